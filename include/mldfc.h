@@ -587,6 +587,178 @@ MLD_API int mld_decoder_step(mld_decoder* dec, const void* x_in, void* x_out, in
  * is then not valid; call mld_decoder_device_status before stepping again). */
 MLD_API int mld_decoder_step_host(mld_decoder* dec, const void* x_host, void* y_host, int32_t pos, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Key/value cache in 4 bits: pages, rotation and norms, attention            */
+/* ------------------------------------------------------------------------ */
+
+/* The reference keeps K and V in float tensors (samples/llm/
+ * qwen3_model_builder.cc:543-846) and serves one sequence; what follows has no
+ * counterpart in it beyond the arithmetic named at each function.
+ *
+ * A cache is a pool of pages that the caller owns (mld_kv4_pool_bytes, one pool
+ * per layer).  32 neighbouring values of a head share a scale:
+ *   scale = fp16(bf16(absmax / 7)), q = clamp(round(x / scale), -7, 7) of x
+ * rounded to fp16, ties to even; a value of the cache is scale * q, which always
+ * is an fp16 number.  Groups with an infinity or a NaN get a NaN scale.  A page
+ * is [kv_heads][page_tokens / 16] tiles of 18 * head_dim bytes (for both K and
+ * V: 144 bytes per token and head of 128, 512 in fp16); what is where in a tile
+ * is the library's matter.  Slot s of a pool is token s % page_tokens of page
+ * s / page_tokens. */
+typedef struct mld_kv4_desc {
+  int32_t kv_heads;          /* 1 to 1024 */
+  int32_t head_dim;          /* 64, 128 or 256 */
+  int32_t page_tokens;       /* multiple of 16, 16 to 65536 */
+  int32_t pages;
+} mld_kv4_desc;
+
+/* 0 for a bad descriptor. */
+MLD_API size_t mld_kv4_page_bytes(const mld_kv4_desc* d);
+MLD_API size_t mld_kv4_pool_bytes(const mld_kv4_desc* d);
+
+/* Keys and values of `tokens` tokens into the pool: token i to slots[i] (int32
+ * on the device, no slot twice; a slot outside the pool is passed over, so -1
+ * marks padding).  k, v: [tokens] rows of kv_heads * head_dim values, fp16 when
+ * f16 else fp32, `stride` elements from token to token, 16-byte aligned. */
+MLD_API int mld_kv4_write(const mld_kv4_desc* d, void* pool, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, int32_t f16, const int32_t* slots, int32_t tokens, void* stream);
+/* The cache's values at `slots`, in fp16 (exactly); zeros for a slot outside
+ * the pool. */
+MLD_API int mld_kv4_read(const mld_kv4_desc* d, const void* pool, const int32_t* slots, int32_t tokens, void* k,
+                         int64_t k_stride, void* v, int64_t v_stride, void* stream);
+/* Copies whole pages from[i] -> to[i] (HOST arrays, checked) in each of `layers`
+ * pools that lie layer_bytes apart.  Copies have no order among them: a page
+ * that is written must appear once.  Lists of up to 480 pages are one launch. */
+MLD_API int mld_kv4_copy_pages(const mld_kv4_desc* d, void* pool, int32_t layers, int64_t layer_bytes,
+                               const int32_t* from, const int32_t* to, int32_t count, void* stream);
+
+/* Who holds which page: host memory only, no CUDA calls, one thread at a time.
+ * Sequences are numbered 0 to max_sequences - 1 in the order of free places. */
+typedef struct mld_kv4_pager mld_kv4_pager;
+MLD_API int mld_kv4_pager_create(int32_t pages, int32_t page_tokens, int32_t max_sequences, mld_kv4_pager** out);
+MLD_API int mld_kv4_pager_destroy(mld_kv4_pager* pager);
+MLD_API int mld_kv4_pager_free_pages(const mld_kv4_pager* pager);
+/* A new, empty sequence; MLD_OUT_OF_RANGE when all are taken. */
+MLD_API int mld_kv4_pager_open(mld_kv4_pager* pager, int32_t* sequence);
+MLD_API int mld_kv4_pager_length(const mld_kv4_pager* pager, int32_t sequence, int32_t* tokens);
+/* The sequence's pages in order: a row of mld_kv4_attn_io.page_table. */
+MLD_API int mld_kv4_pager_table(const mld_kv4_pager* pager, int32_t sequence, int32_t* table, int32_t capacity,
+                                int32_t* count);
+/* Room for `tokens` more: their slots, and, when the last page was shared and
+ * not full, the one copy (copies = 1, from -> to) that has to run before them.
+ * MLD_OUT_OF_RANGE, with nothing changed, when there are not enough pages. */
+MLD_API int mld_kv4_pager_append(mld_kv4_pager* pager, int32_t sequence, int32_t tokens, int32_t* slots,
+                                 int32_t* copy_from, int32_t* copy_to, int32_t* copies);
+/* A second sequence with the same tokens, sharing all pages. */
+MLD_API int mld_kv4_pager_fork(mld_kv4_pager* pager, int32_t sequence, int32_t* fork);
+/* Keeps the first `tokens` tokens (rejected drafts); frees pages behind them. */
+MLD_API int mld_kv4_pager_truncate(mld_kv4_pager* pager, int32_t sequence, int32_t tokens);
+MLD_API int mld_kv4_pager_close(mld_kv4_pager* pager, int32_t sequence);
+/* Moves pages from the end of the pool into holes before it, at most `capacity`
+ * of them; the tables are changed at once, the copies have to run before the
+ * next use of the pool. */
+MLD_API int mld_kv4_pager_compact(mld_kv4_pager* pager, int32_t* copy_from, int32_t* copy_to, int32_t capacity,
+                                  int32_t* copies);
+
+typedef enum mld_rope_pairing {
+  MLD_ROPE_HALVES = 0,       /* value i with value i + rotary_dim / 2
+                                (common/kernels/rope.cc:70-89) */
+  MLD_ROPE_NEIGHBOURS = 1    /* value 2 i with value 2 i + 1 */
+} mld_rope_pairing;
+
+/* RMS norm of every query and key head, y = x w / sqrt(mean(x^2) + eps), and
+ * the rotation of its first rotary_dim values in the same pass: pair i turns by
+ *   position / (min_timescale (max_timescale / min_timescale)^(2 i / rotary_dim)).
+ * Positions have 1 to 4 axes (text: one; time, height, width: three): the first
+ * sections[0] pairs turn by axis 0, the next sections[1] by axis 1, ... */
+typedef struct mld_qk_rope_desc {
+  int32_t heads, kv_heads;   /* either may be 0 */
+  int32_t head_dim;          /* 64, 128 or 256 */
+  int32_t rotary_dim;        /* multiple of 16 up to head_dim; 0: no rotation */
+  int32_t pairing;           /* mld_rope_pairing */
+  int32_t axes;              /* 1 to 4 */
+  int32_t sections[4];       /* pairs per axis, rotary_dim / 2 in all */
+  float min_timescale, max_timescale;
+  float rms_eps;
+  int32_t f16;               /* 1: tensors and weights are fp16, 0: fp32 */
+} mld_qk_rope_desc;
+
+/* Tensors of a call: rows of heads * head_dim values, `stride` elements from
+ * token to token, 16-byte aligned.  q_out may be q and k_out may be k (with the
+ * same stride); otherwise outputs must not overlap inputs. */
+typedef struct mld_qk_rope_io {
+  const void* q;
+  int64_t q_stride;
+  const void* k;
+  int64_t k_stride;
+  const void* v;             /* with a pool only */
+  int64_t v_stride;
+  const void *q_weight, *k_weight; /* [head_dim]; NULL: no norm */
+  const int32_t* positions;  /* device, [axes][tokens] */
+  void* q_out;
+  int64_t q_out_stride;
+  void* k_out;               /* may be NULL with a pool */
+  int64_t k_out_stride;
+  const mld_kv4_desc* cache; /* with a pool only */
+  void* pool;                /* not NULL: keys (rounded to the tensors' type, as
+                                in k_out) and values go to `slots` as by
+                                mld_kv4_write, in the same pass */
+  const int32_t* slots;
+} mld_qk_rope_io;
+
+typedef struct mld_qk_rope_plan mld_qk_rope_plan;
+/* A plan holds the frequencies, in host memory, and nothing on the device: it
+ * may be used on any stream, and by several threads at once. */
+MLD_API int mld_qk_rope_plan_create(const mld_qk_rope_desc* d, mld_qk_rope_plan** out);
+MLD_API int mld_qk_rope_plan_destroy(mld_qk_rope_plan* plan);
+MLD_API int mld_qk_rope_run(mld_qk_rope_plan* plan, const mld_qk_rope_io* io, int32_t tokens, void* stream);
+
+/* Attention of new tokens over the cache, which holds their keys and values
+ * already: what the reference assembles from FullyConnected(q, K), mask,
+ * SoftmaxReduce and FullyConnected(p, V) (samples/llm/
+ * qwen3_model_builder.cc:983-1017).  Head h reads key/value head
+ * h / (heads / kv_heads).  Query token i of m of a sequence of n cached tokens
+ * stands at n - m + i and sees the tokens at or before it, with a window only
+ * the last `window` of those; a query that sees none gives zeros. */
+typedef struct mld_kv4_attn_desc {
+  mld_kv4_desc cache;
+  int32_t heads;             /* a multiple of cache.kv_heads, up to 4096 */
+  int32_t max_batch;         /* 1 to 1024 sequences in a call */
+  int32_t max_pages;         /* entries of a row of the page table */
+  int32_t window;            /* 0: none */
+  float scale;               /* of q.k; 0: 1 / sqrt(head_dim) */
+  int32_t device;            /* -1 = current */
+} mld_kv4_attn_desc;
+
+typedef struct mld_kv4_attn_io {
+  const void* q;             /* fp16 [q_tokens] rows of heads * head_dim */
+  int64_t q_stride;          /* elements from token to token */
+  const void* pool;
+  const int32_t* page_table; /* device, [batch][max_pages]; entries behind a
+                                sequence's last page are not read */
+  const int32_t* lens;       /* device, [batch]: cached tokens, the new ones
+                                among them; 0 is a length */
+  const int32_t* q_starts;   /* device, [batch + 1]: rows of each sequence in q,
+                                ascending; NULL: one row each */
+  int32_t batch, q_tokens;
+  int32_t max_queries;       /* most rows of one sequence */
+  void* out;                 /* fp16, as q */
+  int64_t out_stride;
+} mld_kv4_attn_io;
+
+typedef struct mld_kv4_attn_plan mld_kv4_attn_plan;
+/* All workspace is allocated here and is clear when the call returns.  A plan
+ * may be used from one stream at a time; calls may be captured. */
+MLD_API int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out);
+MLD_API int mld_kv4_attn_plan_destroy(mld_kv4_attn_plan* plan);
+MLD_API size_t mld_kv4_attn_plan_workspace_bytes(const mld_kv4_attn_plan* plan);
+MLD_API int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* stream);
+/* Synchronous: *code = 0, or what a kernel found since the last call (then
+ * cleared): MLD_OUT_OF_RANGE for a page, length or row range on the device that
+ * does not fit (pages outside the pool are read as page 0, lengths and ranges
+ * are cut, nothing is accessed out of range), MLD_TIMEOUT for a bounded wait
+ * that gave up. */
+MLD_API int mld_kv4_attn_plan_device_status(mld_kv4_attn_plan* plan, int32_t* code);
+
 #ifdef __cplusplus
 }
 #endif

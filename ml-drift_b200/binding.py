@@ -84,6 +84,13 @@ def lib() -> C.CDLL:
         L.mld_attn_decode.argtypes = [p, p, p, p, i, i, i, p]
         L.mld_decoder_step.argtypes = [p, p, p, i, p]
         L.mld_decoder_step_host.argtypes = [p, p, p, i, p]
+        l = C.c_int64
+        L.mld_kv4_page_bytes.restype = L.mld_kv4_pool_bytes.restype = L.mld_kv4_attn_plan_workspace_bytes.restype = C.c_size_t
+        L.mld_kv4_write.argtypes = [p, p, p, l, p, l, i, p, i, p]
+        L.mld_kv4_read.argtypes = [p, p, p, i, p, l, p, l, p]
+        L.mld_kv4_copy_pages.argtypes = [p, p, i, l, p, p, i, p]
+        L.mld_qk_rope_run.argtypes = [p, p, i, p]
+        L.mld_kv4_attn_run.argtypes = [p, p, p]
         _lib = L
     return _lib
 
@@ -448,6 +455,295 @@ class Decoder:
     def close(self):
         if self._h:
             lib().mld_decoder_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# ------------------------------------------------- key/value cache in 4 bits
+ROPE_HALVES, ROPE_NEIGHBOURS = 0, 1
+
+
+class Kv4Desc(C.Structure):
+    _fields_ = [("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("page_tokens", C.c_int32), ("pages", C.c_int32)]
+
+
+class QkRopeDesc(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32), ("rotary_dim", C.c_int32),
+                ("pairing", C.c_int32), ("axes", C.c_int32), ("sections", C.c_int32 * 4), ("min_timescale", C.c_float),
+                ("max_timescale", C.c_float), ("rms_eps", C.c_float), ("f16", C.c_int32)]
+
+
+class QkRopeIo(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("k", C.c_void_p), ("k_stride", C.c_int64), ("v", C.c_void_p),
+                ("v_stride", C.c_int64), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p), ("positions", C.c_void_p),
+                ("q_out", C.c_void_p), ("q_out_stride", C.c_int64), ("k_out", C.c_void_p), ("k_out_stride", C.c_int64),
+                ("cache", C.c_void_p), ("pool", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class Kv4AttnDesc(C.Structure):
+    _fields_ = [("cache", Kv4Desc), ("heads", C.c_int32), ("max_batch", C.c_int32), ("max_pages", C.c_int32),
+                ("window", C.c_int32), ("scale", C.c_float), ("device", C.c_int32)]
+
+
+class Kv4AttnIo(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64), ("pool", C.c_void_p), ("page_table", C.c_void_p),
+                ("lens", C.c_void_p), ("q_starts", C.c_void_p), ("batch", C.c_int32), ("q_tokens", C.c_int32),
+                ("max_queries", C.c_int32), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+def _rows(t, heads, head_dim, dtype, what):
+    """Elements from token to token of a [tokens][heads][head_dim] tensor whose rows are contiguous."""
+    _, h, d = t.shape
+    stride = t.stride()
+    if t.dtype is not dtype or h != heads or d != head_dim or stride[2] != 1 or (stride[1] != head_dim and heads > 1):
+        raise ValueError(f"{what}: expected {dtype} [tokens][{heads}][{head_dim}] with contiguous heads, "
+                         f"got {t.dtype} {tuple(t.shape)} strides {stride}")
+    return stride[0]
+
+
+def _ints(t, shape, what):
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+class Kv4Cache:
+    """A pool of pages for each of `layers` layers: keys and values in 4 bits, scales per 32 values (see mldfc.h)."""
+
+    def __init__(self, kv_heads, head_dim, page_tokens, pages, layers=1, pool=None, device="cuda"):
+        self.desc = Kv4Desc(kv_heads, head_dim, page_tokens, pages)
+        self.layers = layers
+        self.layer_bytes = int(lib().mld_kv4_pool_bytes(C.byref(self.desc)))
+        if self.layer_bytes == 0:
+            raise MldError(INVALID_ARGUMENT, "mld_kv4_pool_bytes")
+        shape = (layers, pages, kv_heads, page_tokens // 16, 18 * head_dim)
+        if pool is None:
+            pool = torch.zeros(shape, dtype=torch.uint8, device=device)
+        if pool.dtype != torch.uint8 or tuple(pool.shape) != shape or not pool.is_contiguous():
+            raise ValueError(f"pool: expected contiguous uint8 {shape}, got {pool.dtype} {tuple(pool.shape)}")
+        self.pool, self.head_dim, self._base = pool, head_dim, pool.data_ptr()
+
+    def address(self, layer=0):
+        if not 0 <= layer < self.layers:
+            raise IndexError(f"layer {layer} of {self.layers}")
+        return self._base + layer * self.layer_bytes
+
+    def write(self, k, v, slots, layer=0, stream=None):
+        """k, v: [tokens][kv_heads][head_dim] fp16 or fp32; slots: int32 [tokens] on the device (-1: passed over)."""
+        d = self.desc
+        ks, vs = (_rows(t, d.kv_heads, d.head_dim, k.dtype, n) for t, n in ((k, "k"), (v, "v")))
+        n = _same_tokens(k, v)
+        _check(lib().mld_kv4_write(C.byref(d), self.address(layer), k.data_ptr(), ks, v.data_ptr(), vs, _f16(k),
+                                   _ints(slots, (n,), "slots"), n, _stream_addr(stream)), "mld_kv4_write")
+
+    def read(self, slots, k, v, layer=0, stream=None):
+        """The cache's values at `slots` into k and v, fp16 [tokens][kv_heads][head_dim]."""
+        d = self.desc
+        hk, hd = d.kv_heads, d.head_dim
+        ks, vs = _rows(k, hk, hd, torch.float16, "k"), _rows(v, hk, hd, torch.float16, "v")
+        n = _same_tokens(k, v)
+        rc = _lib.mld_kv4_read(C.byref(d), self.address(layer), _ints(slots, (n,), "slots"), n, k.data_ptr(), ks, v.data_ptr(), vs,
+                               _stream_addr(stream))
+        if rc != OK:
+            _check(rc, "mld_kv4_read")
+
+    def copy_pages(self, src, dst, stream=None):
+        """Copies whole pages in all layers; src, dst: page numbers on the host."""
+        n = len(src)
+        if len(dst) != n:
+            raise ValueError("src and dst differ in length")
+        ints = C.c_int32 * n
+        _check(lib().mld_kv4_copy_pages(C.byref(self.desc), self.pool.data_ptr(), self.layers, self.layer_bytes, ints(*src),
+                                        ints(*dst), n, _stream_addr(stream)), "mld_kv4_copy_pages")
+
+
+def _tokens(t, n, what):
+    if t.shape[0] != n:
+        raise ValueError(f"{what}: {t.shape[0]} tokens where the others have {n}")
+
+
+def _same_tokens(*tensors):
+    n = tensors[0].shape[0]
+    if any(t.shape[0] != n for t in tensors):
+        raise ValueError(f"tensors of different token counts: {[t.shape[0] for t in tensors]}")
+    return n
+
+
+def _f16(t):
+    if t.dtype not in (torch.float16, torch.float32):
+        raise ValueError(f"expected float16 or float32, got {t.dtype}")
+    return int(t.dtype == torch.float16)
+
+
+class Kv4Pager:
+    """Which sequence holds which page of a pool (host only): open, append, fork, truncate, close, compact."""
+
+    def __init__(self, pages, page_tokens, max_sequences):
+        self._h = C.c_void_p()
+        self.pages = pages
+        _check(lib().mld_kv4_pager_create(pages, page_tokens, max_sequences, C.byref(self._h)), "mld_kv4_pager_create")
+
+    def free_pages(self) -> int:
+        return int(lib().mld_kv4_pager_free_pages(self._h))
+
+    def open(self) -> int:
+        s = C.c_int32()
+        _check(lib().mld_kv4_pager_open(self._h, C.byref(s)), "mld_kv4_pager_open")
+        return s.value
+
+    def length(self, sequence) -> int:
+        n = C.c_int32()
+        _check(lib().mld_kv4_pager_length(self._h, sequence, C.byref(n)), "mld_kv4_pager_length")
+        return n.value
+
+    def table(self, sequence) -> list:
+        buf, n = (C.c_int32 * self.pages)(), C.c_int32()
+        _check(lib().mld_kv4_pager_table(self._h, sequence, buf, self.pages, C.byref(n)), "mld_kv4_pager_table")
+        return list(buf[:n.value])
+
+    def append(self, sequence, tokens):
+        """(slots of the new tokens, [(from, to)] pages to copy before they are written)."""
+        slots = (C.c_int32 * max(tokens, 1))()
+        src, dst, n = C.c_int32(), C.c_int32(), C.c_int32()
+        _check(lib().mld_kv4_pager_append(self._h, sequence, tokens, slots, C.byref(src), C.byref(dst), C.byref(n)),
+               "mld_kv4_pager_append")
+        return list(slots[:tokens]), [(src.value, dst.value)] * n.value
+
+    def fork(self, sequence) -> int:
+        s = C.c_int32()
+        _check(lib().mld_kv4_pager_fork(self._h, sequence, C.byref(s)), "mld_kv4_pager_fork")
+        return s.value
+
+    def truncate(self, sequence, tokens):
+        _check(lib().mld_kv4_pager_truncate(self._h, sequence, tokens), "mld_kv4_pager_truncate")
+
+    def close_sequence(self, sequence):
+        _check(lib().mld_kv4_pager_close(self._h, sequence), "mld_kv4_pager_close")
+
+    def compact(self, most=None):
+        """(src, dst): page copies to run (Kv4Cache.copy_pages) before the pool is used again."""
+        most = self.pages if most is None else most
+        src, dst, n = (C.c_int32 * max(most, 1))(), (C.c_int32 * max(most, 1))(), C.c_int32()
+        _check(lib().mld_kv4_pager_compact(self._h, src, dst, most, C.byref(n)), "mld_kv4_pager_compact")
+        return list(src[:n.value]), list(dst[:n.value])
+
+    def close(self):
+        if self._h:
+            lib().mld_kv4_pager_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class QkNormRope:
+    """Norms of queries and keys per head with the rotation in the same pass; with a cache, keys and values written to it."""
+
+    def __init__(self, heads, kv_heads, head_dim, rotary_dim=None, pairing=ROPE_HALVES, sections=None, min_timescale=1.0,
+                 max_timescale=1.0e6, rms_eps=1e-6, f16=True):
+        rotary_dim = head_dim if rotary_dim is None else rotary_dim
+        sections = [rotary_dim // 2] if sections is None else list(sections)
+        if len(sections) > 4:
+            raise ValueError("positions have 1 to 4 axes")
+        self.desc = QkRopeDesc(heads, kv_heads, head_dim, rotary_dim, pairing, len(sections), (C.c_int32 * 4)(*sections),
+                               min_timescale, max_timescale, rms_eps, int(f16))
+        self.heads, self.kv_heads, self.head_dim, self.axes = heads, kv_heads, head_dim, len(sections)
+        self.dtype = torch.float16 if f16 else torch.float32
+        self._h = C.c_void_p()
+        _check(lib().mld_qk_rope_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_qk_rope_plan_create")
+
+    def run(self, q, k, positions, q_out, k_out=None, q_weight=None, k_weight=None, v=None, cache=None, slots=None, layer=0,
+            stream=None):
+        """q, k, v: [tokens][heads][head_dim] (rows may be strided); positions: int32 [tokens] or [axes][tokens] on the device."""
+        h, hk, d, dt = self.heads, self.kv_heads, self.head_dim, self.dtype
+        n = (q if h else k).shape[0]
+        io = QkRopeIo()
+        if h:
+            io.q, io.q_stride = q.data_ptr(), _rows(q, h, d, dt, "q")
+            io.q_out, io.q_out_stride = q_out.data_ptr(), _rows(q_out, h, d, dt, "q_out")
+            _tokens(q_out, n, "q_out")
+        if hk:
+            io.k, io.k_stride = k.data_ptr(), _rows(k, hk, d, dt, "k")
+            _tokens(k, n, "k")
+            if k_out is not None:
+                io.k_out, io.k_out_stride = k_out.data_ptr(), _rows(k_out, hk, d, dt, "k_out")
+                _tokens(k_out, n, "k_out")
+        for w in (q_weight, k_weight):
+            if w is not None and (w.dtype is not dt or w.shape != (d,) or not w.is_contiguous()):
+                raise ValueError(f"norm weights: expected contiguous {dt} [{d}]")
+        if q_weight is not None:
+            io.q_weight = q_weight.data_ptr()
+        if k_weight is not None:
+            io.k_weight = k_weight.data_ptr()
+        if positions is not None:
+            io.positions = _ints(positions, (n,) if self.axes == 1 and positions.dim() == 1 else (self.axes, n), "positions")
+        if cache is not None:
+            if v is None or slots is None:
+                raise ValueError("a cache needs v and slots")
+            io.v, io.v_stride = v.data_ptr(), _rows(v, hk, d, dt, "v")
+            _tokens(v, n, "v")
+            io.cache, io.pool, io.slots = C.addressof(cache.desc), cache.address(layer), _ints(slots, (n,), "slots")
+        rc = _lib.mld_qk_rope_run(self._h, C.byref(io), n, _stream_addr(stream))
+        if rc != OK:
+            _check(rc, "mld_qk_rope_run")
+
+    def close(self):
+        if self._h:
+            lib().mld_qk_rope_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Kv4Attention:
+    """Attention of new tokens over a Kv4Cache (which holds their keys and values already)."""
+
+    def __init__(self, cache, heads, max_batch, max_pages, window=0, scale=0.0, device=-1):
+        self.cache, self.heads, self.max_pages = cache, heads, max_pages
+        self.desc = Kv4AttnDesc(cache.desc, heads, max_batch, max_pages, window, scale, device)
+        self._h = C.c_void_p()
+        _check(lib().mld_kv4_attn_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_kv4_attn_plan_create")
+
+    def run(self, q, page_table, lens, out, q_starts=None, max_queries=1, layer=0, stream=None):
+        """q, out: fp16 [tokens][heads][head_dim]; page_table: int32 [batch][max_pages]; lens: int32 [batch]; q_starts: int32
+        [batch + 1], the rows of each sequence, of which none has more than max_queries (None: one row each)."""
+        d, h = self.cache.head_dim, self.heads
+        batch, n = lens.shape[0], q.shape[0]
+        _tokens(out, n, "out")
+        io = Kv4AttnIo(q.data_ptr(), _rows(q, h, d, torch.float16, "q"), self.cache.address(layer),
+                       _ints(page_table, (batch, self.max_pages), "page_table"), _ints(lens, (batch,), "lens"),
+                       None if q_starts is None else _ints(q_starts, (batch + 1,), "q_starts"), batch, n, max_queries,
+                       out.data_ptr(), _rows(out, h, d, torch.float16, "out"))
+        rc = _lib.mld_kv4_attn_run(self._h, C.byref(io), _stream_addr(stream))
+        if rc != OK:
+            _check(rc, "mld_kv4_attn_run")
+
+    def workspace_bytes(self) -> int:
+        return int(lib().mld_kv4_attn_plan_workspace_bytes(self._h))
+
+    def device_status(self) -> int:
+        """0, or the code of what a kernel found out of range or gave up waiting for (then cleared)."""
+        code = C.c_int32(0)
+        rc = lib().mld_kv4_attn_plan_device_status(self._h, C.byref(code))
+        if rc not in (OK, TIMEOUT, OUT_OF_RANGE):
+            raise MldError(rc, "mld_kv4_attn_plan_device_status")
+        return code.value
+
+    def close(self):
+        if self._h:
+            lib().mld_kv4_attn_plan_destroy(self._h)
             self._h = C.c_void_p()
 
     def __del__(self):

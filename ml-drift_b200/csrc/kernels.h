@@ -18,6 +18,10 @@ int pack_scales_impl(const float* src, int32_t o, int32_t g, int32_t dst_f16, vo
 int quantize_weights_impl(const float* w, int32_t o, int32_t i, int32_t bits, int32_t block, int8_t* q,
                           float* scale, cudaStream_t stream);
 
+// ------------------------------------------------------------------ 4-bit cache
+constexpr int kKv4MaxBatch = 1024;
+int check_kv4_desc(const mld_kv4_desc* d);
+
 // ------------------------------------------------------------------ decode GEMV
 struct GenericArgs {
   const void* x;
