@@ -14,8 +14,8 @@ OUT = os.path.join(HERE, "libmldfc.so")
 
 SOURCES = ["api.cu", "pack_kernels.cu", "gemv_generic.cu", "gemv_stream.cu", "decode_step.cu", "decode_mega.cu",
            "gemm_umma.cu", "gemm_pair.cu", "gemm_wtmem.cu", "shard_group.cu", "embedding.cu", "loader.cu",
-           "qk_rope.cu", "kv4_attn.cu", "kv4_pages.cu"]
-HEADERS = ["common.cuh", "kernels.h", "nccl_lazy.h", "pair_common.cuh", "ring_order.h", "kv4.cuh", os.path.join(ROOT, "include", "mldfc.h")]
+           "qk_rope.cu", "kv4_attn.cu", "kv4_prefill.cu", "kv4_pages.cu"]
+HEADERS = ["common.cuh", "kernels.h", "nccl_lazy.h", "pair_common.cuh", "ring_order.h", "kv4.cuh", "kv4_attn.cuh", os.path.join(ROOT, "include", "mldfc.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

@@ -125,8 +125,7 @@ __device__ __forceinline__ void tmem_alloc_all(uint32_t* smem_dst) {
     tmem_alloc_pair(smem_dst, 512);
     tmem_relinquish_pair();
   } else {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(smem_dst)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    tmem_alloc_512(smem_dst);
   }
 }
 template <bool PAIR>
@@ -134,7 +133,7 @@ __device__ __forceinline__ void tmem_dealloc_all(uint32_t taddr) {
   if constexpr (PAIR) {
     tmem_dealloc_pair(taddr, 512);
   } else {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
+    tmem_dealloc_512(taddr);
   }
 }
 

@@ -27,31 +27,13 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
+#include "kv4_attn.cuh"
 
 namespace mld {
 namespace {
 
 constexpr int kMaxGrid = 256;
-
-struct AttnArgs {
-  const __half* q;
-  __half* out;
-  long long q_stride, out_stride;  // elements from token to token
-  const uint8_t* pool;
-  const int32_t* table;  // [batch][max_pages]
-  const int32_t* lens;   // [batch]
-  const int32_t* starts; // [batch + 1], or null: one query token per sequence
-  int batch, max_pages, q_tokens, max_queries;
-  int heads, kv_heads, group;
-  int page_tiles, pages;
-  int window;
-  float scale_log2; // of the scores as the products give them
-  float* part;      // [grid][2][rows][D + 4]
-  int* tickets;     // [grid], zero between launches
-  int* error;
-};
-
-enum { kErrWait = 40, kErrPage = 41, kErrLength = 42 };
+constexpr int kFewRows = 64;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm(
@@ -86,25 +68,6 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t x, float scale, float off
 __device__ __forceinline__ uint32_t code_lo(uint32_t x) { return fma_half2(x & 0x000F000Fu, 32768.0f, -0.015625f); }
 __device__ __forceinline__ uint32_t code_hi(uint32_t x) { return fma_half2(x & 0x00F000F0u, 2048.0f, -0.015625f); }
 
-// Words from shared memory as one access.
-template <int N>
-__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[N]) {
-  if constexpr (N == 1) {
-    w[0] = *reinterpret_cast<const uint32_t*>(p);
-  } else if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-  } else {
-    static_assert(N == 4, "");
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-  }
-}
-
 constexpr float kFloor = -1e30f;   // reference of a row that has seen nothing
 constexpr float kHeadroom = 2.0f;  // how far weights may exceed the reference, as a power of two
 constexpr float kLift = 13.0f;
@@ -129,31 +92,18 @@ struct Span {
 };
 
 template <int D, int NT>
-__device__ __forceinline__ Span span_of(const AttnArgs& a, int b) {
+__device__ __forceinline__ Span span_of(const Kv4AttnArgs& a, int b) {
   using S = Shape<D, NT>;
+  const Kv4Sequence q = kv4_sequence(a, b);
   Span s;
-  const long long most = static_cast<long long>(a.max_pages) * a.page_tiles * kv4::kTile;
-  const int len = __ldg(a.lens + b);
-  s.n = len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
-  s.m = 1;
-  s.first_row_token = b;
-  if (a.starts != nullptr) {
-    int lo = __ldg(a.starts + b), hi = __ldg(a.starts + b + 1);
-    lo = min(max(lo, 0), a.q_tokens);
-    hi = min(max(hi, lo), a.q_tokens);
-    s.m = min(hi - lo, a.max_queries);
-    s.first_row_token = lo;
-  }
+  s.n = q.n;
+  s.m = q.m;
+  s.first_row_token = q.first_token;
   const int first = a.window > 0 ? max(0, s.n - s.m + 1 - a.window) : 0;
   s.c0 = first / S::kChunk;
   s.chunks = max(1, (s.n + S::kChunk - 1) / S::kChunk - s.c0);
   s.blocks = (s.m * a.group + S::kRows - 1) / S::kRows;
   return s;
-}
-
-// Whether the sequence's length and queries were what the call allows (they are cut to that otherwise).
-__device__ __forceinline__ bool fits(const AttnArgs& a, int b, int n, int m) {
-  return a.lens[b] == n && (a.starts == nullptr || (a.starts[b] >= 0 && a.starts[b + 1] - a.starts[b] == m && a.starts[b + 1] <= a.q_tokens));
 }
 
 // Where an item of the work list lies: sequence, key/value head, block of rows, chunk.
@@ -164,7 +114,7 @@ struct Place {
 };
 
 template <int D, int NT>
-__device__ __forceinline__ Place locate(const AttnArgs& a, const int* prefix, int item) {
+__device__ __forceinline__ Place locate(const Kv4AttnArgs& a, const int* prefix, int item) {
   int lo = 0, hi = a.batch - 1;
   while (lo < hi) {  // the last sequence that begins at or before the item
     const int mid = (lo + hi + 1) >> 1;
@@ -230,7 +180,7 @@ struct Rows {
 
 // Query rows of a block as the MMAs' B operand: lane (g, t) holds values 8 t.. of row 8 i + g.
 template <int D, int NT>
-__device__ __forceinline__ void load_q(const AttnArgs& a, const Place& p, const LaneAt<D>& at, Rows<D, NT>& w) {
+__device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Place& p, const LaneAt<D>& at, Rows<D, NT>& w) {
   using S = Shape<D, NT>;
 #pragma unroll
   for (int i = 0; i < NT; ++i) {
@@ -259,10 +209,10 @@ __device__ __forceinline__ void tile_scores(const uint8_t* tile, const LaneAt<D>
   for (int u = 0; u < kG / kW; ++u) {
     uint32_t k0[kW], k1[kW], sc0[kW / 2], sc1[kW / 2];
     const uint8_t* row = tile + (u == 0 ? at.k : at.k2);
-    lds(row, k0);
-    lds(row + 8 * (D / 2), k1);
-    lds(tile + at.ks + 8 * u, sc0);
-    lds(tile + at.ks + 8 * u + 8 * (D / 16), sc1);
+    kv4_lds(row, k0);
+    kv4_lds(row + 8 * (D / 2), k1);
+    kv4_lds(tile + at.ks + 8 * u, sc0);
+    kv4_lds(tile + at.ks + 8 * u + 8 * (D / 16), sc1);
 #pragma unroll
     for (int v = 0; v < kW; ++v) {
       const int j = u * kW + v;
@@ -298,10 +248,10 @@ __device__ __forceinline__ void tile_values(const uint8_t* tile, const LaneAt<D>
                                             const uint32_t (&v0)[D / 64], const uint32_t (&v1)[D / 64]) {
   constexpr int kG = D / 32;
   uint32_t va[kG / 2], vb[kG / 2], vc[kG / 2], vd[kG / 2];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-  lds(tile + at.v, va);
-  lds(tile + at.v + 4 * (D / 2), vb);
-  lds(tile + at.v + 8 * (D / 2), vc);
-  lds(tile + at.v + 12 * (D / 2), vd);
+  kv4_lds(tile + at.v, va);
+  kv4_lds(tile + at.v + 4 * (D / 2), vb);
+  kv4_lds(tile + at.v + 8 * (D / 2), vc);
+  kv4_lds(tile + at.v + 12 * (D / 2), vd);
 #pragma unroll
   for (int j = 0; j < kG; ++j) {
     const float2 f0 = unpack_half2(v0[j >> 1]), f1 = unpack_half2(v1[j >> 1]);
@@ -337,8 +287,8 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
 #pragma unroll
   for (int k = 0; k < TILES; ++k) {
     tile_scores<D, NT>(tiles + k * S::kTileBytes, at, w, s[k]);
-    lds(tiles + k * S::kTileBytes + at.vs, v0[k]);
-    lds(tiles + k * S::kTileBytes + at.vs + 8 * (D / 16), v1[k]);
+    kv4_lds(tiles + k * S::kTileBytes + at.vs, v0[k]);
+    kv4_lds(tiles + k * S::kTileBytes + at.vs + 8 * (D / 16), v1[k]);
   }
   if (MASKED) {
 #pragma unroll
@@ -427,7 +377,7 @@ __device__ __forceinline__ void put4(__half* p, float a, float b, float c, float
 
 // Row `row` of a block in the output tensor; null beyond the sequence's rows.
 template <int D, int NT>
-__device__ __forceinline__ __half* out_row(const AttnArgs& a, const Place& p, int row) {
+__device__ __forceinline__ __half* out_row(const Kv4AttnArgs& a, const Place& p, int row) {
   row += p.r * Shape<D, NT>::kRows;
   if (row >= p.s.m * a.group) return nullptr;
   const int token = row / a.group, head = p.h * a.group + row - token * a.group;
@@ -437,7 +387,7 @@ __device__ __forceinline__ __half* out_row(const AttnArgs& a, const Place& p, in
 // Ends a warp's part of a segment: `slot` null: it is the whole segment, the rows are written out; else the values as they
 // are, the references and the sums go to the slot.
 template <int D, int NT>
-__device__ __forceinline__ void finish(const AttnArgs& a, const Place& p, const LaneAt<D>& at, Rows<D, NT>& w, float* slot) {
+__device__ __forceinline__ void finish(const Kv4AttnArgs& a, const Place& p, const LaneAt<D>& at, Rows<D, NT>& w, float* slot) {
   using S = Shape<D, NT>;
   const int g = at.g, t = at.t;
 #pragma unroll
@@ -559,7 +509,7 @@ struct Shares {
 };
 
 template <int D, int NT, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   using S = Shape<D, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* const ring_all = smem;                                                                 // [WARPS][kStages][kStageBytes]
@@ -587,7 +537,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     int mine = 0, mine_segs = 0;
     for (int b = b0; b < b1; ++b) {
       const Span s = span_of<D, NT>(a, b);
-      if (blockIdx.x == 0 && !fits(a, b, s.n, s.m)) atomicExch(a.error, kErrLength);
+      if (blockIdx.x == 0 && !kv4_fits(a, b, {s.n, s.m, s.first_row_token})) atomicExch(a.error, kErrLength);
       mine += a.kv_heads * s.blocks * s.chunks;
       mine_segs += a.kv_heads * s.blocks;
     }
@@ -642,7 +592,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     pi.end = wlo;
     int ii = wlo, pid = 0;
     const LaneAt<D> at(lane);
-    const float inv_scale = 1.0f / a.scale_log2;
+    const float cs = a.scale_log2 * kCodeUnit, inv_scale = 1.0f / cs;  // scores come in units of the codes
     // Lane l of the first kTiles brings tile l of a chunk: its page's number is asked for one chunk ahead.
     const auto next_page = [&]() {
       if (ii == pi.end) pi = locate<D, NT>(a, prefix, ii); else ++pi.c;
@@ -691,39 +641,53 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
         }
       const int sees_lo = p.s.n - p.s.m + p.r * S::kRows / a.group;
       const int sees_hi = p.s.n - p.s.m + min(p.r * S::kRows + S::kRows - 1, p.s.m * a.group - 1) / a.group;
-      // steps that begin here are whole: [whole_lo, whole_hi]
-      const int whole_lo = a.window > 0 ? sees_hi - a.window + 1 : 0, whole_hi = sees_lo - S::kStep * kv4::kTile + 1;
+      // chunks that begin in [whole_lo, whole_hi] are seen by all rows; [first_lo, sees_hi] by any
+      const int whole_lo = a.window > 0 ? sees_hi - a.window + 1 : 0, whole_hi = sees_lo - S::kChunk + 1;
       const int first_lo = a.window > 0 ? sees_lo - a.window + 1 : 0;
       int token = (p.s.c0 + p.c) * S::kChunk;
-#pragma unroll 1
-      for (; item < end; ++item) {
+      const auto arrive = [&]() {
         if (alive) alive = mbar_wait(bars + stage, phase);
-        if (alive) {
-          const uint8_t* chunk = ring + stage * S::kStageBytes;
-#pragma unroll 1
-          for (int k = 0; k < S::kTiles; k += S::kStep, token += S::kStep * kv4::kTile) {
-            if (token > sees_hi || token + S::kStep * kv4::kTile <= first_lo) continue;
-            int last[NT][2], first[NT][2];
-            if (token >= whole_lo && token <= whole_hi) {
-              step<D, NT, S::kStep, false>(chunk + k * S::kTileBytes, at, a.scale_log2, inv_scale, w, last, first, 0);
-            } else {
-#pragma unroll
-              for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  last[i][c] = sees[i][c] - token;
-                  first[i][c] = a.window > 0 ? sees[i][c] - a.window + 1 - token : 0;
-                }
-              step<D, NT, S::kStep, true>(chunk + k * S::kTileBytes, at, a.scale_log2, inv_scale, w, last, first, p.s.n - token);
-            }
-          }
-        }
+      };
+      const auto release = [&]() {
         __syncwarp();
         if (ii < whi && alive) ask(stage);
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1;
         }
+        ++item;
+        token += S::kChunk;
+      };
+      while (item < end) {
+        // two loops: one for both kinds moves the accumulators between registers where its branches meet
+#pragma unroll 1
+        while (item < end && token >= whole_lo && token <= whole_hi) {
+          arrive();
+          if (!alive) break;
+          int none[NT][2];
+#pragma unroll
+          for (int k = 0; k < S::kTiles; k += S::kStep)
+            step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, cs, inv_scale, w, none, none, 0);
+          release();
+        }
+        if (item >= end) break;
+        arrive();
+#pragma unroll 1
+        for (int k = 0; k < S::kTiles; k += S::kStep) {
+          const int from = token + k * kv4::kTile;
+          if (!alive || from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
+          int last[NT][2], first[NT][2];
+#pragma unroll
+          for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              last[i][c] = sees[i][c] - from;
+              first[i][c] = a.window > 0 ? sees[i][c] - a.window + 1 - from : 0;
+            }
+          step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, cs, inv_scale, w, last, first,
+                                      p.s.n - from);
+        }
+        release();
       }
       // a segment that ends here and began here is done; else its part goes to the warp's slot: the ring's place for one that
       // began here (nothing is asked for any more), a place of its own for one that began before
@@ -822,7 +786,7 @@ size_t attn_smem(int batch) {
 }
 
 template <int D, int NT, int WARPS>
-int launch_attn_t(const AttnArgs& a, int grid, cudaStream_t stream) {
+int launch_attn_t(const Kv4AttnArgs& a, int grid, cudaStream_t stream) {
   static bool configured[kMaxDevices];
   int dev;
   const size_t most = attn_smem<D, NT, WARPS>(kKv4MaxBatch);
@@ -932,7 +896,7 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   MLD_REQUIRE(io->q_stride % 8 == 0 && io->out_stride % 8 == 0, "token strides must be multiples of 16 bytes");
   MLD_REQUIRE(io->q_tokens == 1 || (io->q_stride >= width && io->out_stride >= width),
               "token strides must not be shorter than a token");
-  AttnArgs a = {};
+  Kv4AttnArgs a = {};
   a.q = static_cast<const __half*>(io->q);
   a.out = static_cast<__half*>(io->out);
   a.q_stride = io->q_stride;
@@ -952,7 +916,7 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   a.pages = d.cache.pages;
   a.window = d.window;
   const float scale = d.scale > 0.0f ? d.scale : 1.0f / sqrtf(static_cast<float>(d.cache.head_dim));
-  a.scale_log2 = scale * 1.4426950408889634f * kCodeUnit;  // scores come in units of the codes
+  a.scale_log2 = scale * 1.4426950408889634f;
   a.part = plan->part;
   a.tickets = plan->tickets;
   a.error = plan->error;
@@ -964,6 +928,8 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
     set_last_error_text("more work than one call can count: fewer sequences, or a narrower page table");
     return MLD_OUT_OF_RANGE;
   }
+  // Many rows: the tensor cores' own kernel.
+  if (rows > kFewRows) return launch_kv4_prefill(a, d.cache.head_dim, stream);
   const bool few = static_cast<int64_t>(io->max_queries) * a.group <= 8;
   switch (d.cache.head_dim) {
     case 64:

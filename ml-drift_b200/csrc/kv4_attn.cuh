@@ -1,0 +1,82 @@
+// Shared by the two attention kernels over the 4-bit cache: arguments and what a sequence has of them.
+#pragma once
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "kv4.cuh"
+
+namespace mld {
+
+struct Kv4AttnArgs {
+  const __half* q;
+  __half* out;
+  long long q_stride, out_stride;  // elements from token to token
+  const uint8_t* pool;
+  const int32_t* table;   // [batch][max_pages]
+  const int32_t* lens;    // [batch]
+  const int32_t* starts;  // [batch + 1], or null: one query token per sequence
+  int batch, max_pages, q_tokens, max_queries;
+  int heads, kv_heads, group;
+  int page_tiles, pages;
+  int window;
+  float scale_log2;  // log2(e) times the scale of the scores
+  float* part;       // [grid][2][rows][D + 4]
+  int* tickets;      // [grid], zero between launches
+  int* error;
+};
+
+int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, cudaStream_t stream);
+
+#ifdef __CUDACC__
+namespace {
+
+enum { kErrWait = 40, kErrPage = 41, kErrLength = 42 };
+
+struct Kv4Sequence {
+  int n, m, first_token;  // cached tokens, queries, the first query's row in q
+};
+__device__ __forceinline__ Kv4Sequence kv4_sequence(const Kv4AttnArgs& a, int b) {
+  Kv4Sequence s;
+  const long long most = static_cast<long long>(a.max_pages) * a.page_tiles * kv4::kTile;
+  const int len = __ldg(a.lens + b);
+  s.n = len < 0 ? 0 : len > most ? static_cast<int>(most) : len;
+  s.m = 1;
+  s.first_token = b;
+  if (a.starts != nullptr) {
+    int lo = __ldg(a.starts + b), hi = __ldg(a.starts + b + 1);
+    lo = min(max(lo, 0), a.q_tokens);
+    hi = min(max(hi, lo), a.q_tokens);
+    s.m = min(hi - lo, a.max_queries);
+    s.first_token = lo;
+  }
+  return s;
+}
+// Whether the sequence's length and queries were what the call allows (they are cut to that otherwise).
+__device__ __forceinline__ bool kv4_fits(const Kv4AttnArgs& a, int b, const Kv4Sequence& s) {
+  return a.lens[b] == s.n && (a.starts == nullptr || (a.starts[b] >= 0 && a.starts[b + 1] - a.starts[b] == s.m && a.starts[b + 1] <= a.q_tokens));
+}
+
+// Words from shared memory as one access.
+template <int N>
+__device__ __forceinline__ void kv4_lds(const uint8_t* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(p);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    static_assert(N == 4, "");
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  }
+}
+
+}  // namespace
+#endif
+
+}  // namespace mld

@@ -1,0 +1,538 @@
+// Attention over the 4-bit cache for many query rows per key/value head (prompts, chunks of prompts), on tcgen05.
+//
+// The rows of a block are the queries of 256 / group tokens for all heads that share a key/value head: two tiles of 128 rows (one
+// for heads of 256 values).  A block walks the cached tokens in steps of N (128; 64 for heads of 256):
+//   S = Q K^T        both operands fp16 from shared memory, 128 x N fp32 in tensor memory
+//   P = 2^(S - ref)  a thread per row; written over S as fp16, where the next product takes it from
+//   O += P V         V from shared memory, 128 x D fp32 in tensor memory
+// The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
+// cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
+// ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
+// by the thread itself, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
+// The two tiles take turns: one's P is made while the other's products run.
+//
+// Roles of the sixteen warps: 0-7 make P and write the rows out, 8-11 unpack, 12 asks for packed tiles, 13 issues the products.
+#include <cuda_fp16.h>
+#include <math.h>
+
+#include "common.cuh"
+#include "kernels.h"
+#include "kv4.cuh"
+#include "kv4_attn.cuh"
+#include "pair_common.cuh"
+
+namespace mld {
+namespace {
+
+constexpr int kPrefillThreads = 512;
+constexpr int kRowsPerTile = 128;
+constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
+constexpr int kMaskedBlocks = 16;  // blocks of tokens that only some rows of a block of rows see, at most
+
+template <int D>
+struct Prefill {
+  static constexpr int kTilesM = D == 256 ? 1 : 2;
+  static constexpr int kRows = kTilesM * kRowsPerTile;
+  static constexpr int kN = D == 256 ? 64 : 128;             // tokens of a step
+  static constexpr int kQBytes = kRowsPerTile * D * 2;       // of a tile
+  static constexpr int kKvBytes = kN * D * 2;                // of K or V of a step
+  static constexpr int kTileBytes = kv4::tile_bytes(D);
+  static constexpr int kPackTiles = 512 / D;                 // packed tiles of a stage of the ring
+  static constexpr int kPackBytes = kPackTiles * kTileBytes; // 9216
+  static constexpr int kPacks = kN / (16 * kPackTiles);      // stages of a step
+  static constexpr int kRing = 3;
+  static constexpr int kO = 256;                             // tensor-memory column of the first O
+  static constexpr size_t kSmem = 1024 + kTilesM * kQBytes + 4 * kKvBytes + kRing * kPackBytes + kMaskedBlocks * kN;
+};
+
+struct PrefillBars {
+  uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+};
+
+__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      : "memory");
+}
+__device__ __forceinline__ void umma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Descriptor of an operand whose 128-byte rows (128-byte swizzle) hold 64 values along M / N, a row per step of K: `columns`
+// bytes between neighbouring 64 values, 1024 bytes from eight rows to the next.
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr, uint32_t columns) {
+  uint64_t d = make_desc(smem_addr);
+  d &= ~(static_cast<uint64_t>(0x3FFF) << 16);
+  return d | static_cast<uint64_t>(columns >> 4) << 16;
+}
+
+__device__ __forceinline__ uint32_t lop3_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+// s (u - 8), exactly, of the codes in bits 0..3 (lo), 4..7 (hi) of both halves.
+__device__ __forceinline__ uint32_t value_lo(uint32_t x, __half2 s) {
+  const uint32_t b = lop3_and_or(x, 0x000F000Fu, 0x64006400u);  // 1024 + u
+  const __half2 h = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1032.0f)), s);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t value_hi(uint32_t x, __half2 s) {
+  const uint32_t b = lop3_and_or(x, 0x00F000F0u, 0x64006400u);  // 1024 + 16 u
+  const __half2 h = __hmul2(__hfma2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(0.0625f), __float2half2_rn(-72.0f)), s);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint4 values8(uint32_t x, __half2 s) {
+  const uint32_t y = x >> 8;
+  return make_uint4(value_lo(x, s), value_hi(x, s), value_lo(y, s), value_hi(y, s));
+}
+
+// Two weights at once: 2^(s * scale - ref).
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+__device__ __forceinline__ float exp2_hw(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks) {
+  using S = Prefill<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* const s_q = smem;                                  // [kTilesM][D / 64][128 rows][128 bytes]
+  uint8_t* const s_k = s_q + S::kTilesM * S::kQBytes;         // [2][D / 64][kN rows][128 bytes]
+  uint8_t* const s_v = s_k + 2 * S::kKvBytes;                 // [2][D / 64][kN rows][128 bytes]
+  uint8_t* const s_pack = s_v + 2 * S::kKvBytes;              // [kRing][kPackBytes]
+  uint8_t* const s_bad = s_pack + S::kRing * S::kPackBytes;   // [kMaskedBlocks][kN]: groups of V that are not finite
+  __shared__ PrefillBars bars;
+  __shared__ uint32_t tmem_base;
+  __shared__ int any_bad;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < S::kRing; ++i) {
+      mbar_init(&bars.pack_full[i], 1);
+      mbar_init(&bars.pack_empty[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bars.k_full[i], 4);
+      mbar_init(&bars.k_empty[i], 1);
+      mbar_init(&bars.v_full[i], 4);
+      mbar_init(&bars.v_empty[i], 1);
+      mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.pv_done[i], 1);
+    }
+    fence_barrier_init();
+    any_bad = 0;
+  }
+  pdl_wait();
+  // ---- which rows: the blocks with the most tokens ahead of them first
+  const int unit = blockIdx.x / row_blocks;
+  const int b = unit / a.kv_heads, h = unit - b * a.kv_heads;
+  const int block = row_blocks - 1 - (blockIdx.x - unit * row_blocks);
+  const Kv4Sequence q = kv4_sequence(a, b);
+  if (blockIdx.x == 0) {
+    for (int i = threadIdx.x; i < a.batch; i += kPrefillThreads)
+      if (!kv4_fits(a, i, kv4_sequence(a, i))) atomicExch(a.error, kErrLength);
+  }
+  const int rows = q.m * a.group, row0 = block * S::kRows;
+  if (row0 >= rows) return;
+  const int row_end = min(rows, row0 + S::kRows);
+  const int at_lo = q.n - q.m + row0 / a.group, at_hi = q.n - q.m + (row_end - 1) / a.group;  // what the rows see ends here
+  const int first = a.window > 0 ? max(0, at_lo - a.window + 1) : 0;
+  const int step0 = first / S::kN, steps = at_hi < 0 ? 0 : at_hi / S::kN + 1 - step0;
+  // whether all rows see all of a step's tokens
+  const auto whole = [&](int t0, int lo, int hi) { return t0 + S::kN - 1 <= lo && (a.window == 0 || t0 >= hi - a.window + 1); };
+
+  if (warp == 13) tmem_alloc_512(&tmem_base);
+  for (int i = threadIdx.x; i < S::kTilesM * kRowsPerTile * (D / 8); i += kPrefillThreads) {
+    const int r = i / (D / 8), c = i - r * (D / 8);
+    const int row = row0 + r, token = row / a.group, head = h * a.group + row - token * a.group;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < rows) v = __ldg(reinterpret_cast<const uint4*>(a.q + (q.first_token + token) * a.q_stride + static_cast<long long>(head) * D) + c);
+    *reinterpret_cast<uint4*>(s_q + (r / kRowsPerTile) * S::kQBytes + (c >> 3) * (kRowsPerTile * 128) + (r % kRowsPerTile) * 128 +
+                              (((c & 7) ^ (r & 7)) << 4)) = v;
+  }
+  for (int i = threadIdx.x; i < kMaskedBlocks * S::kN / 4; i += kPrefillThreads) reinterpret_cast<uint32_t*>(s_bad)[i] = 0;
+  fence_proxy_async();
+  tc_before();
+  __syncthreads();
+  tc_after();
+  const uint32_t tmem = tmem_base;
+  bool ok = true;
+
+  if (warp < 8) {
+    // ------------------------------------------------------------------ weights, rows
+    const int tile = warp >> 2;
+    if (tile < S::kTilesM) {
+      const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+      const uint32_t t_s = tmem + lanes + tile * S::kN, t_o = tmem + lanes + S::kO + tile * D;
+      const int row = row0 + tile * kRowsPerTile + (warp & 3) * 32 + lane;
+      const int at = q.n - q.m + min(row, rows - 1) / a.group;
+      const int tile_lo = q.n - q.m + min(row0 + tile * kRowsPerTile, rows - 1) / a.group;
+      const int tile_hi = q.n - q.m + min(row0 + tile * kRowsPerTile + kRowsPerTile - 1, rows - 1) / a.group;
+      float top = kPrefillFloor, minus_ref = -kPrefillFloor;
+      float2 sum = make_float2(0.0f, 0.0f);
+      const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
+      const float inv_scale = 1.0f / a.scale_log2;
+      float limit = kPrefillFloor * inv_scale;  // scores that may not be exceeded
+#pragma unroll 1
+      for (int j = 0; j < steps; ++j) {
+        ok = mbar_wait(&bars.s_full[tile], j & 1);
+        if (!ok) break;
+        tc_after();
+        const int t0 = (step0 + j) * S::kN;
+        const bool all = whole(t0, tile_lo, tile_hi);
+        const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of the step
+        uint32_t p[S::kN / 2];
+        float2 part;
+        const auto pass = [&](bool only_max) {
+          float m = -INFINITY;
+          part = make_float2(0.0f, 0.0f);
+          const float2 ref2 = make_float2(minus_ref, minus_ref);
+#pragma unroll
+          for (int c = 0; c < S::kN; c += 32) {
+            uint32_t s[32];
+            tmem_ld32(t_s + c, s);
+            tmem_ld_wait();
+            if (!all) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (c + e > hi || c + e < lo) s[e] = 0xFF800000u;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              float2 x = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+              m = fmaxf(m, fmaxf(x.x, x.y));
+              x = fma2(x, scale2, ref2);
+              x.x = exp2_hw(x.x);
+              x.y = exp2_hw(x.y);
+              part = add2(part, x);
+              p[(c + e) / 2] = half2_bits(x.x, x.y);
+            }
+          }
+          return m;
+        };
+        const float m = pass(false);
+        if (__any_sync(0xFFFFFFFFu, m > limit)) {
+          const float new_top = m > limit ? m * a.scale_log2 : top;
+          const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
+          const float f = exp2_hw(-minus_ref - ref);
+          top = new_top;
+          minus_ref = -ref;
+          limit = new_top > kPrefillFloor ? (new_top + kPrefillHeadroom) * inv_scale : kPrefillFloor * inv_scale;
+          sum.x *= f;
+          sum.y *= f;
+          if (j > 0) {
+            ok = mbar_wait(&bars.pv_done[tile], (j - 1) & 1);
+            if (!ok) break;
+            tc_after();
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(t_o + c, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st32(t_o + c, o);
+            }
+          }
+          pass(false);
+        }
+        sum = add2(sum, part);
+#pragma unroll
+        for (int c = 0; c < S::kN / 2; c += 32) tmem_st32(t_s + c, reinterpret_cast<const uint32_t(&)[32]>(p[c]));
+        tmem_st_wait();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[tile]);
+      }
+      // ---- out
+      if (steps > 0 && ok) ok = mbar_wait(&bars.pv_done[tile], (steps - 1) & 1);
+      tc_after();
+      uint32_t bad = 0;  // groups of the row's values that are not finite
+      if (any_bad) {
+        int k = 0;
+        for (int j = 0; j < steps; ++j) {
+          const int t0 = (step0 + j) * S::kN;
+          if (whole(t0, at_lo, at_hi)) continue;
+          for (int t = 0; t < S::kN; ++t)
+            if (t0 + t <= at && (a.window == 0 || t0 + t > at - a.window)) bad |= s_bad[min(k, kMaskedBlocks - 1) * S::kN + t];
+          ++k;
+        }
+      }
+      const float l = sum.x + sum.y;
+      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+      const int token = row / a.group, head = h * a.group + row - token * a.group;
+      __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (steps > 0 && ok) {
+          tmem_ld32(t_o + c, o);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        const float f = (bad >> (c / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
+        if (row < rows) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            // value k of eight lies in column 2 k, value 4 + k in column 2 k + 1
+            const auto x = [&](int k) { return __uint_as_float(o[e + (k < 4 ? 2 * k : 2 * k - 7)]) * f; };
+            *reinterpret_cast<uint4*>(dst + c + e) =
+                make_uint4(half2_bits(x(0), x(1)), half2_bits(x(2), x(3)), half2_bits(x(4), x(5)), half2_bits(x(6), x(7)));
+          }
+        }
+      }
+      tc_before();
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------------ unpacking
+    const int w = warp - 8;
+    // lanes of one 128-byte access lie four rows apart, so that the swizzle spreads them over all banks
+    const int g = lane >> 2, t = lane & 3, in8 = (g >> 1) | (g & 1) << 2;
+    int stage = 0, phase = 0, masked = -1;
+    constexpr int kWords = D / 32 < 4 ? D / 32 : 4;  // groups of an access
+#pragma unroll 1
+    for (int j = 0; j < steps && ok; ++j) {
+      const int t0 = (step0 + j) * S::kN, buf = j & 1, use = (j >> 1) & 1;
+      const bool all = whole(t0, at_lo, at_hi);
+      if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
+      // K of all packed stages of the step, then V
+#pragma unroll 1
+      for (int kind = 0; kind < 2; ++kind) {
+        ok = mbar_wait(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
+        if (!ok) break;
+        uint8_t* const dst0 = (kind ? s_v : s_k) + buf * S::kKvBytes;
+#pragma unroll 1
+        for (int pk = 0; pk < S::kPacks; ++pk) {
+          int st = stage + pk, ph = phase;
+          if (st >= S::kRing) {
+            st -= S::kRing;
+            ph ^= 1;
+          }
+          if (kind == 0) ok = mbar_wait(&bars.pack_full[st], ph);
+          if (!ok) break;
+          const uint8_t* const pack = s_pack + st * S::kPackBytes;
+#pragma unroll 1
+          for (int u = w; u < S::kPackTiles * 2; u += 4) {  // eight tokens of a tile
+            const int tau = (u & 1) * 8 + in8;
+            const int row = pk * S::kPackTiles * 16 + (u >> 1) * 16 + tau;
+            const bool there = t0 + row < q.n;
+            const uint8_t* const tile = pack + (u >> 1) * S::kTileBytes;
+            uint8_t* const dst = dst0 + row * 128;
+#pragma unroll
+            for (int q4 = 0; q4 < D / 32 / kWords; ++q4) {
+              uint32_t x[kWords], sc[kWords / 2];
+              kv4_lds(tile + kv4::scale_at<D>(kind, tau, q4 * kWords), sc);
+              if (kind == 0) {
+                kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), x);
+              } else {
+                // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
+                const int vr = kv4::v_row(tau);
+                const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
+                uint32_t y[kWords / 2], z[kWords / 2];
+                kv4_lds(piece + 8 * q4, y);
+                kv4_lds(piece + D / 16 + 8 * q4, z);
+#pragma unroll
+                for (int e = 0; e < kWords; ++e) x[e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
+              }
+#pragma unroll
+              for (int e = 0; e < kWords; ++e) {
+                const int jg = q4 * kWords + e, c = jg * 4 + t;
+                __half2 s;
+                *reinterpret_cast<uint32_t*>(&s) = __byte_perm(sc[e >> 1], 0, e & 1 ? 0x3232 : 0x1010);
+                uint4 v = values8(x[e], s);
+                bool drop = !there;
+                if (kind == 1 && !all && there && (*reinterpret_cast<const uint32_t*>(&s) & 0x7C00u) == 0x7C00u) {
+                  drop = true;  // a product with a zero weight would not be zero: noted, and told to the rows that see the token
+                  any_bad = 1;
+                  atomicOr(reinterpret_cast<uint32_t*>(s_bad + masked * S::kN + (row & ~3)), 1u << (jg + 8 * (row & 3)));
+                }
+                if (drop) v = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(dst + (c >> 3) * (S::kN * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
+              }
+            }
+          }
+          if (kind == 1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pack_empty[st]);
+          }
+        }
+        if (!ok) break;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+      }
+      stage += S::kPacks;
+      if (stage >= S::kRing) {
+        stage -= S::kRing;
+        phase ^= 1;
+      }
+    }
+  } else if (warp == 12) {
+    // ------------------------------------------------------------------ packed tiles
+    int stage = 0, phase = 0;
+    const int packs = steps * S::kPacks;
+    const auto page_of = [&](int pk) {
+      const int tile = step0 * (S::kN / 16) + pk * S::kPackTiles + lane;
+      return pk < packs && lane < S::kPackTiles && tile * 16 < q.n ? __ldg(a.table + static_cast<long long>(b) * a.max_pages + tile / a.page_tiles) : 0;
+    };
+    int pid = page_of(0);
+#pragma unroll 1
+    for (int pk = 0; pk < packs; ++pk) {
+      ok = mbar_wait(&bars.pack_empty[stage], phase ^ 1);
+      if (!ok) break;
+      const int tile0 = step0 * (S::kN / 16) + pk * S::kPackTiles;
+      const int there = min(S::kPackTiles, max(0, (q.n + 15) / 16 - tile0));
+      if (lane == 0) mbar_arrive_expect_tx(&bars.pack_full[stage], there * S::kTileBytes);
+      __syncwarp();
+      if (lane < there) {
+        const int tile = tile0 + lane;
+        if (pid < 0 || pid >= a.pages) {
+          atomicExch(a.error, kErrPage);
+          pid = 0;
+        }
+        bulk_load_1d(s_pack + stage * S::kPackBytes + lane * S::kTileBytes,
+                     a.pool + ((static_cast<long long>(pid) * a.kv_heads + h) * a.page_tiles + tile % a.page_tiles) * S::kTileBytes,
+                     S::kTileBytes, &bars.pack_full[stage]);
+      }
+      pid = page_of(pk + 1);
+      if (++stage == S::kRing) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (!ok) {  // copies in flight end before the shared memory does
+      for (int i = 0; i < S::kRing; ++i)
+        for (int ph = 0; ph < 2; ++ph) mbar_wait(&bars.pack_full[i], ph);
+    }
+  } else if (warp == 13) {
+    // ------------------------------------------------------------------ products
+    const uint32_t idesc_s = 1u << 4 | static_cast<uint32_t>(S::kN >> 3) << 17 | 8u << 24;
+    const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
+    const auto scores = [&](int i, int buf) {
+      if (elect_one()) {
+        const uint64_t dq = make_desc(smem_u32(s_q + i * S::kQBytes)), dk = make_desc(smem_u32(s_k + buf * S::kKvBytes));
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_ss(tmem + i * S::kN, dq + static_cast<uint64_t>(((k >> 2) * (kRowsPerTile * 128) + (k & 3) * 32) >> 4),
+                  dk + static_cast<uint64_t>(((k >> 2) * (S::kN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
+        if (i == S::kTilesM - 1) umma_commit(&bars.k_empty[buf]);
+        umma_commit(&bars.s_full[i]);
+      }
+      __syncwarp();
+    };
+    if (steps > 0) {
+      ok = mbar_wait(&bars.k_full[0], 0);
+      tc_after();
+      if (ok)
+        for (int i = 0; i < S::kTilesM; ++i) scores(i, 0);
+    }
+#pragma unroll 1
+    for (int j = 0; j < steps && ok; ++j) {
+      const int buf = j & 1;
+#pragma unroll 1
+      for (int i = 0; i < S::kTilesM && ok; ++i) {
+        if (i == 0) ok = mbar_wait(&bars.v_full[buf], (j >> 1) & 1);
+        if (ok) ok = mbar_wait(&bars.p_full[i], j & 1);
+        if (!ok) break;
+        tc_after();
+        if (elect_one()) {
+          const uint64_t dv = make_desc_mn(smem_u32(s_v + buf * S::kKvBytes), S::kN * 128);
+#pragma unroll
+          for (int k = 0; k < S::kN / 16; ++k)
+            umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + 8 * k, dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
+          if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
+          umma_commit(&bars.pv_done[i]);  // last: the block ends after it
+        }
+        __syncwarp();
+        if (j + 1 < steps) {
+          if (i == 0) {
+            ok = mbar_wait(&bars.k_full[buf ^ 1], ((j + 1) >> 1) & 1);
+            if (!ok) break;
+            tc_after();
+          }
+          scores(i, buf ^ 1);
+        }
+      }
+    }
+  }
+  if (!ok && lane == 0) atomicExch(a.error, kErrWait);
+  tc_before();
+  __syncthreads();
+  tc_after();
+  if (warp == 13) tmem_dealloc_512(tmem);
+}
+
+template <int D>
+int launch_prefill_t(const Kv4AttnArgs& a, cudaStream_t stream) {
+  using S = Prefill<D>;
+  static bool configured[kMaxDevices];
+  int dev;
+  if (needs_configure(configured, &dev)) {
+    MLD_CUDA_CHECK(cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+    if (dev >= 0) configured[dev] = true;
+  }
+  const int64_t row_blocks = div_up64(static_cast<int64_t>(a.max_queries) * a.group, S::kRows);
+  const int64_t grid = row_blocks * a.batch * a.kv_heads;
+  if (grid > 0x7FFFFFFF) {
+    set_last_error_text("more work than one call can count: fewer sequences or queries");
+    return MLD_OUT_OF_RANGE;
+  }
+  MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kPrefillThreads), S::kSmem, stream, a,
+                                   static_cast<int>(row_blocks)));
+  MLD_LAUNCH_CHECK();
+  return MLD_OK;
+}
+
+}  // namespace
+
+int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? launch_prefill_t<64>(a, stream) : head_dim == 128 ? launch_prefill_t<128>(a, stream) : launch_prefill_t<256>(a, stream);
+}
+
+}  // namespace mld
