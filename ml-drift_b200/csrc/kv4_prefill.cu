@@ -11,7 +11,8 @@
 // by the thread itself, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
 // The two tiles take turns: one's P is made while the other's products run.
 //
-// Roles of the sixteen warps: 0-7 make P and write the rows out, 8-11 unpack, 12 asks for packed tiles, 13 issues the products.
+// Roles of the twenty warps: 0-7 make P and write the rows out (a warpgroup to a tile), 8-15 unpack, 16 asks for packed tiles, 17
+// issues the products.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -24,7 +25,10 @@
 namespace mld {
 namespace {
 
-constexpr int kPrefillThreads = 512;
+constexpr int kPrefillThreads = 640;
+constexpr int kUnpackWarps = 8, kLoadWarp = 16, kMmaWarp = 17;
+// Registers a thread: 640 x 96 at launch, dealt out anew as 256 x 128 + 256 x 80 + 128 x 64.
+constexpr int kRegsRows = 128, kRegsUnpack = 80, kRegsRest = 64;
 constexpr int kRowsPerTile = 128;
 constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
 constexpr int kMaskedBlocks = 16;  // blocks of tokens that only some rows of a block of rows see, at most
@@ -75,6 +79,13 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
       "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -134,6 +145,15 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 template <int D>
 __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks) {
   using S = Prefill<D>;
@@ -152,12 +172,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   if (threadIdx.x == 0) {
     for (int i = 0; i < S::kRing; ++i) {
       mbar_init(&bars.pack_full[i], 1);
-      mbar_init(&bars.pack_empty[i], 4);
+      mbar_init(&bars.pack_empty[i], kUnpackWarps);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bars.k_full[i], 4);
+      mbar_init(&bars.k_full[i], kUnpackWarps);
       mbar_init(&bars.k_empty[i], 1);
-      mbar_init(&bars.v_full[i], 4);
+      mbar_init(&bars.v_full[i], kUnpackWarps);
       mbar_init(&bars.v_empty[i], 1);
       mbar_init(&bars.s_full[i], 1);
       mbar_init(&bars.p_full[i], 4);
@@ -168,9 +188,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   }
   pdl_wait();
   // ---- which rows: the blocks with the most tokens ahead of them first
-  const int unit = blockIdx.x / row_blocks;
+  const int units = a.batch * a.kv_heads, rank = blockIdx.x / units, unit = blockIdx.x - rank * units;
   const int b = unit / a.kv_heads, h = unit - b * a.kv_heads;
-  const int block = row_blocks - 1 - (blockIdx.x - unit * row_blocks);
+  const int block = row_blocks - 1 - rank;
   const Kv4Sequence q = kv4_sequence(a, b);
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.batch; i += kPrefillThreads)
@@ -185,7 +205,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   // whether all rows see all of a step's tokens
   const auto whole = [&](int t0, int lo, int hi) { return t0 + S::kN - 1 <= lo && (a.window == 0 || t0 >= hi - a.window + 1); };
 
-  if (warp == 13) tmem_alloc_512(&tmem_base);
+  if (warp == kMmaWarp) tmem_alloc_512(&tmem_base);
   for (int i = threadIdx.x; i < S::kTilesM * kRowsPerTile * (D / 8); i += kPrefillThreads) {
     const int r = i / (D / 8), c = i - r * (D / 8);
     const int row = row0 + r, token = row / a.group, head = h * a.group + row - token * a.group;
@@ -203,6 +223,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   bool ok = true;
 
   if (warp < 8) {
+    more_registers<kRegsRows>();
     // ------------------------------------------------------------------ weights, rows
     const int tile = warp >> 2;
     if (tile < S::kTilesM) {
@@ -225,36 +246,28 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         const int t0 = (step0 + j) * S::kN;
         const bool all = whole(t0, tile_lo, tile_hi);
         const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of the step
-        uint32_t p[S::kN / 2];
-        float2 part;
-        const auto pass = [&](bool only_max) {
-          float m = -INFINITY;
-          part = make_float2(0.0f, 0.0f);
-          const float2 ref2 = make_float2(minus_ref, minus_ref);
+        // The step's scores, 32 at a time, the next ones on their way while f works on these.
+        const auto scores = [&](auto&& f) {
+          uint32_t buf[2][32];
+          tmem_ld32(t_s, buf[0]);
 #pragma unroll
           for (int c = 0; c < S::kN; c += 32) {
-            uint32_t s[32];
-            tmem_ld32(t_s + c, s);
+            uint32_t(&s)[32] = buf[(c / 32) & 1];
             tmem_ld_wait();
+            if (c + 32 < S::kN) tmem_ld32(t_s + c + 32, buf[(c / 32 + 1) & 1]);
             if (!all) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (c + e > hi || c + e < lo) s[e] = 0xFF800000u;
             }
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              float2 x = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-              m = fmaxf(m, fmaxf(x.x, x.y));
-              x = fma2(x, scale2, ref2);
-              x.x = exp2_hw(x.x);
-              x.y = exp2_hw(x.y);
-              part = add2(part, x);
-              p[(c + e) / 2] = half2_bits(x.x, x.y);
-            }
+            f(c, s);
           }
-          return m;
         };
-        const float m = pass(false);
+        float m = -INFINITY;
+        scores([&](int, const uint32_t(&s)[32]) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) m = fmaxf(m, fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+        });
         if (__any_sync(0xFFFFFFFFu, m > limit)) {
           const float new_top = m > limit ? m * a.scale_log2 : top;
           const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
@@ -278,11 +291,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
               tmem_st32(t_o + c, o);
             }
           }
-          pass(false);
         }
-        sum = add2(sum, part);
+        const float2 ref2 = make_float2(minus_ref, minus_ref);
+        scores([&](int c, const uint32_t(&s)[32]) {
+          uint32_t p[16];
 #pragma unroll
-        for (int c = 0; c < S::kN / 2; c += 32) tmem_st32(t_s + c, reinterpret_cast<const uint32_t(&)[32]>(p[c]));
+          for (int e = 0; e < 32; e += 2) {
+            float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, ref2);
+            x.x = exp2_hw(x.x);
+            x.y = exp2_hw(x.y);
+            sum = add2(sum, x);
+            p[e / 2] = half2_bits(x.x, x.y);
+          }
+          tmem_st16(t_s + c / 2, p);  // over scores that have been read
+        });
         tmem_st_wait();
         tc_before();
         __syncwarp();
@@ -329,91 +351,103 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       }
       tc_before();
     }
-  } else if (warp < 12) {
+  } else if (warp < kLoadWarp) {
+    fewer_registers<kRegsUnpack>();
     // ------------------------------------------------------------------ unpacking
     const int w = warp - 8;
     // lanes of one 128-byte access lie four rows apart, so that the swizzle spreads them over all banks
     const int g = lane >> 2, t = lane & 3, in8 = (g >> 1) | (g & 1) << 2;
+    constexpr int kG = D / 32, kWords = kG < 4 ? kG : 4, kAtOnce = S::kN / 8 / kUnpackWarps;  // a unit is eight tokens
     int stage = 0, phase = 0, masked = -1;
-    constexpr int kWords = D / 32 < 4 ? D / 32 : 4;  // groups of an access
 #pragma unroll 1
     for (int j = 0; j < steps && ok; ++j) {
       const int t0 = (step0 + j) * S::kN, buf = j & 1, use = (j >> 1) & 1;
       const bool all = whole(t0, at_lo, at_hi);
       if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
-      // K of all packed stages of the step, then V
-#pragma unroll 1
+      int next = stage, next_phase = phase;
+#pragma unroll
+      for (int pk = 0; pk < S::kPacks; ++pk) {
+        ok = ok && mbar_wait(&bars.pack_full[next], next_phase);
+        if (++next == S::kRing) {
+          next = 0;
+          next_phase ^= 1;
+        }
+      }
+      // K, then V; all of a warp's words are asked for before the first is turned into values
+#pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        ok = mbar_wait(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
+        ok = ok && mbar_wait(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
         if (!ok) break;
-        uint8_t* const dst0 = (kind ? s_v : s_k) + buf * S::kKvBytes;
-#pragma unroll 1
-        for (int pk = 0; pk < S::kPacks; ++pk) {
-          int st = stage + pk, ph = phase;
-          if (st >= S::kRing) {
-            st -= S::kRing;
-            ph ^= 1;
+        uint8_t* const dst = (kind ? s_v : s_k) + buf * S::kKvBytes;
+        uint32_t x[kAtOnce][kG], sc[kAtOnce][kG / 2];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int u = w + i * kUnpackWarps, tau = (u & 1) * 8 + in8;
+          int st = stage + (u >> 1) / S::kPackTiles;
+          if (st >= S::kRing) st -= S::kRing;
+          const uint8_t* const tile = s_pack + st * S::kPackBytes + (u >> 1) % S::kPackTiles * S::kTileBytes;
+          kv4_lds(tile + kv4::scale_at<D>(kind, tau, 0), sc[i]);
+          if (kind == 0) {
+#pragma unroll
+            for (int q4 = 0; q4 < kG / kWords; ++q4)
+              kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), reinterpret_cast<uint32_t(&)[kWords]>(x[i][q4 * kWords]));
+          } else {
+            // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
+            const int vr = kv4::v_row(tau);
+            const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
+            uint32_t y[kG / 2], z[kG / 2];
+            kv4_lds(piece, y);
+            kv4_lds(piece + D / 16, z);
+#pragma unroll
+            for (int e = 0; e < kG; ++e) x[i][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
           }
-          if (kind == 0) ok = mbar_wait(&bars.pack_full[st], ph);
-          if (!ok) break;
-          const uint8_t* const pack = s_pack + st * S::kPackBytes;
-#pragma unroll 1
-          for (int u = w; u < S::kPackTiles * 2; u += 4) {  // eight tokens of a tile
-            const int tau = (u & 1) * 8 + in8;
-            const int row = pk * S::kPackTiles * 16 + (u >> 1) * 16 + tau;
-            const bool there = t0 + row < q.n;
-            const uint8_t* const tile = pack + (u >> 1) * S::kTileBytes;
-            uint8_t* const dst = dst0 + row * 128;
+        }
+        if (!all) {
 #pragma unroll
-            for (int q4 = 0; q4 < D / 32 / kWords; ++q4) {
-              uint32_t x[kWords], sc[kWords / 2];
-              kv4_lds(tile + kv4::scale_at<D>(kind, tau, q4 * kWords), sc);
-              if (kind == 0) {
-                kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), x);
-              } else {
-                // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
-                const int vr = kv4::v_row(tau);
-                const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
-                uint32_t y[kWords / 2], z[kWords / 2];
-                kv4_lds(piece + 8 * q4, y);
-                kv4_lds(piece + D / 16 + 8 * q4, z);
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int row = (w + i * kUnpackWarps) * 8 + in8;
 #pragma unroll
-                for (int e = 0; e < kWords; ++e) x[e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
-              }
-#pragma unroll
-              for (int e = 0; e < kWords; ++e) {
-                const int jg = q4 * kWords + e, c = jg * 4 + t;
-                __half2 s;
-                *reinterpret_cast<uint32_t*>(&s) = __byte_perm(sc[e >> 1], 0, e & 1 ? 0x3232 : 0x1010);
-                uint4 v = values8(x[e], s);
-                bool drop = !there;
-                if (kind == 1 && !all && there && (*reinterpret_cast<const uint32_t*>(&s) & 0x7C00u) == 0x7C00u) {
-                  drop = true;  // a product with a zero weight would not be zero: noted, and told to the rows that see the token
-                  any_bad = 1;
-                  atomicOr(reinterpret_cast<uint32_t*>(s_bad + masked * S::kN + (row & ~3)), 1u << (jg + 8 * (row & 3)));
-                }
-                if (drop) v = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4*>(dst + (c >> 3) * (S::kN * 128) + (((c & 7) ^ (row & 7)) << 4)) = v;
+            for (int e = 0; e < kG; ++e) {
+              const uint32_t bits = 0x7C00u << (16 * (e & 1));
+              const bool there = t0 + row < q.n;  // behind the end lies anything
+              if (there && (kind == 0 || (sc[i][e >> 1] & bits) != bits)) continue;
+              // A NaN scale of V: its product with a zero weight would not be zero; noted, and told to the rows that see the token.
+              sc[i][e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+              if (there) {
+                any_bad = 1;
+                atomicOr(reinterpret_cast<uint32_t*>(s_bad + masked * S::kN + (row & ~3)), 1u << (e + 8 * (row & 3)));
               }
             }
           }
-          if (kind == 1) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.pack_empty[st]);
+        }
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+          const int row = (w + i * kUnpackWarps) * 8 + in8;
+#pragma unroll
+          for (int e = 0; e < kG; ++e) {
+            const int c = e * 4 + t;
+            const uint32_t s2 = __byte_perm(sc[i][e >> 1], 0, e & 1 ? 0x3232 : 0x1010);
+            *reinterpret_cast<uint4*>(dst + row * 128 + (c >> 3) * (S::kN * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+                values8(x[i][e], *reinterpret_cast<const __half2*>(&s2));
           }
         }
-        if (!ok) break;
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+        if (lane == 0) {
+          mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+          if (kind == 1) {
+#pragma unroll
+            for (int pk = 0; pk < S::kPacks; ++pk) mbar_arrive(&bars.pack_empty[stage + pk < S::kRing ? stage + pk : stage + pk - S::kRing]);
+          }
+        }
       }
-      stage += S::kPacks;
-      if (stage >= S::kRing) {
-        stage -= S::kRing;
-        phase ^= 1;
-      }
+      stage = next;
+      phase = next_phase;
     }
-  } else if (warp == 12) {
+  } else {
+    fewer_registers<kRegsRest>();
+  }
+  if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ packed tiles
     int stage = 0, phase = 0;
     const int packs = steps * S::kPacks;
@@ -450,7 +484,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       for (int i = 0; i < S::kRing; ++i)
         for (int ph = 0; ph < 2; ++ph) mbar_wait(&bars.pack_full[i], ph);
     }
-  } else if (warp == 13) {
+  } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products
     const uint32_t idesc_s = 1u << 4 | static_cast<uint32_t>(S::kN >> 3) << 17 | 8u << 24;
     const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
@@ -505,7 +539,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == 13) tmem_dealloc_512(tmem);
+  if (warp == kMmaWarp) tmem_dealloc_512(tmem);
 }
 
 template <int D>
