@@ -50,7 +50,7 @@ struct Prefill {
 };
 
 struct PrefillBars {
-  uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+  uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
 };
 
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       mbar_init(&bars.v_full[i], kUnpackWarps);
       mbar_init(&bars.v_empty[i], 1);
       mbar_init(&bars.s_full[i], 1);
+      mbar_init(&bars.p_half[i], 4);
       mbar_init(&bars.p_full[i], 4);
       mbar_init(&bars.pv_done[i], 1);
     }
@@ -263,11 +264,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             f(c, s);
           }
         };
-        float m = -INFINITY;
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         scores([&](int, const uint32_t(&s)[32]) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) m = fmaxf(m, fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+          for (int e = 0; e < 32; e += 2)
+            most[e / 2 % 4] = fmaxf(most[e / 2 % 4], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
         });
+        const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         if (__any_sync(0xFFFFFFFFu, m > limit)) {
           const float new_top = m > limit ? m * a.scale_log2 : top;
           const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
@@ -304,11 +307,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             p[e / 2] = half2_bits(x.x, x.y);
           }
           tmem_st16(t_s + c / 2, p);  // over scores that have been read
+          if (c + 32 == S::kN / 2 || c + 32 == S::kN) {  // the product begins with the first half
+            tmem_st_wait();
+            tc_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(c + 32 == S::kN ? &bars.p_full[tile] : &bars.p_half[tile]);
+          }
         });
-        tmem_st_wait();
-        tc_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_full[tile]);
       }
       // ---- out
       if (steps > 0 && ok) ok = mbar_wait(&bars.pv_done[tile], (steps - 1) & 1);
@@ -512,18 +517,24 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
 #pragma unroll 1
       for (int i = 0; i < S::kTilesM && ok; ++i) {
         if (i == 0) ok = mbar_wait(&bars.v_full[buf], (j >> 1) & 1);
-        if (ok) ok = mbar_wait(&bars.p_full[i], j & 1);
-        if (!ok) break;
-        tc_after();
-        if (elect_one()) {
-          const uint64_t dv = make_desc_mn(smem_u32(s_v + buf * S::kKvBytes), S::kN * 128);
+        const uint64_t dv = make_desc_mn(smem_u32(s_v + buf * S::kKvBytes), S::kN * 128);
 #pragma unroll
-          for (int k = 0; k < S::kN / 16; ++k)
-            umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + 8 * k, dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
-          if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
-          umma_commit(&bars.pv_done[i]);  // last: the block ends after it
+        for (int half = 0; half < 2; ++half) {
+          if (ok) ok = mbar_wait(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
+          if (!ok) break;
+          tc_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = half * (S::kN / 32); k < (half + 1) * (S::kN / 32); ++k)
+              umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + 8 * k, dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
+            if (half) {
+              if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
+              umma_commit(&bars.pv_done[i]);  // last: the block ends after it
+            }
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (!ok) break;
         if (j + 1 < steps) {
           if (i == 0) {
             ok = mbar_wait(&bars.k_full[buf ^ 1], ((j + 1) >> 1) & 1);
