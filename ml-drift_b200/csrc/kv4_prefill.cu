@@ -3,15 +3,15 @@
 // The rows of a block are the queries of 256 / group tokens for all heads that share a key/value head: two tiles of 128 rows (one
 // for heads of 256 values).  A block walks the cached tokens in steps of N (128; 64 for heads of 256):
 //   S = Q K^T        both operands fp16 from shared memory, 128 x N fp32 in tensor memory
-//   P = 2^(S - ref)  a thread per row; written over S as fp16, where the next product takes it from
+//   P = 2^(S - ref)  two threads per row, half of the tokens each; written over S as fp16, where the next product takes it from
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
-// by the thread itself, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
+// by its threads themselves, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
 // The two tiles take turns: one's P is made while the other's products run.
 //
-// Roles of the twenty warps: 0-7 make P and write the rows out (a warpgroup to a tile), 8-15 unpack, 16 asks for packed tiles, 17
+// Roles of the 28 warps: 0-15 make P and write the rows out (eight warps to a tile), 16-23 unpack, 24 asks for packed tiles, 25
 // issues the products.
 #include <cuda_fp16.h>
 #include <math.h>
@@ -25,10 +25,10 @@
 namespace mld {
 namespace {
 
-constexpr int kPrefillThreads = 640;
-constexpr int kUnpackWarps = 8, kLoadWarp = 16, kMmaWarp = 17;
-// Registers a thread: 640 x 96 at launch, dealt out anew as 256 x 128 + 256 x 80 + 128 x 64.
-constexpr int kRegsRows = 128, kRegsUnpack = 80, kRegsRest = 64;
+constexpr int kPrefillThreads = 28 * 32;
+constexpr int kRowWarps = 16, kUnpackWarps = 8, kLoadWarp = 24, kMmaWarp = 25;
+// Registers a thread: 896 x 72 at launch, dealt out anew as 512 x 80 + 256 x 64 + 128 x 56.
+constexpr int kRegsRows = 80, kRegsUnpack = 64, kRegsRest = 56;
 constexpr int kRowsPerTile = 128;
 constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
 constexpr int kMaskedBlocks = 16;  // blocks of tokens that only some rows of a block of rows see, at most
@@ -70,23 +70,17 @@ __device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, 
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
-      "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-      "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -145,6 +139,27 @@ __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+// Whether any of the 256 threads that share barrier `id` says yes; all of them call it.
+__device__ __forceinline__ bool any_of_tile(int id, bool yes) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(yes)), "r"(id)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void tile_sync(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
+
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -167,6 +182,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   __shared__ PrefillBars bars;
   __shared__ uint32_t tmem_base;
   __shared__ int any_bad;
+  __shared__ float s_exchange[2][2][kRowsPerTile];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -180,8 +196,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       mbar_init(&bars.v_full[i], kUnpackWarps);
       mbar_init(&bars.v_empty[i], 1);
       mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_half[i], 4);
-      mbar_init(&bars.p_full[i], 4);
+      mbar_init(&bars.p_half[i], 8);
+      mbar_init(&bars.p_full[i], 8);
       mbar_init(&bars.pv_done[i], 1);
     }
     fence_barrier_init();
@@ -223,100 +239,113 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   const uint32_t tmem = tmem_base;
   bool ok = true;
 
-  if (warp < 8) {
+  if (warp < kRowWarps) {
     more_registers<kRegsRows>();
     // ------------------------------------------------------------------ weights, rows
-    const int tile = warp >> 2;
+    const int tile = warp >> 3, half = (warp >> 2) & 1;
     if (tile < S::kTilesM) {
+      constexpr int kMine = S::kN / 2;  // tokens of a step, columns of S
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + lanes + tile * S::kN, t_o = tmem + lanes + S::kO + tile * D;
-      const int row = row0 + tile * kRowsPerTile + (warp & 3) * 32 + lane;
+      const uint32_t t_s = tmem + lanes + tile * S::kN + half * kMine, t_o = tmem + lanes + S::kO + tile * D + half * (D / 2);
+      const int in_tile = (warp & 3) * 32 + lane, row = row0 + tile * kRowsPerTile + in_tile;
+      float* const s_mine = &s_exchange[tile][half][in_tile];
+      const float* const s_other = &s_exchange[tile][half ^ 1][in_tile];
       const int at = q.n - q.m + min(row, rows - 1) / a.group;
       const int tile_lo = q.n - q.m + min(row0 + tile * kRowsPerTile, rows - 1) / a.group;
       const int tile_hi = q.n - q.m + min(row0 + tile * kRowsPerTile + kRowsPerTile - 1, rows - 1) / a.group;
       float top = kPrefillFloor, minus_ref = -kPrefillFloor;
-      float2 sum = make_float2(0.0f, 0.0f);
+      float2 sums[2] = {};
       const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
       const float inv_scale = 1.0f / a.scale_log2;
       float limit = kPrefillFloor * inv_scale;  // scores that may not be exceeded
+      // A wait that gave up ends the waiting, not the loop: the warps of a tile meet at its barrier in every step.
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        ok = mbar_wait(&bars.s_full[tile], j & 1);
-        if (!ok) break;
+        ok = ok && mbar_wait(&bars.s_full[tile], j & 1);
         tc_after();
-        const int t0 = (step0 + j) * S::kN;
-        const bool all = whole(t0, tile_lo, tile_hi);
-        const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of the step
-        // The step's scores, 32 at a time, the next ones on their way while f works on these.
+        const int t0 = (step0 + j) * S::kN + half * kMine;
+        const bool all = whole((step0 + j) * S::kN, tile_lo, tile_hi);
+        const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of these tokens
+        // The scores, 16 at a time, the next ones on their way while f works on these.
         const auto scores = [&](auto&& f) {
-          uint32_t buf[2][32];
-          tmem_ld32(t_s, buf[0]);
+          uint32_t buf[2][16];
+          tmem_ld16(t_s, buf[0]);
 #pragma unroll
-          for (int c = 0; c < S::kN; c += 32) {
-            uint32_t(&s)[32] = buf[(c / 32) & 1];
+          for (int c = 0; c < kMine; c += 16) {
+            uint32_t(&s)[16] = buf[(c / 16) & 1];
             tmem_ld_wait();
-            if (c + 32 < S::kN) tmem_ld32(t_s + c + 32, buf[(c / 32 + 1) & 1]);
+            if (c + 16 < kMine) tmem_ld16(t_s + c + 16, buf[(c / 16 + 1) & 1]);
             if (!all) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e)
+              for (int e = 0; e < 16; ++e)
                 if (c + e > hi || c + e < lo) s[e] = 0xFF800000u;
             }
             f(c, s);
           }
         };
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        scores([&](int, const uint32_t(&s)[32]) {
+        scores([&](int, const uint32_t(&s)[16]) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 2)
+          for (int e = 0; e < 16; e += 2)
             most[e / 2 % 4] = fmaxf(most[e / 2 % 4], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
         });
-        const float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-        if (__any_sync(0xFFFFFFFFu, m > limit)) {
+        float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        if (any_of_tile(1 + tile, m > limit)) {
+          *s_mine = m;
+          tile_sync(1 + tile);
+          m = fmaxf(m, *s_other);
           const float new_top = m > limit ? m * a.scale_log2 : top;
           const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
           const float f = exp2_hw(-minus_ref - ref);
           top = new_top;
           minus_ref = -ref;
           limit = new_top > kPrefillFloor ? (new_top + kPrefillHeadroom) * inv_scale : kPrefillFloor * inv_scale;
-          sum.x *= f;
-          sum.y *= f;
-          if (j > 0) {
-            ok = mbar_wait(&bars.pv_done[tile], (j - 1) & 1);
-            if (!ok) break;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            sums[i].x *= f;
+            sums[i].y *= f;
+          }
+          if (j > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
+            ok = ok && mbar_wait(&bars.pv_done[tile], (j - 1) & 1);
             tc_after();
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
-              uint32_t o[32];
-              tmem_ld32(t_o + c, o);
+            for (int c = 0; c < D / 2; c += 16) {
+              uint32_t o[16];
+              tmem_ld16(t_o + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-              tmem_st32(t_o + c, o);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tmem_st16(t_o + c, o);
             }
           }
         }
         const float2 ref2 = make_float2(minus_ref, minus_ref);
-        scores([&](int c, const uint32_t(&s)[32]) {
-          uint32_t p[16];
+        scores([&](int c, const uint32_t(&s)[16]) {
+          uint32_t p[8];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
+          for (int e = 0; e < 16; e += 2) {
             float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, ref2);
             x.x = exp2_hw(x.x);
             x.y = exp2_hw(x.y);
-            sum = add2(sum, x);
+            sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
             p[e / 2] = half2_bits(x.x, x.y);
           }
-          tmem_st16(t_s + c / 2, p);  // over scores that have been read
-          if (c + 32 == S::kN / 2 || c + 32 == S::kN) {  // the product begins with the first half
+          tmem_st8(t_s + c / 2, p);  // over scores that have been read
+          if (c + 16 == kMine / 2 || c + 16 == kMine) {  // the product begins with the first halves
             tmem_st_wait();
             tc_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(c + 32 == S::kN ? &bars.p_full[tile] : &bars.p_half[tile]);
+            if (lane == 0) mbar_arrive(c + 16 == kMine ? &bars.p_full[tile] : &bars.p_half[tile]);
           }
         });
       }
       // ---- out
-      if (steps > 0 && ok) ok = mbar_wait(&bars.pv_done[tile], (steps - 1) & 1);
+      const float mine = (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
+      tile_sync(1 + tile);  // nobody reads an earlier exchange any more
+      *s_mine = mine;
+      tile_sync(1 + tile);
+      const float l = half ? *s_other + mine : mine + *s_other;
+      if (steps > 0) ok = ok && mbar_wait(&bars.pv_done[tile], (steps - 1) & 1);
       tc_after();
       uint32_t bad = 0;  // groups of the row's values that are not finite
       if (any_bad) {
@@ -329,24 +358,23 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           ++k;
         }
       }
-      const float l = sum.x + sum.y;
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const int token = row / a.group, head = h * a.group + row - token * a.group;
-      __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D;
+      __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D + half * (D / 2);
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t o[32];
-        if (steps > 0 && ok) {
-          tmem_ld32(t_o + c, o);
+      for (int c = 0; c < D / 2; c += 16) {
+        uint32_t o[16];
+        if (steps > 0) {
+          tmem_ld16(t_o + c, o);
           tmem_ld_wait();
         } else {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
+          for (int e = 0; e < 16; ++e) o[e] = 0;
         }
-        const float f = (bad >> (c / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
+        const float f = (bad >> ((half * (D / 2) + c) / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
         if (row < rows) {
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
+          for (int e = 0; e < 16; e += 8) {
             // value k of eight lies in column 2 k, value 4 + k in column 2 k + 1
             const auto x = [&](int k) { return __uint_as_float(o[e + (k < 4 ? 2 * k : 2 * k - 7)]) * f; };
             *reinterpret_cast<uint4*>(dst + c + e) =
@@ -359,7 +387,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   } else if (warp < kLoadWarp) {
     fewer_registers<kRegsUnpack>();
     // ------------------------------------------------------------------ unpacking
-    const int w = warp - 8;
+    const int w = warp - kRowWarps;
     // lanes of one 128-byte access lie four rows apart, so that the swizzle spreads them over all banks
     const int g = lane >> 2, t = lane & 3, in8 = (g >> 1) | (g & 1) << 2;
     constexpr int kG = D / 32, kWords = kG < 4 ? kG : 4, kAtOnce = S::kN / 8 / kUnpackWarps;  // a unit is eight tokens
@@ -525,8 +553,13 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           tc_after();
           if (elect_one()) {
 #pragma unroll
-            for (int k = half * (S::kN / 32); k < (half + 1) * (S::kN / 32); ++k)
-              umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + 8 * k, dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
+            for (int k = 0; k < S::kN / 16; ++k) {
+              // the weights of either half of the tokens lie over that half's scores, and come in two halves again
+              constexpr int kQuarter = S::kN / 64;
+              if ((k / kQuarter & 1) != half) continue;
+              umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + k / (2 * kQuarter) * (S::kN / 2) + k % (2 * kQuarter) * 8,
+                          dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
+            }
             if (half) {
               if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
               umma_commit(&bars.pv_done[i]);  // last: the block ends after it
