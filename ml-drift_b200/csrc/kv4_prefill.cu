@@ -53,6 +53,20 @@ struct PrefillBars {
   uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
 };
 
+// mbar_wait with a hint that lets the hardware hold a waiting warp, so that polling takes no issue slots from the others.
+__device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  for (;;) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
+        : "memory");
+    if (done) return true;
+    if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -261,7 +275,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       // A wait that gave up ends the waiting, not the loop: the warps of a tile meet at its barrier in every step.
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        ok = ok && mbar_wait(&bars.s_full[tile], j & 1);
+        ok = ok && wait_quietly(&bars.s_full[tile], j & 1);
         tc_after();
         const int t0 = (step0 + j) * S::kN + half * kMine;
         const bool all = whole((step0 + j) * S::kN, tile_lo, tile_hi);
@@ -306,7 +320,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             sums[i].y *= f;
           }
           if (j > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
-            ok = ok && mbar_wait(&bars.pv_done[tile], (j - 1) & 1);
+            ok = ok && wait_quietly(&bars.pv_done[tile], (j - 1) & 1);
             tc_after();
 #pragma unroll 1
             for (int c = 0; c < D / 2; c += 16) {
@@ -345,7 +359,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       *s_mine = mine;
       tile_sync(1 + tile);
       const float l = half ? *s_other + mine : mine + *s_other;
-      if (steps > 0) ok = ok && mbar_wait(&bars.pv_done[tile], (steps - 1) & 1);
+      if (steps > 0) ok = ok && wait_quietly(&bars.pv_done[tile], (steps - 1) & 1);
       tc_after();
       uint32_t bad = 0;  // groups of the row's values that are not finite
       if (any_bad) {
@@ -397,44 +411,52 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       const int t0 = (step0 + j) * S::kN, buf = j & 1, use = (j >> 1) & 1;
       const bool all = whole(t0, at_lo, at_hi);
       if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
-      int next = stage, next_phase = phase;
-#pragma unroll
-      for (int pk = 0; pk < S::kPacks; ++pk) {
-        ok = ok && mbar_wait(&bars.pack_full[next], next_phase);
-        if (++next == S::kRing) {
-          next = 0;
-          next_phase ^= 1;
-        }
-      }
       // K, then V; all of a warp's words are asked for before the first is turned into values
 #pragma unroll
       for (int kind = 0; kind < 2; ++kind) {
-        ok = ok && mbar_wait(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
-        if (!ok) break;
-        uint8_t* const dst = (kind ? s_v : s_k) + buf * S::kKvBytes;
         uint32_t x[kAtOnce][kG], sc[kAtOnce][kG / 2];
+        int st = stage, ph = phase;
 #pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-          const int u = w + i * kUnpackWarps, tau = (u & 1) * 8 + in8;
-          int st = stage + (u >> 1) / S::kPackTiles;
-          if (st >= S::kRing) st -= S::kRing;
-          const uint8_t* const tile = s_pack + st * S::kPackBytes + (u >> 1) % S::kPackTiles * S::kTileBytes;
-          kv4_lds(tile + kv4::scale_at<D>(kind, tau, 0), sc[i]);
-          if (kind == 0) {
+        for (int pk = 0; pk < S::kPacks; ++pk) {
+          if (kind == 0) ok = ok && wait_quietly(&bars.pack_full[st], ph);
+          const uint8_t* const pack = s_pack + st * S::kPackBytes;
 #pragma unroll
-            for (int q4 = 0; q4 < kG / kWords; ++q4)
-              kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), reinterpret_cast<uint32_t(&)[kWords]>(x[i][q4 * kWords]));
-          } else {
-            // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
-            const int vr = kv4::v_row(tau);
-            const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
-            uint32_t y[kG / 2], z[kG / 2];
-            kv4_lds(piece, y);
-            kv4_lds(piece + D / 16, z);
+          for (int i = 0; i < kAtOnce; ++i) {
+            if (kAtOnce >= S::kPacks ? i * S::kPacks / kAtOnce != pk : w * S::kPacks / kUnpackWarps != pk) continue;  // in another stage
+            const int u = w + i * kUnpackWarps, tau = (u & 1) * 8 + in8;
+            const uint8_t* const tile = pack + (u >> 1) % S::kPackTiles * S::kTileBytes;
+            kv4_lds(tile + kv4::scale_at<D>(kind, tau, 0), sc[i]);
+            if (kind == 0) {
 #pragma unroll
-            for (int e = 0; e < kG; ++e) x[i][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
+              for (int q4 = 0; q4 < kG / kWords; ++q4)
+                kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), reinterpret_cast<uint32_t(&)[kWords]>(x[i][q4 * kWords]));
+            } else {
+              // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
+              const int vr = kv4::v_row(tau);
+              const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
+              uint32_t y[kG / 2], z[kG / 2];
+              kv4_lds(piece, y);
+              kv4_lds(piece + D / 16, z);
+#pragma unroll
+              for (int e = 0; e < kG; ++e) x[i][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
+            }
+          }
+          if (kind == 1) {  // the words are in registers: the place is free
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars.pack_empty[st]);
+          }
+          if (++st == S::kRing) {
+            st = 0;
+            ph ^= 1;
           }
         }
+        if (kind == 1) {
+          stage = st;
+          phase = ph;
+        }
+        ok = ok && wait_quietly(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
+        if (!ok) break;
+        uint8_t* const dst = (kind ? s_v : s_k) + buf * S::kKvBytes;
         if (!all) {
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
@@ -442,7 +464,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
 #pragma unroll
             for (int e = 0; e < kG; ++e) {
               const uint32_t bits = 0x7C00u << (16 * (e & 1));
-              const bool there = t0 + row < q.n;  // behind the end lies anything
+              const bool there = t0 + row <= at_hi;  // behind lies anything
               if (there && (kind == 0 || (sc[i][e >> 1] & bits) != bits)) continue;
               // A NaN scale of V: its product with a zero weight would not be zero; noted, and told to the rows that see the token.
               sc[i][e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
@@ -466,56 +488,49 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
-          if (kind == 1) {
-#pragma unroll
-            for (int pk = 0; pk < S::kPacks; ++pk) mbar_arrive(&bars.pack_empty[stage + pk < S::kRing ? stage + pk : stage + pk - S::kRing]);
-          }
-        }
+        if (lane == 0) mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
       }
-      stage = next;
-      phase = next_phase;
     }
   } else {
     fewer_registers<kRegsRest>();
   }
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ packed tiles
+    // Lane l looks up every 32nd tile and brings it when its stage's turn comes, with the tiles behind it that lie in the same page.
     int stage = 0, phase = 0;
-    const int packs = steps * S::kPacks;
-    const auto page_of = [&](int pk) {
-      const int tile = step0 * (S::kN / 16) + pk * S::kPackTiles + lane;
-      return pk < packs && lane < S::kPackTiles && tile * 16 < q.n ? __ldg(a.table + static_cast<long long>(b) * a.max_pages + tile / a.page_tiles) : 0;
-    };
-    int pid = page_of(0);
+    const int tiles = (min(at_hi, q.n - 1) >> 4) + 1, tile0 = step0 * (S::kN / 16);
 #pragma unroll 1
-    for (int pk = 0; pk < packs; ++pk) {
-      ok = mbar_wait(&bars.pack_empty[stage], phase ^ 1);
-      if (!ok) break;
-      const int tile0 = step0 * (S::kN / 16) + pk * S::kPackTiles;
-      const int there = min(S::kPackTiles, max(0, (q.n + 15) / 16 - tile0));
-      if (lane == 0) mbar_arrive_expect_tx(&bars.pack_full[stage], there * S::kTileBytes);
-      __syncwarp();
-      if (lane < there) {
-        const int tile = tile0 + lane;
+    for (int from = tile0; from < tile0 + steps * (S::kN / 16) && ok; from += 32) {
+      const int tile = from + lane, page = tile / a.page_tiles, in_page = tile - page * a.page_tiles;
+      int run = 0;
+      const uint8_t* src = nullptr;
+      if (tile < tiles && (in_page == 0 || lane % S::kPackTiles == 0)) {
+        int pid = __ldg(a.table + static_cast<long long>(b) * a.max_pages + page);
         if (pid < 0 || pid >= a.pages) {
           atomicExch(a.error, kErrPage);
           pid = 0;
         }
-        bulk_load_1d(s_pack + stage * S::kPackBytes + lane * S::kTileBytes,
-                     a.pool + ((static_cast<long long>(pid) * a.kv_heads + h) * a.page_tiles + tile % a.page_tiles) * S::kTileBytes,
-                     S::kTileBytes, &bars.pack_full[stage]);
+        run = min(min(a.page_tiles - in_page, S::kPackTiles - lane % S::kPackTiles), tiles - tile);
+        src = a.pool + ((static_cast<long long>(pid) * a.kv_heads + h) * a.page_tiles + in_page) * S::kTileBytes;
       }
-      pid = page_of(pk + 1);
-      if (++stage == S::kRing) {
-        stage = 0;
-        phase ^= 1;
+#pragma unroll 1
+      for (int l = 0; l < 32 && from + l < tile0 + steps * (S::kN / 16); l += S::kPackTiles) {
+        ok = wait_quietly(&bars.pack_empty[stage], phase ^ 1);
+        if (!ok) break;
+        const int there = min(S::kPackTiles, max(0, tiles - from - l));
+        if (lane == 0) mbar_arrive_expect_tx(&bars.pack_full[stage], there * S::kTileBytes);
+        __syncwarp();
+        if (run > 0 && lane >= l && lane < l + S::kPackTiles)
+          bulk_load_1d(s_pack + stage * S::kPackBytes + (lane - l) * S::kTileBytes, src, run * S::kTileBytes, &bars.pack_full[stage]);
+        if (++stage == S::kRing) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
     }
     if (!ok) {  // copies in flight end before the shared memory does
       for (int i = 0; i < S::kRing; ++i)
-        for (int ph = 0; ph < 2; ++ph) mbar_wait(&bars.pack_full[i], ph);
+        for (int ph = 0; ph < 2; ++ph) wait_quietly(&bars.pack_full[i], ph);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------------ products
@@ -534,7 +549,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       __syncwarp();
     };
     if (steps > 0) {
-      ok = mbar_wait(&bars.k_full[0], 0);
+      ok = wait_quietly(&bars.k_full[0], 0);
       tc_after();
       if (ok)
         for (int i = 0; i < S::kTilesM; ++i) scores(i, 0);
@@ -544,11 +559,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       const int buf = j & 1;
 #pragma unroll 1
       for (int i = 0; i < S::kTilesM && ok; ++i) {
-        if (i == 0) ok = mbar_wait(&bars.v_full[buf], (j >> 1) & 1);
+        if (i == 0) ok = wait_quietly(&bars.v_full[buf], (j >> 1) & 1);
         const uint64_t dv = make_desc_mn(smem_u32(s_v + buf * S::kKvBytes), S::kN * 128);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (ok) ok = mbar_wait(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
+          if (ok) ok = wait_quietly(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
           if (!ok) break;
           tc_after();
           if (elect_one()) {
@@ -570,7 +585,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         if (!ok) break;
         if (j + 1 < steps) {
           if (i == 0) {
-            ok = mbar_wait(&bars.k_full[buf ^ 1], ((j + 1) >> 1) & 1);
+            ok = wait_quietly(&bars.k_full[buf ^ 1], ((j + 1) >> 1) & 1);
             if (!ok) break;
             tc_after();
           }
