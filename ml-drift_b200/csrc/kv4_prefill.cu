@@ -55,6 +55,7 @@ struct PrefillBars {
 
 // mbar_wait with a hint that lets the hardware hold a waiting warp, so that polling takes no issue slots from the others.
 __device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
   const unsigned long long t0 = globaltimer_ns();
   for (;;) {
     uint32_t done;
@@ -67,18 +68,21 @@ __device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
     if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
   }
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+// Products of one issue: descriptors come as their low words, the high word is the same for all operands here (1024 bytes from
+// eight rows to the next, 128-byte swizzle), so that few registers have to be made uniform ahead of each.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(0u)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
@@ -98,13 +102,9 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Descriptor of an operand whose 128-byte rows (128-byte swizzle) hold 64 values along M / N, a row per step of K: `columns`
-// bytes between neighbouring 64 values, 1024 bytes from eight rows to the next.
-__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr, uint32_t columns) {
-  uint64_t d = make_desc(smem_addr);
-  d &= ~(static_cast<uint64_t>(0x3FFF) << 16);
-  return d | static_cast<uint64_t>(columns >> 4) << 16;
-}
+// Low word of an operand's descriptor: its address, and for V, whose 128-byte rows hold 64 of a head's values (along N, a row per
+// step of K), the bytes between neighbouring 64 values.
+__device__ __forceinline__ uint32_t desc_low(const uint8_t* p, uint32_t columns) { return smem_u32(p) >> 4 | columns >> 4 << 16; }
 
 __device__ __forceinline__ uint32_t lop3_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
   uint32_t y;
@@ -536,13 +536,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     // ------------------------------------------------------------------ products
     const uint32_t idesc_s = 1u << 4 | static_cast<uint32_t>(S::kN >> 3) << 17 | 8u << 24;
     const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
+    const uint32_t q_low = desc_low(s_q, 16), k_low = desc_low(s_k, 16), v_low = desc_low(s_v, S::kN * 128);
     const auto scores = [&](int i, int buf) {
       if (elect_one()) {
-        const uint64_t dq = make_desc(smem_u32(s_q + i * S::kQBytes)), dk = make_desc(smem_u32(s_k + buf * S::kKvBytes));
+        const uint32_t dq = q_low + i * (S::kQBytes >> 4), dk = k_low + buf * (S::kKvBytes >> 4);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_ss(tmem + i * S::kN, dq + static_cast<uint64_t>(((k >> 2) * (kRowsPerTile * 128) + (k & 3) * 32) >> 4),
-                  dk + static_cast<uint64_t>(((k >> 2) * (S::kN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
+          umma_ss(tmem + i * S::kN, dq + (((k >> 2) * (kRowsPerTile * 128) + (k & 3) * 32) >> 4),
+                  dk + (((k >> 2) * (S::kN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
         if (i == S::kTilesM - 1) umma_commit(&bars.k_empty[buf]);
         umma_commit(&bars.s_full[i]);
       }
@@ -551,19 +552,21 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     if (steps > 0) {
       ok = wait_quietly(&bars.k_full[0], 0);
       tc_after();
-      if (ok)
+      if (ok) {
+#pragma unroll
         for (int i = 0; i < S::kTilesM; ++i) scores(i, 0);
+      }
     }
 #pragma unroll 1
     for (int j = 0; j < steps && ok; ++j) {
       const int buf = j & 1;
-#pragma unroll 1
-      for (int i = 0; i < S::kTilesM && ok; ++i) {
-        if (i == 0) ok = wait_quietly(&bars.v_full[buf], (j >> 1) & 1);
-        const uint64_t dv = make_desc_mn(smem_u32(s_v + buf * S::kKvBytes), S::kN * 128);
+      const uint32_t dv = v_low + buf * (S::kKvBytes >> 4);
+#pragma unroll
+      for (int i = 0; i < S::kTilesM; ++i) {
+        if (i == 0) ok = wait_quietly(&bars.v_full[buf], j >> 1 & 1);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (ok) ok = wait_quietly(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
+          ok = ok && wait_quietly(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
           if (!ok) break;
           tc_after();
           if (elect_one()) {
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
               constexpr int kQuarter = S::kN / 64;
               if ((k / kQuarter & 1) != half) continue;
               umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + k / (2 * kQuarter) * (S::kN / 2) + k % (2 * kQuarter) * 8,
-                          dv + static_cast<uint64_t>((k * 2048) >> 4), idesc_o, j > 0 || k > 0);
+                          dv + (k * 2048 >> 4), idesc_o, k > 0 ? 1u : static_cast<uint32_t>(j));
             }
             if (half) {
               if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
@@ -585,7 +588,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         if (!ok) break;
         if (j + 1 < steps) {
           if (i == 0) {
-            ok = wait_quietly(&bars.k_full[buf ^ 1], ((j + 1) >> 1) & 1);
+            const uint32_t next_use = (j + 1) >> 1 & 1;
+            ok = wait_quietly(&bars.k_full[buf ^ 1], next_use);
             if (!ok) break;
             tc_after();
           }
