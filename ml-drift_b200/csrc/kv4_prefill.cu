@@ -16,6 +16,8 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -142,6 +144,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=l"(reinterpret_cast<unsigned long long&>(d))
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float y;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
 }
 __device__ __forceinline__ float exp2_hw(float x) {
   float y;
@@ -281,7 +288,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         const bool all = whole((step0 + j) * S::kN, tile_lo, tile_hi);
         const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of these tokens
         // The scores, 16 at a time, the next ones on their way while f works on these.
-        const auto scores = [&](auto&& f) {
+        const auto scores_as = [&](auto masked, auto&& f) {
           uint32_t buf[2][16];
           tmem_ld16(t_s, buf[0]);
 #pragma unroll
@@ -289,7 +296,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             uint32_t(&s)[16] = buf[(c / 16) & 1];
             tmem_ld_wait();
             if (c + 16 < kMine) tmem_ld16(t_s + c + 16, buf[(c / 16 + 1) & 1]);
-            if (!all) {
+            if constexpr (decltype(masked)::value) {
 #pragma unroll
               for (int e = 0; e < 16; ++e)
                 if (c + e > hi || c + e < lo) s[e] = 0xFF800000u;
@@ -297,11 +304,15 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             f(c, s);
           }
         };
+        // Two copies of the code: one with a branch inside would carry the masks' instructions through every step.
+        const auto scores = [&](auto&& f) {
+          if (all) scores_as(std::false_type(), f); else scores_as(std::true_type(), f);
+        };
         float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
         scores([&](int, const uint32_t(&s)[16]) {
 #pragma unroll
           for (int e = 0; e < 16; e += 2)
-            most[e / 2 % 4] = fmaxf(most[e / 2 % 4], fmaxf(__uint_as_float(s[e]), __uint_as_float(s[e + 1])));
+            most[e / 2 % 4] = max3(most[e / 2 % 4], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
         });
         float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         if (any_of_tile(1 + tile, m > limit)) {
