@@ -55,19 +55,23 @@ struct PrefillBars {
   uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
 };
 
-// mbar_wait with a hint that lets the hardware hold a waiting warp, so that polling takes no issue slots from the others.
+// mbar_wait that looks at the clock only now and then: a waiting warp's polls take issue slots from the others.
 __device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const unsigned long long t0 = globaltimer_ns();
+  unsigned long long t0 = 0;
   for (;;) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(100000u)
-        : "memory");
-    if (done) return true;
-    if (globaltimer_ns() - t0 > kWaitLimitNs) return false;
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.b32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(smem_u32(bar)), "r"(parity), "r"(1000000u)
+          : "memory");
+      if (done) return true;
+    }
+    const unsigned long long t = globaltimer_ns();
+    if (t0 == 0) t0 = t;
+    if (t - t0 > kWaitLimitNs) return false;
   }
 }
 // Products of one issue: descriptors come as their low words, the high word is the same for all operands here (1024 bytes from
@@ -179,7 +183,8 @@ __device__ __forceinline__ bool any_of_tile(int id, bool yes) {
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ void tile_sync(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
+// Barrier `id` of 256 threads.  One warp of them waits for a transaction barrier and the others for it here, without polls.
+__device__ __forceinline__ void sync_256(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
 
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -279,10 +284,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
       const float inv_scale = 1.0f / a.scale_log2;
       float limit = kPrefillFloor * inv_scale;  // scores that may not be exceeded
-      // A wait that gave up ends the waiting, not the loop: the warps of a tile meet at its barrier in every step.
+      // A wait that gave up ends the waiting, not the loop: warps meet at their barriers in every step.
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        ok = ok && wait_quietly(&bars.s_full[tile], j & 1);
+        if ((warp & 7) == 0) ok = ok && wait_quietly(&bars.s_full[tile], j & 1);
+        sync_256(1 + tile);
         tc_after();
         const int t0 = (step0 + j) * S::kN + half * kMine;
         const bool all = whole((step0 + j) * S::kN, tile_lo, tile_hi);
@@ -317,7 +323,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
         if (any_of_tile(1 + tile, m > limit)) {
           *s_mine = m;
-          tile_sync(1 + tile);
+          sync_256(1 + tile);
           m = fmaxf(m, *s_other);
           const float new_top = m > limit ? m * a.scale_log2 : top;
           const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
@@ -366,9 +372,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       }
       // ---- out
       const float mine = (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
-      tile_sync(1 + tile);  // nobody reads an earlier exchange any more
+      sync_256(1 + tile);  // nobody reads an earlier exchange any more
       *s_mine = mine;
-      tile_sync(1 + tile);
+      sync_256(1 + tile);
       const float l = half ? *s_other + mine : mine + *s_other;
       if (steps > 0) ok = ok && wait_quietly(&bars.pv_done[tile], (steps - 1) & 1);
       tc_after();
@@ -418,7 +424,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     constexpr int kG = D / 32, kWords = kG < 4 ? kG : 4, kAtOnce = S::kN / 8 / kUnpackWarps;  // a unit is eight tokens
     int stage = 0, phase = 0, masked = -1;
 #pragma unroll 1
-    for (int j = 0; j < steps && ok; ++j) {
+    for (int j = 0; j < steps; ++j) {
       const int t0 = (step0 + j) * S::kN, buf = j & 1, use = (j >> 1) & 1;
       const bool all = whole(t0, at_lo, at_hi);
       if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
@@ -429,7 +435,10 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         int st = stage, ph = phase;
 #pragma unroll
         for (int pk = 0; pk < S::kPacks; ++pk) {
-          if (kind == 0) ok = ok && wait_quietly(&bars.pack_full[st], ph);
+          if (kind == 0) {
+            if (w == 0) ok = ok && wait_quietly(&bars.pack_full[st], ph);
+            sync_256(3);
+          }
           const uint8_t* const pack = s_pack + st * S::kPackBytes;
 #pragma unroll
           for (int i = 0; i < kAtOnce; ++i) {
@@ -465,8 +474,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           stage = st;
           phase = ph;
         }
-        ok = ok && wait_quietly(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
-        if (!ok) break;
+        if (w == 0) ok = ok && wait_quietly(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
+        sync_256(3);
         uint8_t* const dst = (kind ? s_v : s_k) + buf * S::kKvBytes;
         if (!all) {
 #pragma unroll
