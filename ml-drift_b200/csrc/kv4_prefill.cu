@@ -1,18 +1,19 @@
 // Attention over the 4-bit cache for many query rows per key/value head (prompts, chunks of prompts), on tcgen05.
 //
 // The rows of a block are the queries of 256 / group tokens for all heads that share a key/value head: two tiles of 128 rows (one
-// for heads of 256 values).  A block walks the cached tokens in steps of N (128; 64 for heads of 256):
-//   S = Q K^T        both operands fp16 from shared memory, 128 x N fp32 in tensor memory
+// for heads of 256 values).  A block walks the cached tokens in steps of 64:
+//   S = Q K^T        both operands fp16 from shared memory, 128 x 64 fp32 in tensor memory, two of them per tile
 //   P = 2^(S - ref)  two threads per row, half of the tokens each; written over S as fp16, where the next product takes it from
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
+// The next step's S is asked for ahead of this step's O, so that the threads that make P find it ready: steps of 128 tokens, of
+// which tensor memory holds one S per tile beside O, had every thread wait for its own products (0.52 of the tensor cores' rate).
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
 // by its threads themselves, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
-// The two tiles take turns: one's P is made while the other's products run.
 //
-// Roles of the 28 warps: 0-15 make P and write the rows out (eight warps to a tile), 16-23 unpack, 24 asks for packed tiles, 25
-// issues the products.
+// Roles of the 28 warps: 0-15 make P and write the rows out (eight warps to a tile), 16-23 unpack, 24 asks for packed tiles, 25 and
+// 26 issue the products, a tile each (one warp for both took as long to issue as the products take).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -28,31 +29,33 @@ namespace mld {
 namespace {
 
 constexpr int kPrefillThreads = 28 * 32;
-constexpr int kRowWarps = 16, kUnpackWarps = 8, kLoadWarp = 24, kMmaWarp = 25;
+constexpr int kRowWarps = 16, kUnpackWarps = 8, kLoadWarp = 24, kMmaWarp = 25;  // and the one behind it for a second tile
 // Registers a thread: 896 x 72 at launch, dealt out anew as 512 x 80 + 256 x 64 + 128 x 56.
 constexpr int kRegsRows = 80, kRegsUnpack = 64, kRegsRest = 56;
 constexpr int kRowsPerTile = 128;
 constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
-constexpr int kMaskedBlocks = 16;  // blocks of tokens that only some rows of a block of rows see, at most
+constexpr int kMaskedBlocks = 24;  // blocks of tokens that only some rows of a block of rows see, at most
 
 template <int D>
 struct Prefill {
   static constexpr int kTilesM = D == 256 ? 1 : 2;
   static constexpr int kRows = kTilesM * kRowsPerTile;
-  static constexpr int kN = D == 256 ? 64 : 128;             // tokens of a step
+  static constexpr int kN = 64;                              // tokens of a step
   static constexpr int kQBytes = kRowsPerTile * D * 2;       // of a tile
   static constexpr int kKvBytes = kN * D * 2;                // of K or V of a step
+  static constexpr int kBuffers = D == 256 ? 2 : 4;          // of K and of V
   static constexpr int kTileBytes = kv4::tile_bytes(D);
-  static constexpr int kPackTiles = 512 / D;                 // packed tiles of a stage of the ring
-  static constexpr int kPackBytes = kPackTiles * kTileBytes; // 9216
-  static constexpr int kPacks = kN / (16 * kPackTiles);      // stages of a step
-  static constexpr int kRing = 3;
+  static constexpr int kPackTiles = kN / 16;                 // packed tiles of a step
+  static constexpr int kPackBytes = kPackTiles * kTileBytes;
+  static constexpr int kRing = D == 256 ? 1 : 3;             // steps that are in flight packed
   static constexpr int kO = 256;                             // tensor-memory column of the first O
-  static constexpr size_t kSmem = 1024 + kTilesM * kQBytes + 4 * kKvBytes + kRing * kPackBytes + kMaskedBlocks * kN;
+  static constexpr size_t kSmem = 1024 + kTilesM * kQBytes + 2 * kBuffers * kKvBytes + kRing * kPackBytes + kMaskedBlocks * kN;
 };
 
 struct PrefillBars {
-  uint64_t pack_full[3], pack_empty[3], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2], p_full[2], pv_done[2];
+  // What is numbered by steps has as many barriers as there are buffers of K and V: a step's products are also what its buffers
+  // become free by.
+  uint64_t pack_full[3], pack_empty[3], k_full[4], v_full[4], s_full[2][4], p_full[2][4], pv_done[2][4];
 };
 
 // mbar_wait that looks at the clock only now and then: a waiting warp's polls take issue slots from the others.
@@ -74,25 +77,35 @@ __device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
     if (t - t0 > kWaitLimitNs) return false;
   }
 }
-// Products of one issue: descriptors come as their low words, the high word is the same for all operands here (1024 bytes from
-// eight rows to the next, 128-byte swizzle), so that few registers have to be made uniform ahead of each.
+// Products are issued by one elected lane, predicated inside a block without branches: the warp stays together, so that the
+// operands can live in uniform registers, which the instruction takes them from.  Descriptors come as their low words, the high
+// word is the same for all operands here (1024 bytes from eight rows to the next, 128-byte swizzle).
 constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ uint32_t elected() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void umma_ss(uint32_t issue, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\tmov.b64 da, {%1, %5};\n\t"
+      "mov.b64 db, {%2, %5};\n\t@e tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh), "r"(issue)
       : "memory");
 }
-__device__ __forceinline__ void umma_tmem_a(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_tmem_a(uint32_t issue, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 db, {%2, %5};\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
-      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh)
+      "{\n\t.reg .pred p, e;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %6, 0;\n\tmov.b64 db, {%2, %5};\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(accumulate), "r"(kDescHigh), "r"(issue)
       : "memory");
 }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void umma_commit(uint32_t issue, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(issue)
+      : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -100,11 +113,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -201,9 +209,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const s_q = smem;                                  // [kTilesM][D / 64][128 rows][128 bytes]
-  uint8_t* const s_k = s_q + S::kTilesM * S::kQBytes;         // [2][D / 64][kN rows][128 bytes]
-  uint8_t* const s_v = s_k + 2 * S::kKvBytes;                 // [2][D / 64][kN rows][128 bytes]
-  uint8_t* const s_pack = s_v + 2 * S::kKvBytes;              // [kRing][kPackBytes]
+  uint8_t* const s_k = s_q + S::kTilesM * S::kQBytes;         // [kBuffers][D / 64][kN rows][128 bytes]
+  uint8_t* const s_v = s_k + S::kBuffers * S::kKvBytes;       // [kBuffers][D / 64][kN rows][128 bytes]
+  uint8_t* const s_pack = s_v + S::kBuffers * S::kKvBytes;    // [kRing][kPackBytes]
   uint8_t* const s_bad = s_pack + S::kRing * S::kPackBytes;   // [kMaskedBlocks][kN]: groups of V that are not finite
   __shared__ PrefillBars bars;
   __shared__ uint32_t tmem_base;
@@ -216,15 +224,14 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       mbar_init(&bars.pack_full[i], 1);
       mbar_init(&bars.pack_empty[i], kUnpackWarps);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < S::kBuffers; ++i) {
       mbar_init(&bars.k_full[i], kUnpackWarps);
-      mbar_init(&bars.k_empty[i], 1);
       mbar_init(&bars.v_full[i], kUnpackWarps);
-      mbar_init(&bars.v_empty[i], 1);
-      mbar_init(&bars.s_full[i], 1);
-      mbar_init(&bars.p_half[i], 8);
-      mbar_init(&bars.p_full[i], 8);
-      mbar_init(&bars.pv_done[i], 1);
+      for (int t = 0; t < S::kTilesM; ++t) {
+        mbar_init(&bars.s_full[t][i], 1);
+        mbar_init(&bars.p_full[t][i], 8);
+        mbar_init(&bars.pv_done[t][i], 1);
+      }
     }
     fence_barrier_init();
     any_bad = 0;
@@ -262,7 +269,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   tc_before();
   __syncthreads();
   tc_after();
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = 0;  // all columns are this block's: they begin at 0
+  constexpr int kB = S::kBuffers;
   bool ok = true;
 
   if (warp < kRowWarps) {
@@ -272,7 +280,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     if (tile < S::kTilesM) {
       constexpr int kMine = S::kN / 2;  // tokens of a step, columns of S
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t t_s = tmem + lanes + tile * S::kN + half * kMine, t_o = tmem + lanes + S::kO + tile * D + half * (D / 2);
+      const uint32_t t_s0 = tmem + lanes + tile * 2 * S::kN + half * kMine, t_o = tmem + lanes + S::kO + tile * D + half * (D / 2);
       const int in_tile = (warp & 3) * 32 + lane, row = row0 + tile * kRowsPerTile + in_tile;
       float* const s_mine = &s_exchange[tile][half][in_tile];
       const float* const s_other = &s_exchange[tile][half ^ 1][in_tile];
@@ -287,40 +295,23 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       // A wait that gave up ends the waiting, not the loop: warps meet at their barriers in every step.
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        if ((warp & 7) == 0) ok = ok && wait_quietly(&bars.s_full[tile], j & 1);
-        sync_256(1 + tile);
+        ok = ok && wait_quietly(&bars.s_full[tile][j % kB], j / kB & 1);
         tc_after();
+        const uint32_t t_s = t_s0 + (j & 1) * S::kN;
         const int t0 = (step0 + j) * S::kN + half * kMine;
-        const bool all = whole((step0 + j) * S::kN, tile_lo, tile_hi);
-        const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of these tokens
-        // The scores, 16 at a time, the next ones on their way while f works on these.
-        const auto scores_as = [&](auto masked, auto&& f) {
-          uint32_t buf[2][16];
-          tmem_ld16(t_s, buf[0]);
+        uint32_t s[kMine];
+        tmem_ld32(t_s, s);
+        tmem_ld_wait();
+        if (!whole((step0 + j) * S::kN, tile_lo, tile_hi)) {
+          const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of these tokens
 #pragma unroll
-          for (int c = 0; c < kMine; c += 16) {
-            uint32_t(&s)[16] = buf[(c / 16) & 1];
-            tmem_ld_wait();
-            if (c + 16 < kMine) tmem_ld16(t_s + c + 16, buf[(c / 16 + 1) & 1]);
-            if constexpr (decltype(masked)::value) {
+          for (int e = 0; e < kMine; ++e)
+            if (e > hi || e < lo) s[e] = 0xFF800000u;
+        }
+        float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (c + e > hi || c + e < lo) s[e] = 0xFF800000u;
-            }
-            f(c, s);
-          }
-        };
-        // Two copies of the code: one with a branch inside would carry the masks' instructions through every step.
-        const auto scores = [&](auto&& f) {
-          if (all) scores_as(std::false_type(), f); else scores_as(std::true_type(), f);
-        };
-        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        scores([&](int, const uint32_t(&s)[16]) {
-#pragma unroll
-          for (int e = 0; e < 16; e += 2)
-            most[e / 2 % 4] = max3(most[e / 2 % 4], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-        });
-        float m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+        for (int e = 0; e < kMine; e += 2) most[e / 2 % 2] = max3(most[e / 2 % 2], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
+        float m = fmaxf(most[0], most[1]);
         if (any_of_tile(1 + tile, m > limit)) {
           *s_mine = m;
           sync_256(1 + tile);
@@ -337,7 +328,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             sums[i].y *= f;
           }
           if (j > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
-            ok = ok && wait_quietly(&bars.pv_done[tile], (j - 1) & 1);
+            ok = ok && wait_quietly(&bars.pv_done[tile][(j - 1) % kB], (j - 1) / kB & 1);
             tc_after();
 #pragma unroll 1
             for (int c = 0; c < D / 2; c += 16) {
@@ -351,24 +342,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           }
         }
         const float2 ref2 = make_float2(minus_ref, minus_ref);
-        scores([&](int c, const uint32_t(&s)[16]) {
-          uint32_t p[8];
+        uint32_t p[kMine / 2];
 #pragma unroll
-          for (int e = 0; e < 16; e += 2) {
-            float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, ref2);
-            x.x = exp2_hw(x.x);
-            x.y = exp2_hw(x.y);
-            sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
-            p[e / 2] = half2_bits(x.x, x.y);
-          }
-          tmem_st8(t_s + c / 2, p);  // over scores that have been read
-          if (c + 16 == kMine / 2 || c + 16 == kMine) {  // the product begins with the first halves
-            tmem_st_wait();
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(c + 16 == kMine ? &bars.p_full[tile] : &bars.p_half[tile]);
-          }
-        });
+        for (int e = 0; e < kMine; e += 2) {
+          float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, ref2);
+          x.x = exp2_hw(x.x);
+          x.y = exp2_hw(x.y);
+          sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
+          p[e / 2] = half2_bits(x.x, x.y);
+        }
+        tmem_st16(t_s, p);  // over the thread's own scores
+        tmem_st_wait();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_full[tile][j % kB]);
       }
       // ---- out
       const float mine = (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
@@ -376,7 +363,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       *s_mine = mine;
       sync_256(1 + tile);
       const float l = half ? *s_other + mine : mine + *s_other;
-      if (steps > 0) ok = ok && wait_quietly(&bars.pv_done[tile], (steps - 1) & 1);
+      if (steps > 0) ok = ok && wait_quietly(&bars.pv_done[tile][(steps - 1) % kB], (steps - 1) / kB & 1);
       tc_after();
       uint32_t bad = 0;  // groups of the row's values that are not finite
       if (any_bad) {
@@ -421,94 +408,78 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     const int w = warp - kRowWarps;
     // lanes of one 128-byte access lie four rows apart, so that the swizzle spreads them over all banks
     const int g = lane >> 2, t = lane & 3, in8 = (g >> 1) | (g & 1) << 2;
-    constexpr int kG = D / 32, kWords = kG < 4 ? kG : 4, kAtOnce = S::kN / 8 / kUnpackWarps;  // a unit is eight tokens
-    int stage = 0, phase = 0, masked = -1;
+    constexpr int kG = D / 32, kWords = kG < 4 ? kG : 4;
+    const int tau = (w & 1) * 8 + in8, row = (w >> 1) * 16 + tau;  // a warp takes eight tokens of a step
+    uint8_t* const dst = s_k + row * 128;
+    int stage = 0, phase = 0, masked = -1, buf = 0, use = 0;
 #pragma unroll 1
     for (int j = 0; j < steps; ++j) {
-      const int t0 = (step0 + j) * S::kN, buf = j & 1, use = (j >> 1) & 1;
+      const int t0 = (step0 + j) * S::kN;
       const bool all = whole(t0, at_lo, at_hi);
       if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
-      // K, then V; all of a warp's words are asked for before the first is turned into values
+      if (w == 0) {
+        ok = ok && wait_quietly(&bars.pack_full[stage], phase);
+        for (int i = 0; i < S::kTilesM; ++i) ok = ok && wait_quietly(&bars.pv_done[i][buf], use ^ 1);  // then K is free as well
+      }
+      sync_256(3);
+      // all of the lane's words of K and V are asked for before the first is turned into values
+      const uint8_t* const tile = s_pack + stage * S::kPackBytes + (w >> 1) * S::kTileBytes;
+      uint32_t x[2][kG], sc[2][kG / 2];
 #pragma unroll
-      for (int kind = 0; kind < 2; ++kind) {
-        uint32_t x[kAtOnce][kG], sc[kAtOnce][kG / 2];
-        int st = stage, ph = phase;
+      for (int kind = 0; kind < 2; ++kind) kv4_lds(tile + kv4::scale_at<D>(kind, tau, 0), sc[kind]);
 #pragma unroll
-        for (int pk = 0; pk < S::kPacks; ++pk) {
-          if (kind == 0) {
-            if (w == 0) ok = ok && wait_quietly(&bars.pack_full[st], ph);
-            sync_256(3);
-          }
-          const uint8_t* const pack = s_pack + st * S::kPackBytes;
+      for (int q4 = 0; q4 < kG / kWords; ++q4)
+        kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), reinterpret_cast<uint32_t(&)[kWords]>(x[0][q4 * kWords]));
+      {
+        // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
+        const int vr = kv4::v_row(tau);
+        const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
+        uint32_t y[kG / 2], z[kG / 2];
+        kv4_lds(piece, y);
+        kv4_lds(piece + D / 16, z);
 #pragma unroll
-          for (int i = 0; i < kAtOnce; ++i) {
-            if (kAtOnce >= S::kPacks ? i * S::kPacks / kAtOnce != pk : w * S::kPacks / kUnpackWarps != pk) continue;  // in another stage
-            const int u = w + i * kUnpackWarps, tau = (u & 1) * 8 + in8;
-            const uint8_t* const tile = pack + (u >> 1) % S::kPackTiles * S::kTileBytes;
-            kv4_lds(tile + kv4::scale_at<D>(kind, tau, 0), sc[i]);
-            if (kind == 0) {
+        for (int e = 0; e < kG; ++e) x[1][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars.pack_empty[stage]);  // the words are in registers: the place is free
+      if (!all) {
 #pragma unroll
-              for (int q4 = 0; q4 < kG / kWords; ++q4)
-                kv4_lds(tile + kv4::k_word<D>(tau, q4 * kWords, t), reinterpret_cast<uint32_t(&)[kWords]>(x[i][q4 * kWords]));
-            } else {
-              // pieces 2 t and 2 t + 1 lie side by side; two bytes of each make a word of eight neighbours
-              const int vr = kv4::v_row(tau);
-              const uint8_t* piece = tile + 8 * D + vr * (D / 2) + kv4::v_piece<D>(vr, 2 * t) * (D / 16);
-              uint32_t y[kG / 2], z[kG / 2];
-              kv4_lds(piece, y);
-              kv4_lds(piece + D / 16, z);
-#pragma unroll
-              for (int e = 0; e < kG; ++e) x[i][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
-            }
-          }
-          if (kind == 1) {  // the words are in registers: the place is free
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&bars.pack_empty[st]);
-          }
-          if (++st == S::kRing) {
-            st = 0;
-            ph ^= 1;
-          }
-        }
-        if (kind == 1) {
-          stage = st;
-          phase = ph;
-        }
-        if (w == 0) ok = ok && wait_quietly(kind ? &bars.v_empty[buf] : &bars.k_empty[buf], use ^ 1);
-        sync_256(3);
-        uint8_t* const dst = (kind ? s_v : s_k) + buf * S::kKvBytes;
-        if (!all) {
-#pragma unroll
-          for (int i = 0; i < kAtOnce; ++i) {
-            const int row = (w + i * kUnpackWarps) * 8 + in8;
-#pragma unroll
-            for (int e = 0; e < kG; ++e) {
-              const uint32_t bits = 0x7C00u << (16 * (e & 1));
-              const bool there = t0 + row <= at_hi;  // behind lies anything
-              if (there && (kind == 0 || (sc[i][e >> 1] & bits) != bits)) continue;
-              // A NaN scale of V: its product with a zero weight would not be zero; noted, and told to the rows that see the token.
-              sc[i][e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-              if (there) {
-                any_bad = 1;
-                atomicOr(reinterpret_cast<uint32_t*>(s_bad + masked * S::kN + (row & ~3)), 1u << (e + 8 * (row & 3)));
-              }
-            }
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-          const int row = (w + i * kUnpackWarps) * 8 + in8;
+        for (int kind = 0; kind < 2; ++kind) {
 #pragma unroll
           for (int e = 0; e < kG; ++e) {
-            const int c = e * 4 + t;
-            const uint32_t s2 = __byte_perm(sc[i][e >> 1], 0, e & 1 ? 0x3232 : 0x1010);
-            *reinterpret_cast<uint4*>(dst + row * 128 + (c >> 3) * (S::kN * 128) + (((c & 7) ^ (row & 7)) << 4)) =
-                values8(x[i][e], *reinterpret_cast<const __half2*>(&s2));
+            const uint32_t bits = 0x7C00u << (16 * (e & 1));
+            const bool there = t0 + row <= at_hi;  // behind lies anything
+            if (there && (kind == 0 || (sc[kind][e >> 1] & bits) != bits)) continue;
+            // A NaN scale of V: its product with a zero weight would not be zero; noted, and told to the rows that see the token.
+            sc[kind][e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+            if (there) {
+              any_bad = 1;
+              atomicOr(reinterpret_cast<uint32_t*>(s_bad + masked * S::kN + (row & ~3)), 1u << (e + 8 * (row & 3)));
+            }
           }
+        }
+      }
+#pragma unroll
+      for (int kind = 0; kind < 2; ++kind) {
+        uint8_t* const to = dst + (kind * S::kBuffers + buf) * S::kKvBytes;  // V's buffers follow K's
+#pragma unroll
+        for (int e = 0; e < kG; ++e) {
+          const int c = e * 4 + t;
+          const uint32_t s2 = __byte_perm(sc[kind][e >> 1], 0, e & 1 ? 0x3232 : 0x1010);
+          *reinterpret_cast<uint4*>(to + (c >> 3) * (S::kN * 128) + (((c & 7) ^ (row & 7)) << 4)) =
+              values8(x[kind][e], *reinterpret_cast<const __half2*>(&s2));
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+      }
+      if (++stage == S::kRing) {
+        stage = 0;
+        phase ^= 1;
+      }
+      if (++buf == S::kBuffers) {
+        buf = 0;
+        use ^= 1;
       }
     }
   } else {
@@ -552,77 +523,45 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       for (int i = 0; i < S::kRing; ++i)
         for (int ph = 0; ph < 2; ++ph) wait_quietly(&bars.pack_full[i], ph);
     }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------------ products
+  } else if (warp >= kMmaWarp && warp < kMmaWarp + S::kTilesM) {
+    // ------------------------------------------------------------------ products of a tile
+    const int tile = warp - kMmaWarp;
     const uint32_t idesc_s = 1u << 4 | static_cast<uint32_t>(S::kN >> 3) << 17 | 8u << 24;
     const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
-    const uint32_t q_low = desc_low(s_q, 16), k_low = desc_low(s_k, 16), v_low = desc_low(s_v, S::kN * 128);
-    const auto scores = [&](int i, int buf) {
-      if (elect_one()) {
-        const uint32_t dq = q_low + i * (S::kQBytes >> 4), dk = k_low + buf * (S::kKvBytes >> 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          umma_ss(tmem + i * S::kN, dq + (((k >> 2) * (kRowsPerTile * 128) + (k & 3) * 32) >> 4),
-                  dk + (((k >> 2) * (S::kN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
-        if (i == S::kTilesM - 1) umma_commit(&bars.k_empty[buf]);
-        umma_commit(&bars.s_full[i]);
-      }
-      __syncwarp();
-    };
-    if (steps > 0) {
-      ok = wait_quietly(&bars.k_full[0], 0);
+    const uint32_t q_low = desc_low(s_q + tile * S::kQBytes, 16), k_low = desc_low(s_k, 16), v_low = desc_low(s_v, S::kN * 128);
+    const uint32_t t_s = tmem + tile * 2 * S::kN, t_o = tmem + S::kO + tile * D, me = elected();
+    const auto wait_all = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_quietly(bar, parity)) != 0; };
+    const auto scores = [&](int j) {  // of step j, into the tile's j % 2nd place
+      ok = wait_all(&bars.k_full[j % kB], j / kB & 1);
+      if (j > 1) ok = ok && wait_all(&bars.pv_done[tile][(j - 2) % kB], (j - 2) / kB & 1);  // whose weights lie there
+      if (!ok) return;
       tc_after();
-      if (ok) {
+      const uint32_t dk = k_low + j % kB * (S::kKvBytes >> 4);
 #pragma unroll
-        for (int i = 0; i < S::kTilesM; ++i) scores(i, 0);
-      }
-    }
+      for (int k = 0; k < D / 16; ++k)
+        umma_ss(me, t_s + (j & 1) * S::kN, q_low + (((k >> 2) * (kRowsPerTile * 128) + (k & 3) * 32) >> 4),
+                dk + (((k >> 2) * (S::kN * 128) + (k & 3) * 32) >> 4), idesc_s, k > 0);
+      umma_commit(me, &bars.s_full[tile][j % kB]);
+    };
+    if (steps > 0) scores(0);
 #pragma unroll 1
     for (int j = 0; j < steps && ok; ++j) {
-      const int buf = j & 1;
-      const uint32_t dv = v_low + buf * (S::kKvBytes >> 4);
+      if (j + 1 < steps) scores(j + 1);
+      ok = ok && wait_all(&bars.v_full[j % kB], j / kB & 1) && wait_all(&bars.p_full[tile][j % kB], j / kB & 1);
+      if (!ok) break;
+      tc_after();
+      const uint32_t dv = v_low + j % kB * (S::kKvBytes >> 4), p = t_s + (j & 1) * S::kN;
 #pragma unroll
-      for (int i = 0; i < S::kTilesM; ++i) {
-        if (i == 0) ok = wait_quietly(&bars.v_full[buf], j >> 1 & 1);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          ok = ok && wait_quietly(half ? &bars.p_full[i] : &bars.p_half[i], j & 1);
-          if (!ok) break;
-          tc_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < S::kN / 16; ++k) {
-              // the weights of either half of the tokens lie over that half's scores, and come in two halves again
-              constexpr int kQuarter = S::kN / 64;
-              if ((k / kQuarter & 1) != half) continue;
-              umma_tmem_a(tmem + S::kO + i * D, tmem + i * S::kN + k / (2 * kQuarter) * (S::kN / 2) + k % (2 * kQuarter) * 8,
-                          dv + (k * 2048 >> 4), idesc_o, k > 0 ? 1u : static_cast<uint32_t>(j));
-            }
-            if (half) {
-              if (i == S::kTilesM - 1) umma_commit(&bars.v_empty[buf]);
-              umma_commit(&bars.pv_done[i]);  // last: the block ends after it
-            }
-          }
-          __syncwarp();
-        }
-        if (!ok) break;
-        if (j + 1 < steps) {
-          if (i == 0) {
-            const uint32_t next_use = (j + 1) >> 1 & 1;
-            ok = wait_quietly(&bars.k_full[buf ^ 1], next_use);
-            if (!ok) break;
-            tc_after();
-          }
-          scores(i, buf ^ 1);
-        }
-      }
+      for (int k = 0; k < S::kN / 16; ++k)  // the weights of either half of the tokens lie over that half's scores
+        umma_tmem_a(me, t_o, p + k / 2 * (S::kN / 2) + k % 2 * 8, dv + (k * 2048 >> 4), idesc_o, k > 0 ? 1u : static_cast<uint32_t>(j));
+      umma_commit(me, &bars.pv_done[tile][j % kB]);
     }
   }
   if (!ok && lane == 0) atomicExch(a.error, kErrWait);
   tc_before();
   __syncthreads();
   tc_after();
-  if (warp == kMmaWarp) tmem_dealloc_512(tmem);
+  if (warp == kMmaWarp) tmem_dealloc_512(tmem_base);
 }
 
 template <int D>
