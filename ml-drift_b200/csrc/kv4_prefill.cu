@@ -3,17 +3,17 @@
 // The rows of a block are the queries of 256 / group tokens for all heads that share a key/value head: two tiles of 128 rows (one
 // for heads of 256 values).  A block walks the cached tokens in steps of 64:
 //   S = Q K^T        both operands fp16 from shared memory, 128 x 64 fp32 in tensor memory, two of them per tile
-//   P = 2^(S - ref)  two threads per row, half of the tokens each; written over S as fp16, where the next product takes it from
+//   P = 2^(S - ref)  a thread per row; written over S as fp16, where the next product takes it from
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
 // The next step's S is asked for ahead of this step's O, so that the threads that make P find it ready: steps of 128 tokens, of
 // which tensor memory holds one S per tile beside O, had every thread wait for its own products (0.52 of the tensor cores' rate).
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
-// by its threads themselves, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
+// by its thread itself, after the last product.  Weights are 2^10 at ref, so that fp16 holds 2^-24 of it as a normal number.
 //
-// Roles of the 28 warps: 0-15 make P and write the rows out (eight warps to a tile), 16-23 unpack, 24 asks for packed tiles, 25 and
-// 26 issue the products, a tile each (one warp for both took as long to issue as the products take).
+// Roles of the twenty warps: 0-7 make P and write the rows out (a warpgroup to a tile), 8-15 unpack, 16 asks for packed tiles, 17
+// and 18 issue the products, a tile each (one warp for both took as long to issue as the products take).
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -28,10 +28,10 @@
 namespace mld {
 namespace {
 
-constexpr int kPrefillThreads = 28 * 32;
-constexpr int kRowWarps = 16, kUnpackWarps = 8, kLoadWarp = 24, kMmaWarp = 25;  // and the one behind it for a second tile
-// Registers a thread: 896 x 72 at launch, dealt out anew as 512 x 80 + 256 x 64 + 128 x 56.
-constexpr int kRegsRows = 80, kRegsUnpack = 64, kRegsRest = 56;
+constexpr int kPrefillThreads = 20 * 32;
+constexpr int kRowWarps = 8, kUnpackWarps = 8, kLoadWarp = 16, kMmaWarp = 17;  // and the one behind it for a second tile
+// Registers a thread: 640 x 96 at launch, dealt out anew as 256 x 136 + 256 x 72 + 128 x 64.
+constexpr int kRegsRows = 136, kRegsUnpack = 72, kRegsRest = 64;
 constexpr int kRowsPerTile = 128;
 constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
 constexpr int kMaskedBlocks = 24;  // blocks of tokens that only some rows of a block of rows see, at most
@@ -181,16 +181,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-// Whether any of the 256 threads that share barrier `id` says yes; all of them call it.
-__device__ __forceinline__ bool any_of_tile(int id, bool yes) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, %2, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"(static_cast<uint32_t>(yes)), "r"(id)
-      : "memory");
-  return r != 0;
-}
 // Barrier `id` of 256 threads.  One warp of them waits for a transaction barrier and the others for it here, without polls.
 __device__ __forceinline__ void sync_256(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
 
@@ -216,7 +206,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   __shared__ PrefillBars bars;
   __shared__ uint32_t tmem_base;
   __shared__ int any_bad;
-  __shared__ float s_exchange[2][2][kRowsPerTile];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -229,7 +218,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       mbar_init(&bars.v_full[i], kUnpackWarps);
       for (int t = 0; t < S::kTilesM; ++t) {
         mbar_init(&bars.s_full[t][i], 1);
-        mbar_init(&bars.p_full[t][i], 8);
+        mbar_init(&bars.p_full[t][i], 4);
         mbar_init(&bars.pv_done[t][i], 1);
       }
     }
@@ -276,14 +265,11 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   if (warp < kRowWarps) {
     more_registers<kRegsRows>();
     // ------------------------------------------------------------------ weights, rows
-    const int tile = warp >> 3, half = (warp >> 2) & 1;
+    const int tile = warp >> 2;
     if (tile < S::kTilesM) {
-      constexpr int kMine = S::kN / 2;  // tokens of a step, columns of S
       const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-      const uint32_t t_s0 = tmem + lanes + tile * 2 * S::kN + half * kMine, t_o = tmem + lanes + S::kO + tile * D + half * (D / 2);
-      const int in_tile = (warp & 3) * 32 + lane, row = row0 + tile * kRowsPerTile + in_tile;
-      float* const s_mine = &s_exchange[tile][half][in_tile];
-      const float* const s_other = &s_exchange[tile][half ^ 1][in_tile];
+      const uint32_t t_s0 = tmem + lanes + tile * 2 * S::kN, t_o = tmem + lanes + S::kO + tile * D;
+      const int row = row0 + tile * kRowsPerTile + (warp & 3) * 32 + lane;
       const int at = q.n - q.m + min(row, rows - 1) / a.group;
       const int tile_lo = q.n - q.m + min(row0 + tile * kRowsPerTile, rows - 1) / a.group;
       const int tile_hi = q.n - q.m + min(row0 + tile * kRowsPerTile + kRowsPerTile - 1, rows - 1) / a.group;
@@ -292,30 +278,29 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       const float2 scale2 = make_float2(a.scale_log2, a.scale_log2);
       const float inv_scale = 1.0f / a.scale_log2;
       float limit = kPrefillFloor * inv_scale;  // scores that may not be exceeded
-      // A wait that gave up ends the waiting, not the loop: warps meet at their barriers in every step.
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        ok = ok && wait_quietly(&bars.s_full[tile][j % kB], j / kB & 1);
+        ok = wait_quietly(&bars.s_full[tile][j % kB], j / kB & 1);
+        if (!ok) break;
         tc_after();
         const uint32_t t_s = t_s0 + (j & 1) * S::kN;
-        const int t0 = (step0 + j) * S::kN + half * kMine;
-        uint32_t s[kMine];
-        tmem_ld32(t_s, s);
+        const int t0 = (step0 + j) * S::kN;
+        uint32_t s[2][32];
+        tmem_ld32(t_s, s[0]);
+        tmem_ld32(t_s + 32, s[1]);
         tmem_ld_wait();
-        if (!whole((step0 + j) * S::kN, tile_lo, tile_hi)) {
-          const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of these tokens
+        if (!whole(t0, tile_lo, tile_hi)) {
+          const int hi = at - t0, lo = a.window > 0 ? hi - a.window + 1 : 0;  // what the row sees of the step
 #pragma unroll
-          for (int e = 0; e < kMine; ++e)
-            if (e > hi || e < lo) s[e] = 0xFF800000u;
+          for (int e = 0; e < S::kN; ++e)
+            if (e > hi || e < lo) s[e / 32][e % 32] = 0xFF800000u;
         }
-        float most[2] = {-INFINITY, -INFINITY};
+        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int e = 0; e < kMine; e += 2) most[e / 2 % 2] = max3(most[e / 2 % 2], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-        float m = fmaxf(most[0], most[1]);
-        if (any_of_tile(1 + tile, m > limit)) {
-          *s_mine = m;
-          sync_256(1 + tile);
-          m = fmaxf(m, *s_other);
+        for (int e = 0; e < S::kN; e += 2)
+          most[e / 2 % 4] = max3(most[e / 2 % 4], __uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1]));
+        const float m = fmaxf(max3(most[0], most[1], most[2]), most[3]);
+        if (__any_sync(0xFFFFFFFFu, m > limit)) {
           const float new_top = m > limit ? m * a.scale_log2 : top;
           const float ref = new_top > kPrefillFloor ? new_top - kPrefillLift : kPrefillFloor;
           const float f = exp2_hw(-minus_ref - ref);
@@ -327,11 +312,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             sums[i].x *= f;
             sums[i].y *= f;
           }
-          if (j > 0 && __any_sync(0xFFFFFFFFu, f != 1.0f)) {
-            ok = ok && wait_quietly(&bars.pv_done[tile][(j - 1) % kB], (j - 1) / kB & 1);
+          if (j > 0) {
+            ok = wait_quietly(&bars.pv_done[tile][(j - 1) % kB], (j - 1) / kB & 1);
+            if (!ok) break;
             tc_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 2; c += 16) {
+            for (int c = 0; c < D; c += 16) {
               uint32_t o[16];
               tmem_ld16(t_o + c, o);
               tmem_ld_wait();
@@ -342,27 +328,26 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           }
         }
         const float2 ref2 = make_float2(minus_ref, minus_ref);
-        uint32_t p[kMine / 2];
 #pragma unroll
-        for (int e = 0; e < kMine; e += 2) {
-          float2 x = fma2(make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale2, ref2);
-          x.x = exp2_hw(x.x);
-          x.y = exp2_hw(x.y);
-          sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
-          p[e / 2] = half2_bits(x.x, x.y);
+        for (int h2 = 0; h2 < 2; ++h2) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            float2 x = fma2(make_float2(__uint_as_float(s[h2][e]), __uint_as_float(s[h2][e + 1])), scale2, ref2);
+            x.x = exp2_hw(x.x);
+            x.y = exp2_hw(x.y);
+            sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
+            p[e / 2] = half2_bits(x.x, x.y);
+          }
+          tmem_st16(t_s + 16 * h2, p);  // over the thread's own scores
         }
-        tmem_st16(t_s, p);  // over the thread's own scores
         tmem_st_wait();
         tc_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&bars.p_full[tile][j % kB]);
       }
       // ---- out
-      const float mine = (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
-      sync_256(1 + tile);  // nobody reads an earlier exchange any more
-      *s_mine = mine;
-      sync_256(1 + tile);
-      const float l = half ? *s_other + mine : mine + *s_other;
+      const float l = (sums[0].x + sums[1].x) + (sums[0].y + sums[1].y);
       if (steps > 0) ok = ok && wait_quietly(&bars.pv_done[tile][(steps - 1) % kB], (steps - 1) / kB & 1);
       tc_after();
       uint32_t bad = 0;  // groups of the row's values that are not finite
@@ -378,9 +363,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       }
       const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const int token = row / a.group, head = h * a.group + row - token * a.group;
-      __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D + half * (D / 2);
+      __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D;
 #pragma unroll 1
-      for (int c = 0; c < D / 2; c += 16) {
+      for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
         if (steps > 0) {
           tmem_ld16(t_o + c, o);
@@ -389,7 +374,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0;
         }
-        const float f = (bad >> ((half * (D / 2) + c) / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
+        const float f = (bad >> (c / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
         if (row < rows) {
 #pragma unroll
           for (int e = 0; e < 16; e += 8) {
@@ -530,7 +515,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
     const uint32_t q_low = desc_low(s_q + tile * S::kQBytes, 16), k_low = desc_low(s_k, 16), v_low = desc_low(s_v, S::kN * 128);
     const uint32_t t_s = tmem + tile * 2 * S::kN, t_o = tmem + S::kO + tile * D, me = elected();
-    const auto wait_all = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_quietly(bar, parity)) != 0; };
+    const auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_quietly(bar, parity)) != 0; };
     const auto scores = [&](int j) {  // of step j, into the tile's j % 2nd place
       ok = wait_all(&bars.k_full[j % kB], j / kB & 1);
       if (j > 1) ok = ok && wait_all(&bars.pv_done[tile][(j - 2) % kB], (j - 2) / kB & 1);  // whose weights lie there
@@ -552,8 +537,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       tc_after();
       const uint32_t dv = v_low + j % kB * (S::kKvBytes >> 4), p = t_s + (j & 1) * S::kN;
 #pragma unroll
-      for (int k = 0; k < S::kN / 16; ++k)  // the weights of either half of the tokens lie over that half's scores
-        umma_tmem_a(me, t_o, p + k / 2 * (S::kN / 2) + k % 2 * 8, dv + (k * 2048 >> 4), idesc_o, k > 0 ? 1u : static_cast<uint32_t>(j));
+      for (int k = 0; k < S::kN / 16; ++k)
+        umma_tmem_a(me, t_o, p + 8 * k, dv + (k * 2048 >> 4), idesc_o, k > 0 ? 1u : static_cast<uint32_t>(j));
       umma_commit(me, &bars.pv_done[tile][j % kB]);
     }
   }
