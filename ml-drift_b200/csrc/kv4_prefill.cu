@@ -144,7 +144,7 @@ __device__ __forceinline__ uint4 values8(uint32_t x, __half2 s) {
 // Two weights at once: 2^(s * scale - ref).
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+  asm volatile("fma.rn.f32x2 %0, %1, %2, %3;"
       : "=l"(reinterpret_cast<unsigned long long&>(d))
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
         "l"(reinterpret_cast<unsigned long long&>(c)));
@@ -152,7 +152,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 d;
-  asm("add.rn.f32x2 %0, %1, %2;"
+  asm volatile("add.rn.f32x2 %0, %1, %2;"
       : "=l"(reinterpret_cast<unsigned long long&>(d))
       : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
   return d;
@@ -164,7 +164,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 __device__ __forceinline__ float exp2_hw(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
@@ -328,19 +328,27 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           }
         }
         const float2 ref2 = make_float2(minus_ref, minus_ref);
+        // Three pairs are in the works at a time, so that the exponentials' unit, which takes an instruction in eight cycles, has
+        // the next one while the pair before is added up and packed.
+        const auto pair = [&](int e) { return make_float2(__uint_as_float(s[e / 32][e % 32]), __uint_as_float(s[e / 32][e % 32 + 1])); };
+        uint32_t p[2][16];
+        float2 x0 = fma2(pair(0), scale2, ref2), x1 = fma2(pair(2), scale2, ref2), y;
+        x0.x = exp2_hw(x0.x);
+        x0.y = exp2_hw(x0.y);
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-          uint32_t p[16];
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float2 x = fma2(make_float2(__uint_as_float(s[h2][e]), __uint_as_float(s[h2][e + 1])), scale2, ref2);
-            x.x = exp2_hw(x.x);
-            x.y = exp2_hw(x.y);
-            sums[e / 2 & 1] = add2(sums[e / 2 & 1], x);
-            p[e / 2] = half2_bits(x.x, x.y);
+        for (int e = 0; e < S::kN; e += 2) {
+          if (e + 2 < S::kN) {
+            y = x1;
+            y.x = exp2_hw(y.x);
           }
-          tmem_st16(t_s + 16 * h2, p);  // over the thread's own scores
+          if (e + 4 < S::kN) x1 = fma2(pair(e + 4), scale2, ref2);
+          sums[e / 2 & 1] = add2(sums[e / 2 & 1], x0);
+          if (e + 2 < S::kN) y.y = exp2_hw(y.y);
+          p[e / 32][e % 32 / 2] = half2_bits(x0.x, x0.y);
+          x0 = y;
+          if (e == 30) tmem_st16(t_s, p[0]);  // over the thread's own scores
         }
+        tmem_st16(t_s + 16, p[1]);
         tmem_st_wait();
         tc_before();
         __syncwarp();

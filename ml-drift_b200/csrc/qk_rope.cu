@@ -8,8 +8,10 @@
 // The angle is taken in turns, as a product of 32 x 64-bit integers modulo one turn (2^64), since a 32-bit float loses the
 // decimals of position * frequency for long contexts (position 131071: 0.008 rad); what is left is exact to 2^-31 turns.
 //
-// D / 8 lanes hold a head, eight neighbouring values each (one 16-byte load); a block takes 2048 values of one token.
-// Cosines and sines of a token are worked out once per block.
+// D / 8 lanes hold a head, eight neighbouring values each (16 bytes of fp16), and go through heads of one token.  With x' a value's
+// partner in its pair, a turned value is r (x A + x' B), r = 1 / sqrt(...): A = w cos and B = -+ w' sin are worked out once per token
+// and lane, so that a head costs an exchange of the raw values and three operations per value; all of a lane's heads are asked for
+// before the token's cosines are there.  What bounds a prompt is memory: q, k, v once in, q and the cache out.
 #include <cuda_fp16.h>
 #include <math.h>
 #include <string.h>
@@ -23,8 +25,9 @@
 namespace mld {
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 64;  // few lanes to a token: each works out its cosines and weights once for all its heads
 constexpr int kMaxPairs = 128;
+constexpr int kAhead = 2;  // heads that a lane asks for at once
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -44,173 +47,275 @@ struct RopeArgs {
   unsigned long long steps[kMaxPairs];  // 2^-64 turns per position
 };
 
+// Two 32-bit operations in one.
+__device__ __forceinline__ float2 pair(const float (&x)[8], int i) { return make_float2(x[i], x[i + 1]); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+        "l"(reinterpret_cast<unsigned long long&>(c)));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<unsigned long long&>(d))
+      : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+  return d;
+}
+
+// Eight neighbouring values as they lie in memory.
 template <typename T>
 struct Eight;
 template <>
 struct Eight<__half> {
-  static __device__ __forceinline__ void load(const __half* p, float (&x)[8]) {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const __half* p) {
     const uint4 r = *reinterpret_cast<const uint4*>(p);
-    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    w[0] = r.x;
+    w[1] = r.y;
+    w[2] = r.z;
+    w[3] = r.w;
+  }
+  __device__ __forceinline__ void store(__half* p) const { *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float2 f = __half22float2(h[i]);
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
       x[2 * i] = f.x;
       x[2 * i + 1] = f.y;
     }
   }
-  static __device__ __forceinline__ void store(__half* p, const float (&x)[8]) {
-    __align__(16) __half2 h[4];
+  __device__ __forceinline__ void put(const float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
-    *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
   }
+  __device__ __forceinline__ Eight from(unsigned mask, int lane) const {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r.w[i] = __shfl_sync(mask, w[i], lane);
+    return r;
+  }
+  __device__ __forceinline__ Eight<__half> halves() const { return *this; }
 };
 template <>
 struct Eight<float> {
-  static __device__ __forceinline__ void load(const float* p, float (&x)[8]) {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const float4 f = reinterpret_cast<const float4*>(p)[i];
-      x[4 * i] = f.x;
-      x[4 * i + 1] = f.y;
-      x[4 * i + 2] = f.z;
-      x[4 * i + 3] = f.w;
+      v[4 * i] = f.x;
+      v[4 * i + 1] = f.y;
+      v[4 * i + 2] = f.z;
+      v[4 * i + 3] = f.w;
     }
   }
-  static __device__ __forceinline__ void store(float* p, const float (&x)[8]) {
+  __device__ __forceinline__ void store(float* p) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      reinterpret_cast<float4*>(p)[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      reinterpret_cast<float4*>(p)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = v[i];
+  }
+  __device__ __forceinline__ void put(const float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = x[i];
+  }
+  __device__ __forceinline__ Eight from(unsigned mask, int lane) const {
+    Eight r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r.v[i] = __shfl_sync(mask, v[i], lane);
+    return r;
+  }
+  __device__ __forceinline__ Eight<__half> halves() const {
+    Eight<__half> h;
+    h.put(v);
+    return h;
   }
 };
 
 // Quantises the eight values of a lane (its place in the head: l) into the tile at `tile`; the four lanes of a group of 32
 // call it together.  A group that holds an infinity or a NaN gets a NaN scale.
 template <int D>
-__device__ __forceinline__ void put_eight(uint8_t* tile, bool is_v, int tau, int l, const float (&x)[8], unsigned mask, bool store) {
-  float r[8], top = 0.0f;
-  bool finite = true;
+__device__ __forceinline__ void put_eight(uint8_t* tile, bool is_v, int tau, int l, const Eight<__half>& h, unsigned mask, bool store) {
+  uint32_t top2 = 0;  // of magnitudes, as bits: infinities and NaN are above all numbers
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    r[i] = __half2float(__float2half_rn(x[i]));
-    top = fmaxf(top, fabsf(r[i]));
-    finite = finite && fabsf(r[i]) <= 65504.0f;
-  }
-  if (!finite) top = INFINITY;
-  top = fmaxf(top, __shfl_xor_sync(mask, top, 1));
-  top = fmaxf(top, __shfl_xor_sync(mask, top, 2));
+  for (int i = 0; i < 4; ++i) top2 = __vmaxu2(top2, h.w[i] & 0x7FFF7FFFu);
+  top2 = __vmaxu2(top2, __shfl_xor_sync(mask, top2, 1));
+  top2 = __vmaxu2(top2, __shfl_xor_sync(mask, top2, 2));
+  const uint32_t top = max(top2 & 0xFFFFu, top2 >> 16);
   // eight significant bits (round to nearest even), then fp16, which rounds only what is below its normal range
-  uint32_t bits = __float_as_uint(__fdiv_rn(top, 7.0f));
+  uint32_t bits = __float_as_uint(__fdiv_rn(__half2float(__ushort_as_half(static_cast<unsigned short>(top))), 7.0f));
   bits = (bits + 0x7FFFu + ((bits >> 16) & 1u)) & 0xFFFF0000u;
-  const __half scale = top == INFINITY ? __ushort_as_half(0x7E00) : __float2half_rn(__uint_as_float(bits));
+  const __half scale = top >= 0x7C00u ? __ushort_as_half(0x7E00) : __float2half_rn(__uint_as_float(bits));
   const float s = __half2float(scale);
+  float r[8];
+  h.get(r);
+  // The product with the reciprocal decides, unless it is within 10^-5 of a halfway point (it is off by less than 2 10^-6), or
+  // the scale is one of fp16's subnormal numbers, whose rounding may leave more than 7.
+  constexpr float kMagic = 12582920.0f;  // 1.5 2^23 + 8: a sum's low bits are the code
+  const float inv = __frcp_rn(s);
   uint32_t code[8];
+  float off = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float c = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(r[i], s)), -7.0f), 7.0f) : 0.0f;
-    code[i] = static_cast<uint32_t>(static_cast<int>(c) + 8);
+    const float t = r[i] * inv, y = t + kMagic;
+    off = fmaxf(off, fabsf(t - (y - kMagic)));
+    code[i] = __float_as_uint(y);
+  }
+  if (!(off < 0.49999f) || !(s >= 6.103515625e-05f)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float c = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(r[i], s)), -7.0f), 7.0f) : 0.0f;
+      code[i] = static_cast<uint32_t>(static_cast<int>(c) + 8);
+    }
   }
   if (!store) return;
   const int j = l >> 2, t = l & 3;
-  if (!is_v) {
-    uint32_t w = 0;
+  // nibble p of the low half and of the high half: values 2 p and 2 p + 1 of K, p and 4 + p of V
+  uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= code[i] << (4 * (4 * (i & 1) + (i >> 1)));
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t two = is_v ? __byte_perm(code[p], code[4 + p], 0x5410) : __byte_perm(code[2 * p], code[2 * p + 1], 0x5410);
+    w |= (two << (4 * p)) & (0x000F000Fu << (4 * p));
+  }
+  if (!is_v) {
     *reinterpret_cast<uint32_t*>(tile + kv4::k_word<D>(tau, j, t)) = w;
   } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      *reinterpret_cast<uint16_t*>(tile + kv4::v_half<D>(tau, j, 2 * t + h)) =
-          static_cast<uint16_t>(code[4 * h] | code[4 * h + 1] << 4 | code[4 * h + 2] << 8 | code[4 * h + 3] << 12);
+    uint8_t* const at = tile + kv4::v_half<D>(tau, j, 2 * t);
+    *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w);
+    *reinterpret_cast<uint16_t*>(at + D / 16) = static_cast<uint16_t>(w >> 16);
   }
   if (t == 0) *reinterpret_cast<__half*>(tile + kv4::scale_at<D>(is_v, tau, j)) = scale;
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
+// Blocks: tokens along x; along y, parts of a token's heads (each takes every gridDim.y-th of the groups of kHeads heads).
+template <typename T, int D, bool NEIGHBOURS>
+__global__ void __launch_bounds__(kThreads, 12) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kLanes = D / 8;
   constexpr int kHeads = kThreads / kLanes;
-  __shared__ float cosines[kMaxPairs], sines[kMaxPairs];
+  __shared__ float2 turned[8][kMaxPairs / 8];  // cosine, sine of pair 8 j + i at [i][j]
   pdl_wait();
   const int token = blockIdx.x;
   const int l = threadIdx.x % kLanes;
-  const int head = blockIdx.y * kHeads + threadIdx.x / kLanes;
-  const bool is_q = head < a.q_heads;
-  const bool is_k = !is_q && head < a.q_heads + a.k_heads;
-  const bool is_v = !is_q && !is_k && head < a.q_heads + a.k_heads + a.v_heads;
-  const int h = is_q ? head : is_k ? head - a.q_heads : head - a.q_heads - a.k_heads;
-  float x[8] = {};
-  if (is_q || is_k || is_v) {
-    const T* src = is_q   ? static_cast<const T*>(a.q) + token * a.q_stride
-                   : is_k ? static_cast<const T*>(a.k) + token * a.k_stride
-                          : static_cast<const T*>(a.v) + token * a.v_stride;
-    Eight<T>::load(src + h * D + 8 * l, x);
-  }
+  const int step = kHeads * gridDim.y, head0 = blockIdx.y * kHeads + threadIdx.x / kLanes;
+  Eight<T> ahead[kAhead];
+  const T* src = static_cast<const T*>(a.q) + token * a.q_stride + 8 * l;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i)
+    if (head0 + i * step < a.q_heads) ahead[i].load(src + (head0 + i * step) * D);
   for (int i = threadIdx.x; i < a.half_pairs; i += kThreads) {
     int axis = 0;
 #pragma unroll
     for (int s = 0; s < 3; ++s) axis += i >= a.section_end[s] ? 1 : 0;
     const long long pos = a.positions[static_cast<long long>(axis) * a.tokens + token];
     const unsigned long long turn = static_cast<unsigned long long>(pos) * a.steps[i];
-    sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f, &sines[i], &cosines[i]);
+    float sine, cosine;
+    sincospif(static_cast<float>(static_cast<int>(turn >> 32)) * 4.656612873077393e-10f, &sine, &cosine);
+    turned[i & 7][i >> 3] = make_float2(cosine, sine);
+  }
+  int slot = -1, in_page = 0;
+  uint8_t* tile0 = a.pool;
+  const int page_tiles = a.page_tokens / kv4::kTile;
+  if (a.pool != nullptr) {
+    slot = a.slots[token];
+    if (slot < 0 || slot >= a.slots_end) slot = -1;
+    const int page = max(slot, 0) / a.page_tokens;
+    in_page = max(slot, 0) - page * a.page_tokens;
+    tile0 += (static_cast<long long>(page) * a.kv_heads_pool * page_tiles + in_page / kv4::kTile) * kv4::tile_bytes(D);
   }
   __syncthreads();
   // the lanes of a head stay together in what follows
   const unsigned mask = kLanes == 32 ? 0xFFFFFFFFu : ((1u << kLanes) - 1u) << ((threadIdx.x & 31) / kLanes * kLanes);
-  if (is_q || is_k) {
-    const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
-    if (w != nullptr) {
-      float sum = 0.0f;
+  const int far = a.half_pairs / 8;  // lanes between the halves of a pair
+  const bool turns = 8 * l < 2 * a.half_pairs, second = l >= far;
+  const int partner = NEIGHBOURS || !turns ? l : second ? l - far : l + far;
+  const int from = ((threadIdx.x & 31) - l) + partner;
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const int count = kind ? a.k_heads : a.q_heads;
+    const T* const w = static_cast<const T*>(kind ? a.k_weight : a.q_weight);
+    // what multiplies a value and its partner
+    float mine[8], other[8];
+    {
+      float wm[8], wo[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-      const float r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
-      float wf[8];
-      Eight<T>::load(w + 8 * l, wf);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wf[i];
-    }
-    const int rot = 2 * a.half_pairs;
-    if (a.neighbours) {
-      if (8 * l < rot) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float c = cosines[4 * l + i], s = sines[4 * l + i], p = x[2 * i], n = x[2 * i + 1];
-          x[2 * i] = p * c - n * s;
-          x[2 * i + 1] = n * c + p * s;
-        }
+      for (int i = 0; i < 8; ++i) wm[i] = wo[i] = 1.0f;
+      if (w != nullptr) {
+        Eight<T> e;
+        e.load(w + 8 * l);
+        e.get(wm);
+        e.load(w + 8 * partner);
+        e.get(wo);
       }
-    } else {
-      const int far = a.half_pairs / 8;  // lanes between the halves of a pair
-      const bool second = l >= far;
-      const int other = l < far ? l + far : l < 2 * far ? l - far : l;
-      const int from = ((threadIdx.x & 31) - l) + other;
-      float y[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(mask, x[i], from);
-      if (l < 2 * far) {
-        const int at = 8 * (second ? other : l);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float c = cosines[at + i], s = sines[at + i];
-          x[i] = second ? x[i] * c + y[i] * s : x[i] * c - y[i] * s;
-        }
+      for (int i = 0; i < 8; ++i) {
+        float2 cs = make_float2(1.0f, 0.0f);
+        if (turns) cs = NEIGHBOURS ? turned[4 * (l & 1) + i / 2][l >> 1] : turned[i][second ? partner : l];
+        mine[i] = wm[i] * cs.x;
+        other[i] = (NEIGHBOURS ? wo[i ^ 1] : wo[i]) * ((NEIGHBOURS ? (i & 1) == 0 : !second) ? -cs.y : cs.y);
       }
     }
-    if (is_q) {
-      Eight<T>::store(static_cast<T*>(a.q_out) + token * a.q_out_stride + h * D + 8 * l, x);
-    } else if (a.k_out != nullptr) {
-      Eight<T>::store(static_cast<T*>(a.k_out) + token * a.k_out_stride + h * D + 8 * l, x);
+    if (kind) {
+      src = static_cast<const T*>(a.k) + token * a.k_stride + 8 * l;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i)
+        if (head0 + i * step < count) ahead[i].load(src + (head0 + i * step) * D);
+    }
+    T* const out = kind ? static_cast<T*>(a.k_out) : static_cast<T*>(a.q_out);
+    T* const dst = out == nullptr ? nullptr : out + token * (kind ? a.k_out_stride : a.q_out_stride) + 8 * l;
+#pragma unroll 1
+    for (int base = head0; base < count; base += kAhead * step) {
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int h = base + i * step;
+        if (h >= count) break;
+        Eight<T> e = ahead[i];
+        if (h + kAhead * step < count) ahead[i].load(src + (h + kAhead * step) * D);
+        float x[8], y[8];
+        e.get(x);
+        float r = 1.0f;
+        if (w != nullptr) {
+          float2 two = make_float2(0.0f, 0.0f);
+#pragma unroll
+          for (int c = 0; c < 8; c += 2) two = fma2(pair(x, c), pair(x, c), two);
+          float sum = two.x + two.y;
+#pragma unroll
+          for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+          r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
+        }
+        if (NEIGHBOURS) {
+#pragma unroll
+          for (int c = 0; c < 8; ++c) y[c] = x[c ^ 1];
+        } else {
+          e.from(mask, from).get(y);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; c += 2) {
+          const float2 z = mul2(make_float2(r, r), fma2(pair(x, c), pair(mine, c), mul2(pair(y, c), pair(other, c))));
+          x[c] = z.x;
+          x[c + 1] = z.y;
+        }
+        e.put(x);
+        if (dst != nullptr) e.store(dst + h * D);
+        if (kind && a.pool != nullptr)
+          put_eight<D>(tile0 + static_cast<long long>(h) * page_tiles * kv4::tile_bytes(D), false, in_page % kv4::kTile, l, e.halves(), mask, slot >= 0);
+      }
     }
   }
-  if ((is_k || is_v) && a.pool != nullptr) {
-    const int slot = a.slots[token];
-    const bool store = slot >= 0 && slot < a.slots_end;
-    const int page = store ? slot / a.page_tokens : 0, in_page = store ? slot - page * a.page_tokens : 0;
-    uint8_t* tile = a.pool + ((static_cast<long long>(page) * a.kv_heads_pool + h) * (a.page_tokens / kv4::kTile) +
-                              in_page / kv4::kTile) * kv4::tile_bytes(D);
-    put_eight<D>(tile, is_v, in_page % kv4::kTile, l, x, mask, store);
+  src = static_cast<const T*>(a.v) + token * a.v_stride + 8 * l;
+#pragma unroll 1
+  for (int h = head0; h < a.v_heads; h += step) {
+    Eight<T> e;
+    e.load(src + h * D);
+    put_eight<D>(tile0 + static_cast<long long>(h) * page_tiles * kv4::tile_bytes(D), true, in_page % kv4::kTile, l, e.halves(), mask, slot >= 0);
   }
 }
 
@@ -222,47 +327,57 @@ struct ReadArgs {
   int slots_end, page_tokens, kv_heads, tokens;
 };
 
-// One lane gives eight neighbouring values of a token's key or value.  A slot outside the pool gives zeros.
+// One lane gives eight neighbouring values of a token's key or value at a time.  A slot outside the pool gives zeros.
 template <int D>
 __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
   constexpr int kLanes = D / 8;
+  constexpr int kHeads = kThreads / kLanes;
   pdl_wait();
-  const int unit = blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes;
-  if (unit >= 2 * a.kv_heads) return;
   const int token = blockIdx.x, l = threadIdx.x % kLanes, j = l >> 2, t = l & 3;
-  const bool is_v = unit >= a.kv_heads;
-  const int h = is_v ? unit - a.kv_heads : unit;
   const int slot = a.slots[token];
-  __align__(16) __half2 y[4] = {};
-  if (slot >= 0 && slot < a.slots_end) {
-    const int page = slot / a.page_tokens, in_page = slot - page * a.page_tokens, tau = in_page % kv4::kTile;
-    const uint8_t* tile = a.pool + ((static_cast<long long>(page) * a.kv_heads + h) * (a.page_tokens / kv4::kTile) +
-                                    in_page / kv4::kTile) * kv4::tile_bytes(D);
-    const float s = __half2float(*reinterpret_cast<const __half*>(tile + kv4::scale_at<D>(is_v, tau, j)));
-    float c[8];
-    if (!is_v) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + kv4::k_word<D>(tau, j, t));
+  const bool there = slot >= 0 && slot < a.slots_end;
+  const int page = there ? slot / a.page_tokens : 0, in_page = there ? slot - page * a.page_tokens : 0, tau = in_page % kv4::kTile;
+  const long long head_bytes = static_cast<long long>(a.page_tokens / kv4::kTile) * kv4::tile_bytes(D);
+  const uint8_t* const tile0 = a.pool + static_cast<long long>(page) * a.kv_heads * head_bytes + in_page / kv4::kTile * kv4::tile_bytes(D);
+  const int at_k = kv4::k_word<D>(tau, j, t), at_v = kv4::v_half<D>(tau, j, 2 * t);
+  __half* const k = a.k + token * a.k_stride + 8 * l;
+  __half* const v = a.v + token * a.v_stride + 8 * l;
+#pragma unroll 2
+  for (int unit = blockIdx.y * kHeads + threadIdx.x / kLanes; unit < 2 * a.kv_heads; unit += kHeads * gridDim.y) {
+    const bool is_v = unit >= a.kv_heads;
+    const int h = is_v ? unit - a.kv_heads : unit;
+    uint4 y = make_uint4(0, 0, 0, 0);
+    if (there) {
+      const uint8_t* const tile = tile0 + h * head_bytes;
+      const __half2 s = __half2half2(*reinterpret_cast<const __half*>(tile + kv4::scale_at<D>(is_v, tau, j)));
+      uint32_t w;
+      if (!is_v)
+        w = *reinterpret_cast<const uint32_t*>(tile + at_k);
+      else
+        w = *reinterpret_cast<const uint16_t*>(tile + at_v) | static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(tile + at_v + D / 16)) << 16;
+      uint32_t p[4];  // values 2 i and 2 i + 1 of K, i and 4 + i of V
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = static_cast<float>(static_cast<int>(w >> (4 * (4 * (i & 1) + (i >> 1))) & 15u) - 8);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const uint32_t w = *reinterpret_cast<const uint16_t*>(tile + kv4::v_half<D>(tau, j, 2 * t + i));
-#pragma unroll
-        for (int e = 0; e < 4; ++e) c[4 * i + e] = static_cast<float>(static_cast<int>(w >> (4 * e) & 15u) - 8);
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t b = (w >> (4 * i) & 0x000F000Fu) | 0x64006400u;  // 1024 + u
+        const __half2 x = __hmul2(__hsub2(*reinterpret_cast<const __half2*>(&b), __float2half2_rn(1032.0f)), s);
+        p[i] = *reinterpret_cast<const uint32_t*>(&x);
       }
+      y = is_v ? make_uint4(__byte_perm(p[0], p[1], 0x5410), __byte_perm(p[2], p[3], 0x5410), __byte_perm(p[0], p[1], 0x7632),
+                            __byte_perm(p[2], p[3], 0x7632))
+               : make_uint4(p[0], p[1], p[2], p[3]);
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __floats2half2_rn(c[2 * i] * s, c[2 * i + 1] * s);
+    *reinterpret_cast<uint4*>((is_v ? v : k) + h * D) = y;
   }
-  __half* dst = is_v ? a.v + token * a.v_stride : a.k + token * a.k_stride;
-  *reinterpret_cast<uint4*>(dst + h * D + 8 * l) = *reinterpret_cast<const uint4*>(y);
 }
+
+// Blocks of a token: as many as it has groups of heads while the GPU has room for them at once, else one.
+int parts_of_token(int tokens, int groups) { return groups < 1 ? 1 : static_cast<int64_t>(tokens) * groups <= 4 * 148 ? groups : 1; }
 
 template <typename T, int D>
 int launch_rope_t(const RopeArgs& a, cudaStream_t stream) {
-  const dim3 grid(a.tokens, div_up(a.q_heads + a.k_heads + a.v_heads, kThreads / (D / 8)));
-  MLD_CUDA_CHECK(launch_overlapped(qk_rope_kernel<T, D>, grid, dim3(kThreads), 0, stream, a));
+  const int most = a.q_heads > a.k_heads ? a.q_heads : a.k_heads;
+  const dim3 grid(a.tokens, parts_of_token(a.tokens, div_up(most, kThreads / (D / 8))));
+  MLD_CUDA_CHECK(launch_overlapped(a.neighbours ? qk_rope_kernel<T, D, true> : qk_rope_kernel<T, D, false>, grid, dim3(kThreads), 0, stream, a));
   MLD_LAUNCH_CHECK();
   return MLD_OK;
 }
@@ -441,7 +556,7 @@ int mld_kv4_read(const mld_kv4_desc* d, const void* pool, const int32_t* slots, 
   MLD_REQUIRE(tokens == 1 || (k_stride >= width && v_stride >= width), "token strides must not be shorter than a token");
   ReadArgs a = {static_cast<const uint8_t*>(pool), slots, static_cast<__half*>(k), static_cast<__half*>(v), k_stride, v_stride,
                 d->pages * d->page_tokens, d->page_tokens, d->kv_heads, tokens};
-  const dim3 grid(tokens, div_up(2 * d->kv_heads, kThreads / (d->head_dim / 8)));
+  const dim3 grid(tokens, parts_of_token(tokens, div_up(2 * d->kv_heads, kThreads / (d->head_dim / 8))));
   auto kern = d->head_dim == 64 ? kv4_read_kernel<64> : d->head_dim == 128 ? kv4_read_kernel<128> : kv4_read_kernel<256>;
   MLD_CUDA_CHECK(launch_overlapped(kern, grid, dim3(kThreads), 0, static_cast<cudaStream_t>(stream), a));
   MLD_LAUNCH_CHECK();
