@@ -496,12 +496,13 @@ class Kv4AttnIo(C.Structure):
                 ("max_queries", C.c_int32), ("out", C.c_void_p), ("out_stride", C.c_int64)]
 
 
-def _rows(t, heads, head_dim, dtype, what):
+def _rows(t, tokens, heads, head_dim, dtype, what):
     """Elements from token to token of a [tokens][heads][head_dim] tensor whose rows are contiguous."""
-    _, h, d = t.shape
+    n, h, d = t.shape
     stride = t.stride()
-    if t.dtype is not dtype or h != heads or d != head_dim or stride[2] != 1 or (stride[1] != head_dim and heads > 1):
-        raise ValueError(f"{what}: expected {dtype} [tokens][{heads}][{head_dim}] with contiguous heads, "
+    if n != tokens or t.dtype is not dtype or h != heads or d != head_dim or stride[2] != 1 or \
+            (stride[1] != head_dim and heads > 1):
+        raise ValueError(f"{what}: expected {dtype} [{tokens}][{heads}][{head_dim}] with contiguous heads, "
                          f"got {t.dtype} {tuple(t.shape)} strides {stride}")
     return stride[0]
 
@@ -536,8 +537,8 @@ class Kv4Cache:
     def write(self, k, v, slots, layer=0, stream=None):
         """k, v: [tokens][kv_heads][head_dim] fp16 or fp32; slots: int32 [tokens] on the device (-1: passed over)."""
         d = self.desc
-        ks, vs = (_rows(t, d.kv_heads, d.head_dim, k.dtype, n) for t, n in ((k, "k"), (v, "v")))
-        n = _same_tokens(k, v)
+        n = k.shape[0]
+        ks, vs = (_rows(t, n, d.kv_heads, d.head_dim, k.dtype, what) for t, what in ((k, "k"), (v, "v")))
         _check(lib().mld_kv4_write(C.byref(d), self.address(layer), k.data_ptr(), ks, v.data_ptr(), vs, _f16(k),
                                    _ints(slots, (n,), "slots"), n, _stream_addr(stream)), "mld_kv4_write")
 
@@ -545,8 +546,8 @@ class Kv4Cache:
         """The cache's values at `slots` into k and v, fp16 [tokens][kv_heads][head_dim]."""
         d = self.desc
         hk, hd = d.kv_heads, d.head_dim
-        ks, vs = _rows(k, hk, hd, torch.float16, "k"), _rows(v, hk, hd, torch.float16, "v")
-        n = _same_tokens(k, v)
+        n = k.shape[0]
+        ks, vs = _rows(k, n, hk, hd, torch.float16, "k"), _rows(v, n, hk, hd, torch.float16, "v")
         rc = _lib.mld_kv4_read(C.byref(d), self.address(layer), _ints(slots, (n,), "slots"), n, k.data_ptr(), ks, v.data_ptr(), vs,
                                _stream_addr(stream))
         if rc != OK:
@@ -560,18 +561,6 @@ class Kv4Cache:
         ints = C.c_int32 * n
         _check(lib().mld_kv4_copy_pages(C.byref(self.desc), self.pool.data_ptr(), self.layers, self.layer_bytes, ints(*src),
                                         ints(*dst), n, _stream_addr(stream)), "mld_kv4_copy_pages")
-
-
-def _tokens(t, n, what):
-    if t.shape[0] != n:
-        raise ValueError(f"{what}: {t.shape[0]} tokens where the others have {n}")
-
-
-def _same_tokens(*tensors):
-    n = tensors[0].shape[0]
-    if any(t.shape[0] != n for t in tensors):
-        raise ValueError(f"tensors of different token counts: {[t.shape[0] for t in tensors]}")
-    return n
 
 
 def _f16(t):
@@ -667,17 +656,14 @@ class QkNormRope:
         n = (q if h else k).shape[0]
         io = QkRopeIo()
         if h:
-            io.q, io.q_stride = q.data_ptr(), _rows(q, h, d, dt, "q")
-            io.q_out, io.q_out_stride = q_out.data_ptr(), _rows(q_out, h, d, dt, "q_out")
-            _tokens(q_out, n, "q_out")
+            io.q, io.q_stride = q.data_ptr(), _rows(q, n, h, d, dt, "q")
+            io.q_out, io.q_out_stride = q_out.data_ptr(), _rows(q_out, n, h, d, dt, "q_out")
         if hk:
-            io.k, io.k_stride = k.data_ptr(), _rows(k, hk, d, dt, "k")
-            _tokens(k, n, "k")
+            io.k, io.k_stride = k.data_ptr(), _rows(k, n, hk, d, dt, "k")
             if k_out is not None:
-                io.k_out, io.k_out_stride = k_out.data_ptr(), _rows(k_out, hk, d, dt, "k_out")
-                _tokens(k_out, n, "k_out")
+                io.k_out, io.k_out_stride = k_out.data_ptr(), _rows(k_out, n, hk, d, dt, "k_out")
         for w in (q_weight, k_weight):
-            if w is not None and (w.dtype is not dt or w.shape != (d,) or not w.is_contiguous()):
+            if w is not None and (w.dtype is not dt or w.numel() != d or not w.is_contiguous()):
                 raise ValueError(f"norm weights: expected contiguous {dt} [{d}]")
         if q_weight is not None:
             io.q_weight = q_weight.data_ptr()
@@ -688,8 +674,7 @@ class QkNormRope:
         if cache is not None:
             if v is None or slots is None:
                 raise ValueError("a cache needs v and slots")
-            io.v, io.v_stride = v.data_ptr(), _rows(v, hk, d, dt, "v")
-            _tokens(v, n, "v")
+            io.v, io.v_stride = v.data_ptr(), _rows(v, n, hk, d, dt, "v")
             io.cache, io.pool, io.slots = C.addressof(cache.desc), cache.address(layer), _ints(slots, (n,), "slots")
         rc = _lib.mld_qk_rope_run(self._h, C.byref(io), n, _stream_addr(stream))
         if rc != OK:
@@ -721,11 +706,10 @@ class Kv4Attention:
         [batch + 1], the rows of each sequence, of which none has more than max_queries (None: one row each)."""
         d, h = self.cache.head_dim, self.heads
         batch, n = lens.shape[0], q.shape[0]
-        _tokens(out, n, "out")
-        io = Kv4AttnIo(q.data_ptr(), _rows(q, h, d, torch.float16, "q"), self.cache.address(layer),
+        io = Kv4AttnIo(q.data_ptr(), _rows(q, n, h, d, torch.float16, "q"), self.cache.address(layer),
                        _ints(page_table, (batch, self.max_pages), "page_table"), _ints(lens, (batch,), "lens"),
                        None if q_starts is None else _ints(q_starts, (batch + 1,), "q_starts"), batch, n, max_queries,
-                       out.data_ptr(), _rows(out, h, d, torch.float16, "out"))
+                       out.data_ptr(), _rows(out, n, h, d, torch.float16, "out"))
         rc = _lib.mld_kv4_attn_run(self._h, C.byref(io), _stream_addr(stream))
         if rc != OK:
             _check(rc, "mld_kv4_attn_run")

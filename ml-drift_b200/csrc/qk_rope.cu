@@ -10,8 +10,9 @@
 //
 // D / 8 lanes hold a head, eight neighbouring values each (16 bytes of fp16), and go through heads of one token.  With x' a value's
 // partner in its pair, a turned value is r (x A + x' B), r = 1 / sqrt(...): A = w cos and B = -+ w' sin are worked out once per token
-// and lane, so that a head costs an exchange of the raw values and three operations per value; all of a lane's heads are asked for
-// before the token's cosines are there.  What bounds a prompt is memory: q, k, v once in, q and the cache out.
+// and lane, so that a head costs an exchange of the raw values and three operations per value.  Blocks of two warps, 16 to an SM:
+// 8192 tokens of 32 + 8 + 8 heads of 128 into the cache take 66 us with the read behind it, 71 with 12 blocks of more registers to an
+// SM, 73 to 81 in blocks of four warps; it is bound by instructions (conversions, exchanges, quantisation), not by memory.
 #include <cuda_fp16.h>
 #include <math.h>
 #include <string.h>
@@ -27,7 +28,6 @@ namespace {
 
 constexpr int kThreads = 64;  // few lanes to a token: each works out its cosines and weights once for all its heads
 constexpr int kMaxPairs = 128;
-constexpr int kAhead = 2;  // heads that a lane asks for at once
 
 struct RopeArgs {
   const void *q, *k, *v;
@@ -198,7 +198,7 @@ __device__ __forceinline__ void put_eight(uint8_t* tile, bool is_v, int tau, int
 
 // Blocks: tokens along x; along y, parts of a token's heads (each takes every gridDim.y-th of the groups of kHeads heads).
 template <typename T, int D, bool NEIGHBOURS>
-__global__ void __launch_bounds__(kThreads, 12) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, 16) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kLanes = D / 8;
   constexpr int kHeads = kThreads / kLanes;
   __shared__ float2 turned[8][kMaxPairs / 8];  // cosine, sine of pair 8 j + i at [i][j]
@@ -206,11 +206,9 @@ __global__ void __launch_bounds__(kThreads, 12) qk_rope_kernel(const __grid_cons
   const int token = blockIdx.x;
   const int l = threadIdx.x % kLanes;
   const int step = kHeads * gridDim.y, head0 = blockIdx.y * kHeads + threadIdx.x / kLanes;
-  Eight<T> ahead[kAhead];
+  Eight<T> ahead;  // the next head
   const T* src = static_cast<const T*>(a.q) + token * a.q_stride + 8 * l;
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i)
-    if (head0 + i * step < a.q_heads) ahead[i].load(src + (head0 + i * step) * D);
+  if (head0 < a.q_heads) ahead.load(src + head0 * D);
   for (int i = threadIdx.x; i < a.half_pairs; i += kThreads) {
     int axis = 0;
 #pragma unroll
@@ -265,49 +263,42 @@ __global__ void __launch_bounds__(kThreads, 12) qk_rope_kernel(const __grid_cons
     }
     if (kind) {
       src = static_cast<const T*>(a.k) + token * a.k_stride + 8 * l;
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i)
-        if (head0 + i * step < count) ahead[i].load(src + (head0 + i * step) * D);
+      if (head0 < count) ahead.load(src + head0 * D);
     }
     T* const out = kind ? static_cast<T*>(a.k_out) : static_cast<T*>(a.q_out);
     T* const dst = out == nullptr ? nullptr : out + token * (kind ? a.k_out_stride : a.q_out_stride) + 8 * l;
 #pragma unroll 1
-    for (int base = head0; base < count; base += kAhead * step) {
+    for (int h = head0; h < count; h += step) {
+      Eight<T> e = ahead;
+      if (h + step < count) ahead.load(src + (h + step) * D);
+      float x[8], y[8];
+      e.get(x);
+      float r = 1.0f;
+      if (w != nullptr) {
+        float2 two = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int i = 0; i < kAhead; ++i) {
-        const int h = base + i * step;
-        if (h >= count) break;
-        Eight<T> e = ahead[i];
-        if (h + kAhead * step < count) ahead[i].load(src + (h + kAhead * step) * D);
-        float x[8], y[8];
-        e.get(x);
-        float r = 1.0f;
-        if (w != nullptr) {
-          float2 two = make_float2(0.0f, 0.0f);
+        for (int c = 0; c < 8; c += 2) two = fma2(pair(x, c), pair(x, c), two);
+        float sum = two.x + two.y;
 #pragma unroll
-          for (int c = 0; c < 8; c += 2) two = fma2(pair(x, c), pair(x, c), two);
-          float sum = two.x + two.y;
-#pragma unroll
-          for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-          r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
-        }
-        if (NEIGHBOURS) {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) y[c] = x[c ^ 1];
-        } else {
-          e.from(mask, from).get(y);
-        }
-#pragma unroll
-        for (int c = 0; c < 8; c += 2) {
-          const float2 z = mul2(make_float2(r, r), fma2(pair(x, c), pair(mine, c), mul2(pair(y, c), pair(other, c))));
-          x[c] = z.x;
-          x[c + 1] = z.y;
-        }
-        e.put(x);
-        if (dst != nullptr) e.store(dst + h * D);
-        if (kind && a.pool != nullptr)
-          put_eight<D>(tile0 + static_cast<long long>(h) * page_tiles * kv4::tile_bytes(D), false, in_page % kv4::kTile, l, e.halves(), mask, slot >= 0);
+        for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+        r = rsqrtf(fmaf(sum, 1.0f / D, a.eps));
       }
+      if (NEIGHBOURS) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) y[c] = x[c ^ 1];
+      } else {
+        e.from(mask, from).get(y);
+      }
+#pragma unroll
+      for (int c = 0; c < 8; c += 2) {
+        const float2 z = mul2(make_float2(r, r), fma2(pair(x, c), pair(mine, c), mul2(pair(y, c), pair(other, c))));
+        x[c] = z.x;
+        x[c + 1] = z.y;
+      }
+      e.put(x);
+      if (dst != nullptr) e.store(dst + h * D);
+      if (kind && a.pool != nullptr)
+        put_eight<D>(tile0 + static_cast<long long>(h) * page_tiles * kv4::tile_bytes(D), false, in_page % kv4::kTile, l, e.halves(), mask, slot >= 0);
     }
   }
   src = static_cast<const T*>(a.v) + token * a.v_stride + 8 * l;
