@@ -5,10 +5,13 @@
 // What bounds it is reading the cache once: 18 D / 16 bytes per token and head (144 for D = 128, 3.6 times fewer than fp16).
 // The queries of all heads that share a key/value head, and of all new tokens of a sequence, are the columns of the products,
 // so a code is unpacked once for all of them:
-//   S^T[token][row] = K q:  A = codes of K made (u - 8) 2^-9 in fp16 (exact, and without the cancellation that sums of u would
-//     have), a 32-value group at a time, so that the group's scale multiplies an fp32 sum.
-//   O^T[value][row] = V^T P: the scales of V, which belong to tokens and groups, go into P before it is rounded to fp16, a P
-//     per group.  S^T's accumulator layout becomes P's operand layout by an 8x8 transposition in registers (movmatrix).
+//   S^T[token][row] = K q:  A = codes of K as they lie, masked into fp16 subnormals u 2^-24 (and 16 u 2^-24 for the odd nibbles,
+//     whose q is divided by 16), a 32-value group at a time, so that the group's scale multiplies an fp32 sum; -8 sum(q) is added
+//     to it.  A row of q is scaled by a power of two that leaves its largest value near 2^10, so that a sixteenth of any value
+//     that counts is a normal number.
+//   O^T[value][row] = V^T P: A = codes of V made (u - 8) 2^-9 by a mask and a multiply-add, exactly (sums of P u minus 8 sums of P
+//     would lose what a token of great weight leaves to the others where its own value is zero); the scales of V, which belong to
+//     tokens and groups, go into P before it is rounded to fp16, a P per group.  S^T's accumulator layout becomes P's operand layout by an 8x8 transposition in registers (movmatrix).
 // P's range: 2^top is a row's reference weight and 2^e no smaller than any scale of V so far; weights are taken as
 // 2^(s - top - e + 13), so that weight times scale stays below 2^15 and is a normal number down to 2^-27 of the largest, whatever
 // the values' magnitude.  top and e move only when a step exceeds them (top by 2^2); sums are kept per lane until the end.
@@ -58,8 +61,9 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
 __device__ __forceinline__ float2 unpack_half2(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
 
 // (u - 8) 2^-9 of the codes in bits 0..3 (lo), 4..7 (hi) of both halves: what the mask leaves is an fp16 subnormal, u 2^-24 or
-// u 2^-20, which one fused multiply-add turns into that, exactly.  One mask and one multiply-add per pair of codes is what bounds
-// the kernel's arithmetic.
+// u 2^-20, which one fused multiply-add turns into that, exactly.  Masks, shifts and these multiply-adds share a pipe that takes one
+// in two cycles, which is what bounds the kernel's arithmetic: 64 masks, 24 shifts and permutations and 32 multiply-adds to 16
+// tokens of 128 values.
 constexpr float kCodeUnit = 512.0f;
 __device__ __forceinline__ uint32_t fma_half2(uint32_t x, float scale, float offset) {
   const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(scale), __float2half2_rn(offset));
@@ -153,12 +157,14 @@ struct Rows {
   float o[S::kGroups][2][NT][4];
   float top[NT][2], sum[NT][2];
   float minus_ref[NT][2];  // -(top + e - kLift)
-  float limit[NT][2];      // scores that may not be exceeded: (top + kHeadroom) / scale
+  float limit[NT][2];      // scores that may not be exceeded: (top + kHeadroom) / cs
+  float cs[NT][2];         // log2(e) times the scale of the scores, as the products give them
+  float q8[S::kGroups][NT][2];  // -8 sum(q) of a group, in the codes' units
   uint32_t scale_limit;    // largest scale of V, as the bits of fp16, that e covers
   float e;
   uint32_t q[S::kGroups][NT][4];
 
-  __device__ __forceinline__ void clear(float inv_scale) {
+  __device__ __forceinline__ void clear() {
     scale_limit = 0;
     e = -14.0f;
 #pragma unroll
@@ -171,7 +177,7 @@ struct Rows {
       for (int c = 0; c < 2; ++c) {
         top[i][c] = kFloor;
         minus_ref[i][c] = -kFloor;
-        limit[i][c] = kFloor * inv_scale;
+        limit[i][c] = kFloor / cs[i][c];
         sum[i][c] = 0.0f;
       }
     }
@@ -188,6 +194,7 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Place& p, con
     const bool there = row < p.s.m * a.group;
     const int token = row / a.group, head = p.h * a.group + row - token * a.group;
     const __half* src = a.q + (p.s.first_row_token + token) * a.q_stride + static_cast<long long>(head) * D + 8 * at.t;
+    uint32_t most = 0;
 #pragma unroll
     for (int j = 0; j < S::kGroups; ++j) {
       uint4 v = make_uint4(0, 0, 0, 0);
@@ -196,7 +203,37 @@ __device__ __forceinline__ void load_q(const Kv4AttnArgs& a, const Place& p, con
       w.q[j][i][1] = v.y;
       w.q[j][i][2] = v.z;
       w.q[j][i][3] = v.w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = __vmaxu2(most, w.q[j][i][e] & 0x7FFF7FFFu);
     }
+    most = max(most & 0xFFFFu, most >> 16);
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+    most = max(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+    const int exponent = static_cast<int>(most >> 10);              // 31: an infinity or a NaN, which stays what it is
+    const int up = exponent == 31 ? 0 : 25 - exponent;              // 2^10 for the largest
+    const float by = __int_as_float((127 + up) << 23);
+#pragma unroll
+    for (int j = 0; j < S::kGroups; ++j) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 f = unpack_half2(w.q[j][i][e]);
+        f.x *= by;
+        f.y *= by;
+        sum += f.x + f.y;
+        const float odd = e & 1 ? 0.0625f : 1.0f;
+        w.q[j][i][e] = pack_half2(f.x * odd, f.y * odd);
+      }
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+      sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+      // this lane's columns of the accumulators are rows 2 t and 2 t + 1
+      const float unit = -8.0f / 16777216.0f;
+      w.q8[j][i][0] = unit * __shfl_sync(0xFFFFFFFFu, sum, 8 * at.t);
+      w.q8[j][i][1] = unit * __shfl_sync(0xFFFFFFFFu, sum, 8 * at.t + 4);
+    }
+    const float cs = a.scale_log2 * 16777216.0f * __int_as_float((127 - up) << 23);
+    w.cs[i][0] = __shfl_sync(0xFFFFFFFFu, cs, 8 * at.t);
+    w.cs[i][1] = __shfl_sync(0xFFFFFFFFu, cs, 8 * at.t + 4);
   }
 }
 
@@ -219,13 +256,15 @@ __device__ __forceinline__ void tile_scores(const uint8_t* tile, const LaneAt<D>
       const float2 f0 = unpack_half2(sc0[v >> 1]), f1 = unpack_half2(sc1[v >> 1]);
       const float s0 = v & 1 ? f0.y : f0.x, s1 = v & 1 ? f1.y : f1.x;
       const uint32_t x0 = k0[v], x1 = k1[v], y0 = x0 >> 8, y1 = x1 >> 8;
-      const uint32_t a0 = code_lo(x0), a1 = code_lo(x1), a2 = code_hi(x0), a3 = code_hi(x1);
-      const uint32_t b0 = code_lo(y0), b1 = code_lo(y1), b2 = code_hi(y0), b3 = code_hi(y1);
+      const uint32_t a0 = x0 & 0x000F000Fu, a1 = x1 & 0x000F000Fu, a2 = x0 & 0x00F000F0u, a3 = x1 & 0x00F000F0u;
+      const uint32_t b0 = y0 & 0x000F000Fu, b1 = y1 & 0x000F000Fu, b2 = y0 & 0x00F000F0u, b3 = y1 & 0x00F000F0u;
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         mma16816(c, a0, a1, a2, a3, w.q[j][i][0], w.q[j][i][1]);
         mma16816(c, b0, b1, b2, b3, w.q[j][i][2], w.q[j][i][3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[e] += w.q8[j][i][e & 1];
         if (j == 0) {
           s[i][0] = s0 * c[0];
           s[i][1] = s0 * c[1];
@@ -278,8 +317,7 @@ __device__ __forceinline__ void tile_values(const uint8_t* tile, const LaneAt<D>
 // 16 * TILES tokens.  last[i][c]: the last token of them that the lane's row sees, first[i][c]: the first, exists: how many
 // there are; MASKED: some token is hidden from some row or does not exist.
 template <int D, int NT, int TILES, bool MASKED>
-__device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, float cs, float inv_cs, Rows<D, NT>& w,
-                                     const int (&last)[NT][2], const int (&first)[NT][2], int exists) {
+__device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, Rows<D, NT>& w, const int (&last)[NT][2], const int (&first)[NT][2], int exists) {
   using S = Shape<D, NT>;
   constexpr int kG = S::kGroups;
   float s[TILES][NT][4];
@@ -340,11 +378,11 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
         m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
         m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
         m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-        w.top[i][c] = fmaxf(w.top[i][c], m * cs);
+        w.top[i][c] = fmaxf(w.top[i][c], m * w.cs[i][c]);
         const float ref = w.top[i][c] > kFloor ? w.top[i][c] + w.e - kLift : kFloor;
         const float f = exp2_fast(-w.minus_ref[i][c] - ref);
         w.minus_ref[i][c] = -ref;
-        w.limit[i][c] = w.top[i][c] > kFloor ? (w.top[i][c] + kHeadroom) * inv_cs : kFloor * inv_cs;
+        w.limit[i][c] = (w.top[i][c] > kFloor ? w.top[i][c] + kHeadroom : kFloor) / w.cs[i][c];
         w.sum[i][c] *= f;
 #pragma unroll
         for (int j = 0; j < kG; ++j) {
@@ -363,7 +401,7 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
     for (int i = 0; i < NT; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[k][i][e] = exp2_fast(fmaf(s[k][i][e], cs, w.minus_ref[i][e & 1]));
+        s[k][i][e] = exp2_fast(fmaf(s[k][i][e], w.cs[i][e & 1], w.minus_ref[i][e & 1]));
         w.sum[i][e & 1] += s[k][i][e];
       }
     tile_values<D, NT, MASKED>(tiles + k * S::kTileBytes, at, w, s[k], v0[k], v1[k]);
@@ -375,19 +413,28 @@ __device__ __forceinline__ void put4(__half* p, float a, float b, float c, float
   *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(a, b), pack_half2(c, d));
 }
 
+// What joining the parts of a segment has to know of it.
+struct Segment {
+  int start, end;               // as items; start < 0: no part here
+  int h, r, rows, first_token;  // key/value head, block of rows, rows of the sequence, its first row in q
+};
+template <int D, int NT>
+__device__ __forceinline__ Segment segment_of(const Kv4AttnArgs& a, const Place& p) {
+  return {p.start, p.end, p.h, p.r, p.s.m * a.group, p.s.first_row_token};
+}
 // Row `row` of a block in the output tensor; null beyond the sequence's rows.
 template <int D, int NT>
-__device__ __forceinline__ __half* out_row(const Kv4AttnArgs& a, const Place& p, int row) {
+__device__ __forceinline__ __half* out_row(const Kv4AttnArgs& a, const Segment& p, int row) {
   row += p.r * Shape<D, NT>::kRows;
-  if (row >= p.s.m * a.group) return nullptr;
+  if (row >= p.rows) return nullptr;
   const int token = row / a.group, head = p.h * a.group + row - token * a.group;
-  return a.out + (p.s.first_row_token + token) * a.out_stride + static_cast<long long>(head) * D;
+  return a.out + (p.first_token + token) * a.out_stride + static_cast<long long>(head) * D;
 }
 
 // Ends a warp's part of a segment: `slot` null: it is the whole segment, the rows are written out; else the values as they
 // are, the references and the sums go to the slot.
 template <int D, int NT>
-__device__ __forceinline__ void finish(const Kv4AttnArgs& a, const Place& p, const LaneAt<D>& at, Rows<D, NT>& w, float* slot) {
+__device__ __forceinline__ void finish(const Kv4AttnArgs& a, const Segment& p, const LaneAt<D>& at, Rows<D, NT>& w, float* slot) {
   using S = Shape<D, NT>;
   const int g = at.g, t = at.t;
 #pragma unroll
@@ -422,7 +469,8 @@ __device__ __forceinline__ void finish(const Kv4AttnArgs& a, const Place& p, con
 }
 
 // Sum over `count` records of one row (at `first`, then at `rest` and every `step` floats behind it), a warp together: lane l
-// gets values l VALUES.. of the row, not yet divided by `sum`.
+// gets values l VALUES.. of the row, not yet divided by `sum`.  Records are asked for several at a time; a trip to L2 is what
+// joining costs.
 template <int D>
 struct Joined {
   static constexpr int kValues = D / 32;
@@ -432,41 +480,55 @@ struct Joined {
 template <int D, bool GLOBAL>
 __device__ __forceinline__ Joined<D> join(const float* first, const float* rest, int step, int count, int lane) {
   Joined<D> r;
-  constexpr int kV = Joined<D>::kValues;
-  const auto record = [&](int i) { return i == 0 ? first : rest + static_cast<long long>(i - 1) * step; };
-  float top = kFloor;
-  for (int i = lane; i < count; i += 32) top = fmaxf(top, GLOBAL ? __ldcg(record(i) + D) : record(i)[D]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
-  r.top = top;
+  constexpr int kV = Joined<D>::kValues, kAtOnce = GLOBAL ? (D == 256 ? 4 : 8) : 2;
+  r.top = kFloor;
   r.sum = 0.0f;
 #pragma unroll
   for (int e = 0; e < kV; ++e) r.x[e] = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < count; ++i) {
-    const float* p = record(i);
-    float x[kV];
-    const float2* ml = reinterpret_cast<const float2*>(p + D);
-    const float2 m = GLOBAL ? __ldcg(ml) : *ml;
-    if constexpr (kV == 2) {
-      const float2 v = GLOBAL ? __ldcg(reinterpret_cast<const float2*>(p) + lane) : reinterpret_cast<const float2*>(p)[lane];
-      x[0] = v.x;
-      x[1] = v.y;
-    } else {
+#pragma unroll 1
+  for (int i0 = 0; i0 < count; i0 += kAtOnce) {
+    float x[kAtOnce][kV];
+    float2 m[kAtOnce];
 #pragma unroll
-      for (int e = 0; e < kV; e += 4) {
-        const float4* at = reinterpret_cast<const float4*>(p) + lane * (kV / 4) + e / 4;
-        const float4 v = GLOBAL ? __ldcg(at) : *at;
-        x[e] = v.x;
-        x[e + 1] = v.y;
-        x[e + 2] = v.z;
-        x[e + 3] = v.w;
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int n = min(i0 + i, count - 1);
+      const float* p = n == 0 ? first : rest + static_cast<long long>(n - 1) * step;
+      const float2* ml = reinterpret_cast<const float2*>(p + D);
+      m[i] = GLOBAL ? __ldcg(ml) : *ml;
+      if (i0 + i >= count) m[i] = make_float2(kFloor, 0.0f);
+      if constexpr (kV == 2) {
+        const float2* at = reinterpret_cast<const float2*>(p) + lane;
+        const float2 v = GLOBAL ? __ldcg(at) : *at;
+        x[i][0] = v.x;
+        x[i][1] = v.y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < kV; e += 4) {
+          const float4* at = reinterpret_cast<const float4*>(p) + lane * (kV / 4) + e / 4;
+          const float4 v = GLOBAL ? __ldcg(at) : *at;
+          x[i][e] = v.x;
+          x[i][e + 1] = v.y;
+          x[i][e + 2] = v.z;
+          x[i][e + 3] = v.w;
+        }
       }
     }
-    const float f = exp2_fast(m.x - top);
-    r.sum = fmaf(m.y, f, r.sum);
+    float top = r.top;
 #pragma unroll
-    for (int e = 0; e < kV; ++e) r.x[e] = fmaf(x[e], f, r.x[e]);
+    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, m[i].x);
+    float f = exp2_fast(r.top - top);
+    r.top = top;
+    r.sum *= f;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) r.x[e] *= f;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (i0 + i >= count) break;
+      f = exp2_fast(m[i].x - top);
+      r.sum = fmaf(m[i].y, f, r.sum);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) r.x[e] = fmaf(x[i][e], f, r.x[e]);
+    }
   }
   return r;
 }
@@ -515,8 +577,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   uint8_t* const ring_all = smem;                                                                 // [WARPS][kStages][kStageBytes]
   float* const slots = reinterpret_cast<float*>(smem + WARPS * S::kStages * S::kStageBytes);      // [WARPS][kRows][kRecord]
   uint64_t* const bars_all = reinterpret_cast<uint64_t*>(slots + WARPS * S::kRows * S::kRecord);  // [WARPS][kStages]
-  int* const segs = reinterpret_cast<int*>(bars_all + WARPS * S::kStages);                        // [WARPS][2]: segments of the slots
-  int* const prefix = segs + 2 * WARPS;                                                           // [batch]
+  Segment* const segs = reinterpret_cast<Segment*>(bars_all + WARPS * S::kStages);                // [WARPS][2]: segments of the slots
+  int* const prefix = reinterpret_cast<int*>(segs + 2 * WARPS);                                   // [batch]
   __shared__ int warp_items[WARPS], warp_segs[WARPS];
   __shared__ int is_last[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -526,7 +588,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
 #pragma unroll
     for (int i = 0; i < S::kStages; ++i) mbar_init(bars + i, 1);
     fence_barrier_init();
-    segs[2 * warp] = segs[2 * warp + 1] = -1;
+    segs[2 * warp].start = segs[2 * warp + 1].start = -1;
   }
   pdl_wait();
   // ---- how many items lie ahead of each sequence
@@ -590,33 +652,47 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   if (wlo < whi) {
     Place pi;  // where copies are asked for
     pi.end = wlo;
-    int ii = wlo, pid = 0;
+    int ii = wlo, window = 0, run = 0;
+    const uint8_t* src = nullptr;
     const LaneAt<D> at(lane);
-    const float cs = a.scale_log2 * kCodeUnit, inv_scale = 1.0f / cs;  // scores come in units of the codes
-    // Lane l of the first kTiles brings tile l of a chunk: its page's number is asked for one chunk ahead.
-    const auto next_page = [&]() {
-      if (ii == pi.end) pi = locate<D, NT>(a, prefix, ii); else ++pi.c;
-      const int tile = (pi.s.c0 + pi.c) * S::kTiles + lane;
-      pid = 0;
-      if (lane < S::kTiles && tile * kv4::kTile < pi.s.n) pid = __ldg(a.table + static_cast<long long>(pi.b) * a.max_pages + tile / a.page_tiles);
+    // Lane l looks up every 32nd tile of a segment and brings it when its chunk's turn comes, with the tiles of the chunk behind it
+    // that lie in the same page.
+    const auto look_up = [&]() {
+      window = (pi.s.c0 + pi.c) * S::kTiles;
+      const int tile = window + lane, tiles = (pi.s.n + kv4::kTile - 1) / kv4::kTile;
+      run = 0;
+      if (tile < tiles) {
+        const int page = tile / a.page_tiles, in_page = tile - page * a.page_tiles, in_chunk = lane % S::kTiles;
+        if (in_page == 0 || in_chunk == 0) {
+          int pid = __ldg(a.table + static_cast<long long>(pi.b) * a.max_pages + page);
+          if (pid < 0 || pid >= a.pages) {
+            atomicExch(a.error, kErrPage);
+            pid = 0;
+          }
+          run = min(min(a.page_tiles - in_page, S::kTiles - in_chunk), tiles - tile);
+          src = a.pool + ((static_cast<long long>(pid) * a.kv_heads + pi.h) * a.page_tiles + in_page) * S::kTileBytes;
+        }
+      }
+    };
+    const auto next = [&]() {
+      if (ii == pi.end) {
+        pi = locate<D, NT>(a, prefix, ii);
+        look_up();
+      } else {
+        ++pi.c;
+        if ((pi.s.c0 + pi.c) * S::kTiles == window + 32) look_up();
+      }
     };
     const auto ask = [&](int stage) {
-      const int tile0 = (pi.s.c0 + pi.c) * S::kTiles;
+      const int tile0 = (pi.s.c0 + pi.c) * S::kTiles, first = tile0 - window;
       const int there = min(S::kTiles, max(0, (pi.s.n + kv4::kTile - 1) / kv4::kTile - tile0));
       if (lane == 0) mbar_arrive_expect_tx(bars + stage, there * S::kTileBytes);
       __syncwarp();
-      if (lane < there) {
-        const int tile = tile0 + lane;
-        if (pid < 0 || pid >= a.pages) {
-          atomicExch(a.error, kErrPage);
-          pid = 0;
-        }
-        const uint8_t* src = a.pool + ((static_cast<long long>(pid) * a.kv_heads + pi.h) * a.page_tiles + tile % a.page_tiles) * S::kTileBytes;
-        bulk_load_1d(ring + stage * S::kStageBytes + lane * S::kTileBytes, src, S::kTileBytes, bars + stage);
-      }
-      if (++ii < whi) next_page();
+      if (run > 0 && lane >= first && lane < first + S::kTiles)
+        bulk_load_1d(ring + stage * S::kStageBytes + (lane - first) * S::kTileBytes, src, run * S::kTileBytes, bars + stage);
+      if (++ii < whi) next();
     };
-    next_page();
+    next();
 #pragma unroll 1
     for (int s = 0; s < S::kStages && ii < whi; ++s) ask(s);
 
@@ -629,7 +705,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       const Place p = locate<D, NT>(a, prefix, item);
       const int end = min(p.end, whi);
       load_q<D, NT>(a, p, at, w);
-      w.clear(inv_scale);
+      w.clear();
       // the last token that each of the lane's rows sees
       int sees[NT][2];
 #pragma unroll
@@ -667,7 +743,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
           int none[NT][2];
 #pragma unroll
           for (int k = 0; k < S::kTiles; k += S::kStep)
-            step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, cs, inv_scale, w, none, none, 0);
+            step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, none, none, 0);
           release();
         }
         if (item >= end) break;
@@ -684,7 +760,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
               last[i][c] = sees[i][c] - from;
               first[i][c] = a.window > 0 ? sees[i][c] - a.window + 1 - from : 0;
             }
-          step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, cs, inv_scale, w, last, first,
+          step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, last, first,
                                       p.s.n - from);
         }
         release();
@@ -692,12 +768,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       // a segment that ends here and began here is done; else its part goes to the warp's slot: the ring's place for one that
       // began here (nothing is asked for any more), a place of its own for one that began before
       if (p.start >= wlo && p.end <= whi) {
-        finish<D, NT>(a, p, at, w, nullptr);
+        finish<D, NT>(a, segment_of<D, NT>(a, p), at, w, nullptr);
       } else {
         const int which = p.start >= wlo ? 1 : 0;
         float* slot = which ? reinterpret_cast<float*>(ring) : slots + warp * S::kRows * S::kRecord;
-        finish<D, NT>(a, p, at, w, slot);
-        if (lane == 0) segs[2 * warp + which] = p.start;
+        const Segment seg = segment_of<D, NT>(a, p);
+        finish<D, NT>(a, seg, at, w, slot);
+        if (lane == 0) segs[2 * warp + which] = seg;
       }
     }
     if (!alive && lane == 0) {
@@ -709,27 +786,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   __syncthreads();
 
   // ---- segments that warps share: tasks (run of slots of one segment, row), one to a warp
-  int began_before = -1, begins_here = -1;  // the CTA's segments that other CTAs share
-  Place shared_place[2];
+  int shared[2] = {-1, -1};  // slots of the CTA's segments that other CTAs share: [0] began before, [1] begins here
   {
     int task = 0;
 #pragma unroll 1
     for (int i = 0; i < 2 * WARPS; ++i) {
-      const int seg = segs[i];
-      if (seg < 0) continue;
+      const Segment p = segs[i];
+      if (p.start < 0) continue;
       // the slots of this segment: this one, then the [0] slots of the following warps
       int parts = 1;
-      for (int k = (i / 2 + 1) * 2; k < 2 * WARPS && segs[k] == seg; k += 2) ++parts;
-      const Place p = locate<D, NT>(a, prefix, seg);
+      for (int k = (i / 2 + 1) * 2; k < 2 * WARPS && segs[k].start == p.start; k += 2) ++parts;
       const bool whole = p.start >= lo && p.end <= hi;
       const int which = p.start >= lo ? 1 : 0;
       if (!whole) {
-        (which ? begins_here : began_before) = seg;
-        shared_place[which] = p;
+        if (which) shared[1] = i; else shared[0] = i;
       }
 #pragma unroll 1
-      for (int row = 0; row < S::kRows; ++row, ++task) {
-        if (task % WARPS != warp) continue;
+      for (int row = (warp - task % WARPS + WARPS) % WARPS; row < S::kRows; row += WARPS) {
         // the first part may lie in a ring, the others are in the slots, one after the other
         const float* first = (i & 1 ? reinterpret_cast<const float*>(ring_all + (i / 2) * S::kStages * S::kStageBytes)
                                     : slots + (i / 2) * S::kRows * S::kRecord) + row * S::kRecord;
@@ -741,19 +814,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
           put_record<D>(a.part + ((static_cast<long long>(cta) * 2 + which) * S::kRows + row) * S::kRecord, r, lane);
         }
       }
+      task += S::kRows;
       i += 2 * parts - 2 - (parts > 1 ? i & 1 : 0);  // on to the last of its slots
     }
   }
-  if (began_before < 0 && begins_here < 0) return;
+  if (shared[0] < 0 && shared[1] < 0) return;
 
   // ---- segments that CTAs share: the last of them joins
   __threadfence();
   __syncthreads();
   if (threadIdx.x < 2) {
-    const int seg = threadIdx.x ? begins_here : began_before;
+    const int slot = threadIdx.x ? shared[1] : shared[0];
     int last = 0;
-    if (seg >= 0) {
-      const int c0 = shares.holder(shared_place[threadIdx.x].start), c1 = shares.holder(shared_place[threadIdx.x].end - 1);
+    if (slot >= 0) {
+      const int c0 = shares.holder(segs[slot].start), c1 = shares.holder(segs[slot].end - 1);
       const int parts = c1 - c0 + 1;
       if (atomicAdd(a.tickets + c0, 1) == parts - 1) {
         a.tickets[c0] = 0;
@@ -768,9 +842,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     if (is_last[which] == 0) continue;
     __threadfence();
     const int parts = is_last[which] >> 10, c0 = (is_last[which] & 1023) - 1;
+    const Segment p = segs[which ? shared[1] : shared[0]];
 #pragma unroll 1
     for (int row = warp; row < S::kRows; row += WARPS) {
-      __half* dst = out_row<D, NT>(a, shared_place[which], row);
+      __half* dst = out_row<D, NT>(a, p, row);
       if (dst == nullptr) continue;
       // the first part is a [1] record, the others are [0] records of the CTAs behind it
       const float* first = a.part + (static_cast<long long>(c0) * 2 + 1) * S::kRows * S::kRecord + row * S::kRecord;
@@ -782,7 +857,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
 template <int D, int NT, int WARPS>
 size_t attn_smem(int batch) {
   using S = Shape<D, NT>;
-  return static_cast<size_t>(WARPS) * (S::kStages * S::kStageBytes + S::kSlotBytes + 8 * S::kStages + 8) + 4 * static_cast<size_t>(batch);
+  return static_cast<size_t>(WARPS) * (S::kStages * S::kStageBytes + S::kSlotBytes + 8 * S::kStages + 2 * sizeof(Segment)) + 4 * static_cast<size_t>(batch);
 }
 
 template <int D, int NT, int WARPS>
