@@ -282,9 +282,9 @@ __device__ __forceinline__ void tile_scores(const uint8_t* tile, const LaneAt<D>
 }
 
 // Adds P V of 16 tokens; p: weights in the layout of the scores, v0, v1: scales of V of the tokens g and g + 8.
-template <int D, int NT, bool MASKED>
+template <int D, int NT>
 __device__ __forceinline__ void tile_values(const uint8_t* tile, const LaneAt<D>& at, Rows<D, NT>& w, const float (&p)[NT][4],
-                                            const uint32_t (&v0)[D / 64], const uint32_t (&v1)[D / 64]) {
+                                            const uint32_t (&v0)[D / 64], const uint32_t (&v1)[D / 64], bool wild) {
   constexpr int kG = D / 32;
   uint32_t va[kG / 2], vb[kG / 2], vc[kG / 2], vd[kG / 2];  // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
   kv4_lds(tile + at.v, va);
@@ -303,7 +303,7 @@ __device__ __forceinline__ void tile_values(const uint8_t* tile, const LaneAt<D>
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       float z[4] = {p[i][0] * s0, p[i][1] * s0, p[i][2] * s1, p[i][3] * s1};
-      if (MASKED) {  // a scale that a row does not see may be infinite or NaN
+      if (wild) {  // a scale is NaN: the rows that do not see it keep out of it
 #pragma unroll
         for (int c = 0; c < 4; ++c) z[c] = p[i][c] == 0.0f ? 0.0f : z[c];
       }
@@ -314,10 +314,11 @@ __device__ __forceinline__ void tile_values(const uint8_t* tile, const LaneAt<D>
   }
 }
 
-// 16 * TILES tokens.  last[i][c]: the last token of them that the lane's row sees, first[i][c]: the first, exists: how many
-// there are; MASKED: some token is hidden from some row or does not exist.
+// 16 * TILES tokens, the first of them `from`.  sees[i][c]: the last token that the lane's row sees; MASKED: some token is hidden
+// from some row or does not exist.
 template <int D, int NT, int TILES, bool MASKED>
-__device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, Rows<D, NT>& w, const int (&last)[NT][2], const int (&first)[NT][2], int exists) {
+__device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, Rows<D, NT>& w, const int (&sees)[NT][2], int window,
+                                     int from, int n) {
   using S = Shape<D, NT>;
   constexpr int kG = S::kGroups;
   float s[TILES][NT][4];
@@ -331,18 +332,18 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
   if (MASKED) {
 #pragma unroll
     for (int k = 0; k < TILES; ++k) {
-      const int g = at.g + 16 * k;
+      const int token = from + 16 * k + at.g;
 #pragma unroll
       for (int e = 0; e < kG / 2; ++e) {  // what lies behind the last token is anything
-        if (g >= exists) v0[k][e] = 0;
-        if (g + 8 >= exists) v1[k][e] = 0;
+        if (token >= n) v0[k][e] = 0;
+        if (token + 8 >= n) v1[k][e] = 0;
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int tok = g + (e < 2 ? 0 : 8);
-          if (tok > last[i][e & 1] || tok < first[i][e & 1]) s[k][i][e] = -INFINITY;
+          const int t = token + (e < 2 ? 0 : 8), last = sees[i][e & 1];
+          if (t > last || (window > 0 && t <= last - window)) s[k][i][e] = -INFINITY;
         }
     }
   }
@@ -354,7 +355,8 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
 #pragma unroll
     for (int e = 0; e < kG / 2; ++e) most = __vmaxu2(most, __vmaxu2(v0[k][e], v1[k][e]));
   most = max(most & 0xFFFFu, most >> 16);
-  over = most > w.scale_limit;
+  bool wild = false;
+  over = most > w.scale_limit || most >= 0x7C00u;
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -366,6 +368,7 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
     }
   if (__any_sync(0xFFFFFFFFu, over)) {
     most = __reduce_max_sync(0xFFFFFFFFu, most);
+    wild = most >= 0x7C00u;
     if (most > w.scale_limit) {
       w.scale_limit = most | 0x3FFu;  // the end of its binade
       w.e = static_cast<float>(static_cast<int>(most >> 10) - 14);
@@ -404,7 +407,7 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
         s[k][i][e] = exp2_fast(fmaf(s[k][i][e], w.cs[i][e & 1], w.minus_ref[i][e & 1]));
         w.sum[i][e & 1] += s[k][i][e];
       }
-    tile_values<D, NT, MASKED>(tiles + k * S::kTileBytes, at, w, s[k], v0[k], v1[k]);
+    tile_values<D, NT>(tiles + k * S::kTileBytes, at, w, s[k], v0[k], v1[k], wild);
   }
 }
 
@@ -468,68 +471,50 @@ __device__ __forceinline__ void finish(const Kv4AttnArgs& a, const Segment& p, c
     }
 }
 
-// Sum over `count` records of one row (at `first`, then at `rest` and every `step` floats behind it), a warp together: lane l
-// gets values l VALUES.. of the row, not yet divided by `sum`.  Records are asked for several at a time; a trip to L2 is what
-// joining costs.
+// Adds `count` records of one row in shared memory (at `first`, then at `rest` and every `step` floats behind it), a warp together:
+// lane l has values l VALUES.. of the row, not yet divided by `sum`.
 template <int D>
 struct Joined {
   static constexpr int kValues = D / 32;
   float x[kValues];
   float top, sum;
 };
-template <int D, bool GLOBAL>
-__device__ __forceinline__ Joined<D> join(const float* first, const float* rest, int step, int count, int lane) {
+template <int D>
+__device__ __forceinline__ void join(Joined<D>& r, const float* first, const float* rest, int step, int count, int lane) {
+  constexpr int kV = Joined<D>::kValues;
+#pragma unroll 2
+  for (int i = 0; i < count; ++i) {
+    const float* p = i == 0 ? first : rest + (i - 1) * step;
+    const float2 m = *reinterpret_cast<const float2*>(p + D);
+    float x[kV];
+    if constexpr (kV == 2) {
+      const float2 v = reinterpret_cast<const float2*>(p)[lane];
+      x[0] = v.x;
+      x[1] = v.y;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kV; e += 4) {
+        const float4 v = reinterpret_cast<const float4*>(p)[lane * (kV / 4) + e / 4];
+        x[e] = v.x;
+        x[e + 1] = v.y;
+        x[e + 2] = v.z;
+        x[e + 3] = v.w;
+      }
+    }
+    const float top = fmaxf(r.top, m.x), f = exp2_fast(r.top - top), g = exp2_fast(m.x - top);
+    r.top = top;
+    r.sum = fmaf(m.y, g, r.sum * f);
+#pragma unroll
+    for (int e = 0; e < kV; ++e) r.x[e] = fmaf(x[e], g, r.x[e] * f);
+  }
+}
+template <int D>
+__device__ __forceinline__ Joined<D> nothing_joined() {
   Joined<D> r;
-  constexpr int kV = Joined<D>::kValues, kAtOnce = GLOBAL ? (D == 256 ? 4 : 8) : 2;
   r.top = kFloor;
   r.sum = 0.0f;
 #pragma unroll
-  for (int e = 0; e < kV; ++e) r.x[e] = 0.0f;
-#pragma unroll 1
-  for (int i0 = 0; i0 < count; i0 += kAtOnce) {
-    float x[kAtOnce][kV];
-    float2 m[kAtOnce];
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const int n = min(i0 + i, count - 1);
-      const float* p = n == 0 ? first : rest + static_cast<long long>(n - 1) * step;
-      const float2* ml = reinterpret_cast<const float2*>(p + D);
-      m[i] = GLOBAL ? __ldcg(ml) : *ml;
-      if (i0 + i >= count) m[i] = make_float2(kFloor, 0.0f);
-      if constexpr (kV == 2) {
-        const float2* at = reinterpret_cast<const float2*>(p) + lane;
-        const float2 v = GLOBAL ? __ldcg(at) : *at;
-        x[i][0] = v.x;
-        x[i][1] = v.y;
-      } else {
-#pragma unroll
-        for (int e = 0; e < kV; e += 4) {
-          const float4* at = reinterpret_cast<const float4*>(p) + lane * (kV / 4) + e / 4;
-          const float4 v = GLOBAL ? __ldcg(at) : *at;
-          x[i][e] = v.x;
-          x[i][e + 1] = v.y;
-          x[i][e + 2] = v.z;
-          x[i][e + 3] = v.w;
-        }
-      }
-    }
-    float top = r.top;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) top = fmaxf(top, m[i].x);
-    float f = exp2_fast(r.top - top);
-    r.top = top;
-    r.sum *= f;
-#pragma unroll
-    for (int e = 0; e < kV; ++e) r.x[e] *= f;
-#pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      if (i0 + i >= count) break;
-      f = exp2_fast(m[i].x - top);
-      r.sum = fmaf(m[i].y, f, r.sum);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) r.x[e] = fmaf(x[i][e], f, r.x[e]);
-    }
-  }
+  for (int e = 0; e < Joined<D>::kValues; ++e) r.x[e] = 0.0f;
   return r;
 }
 template <int D>
@@ -581,14 +566,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   int* const prefix = reinterpret_cast<int*>(segs + 2 * WARPS);                                   // [batch]
   __shared__ int warp_items[WARPS], warp_segs[WARPS];
   __shared__ int is_last[2];
+  __shared__ uint64_t join_bar;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* const ring = ring_all + warp * S::kStages * S::kStageBytes;
   uint64_t* const bars = bars_all + warp * S::kStages;
   if (lane == 0) {
 #pragma unroll
     for (int i = 0; i < S::kStages; ++i) mbar_init(bars + i, 1);
-    fence_barrier_init();
     segs[2 * warp].start = segs[2 * warp + 1].start = -1;
+    if (warp == 0) mbar_init(&join_bar, 1);
+    fence_barrier_init();
   }
   pdl_wait();
   // ---- how many items lie ahead of each sequence
@@ -693,89 +680,84 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       if (++ii < whi) next();
     };
     next();
-#pragma unroll 1
-    for (int s = 0; s < S::kStages && ii < whi; ++s) ask(s);
-
     Rows<D, NT> w;
-    int stage = 0, phase = 0;
+    Place p;
+    int stage = 0, phase = 0, asked = 0, sees[NT][2], whole_lo = 0, whole_hi = 0, first_lo = 0, sees_hi = 0, token = 0;
     bool alive = true;
-    int item = wlo;
+    p.end = wlo;
+    const auto ask_ahead = [&](int item) {
 #pragma unroll 1
-    while (item < whi) {
-      const Place p = locate<D, NT>(a, prefix, item);
+      while (alive && ii < whi && ii < item + S::kStages) {
+        ask(asked);
+        if (++asked == S::kStages) asked = 0;
+      }
+    };
+    const auto release = [&]() {
+      __syncwarp();
+      if (++stage == S::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      token += S::kChunk;
+    };
+#pragma unroll 1
+    for (int item = wlo; item < whi;) {
+      ask_ahead(item);
+      if (item == p.end) {
+        p = locate<D, NT>(a, prefix, item);
+        load_q<D, NT>(a, p, at, w);
+        w.clear();
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int row = min(p.r * S::kRows + 8 * i + 2 * at.t + c, p.s.m * a.group - 1);
+            sees[i][c] = p.s.n - p.s.m + row / a.group;
+          }
+        const int sees_lo = p.s.n - p.s.m + p.r * S::kRows / a.group;
+        sees_hi = p.s.n - p.s.m + min(p.r * S::kRows + S::kRows - 1, p.s.m * a.group - 1) / a.group;
+        // chunks that begin in [whole_lo, whole_hi] are seen by all rows; tokens in (first_lo, sees_hi] by any
+        whole_lo = a.window > 0 ? sees_hi - a.window + 1 : 0;
+        whole_hi = sees_lo - S::kChunk + 1;
+        first_lo = a.window > 0 ? sees_lo - a.window + 1 : 0;
+        token = (p.s.c0 + p.c) * S::kChunk;
+      }
       const int end = min(p.end, whi);
-      load_q<D, NT>(a, p, at, w);
-      w.clear();
-      // the last token that each of the lane's rows sees
-      int sees[NT][2];
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int row = min(p.r * S::kRows + 8 * i + 2 * at.t + c, p.s.m * a.group - 1);
-          sees[i][c] = p.s.n - p.s.m + row / a.group;
-        }
-      const int sees_lo = p.s.n - p.s.m + p.r * S::kRows / a.group;
-      const int sees_hi = p.s.n - p.s.m + min(p.r * S::kRows + S::kRows - 1, p.s.m * a.group - 1) / a.group;
-      // chunks that begin in [whole_lo, whole_hi] are seen by all rows; [first_lo, sees_hi] by any
-      const int whole_lo = a.window > 0 ? sees_hi - a.window + 1 : 0, whole_hi = sees_lo - S::kChunk + 1;
-      const int first_lo = a.window > 0 ? sees_lo - a.window + 1 : 0;
-      int token = (p.s.c0 + p.c) * S::kChunk;
-      const auto arrive = [&]() {
-        if (alive) alive = mbar_wait(bars + stage, phase);
-      };
-      const auto release = [&]() {
-        __syncwarp();
-        if (ii < whi && alive) ask(stage);
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
-        ++item;
-        token += S::kChunk;
-      };
-      while (item < end) {
-        // two loops: one for both kinds moves the accumulators between registers where its branches meet
+      // A loop of its own for chunks that all rows see: one for both kinds moves the accumulators between registers where its
+      // branches meet.
 #pragma unroll 1
-        while (item < end && token >= whole_lo && token <= whole_hi) {
-          arrive();
-          if (!alive) break;
-          int none[NT][2];
+      while (item < end && token >= whole_lo && token <= whole_hi) {
+        if (alive) alive = mbar_wait(bars + stage, phase);
+        if (!alive) break;
 #pragma unroll
-          for (int k = 0; k < S::kTiles; k += S::kStep)
-            step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, none, none, 0);
-          release();
-        }
-        if (item >= end) break;
-        arrive();
+        for (int k = 0; k < S::kTiles; k += S::kStep)
+          step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, 0, 0, 0);
+        release();
+        ++item;
+        ask_ahead(item);
+      }
+      if (item < end) {
+        if (alive) alive = mbar_wait(bars + stage, phase);
 #pragma unroll 1
         for (int k = 0; k < S::kTiles; k += S::kStep) {
           const int from = token + k * kv4::kTile;
           if (!alive || from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
-          int last[NT][2], first[NT][2];
-#pragma unroll
-          for (int i = 0; i < NT; ++i)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              last[i][c] = sees[i][c] - from;
-              first[i][c] = a.window > 0 ? sees[i][c] - a.window + 1 - from : 0;
-            }
-          step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, last, first,
-                                      p.s.n - from);
+          step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, a.window, from, p.s.n);
         }
         release();
+        ++item;
       }
+      if (item < p.end && item < whi) continue;
       // a segment that ends here and began here is done; else its part goes to the warp's slot: the ring's place for one that
       // began here (nothing is asked for any more), a place of its own for one that began before
-      if (p.start >= wlo && p.end <= whi) {
-        finish<D, NT>(a, segment_of<D, NT>(a, p), at, w, nullptr);
-      } else {
-        const int which = p.start >= wlo ? 1 : 0;
-        float* slot = which ? reinterpret_cast<float*>(ring) : slots + warp * S::kRows * S::kRecord;
-        const Segment seg = segment_of<D, NT>(a, p);
-        finish<D, NT>(a, seg, at, w, slot);
+      const Segment seg = segment_of<D, NT>(a, p);
+      const int which = p.start >= wlo ? 1 : 0;
+      float* slot = nullptr;
+      if (p.start < wlo || p.end > whi) {
+        slot = which ? reinterpret_cast<float*>(ring) : slots + warp * S::kRows * S::kRecord;
         if (lane == 0) segs[2 * warp + which] = seg;
       }
+      finish<D, NT>(a, seg, at, w, slot);
     }
     if (!alive && lane == 0) {
       atomicExch(a.error, kErrWait);
@@ -785,46 +767,44 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   }
   __syncthreads();
 
-  // ---- segments that warps share: tasks (run of slots of one segment, row), one to a warp
-  int shared[2] = {-1, -1};  // slots of the CTA's segments that other CTAs share: [0] began before, [1] begins here
-  {
-    int task = 0;
+  // ---- segments that warps share: tasks (run of slots of one segment, row) dealt out to the warps
+  // Lane l looks at slot l.  A run begins at a slot whose segment the warp before does not end with, and goes on over the [0] slots
+  // of the following warps.
+  const int my_start = lane < 2 * WARPS ? segs[lane].start : -1, my_end = lane < 2 * WARPS ? segs[lane].end : 0;
+  const int one_before = __shfl_up_sync(0xFFFFFFFFu, my_start, 1), two_before = __shfl_up_sync(0xFFFFFFFFu, my_start, 2);
+  const unsigned slots_used = __ballot_sync(0xFFFFFFFFu, my_start >= 0);
+  const unsigned begins = __ballot_sync(0xFFFFFFFFu, my_start >= 0 && ((lane & 1) || lane < 2 || max(one_before, two_before) != my_start));
+  const unsigned before = __ballot_sync(0xFFFFFFFFu, my_start >= 0 && my_start < lo);
+  const unsigned beyond = __ballot_sync(0xFFFFFFFFu, my_start >= lo && my_end > hi);
+  // the slots of the segments that other CTAs share: [0] began before, [1] begins here
+  const int shared0 = before ? __ffs(before) - 1 : -1, shared1 = beyond ? __ffs(beyond) - 1 : -1;
+  const int runs = __popc(begins);
 #pragma unroll 1
-    for (int i = 0; i < 2 * WARPS; ++i) {
-      const Segment p = segs[i];
-      if (p.start < 0) continue;
-      // the slots of this segment: this one, then the [0] slots of the following warps
-      int parts = 1;
-      for (int k = (i / 2 + 1) * 2; k < 2 * WARPS && segs[k].start == p.start; k += 2) ++parts;
-      const bool whole = p.start >= lo && p.end <= hi;
-      const int which = p.start >= lo ? 1 : 0;
-      if (!whole) {
-        if (which) shared[1] = i; else shared[0] = i;
-      }
-#pragma unroll 1
-      for (int row = (warp - task % WARPS + WARPS) % WARPS; row < S::kRows; row += WARPS) {
-        // the first part may lie in a ring, the others are in the slots, one after the other
-        const float* first = (i & 1 ? reinterpret_cast<const float*>(ring_all + (i / 2) * S::kStages * S::kStageBytes)
-                                    : slots + (i / 2) * S::kRows * S::kRecord) + row * S::kRecord;
-        const Joined<D> r = join<D, false>(first, slots + ((i / 2 + 1) * S::kRows + row) * S::kRecord, S::kRows * S::kRecord, parts, lane);
-        if (whole) {
-          __half* dst = out_row<D, NT>(a, p, row);
-          if (dst != nullptr) put_row<D>(dst, r, lane);
-        } else {
-          put_record<D>(a.part + ((static_cast<long long>(cta) * 2 + which) * S::kRows + row) * S::kRecord, r, lane);
-        }
-      }
-      task += S::kRows;
-      i += 2 * parts - 2 - (parts > 1 ? i & 1 : 0);  // on to the last of its slots
+  for (int task = warp; task < runs * S::kRows; task += WARPS) {
+    const int slot = __fns(begins, 0, task / S::kRows + 1), row = task % S::kRows;
+    const unsigned behind = slot == 31 ? 0u : begins >> (slot + 1) << (slot + 1);
+    const unsigned until = behind ? (1u << (__ffs(behind) - 1)) - 1u : 0xFFFFFFFFu;
+    const int parts = __popc(slots_used & until & ~((1u << slot) - 1u));
+    const Segment p = segs[slot];
+    // the first part may lie in a ring, the others are in the slots, one after the other
+    const float* first = (slot & 1 ? reinterpret_cast<const float*>(ring_all + (slot / 2) * S::kStages * S::kStageBytes)
+                                   : slots + (slot / 2) * S::kRows * S::kRecord) + row * S::kRecord;
+    Joined<D> r = nothing_joined<D>();
+    join<D>(r, first, slots + ((slot / 2 + 1) * S::kRows + row) * S::kRecord, S::kRows * S::kRecord, parts, lane);
+    if (p.start >= lo && p.end <= hi) {
+      __half* dst = out_row<D, NT>(a, p, row);
+      if (dst != nullptr) put_row<D>(dst, r, lane);
+    } else {
+      put_record<D>(a.part + ((static_cast<long long>(cta) * 2 + (p.start >= lo ? 1 : 0)) * S::kRows + row) * S::kRecord, r, lane);
     }
   }
-  if (shared[0] < 0 && shared[1] < 0) return;
+  if (shared0 < 0 && shared1 < 0) return;
 
   // ---- segments that CTAs share: the last of them joins
   __threadfence();
   __syncthreads();
   if (threadIdx.x < 2) {
-    const int slot = threadIdx.x ? shared[1] : shared[0];
+    const int slot = threadIdx.x ? shared1 : shared0;
     int last = 0;
     if (slot >= 0) {
       const int c0 = shares.holder(segs[slot].start), c1 = shares.holder(segs[slot].end - 1);
@@ -837,19 +817,53 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     is_last[threadIdx.x] = last;
   }
   __syncthreads();
+  if (is_last[0] == 0 && is_last[1] == 0) return;
+  // All parts come into the rings' place at once, by bulk copies: they lie far away (a trip takes a microsecond).
+  __threadfence();
+  asm volatile("fence.proxy.async;" ::: "memory");
+  constexpr int kRoom = WARPS * S::kStages * S::kStageBytes / S::kSlotBytes < 32 ? WARPS * S::kStages * S::kStageBytes / S::kSlotBytes : 32;
+  int phase = 0;
 #pragma unroll 1
   for (int which = 0; which < 2; ++which) {
     if (is_last[which] == 0) continue;
-    __threadfence();
     const int parts = is_last[which] >> 10, c0 = (is_last[which] & 1023) - 1;
-    const Segment p = segs[which ? shared[1] : shared[0]];
+    const Segment p = segs[which ? shared1 : shared0];
+    static_assert(S::kRows <= 2 * WARPS, "two rows to a warp at most");
+    Joined<D> r[2] = {nothing_joined<D>(), nothing_joined<D>()};
 #pragma unroll 1
-    for (int row = warp; row < S::kRows; row += WARPS) {
+    for (int base = 0; base < parts; base += kRoom) {
+      const int n = min(kRoom, parts - base);
+      if (warp == 0) {
+        if (lane == 0) mbar_arrive_expect_tx(&join_bar, n * S::kSlotBytes);
+        __syncwarp();
+        // the first part is a [1] record, the others are [0] records of the CTAs behind it
+        const int part = base + lane;
+        if (lane < n)
+          bulk_load_1d(ring_all + lane * S::kSlotBytes,
+                       a.part + (static_cast<long long>(c0 + part) * 2 + (part == 0 ? 1 : 0)) * S::kRows * S::kRecord, S::kSlotBytes, &join_bar);
+      }
+      if (!mbar_wait(&join_bar, phase)) {
+        if (lane == 0) atomicExch(a.error, kErrWait);
+        mbar_wait(&join_bar, phase);  // copies in flight end before the shared memory does
+        return;
+      }
+      phase ^= 1;
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = warp + k * WARPS;
+        if (row >= S::kRows) break;
+        const float* from = reinterpret_cast<const float*>(ring_all) + row * S::kRecord;
+        join<D>(r[k], from, from + S::kRows * S::kRecord, S::kRows * S::kRecord, n, lane);
+      }
+      __syncthreads();
+      asm volatile("fence.proxy.async;" ::: "memory");
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int row = warp + k * WARPS;
+      if (row >= S::kRows) break;
       __half* dst = out_row<D, NT>(a, p, row);
-      if (dst == nullptr) continue;
-      // the first part is a [1] record, the others are [0] records of the CTAs behind it
-      const float* first = a.part + (static_cast<long long>(c0) * 2 + 1) * S::kRows * S::kRecord + row * S::kRecord;
-      put_row<D>(dst, join<D, true>(first, first + S::kRows * S::kRecord, 2 * S::kRows * S::kRecord, parts, lane), lane);
+      if (dst != nullptr) put_row<D>(dst, r[k], lane);
     }
   }
 }
