@@ -6,7 +6,10 @@
 //   P = 2^(S - ref)  a thread per row; written over S as fp16, where the next product takes it from
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
 // The next step's S is asked for ahead of this step's O, so that the threads that make P find it ready: steps of 128 tokens, of
-// which tensor memory holds one S per tile beside O, had every thread wait for its own products (0.52 of the tensor cores' rate).
+// which tensor memory holds one S per tile beside O, had every thread wait for its own products (chunks of 64 sequences 938 us
+// against 902).  Measured: 574 TFLOP/s for a prompt of 2048 (32 heads of 128 over 8), 798 for 552 blocks of chunks, which 148
+// multiprocessors share unevenly (four blocks on most, three on some, of unequal lengths); a step of a pair of tiles takes about
+// 2250 cycles where its products take 1024: exponentials, unpacking and the reads of K and V for 64 columns a product bound it.
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
@@ -433,8 +436,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
 #pragma unroll
         for (int e = 0; e < kG; ++e) x[1][e] = __byte_perm(y[e >> 1], z[e >> 1], e & 1 ? 0x7632 : 0x5410);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars.pack_empty[stage]);  // the words are in registers: the place is free
       if (!all) {
 #pragma unroll
         for (int kind = 0; kind < 2; ++kind) {
@@ -464,7 +465,12 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+        if (lane == 0) {
+          mbar_arrive(kind ? &bars.v_full[buf] : &bars.k_full[buf]);
+          // Behind the fence, which orders the reads ahead of the next copy's writes: an arrival right after them let copies
+          // overtake them.
+          if (kind == 1) mbar_arrive(&bars.pack_empty[stage]);
+        }
       }
       if (++stage == S::kRing) {
         stage = 0;
