@@ -719,6 +719,12 @@ MLD_API int mld_qk_rope_run(mld_qk_rope_plan* plan, const mld_qk_rope_io* io, in
  * h / (heads / kv_heads).  Query token i of m of a sequence of n cached tokens
  * stands at n - m + i and sees the tokens at or before it, with a window only
  * the last `window` of those; a query that sees none gives zeros. */
+typedef enum mld_kv4_path {
+  MLD_KV4_PATH_AUTO = 0,
+  MLD_KV4_PATH_FEW_ROWS = 1, /* cut over all SMs without regard to sequences:
+                                decoding, drafted tokens */
+  MLD_KV4_PATH_MANY_ROWS = 2 /* blocks of 256 rows on the tensor cores: prompts */
+} mld_kv4_path;
 typedef struct mld_kv4_attn_desc {
   mld_kv4_desc cache;
   int32_t heads;             /* a multiple of cache.kv_heads, up to 4096 */
@@ -727,6 +733,8 @@ typedef struct mld_kv4_attn_desc {
   int32_t window;            /* 0: none */
   float scale;               /* of q.k; 0: 1 / sqrt(head_dim) */
   int32_t device;            /* -1 = current */
+  int32_t force_path;        /* mld_kv4_path; 0 = by the measured rule on
+                                batch, heads and max_queries */
 } mld_kv4_attn_desc;
 
 typedef struct mld_kv4_attn_io {

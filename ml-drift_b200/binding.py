@@ -466,6 +466,7 @@ class Decoder:
 
 # ------------------------------------------------- key/value cache in 4 bits
 ROPE_HALVES, ROPE_NEIGHBOURS = 0, 1
+KV4_PATH_AUTO, KV4_PATH_FEW_ROWS, KV4_PATH_MANY_ROWS = 0, 1, 2
 
 
 class Kv4Desc(C.Structure):
@@ -487,7 +488,7 @@ class QkRopeIo(C.Structure):
 
 class Kv4AttnDesc(C.Structure):
     _fields_ = [("cache", Kv4Desc), ("heads", C.c_int32), ("max_batch", C.c_int32), ("max_pages", C.c_int32),
-                ("window", C.c_int32), ("scale", C.c_float), ("device", C.c_int32)]
+                ("window", C.c_int32), ("scale", C.c_float), ("device", C.c_int32), ("force_path", C.c_int32)]
 
 
 class Kv4AttnIo(C.Structure):
@@ -695,9 +696,9 @@ class QkNormRope:
 class Kv4Attention:
     """Attention of new tokens over a Kv4Cache (which holds their keys and values already)."""
 
-    def __init__(self, cache, heads, max_batch, max_pages, window=0, scale=0.0, device=-1):
+    def __init__(self, cache, heads, max_batch, max_pages, window=0, scale=0.0, device=-1, force_path=KV4_PATH_AUTO):
         self.cache, self.heads, self.max_pages = cache, heads, max_pages
-        self.desc = Kv4AttnDesc(cache.desc, heads, max_batch, max_pages, window, scale, device)
+        self.desc = Kv4AttnDesc(cache.desc, heads, max_batch, max_pages, window, scale, device, force_path)
         self._h = C.c_void_p()
         _check(lib().mld_kv4_attn_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_kv4_attn_plan_create")
 

@@ -36,7 +36,6 @@ namespace mld {
 namespace {
 
 constexpr int kMaxGrid = 256;
-constexpr int kFewRows = 64;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm(
@@ -693,6 +692,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       }
     };
     const auto release = [&]() {
+      fence_proxy_async();  // the reads come ahead of the next copy's writes
       __syncwarp();
       if (++stage == S::kStages) {
         stage = 0;
@@ -889,6 +889,26 @@ int launch_attn_t(const Kv4AttnArgs& a, int grid, cudaStream_t stream) {
   return MLD_OK;
 }
 
+// The pieces of work of a call are counted in 32 bits in this kernel.
+bool countable(const mld_kv4_attn_desc& d, int batch, int64_t rows) {
+  const double tiles = static_cast<double>(d.max_pages) * (d.cache.page_tokens / kv4::kTile);
+  return tiles * batch * d.cache.kv_heads * div_up64(rows, 8) <= 2147483647.0;
+}
+
+// Whether a call's rows are worked on here or in blocks of 256 on the tensor cores.  64 tokens cost this kernel a time in
+// proportion to heads x blocks of 16 rows (8 for heads of 256), spread over all SMs; the other one a fixed time per wave of its
+// blocks, of which one walks all tokens.  Both sides, us, 4096 cached tokens: 8 heads of 128, 512 rows 70 / 85, 1024 rows 119 / 85
+// (16384 tokens: 211 / 303, 403 / 304); 32 heads, 128 rows 58 / 83, 256 rows 96 / 85; 128 heads, 32 rows 62 / 85, 64 rows 93 / 86;
+// 64 heads of 64, 128 rows 57 / 75, 256 rows 85 / 76; 16 heads of 64, 512 rows 59 / 75, 1024 rows 96 / 75; 8 heads of 256, 256 rows
+// 67 / 127, 1024 rows 213 / 128.
+bool few_rows(const mld_kv4_attn_desc& d, int batch, int64_t rows, int sms) {
+  const int64_t units = static_cast<int64_t>(batch) * d.cache.kv_heads;
+  const bool wide = d.cache.head_dim == 256;
+  const int64_t blocks = div_up64(rows, wide ? 8 : 16), waves = div_up64(units * div_up64(rows, wide ? 128 : 256), sms);
+  if (!countable(d, batch, rows)) return false;
+  return units * blocks <= (d.cache.head_dim == 64 ? 1000 : wide ? 500 : 450) * waves;
+}
+
 }  // namespace
 }  // namespace mld
 
@@ -913,6 +933,7 @@ int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out
   MLD_REQUIRE(d->max_batch >= 1 && d->max_batch <= kKv4MaxBatch, "max_batch must be 1 to 1024");
   MLD_REQUIRE(d->max_pages >= 1 && static_cast<int64_t>(d->max_pages) * d->cache.page_tokens <= 0x7FFFFFFF,
               "a sequence holds 1 to 2^31 - 1 tokens in whole pages");
+  MLD_REQUIRE(d->force_path >= MLD_KV4_PATH_AUTO && d->force_path <= MLD_KV4_PATH_MANY_ROWS, "bad force_path");
   MLD_REQUIRE(d->window >= 0, "window must not be negative (0: none)");
   MLD_REQUIRE(isfinite(d->scale) && d->scale >= 0.0f, "scale must be a finite positive number (0: 1 / sqrt(head_dim))");
   mld_kv4_attn_plan* p = new (std::nothrow) mld_kv4_attn_plan();
@@ -1010,16 +1031,14 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   a.tickets = plan->tickets;
   a.error = plan->error;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  // pieces of work are counted in 32 bits
   const int64_t rows = static_cast<int64_t>(io->max_queries) * a.group;
-  const int64_t chunks = static_cast<int64_t>(d.max_pages) * a.page_tiles;  // of a tile at least
-  if (static_cast<double>(io->batch) * d.cache.kv_heads * (rows / 8 + 1) * chunks > 2147483647.0) {
-    set_last_error_text("more work than one call can count: fewer sequences, or a narrower page table");
+  if (d.force_path == MLD_KV4_PATH_MANY_ROWS || (d.force_path == MLD_KV4_PATH_AUTO && !few_rows(d, io->batch, rows, plan->grid)))
+    return launch_kv4_prefill(a, d.cache.head_dim, stream);
+  if (!countable(d, io->batch, rows)) {
+    set_last_error_text("more work than one call of this path can count: fewer sequences, or a narrower page table");
     return MLD_OUT_OF_RANGE;
   }
-  // Many rows: the tensor cores' own kernel.
-  if (rows > kFewRows) return launch_kv4_prefill(a, d.cache.head_dim, stream);
-  const bool few = static_cast<int64_t>(io->max_queries) * a.group <= 8;
+  const bool few = rows <= 8;
   switch (d.cache.head_dim) {
     case 64:
       return few ? launch_attn_t<64, 1, 12>(a, plan->grid, stream) : launch_attn_t<64, 2, 12>(a, plan->grid, stream);

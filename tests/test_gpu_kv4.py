@@ -188,23 +188,25 @@ def _attention_case(mld, seed, head_dim, kv_heads, group, page, lens, news, wind
     qw = (rng.standard_normal((total, heads + 1, head_dim)) * spread).astype(np.float16)
     q = _dev(qw)[:, 1:]
     out = torch.full((total, heads + 2, head_dim), float("nan"), dtype=torch.float16, device="cuda")
-    plan = mld.Kv4Attention(cache, heads, batch + 1, table.shape[1], window=window, scale=scale)
+    sc = scale if scale else head_dim ** -0.5
+    wants = [ref.attention(qw[starts[b]:starts[b + 1], 1:], *kept[b], news[b], sc, window) for b in range(batch)]
     one = all(m == 1 for m in news)
     args = dict() if one else dict(q_starts=_dev(starts), max_queries=max(news))
-    plan.run(q, _dev(table), _dev(np.int32(lens)), out[:, :heads], **args)
-    first = out.clone()
-    plan.run(q, _dev(table), _dev(np.int32(lens)), out[:, :heads], **args)
-    assert plan.device_status() == 0
-    got = out[:, :heads].cpu().numpy().astype(np.float64)
-    assert np.array_equal(first[:, :heads].cpu().numpy().astype(np.float64), got), "two runs differ"
-    assert bool(torch.isnan(out[:, heads:]).all()), "wrote beside the output"
-    sc = scale if scale else head_dim ** -0.5
-    for b in range(batch):
-        r0, r1 = int(starts[b]), int(starts[b + 1])
-        want, size = ref.attention(qw[r0:r1, 1:], *kept[b], r1 - r0, sc, window)
-        tol = 1.1 * 2.0 ** -11 * (np.abs(want) + size) + 2.0 ** -25
-        bad = np.abs(got[r0:r1] - want) > tol
-        assert not bad.any(), (b, lens[b], int(bad.sum()), float((np.abs(got[r0:r1] - want) / (tol + 1e-30)).max()))
+    for path in (mld.KV4_PATH_AUTO, mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+        out.fill_(float("nan"))
+        plan = mld.Kv4Attention(cache, heads, batch + 1, table.shape[1], window=window, scale=scale, force_path=path)
+        plan.run(q, _dev(table), _dev(np.int32(lens)), out[:, :heads], **args)
+        first = out.clone()
+        plan.run(q, _dev(table), _dev(np.int32(lens)), out[:, :heads], **args)
+        assert plan.device_status() == 0
+        got = out[:, :heads].cpu().numpy().astype(np.float64)
+        assert np.array_equal(first[:, :heads].cpu().numpy().astype(np.float64), got), "two runs differ"
+        assert bool(torch.isnan(out[:, heads:]).all()), "wrote beside the output"
+        for b, (want, size) in enumerate(wants):
+            r0, r1 = int(starts[b]), int(starts[b + 1])
+            tol = 1.1 * 2.0 ** -11 * (np.abs(want) + size) + 2.0 ** -25
+            bad = np.abs(got[r0:r1] - want) > tol
+            assert not bad.any(), (path, b, lens[b], int(bad.sum()), float((np.abs(got[r0:r1] - want) / (tol + 1e-30)).max()))
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
@@ -260,6 +262,60 @@ def test_several_new_tokens(mld, head_dim, group, news):
 def test_a_whole_prompt(mld, head_dim):
     _attention_case(mld, 21, head_dim, 2, 2, 64, [513], [513])
     _attention_case(mld, 22, head_dim, 1, 3, 16, [200, 129], [200, 128], window=70)
+
+
+@pytest.mark.parametrize("head_dim,group,lens,news,window", [(128, 4, [1500, 300], [700, 65], 0), (64, 8, [700], [333], 129),
+                                                             (256, 2, [1100], [600], 0), (128, 1, [900], [900], 300)])
+def test_prompts_of_many_blocks(mld, head_dim, group, lens, news, window):
+    _attention_case(mld, 23, head_dim, 2, group, 64, lens, news, window=window)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [0, 37])
+def test_nan_and_infinities_at_places_that_a_row_does_not_see_stay_out_of_it(mld, head_dim, window):
+    rng = np.random.default_rng(head_dim)
+    n, m, hk = 300, 90, 2
+    cache = mld.Kv4Cache(hk, head_dim, 32, 10)
+    k, v = (rng.standard_normal((n, hk, head_dim)).astype(np.float16) for _ in range(2))
+    v[250, 1, 33], v[231, 0, 0], k[280, 0, 5] = np.nan, -np.inf, np.inf
+    if window:
+        v[20, 0, 40] = np.nan  # seen by nobody
+    cache.write(_dev(k), _dev(v), torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = rng.standard_normal((m, hk, head_dim)).astype(np.float16)
+    at = np.arange(n - m, n)
+    sees = lambda t: (at >= t) & ((at - t < window) if window else True)  # noqa: E731
+    nan = np.zeros((m, hk, head_dim), bool)
+    nan[sees(250), 1, 32:64] = True
+    nan[sees(231), 0, :32] = True
+    nan[sees(280), 0] = True
+    kr, vr = np.nan_to_num(ref.quantise(k)), np.nan_to_num(ref.quantise(v))
+    want, size = ref.attention(q, kr, vr, m, head_dim ** -0.5, window)
+    table = torch.arange(10, dtype=torch.int32, device="cuda")[None].contiguous()
+    starts = _dev(np.int32([0, m]))
+    for path in (mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+        out = torch.zeros(m, hk, head_dim, dtype=torch.float16, device="cuda")
+        mld.Kv4Attention(cache, hk, 1, 10, window=window, force_path=path).run(_dev(q), table, _dev(np.int32([n])), out, q_starts=starts,
+                                                                               max_queries=m)
+        got = out.cpu().numpy().astype(np.float64)
+        assert np.array_equal(np.isnan(got), nan), (path, np.isnan(got).sum(), nan.sum())
+        tol = 1.1 * 2.0 ** -11 * (np.abs(want) + size) + 2.0 ** -25
+        assert (np.abs(got - want)[~nan] <= tol[~nan]).all()
+
+
+@pytest.mark.parametrize("head_dim,kv_heads,page", [(64, 2, 64), (128, 2, 16), (256, 1, 64)])
+def test_a_hundred_runs_give_the_same_bits(mld, head_dim, kv_heads, page):
+    n, m, g = 2500, 70, 4
+    cache = mld.Kv4Cache(kv_heads, head_dim, page, -(-n // page))
+    k, v = (torch.randn(n, kv_heads, head_dim, device="cuda").half() for _ in range(2))
+    cache.write(k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = (torch.randn(m, kv_heads * g, head_dim, device="cuda") * 1.5).half()
+    table = torch.arange(-(-n // page), dtype=torch.int32, device="cuda")[None].contiguous()
+    for path in (mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+        plan = mld.Kv4Attention(cache, kv_heads * g, 1, table.shape[1], force_path=path)
+        outs = [torch.full_like(q, float("nan")) for _ in range(100)]
+        for out in outs:
+            plan.run(q, table, _dev(np.int32([n])), out, q_starts=_dev(np.int32([0, m])), max_queries=m)
+        assert all(torch.equal(o, outs[0]) for o in outs) and bool(torch.isfinite(outs[0]).all())
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])

@@ -30,10 +30,11 @@ def test_bad_caches_are_refused(mld, kv_heads, head_dim, page, pages):
 
 
 @pytest.mark.parametrize("change", [dict(heads=3), dict(heads=0), dict(max_batch=0), dict(max_batch=1025), dict(max_pages=0), dict(window=-1),
-                                    dict(scale=float("nan")), dict(scale=-1.0)])
+                                    dict(scale=float("nan")), dict(scale=-1.0), dict(force_path=3)])
 def test_bad_attention_plans_are_refused(mld, change):
-    d = dict(heads=4, max_batch=1, max_pages=4, window=0, scale=0.0) | change
-    a = mld.binding.Kv4AttnDesc(mld.binding.Kv4Desc(2, 128, 64, 10), d["heads"], d["max_batch"], d["max_pages"], d["window"], d["scale"], -1)
+    d = dict(heads=4, max_batch=1, max_pages=4, window=0, scale=0.0, force_path=0) | change
+    a = mld.binding.Kv4AttnDesc(mld.binding.Kv4Desc(2, 128, 64, 10), d["heads"], d["max_batch"], d["max_pages"], d["window"], d["scale"], -1,
+                                d["force_path"])
     h = ctypes.c_void_p()
     assert mld.lib().mld_kv4_attn_plan_create(ctypes.byref(a), ctypes.byref(h)) == mld.INVALID_ARGUMENT
 
