@@ -734,7 +734,7 @@ typedef struct mld_kv4_attn_desc {
   float scale;               /* of q.k; 0: 1 / sqrt(head_dim) */
   int32_t device;            /* -1 = current */
   int32_t force_path;        /* mld_kv4_path; 0 = by the measured rule on
-                                batch, heads and max_queries */
+                                batch, heads, max_queries and max_pages */
 } mld_kv4_attn_desc;
 
 typedef struct mld_kv4_attn_io {
@@ -754,8 +754,11 @@ typedef struct mld_kv4_attn_io {
 } mld_kv4_attn_io;
 
 typedef struct mld_kv4_attn_plan mld_kv4_attn_plan;
-/* All workspace is allocated here and is clear when the call returns.  A plan
- * may be used from one stream at a time; calls may be captured. */
+/* All workspace is allocated here and is clear when the call returns: about
+ * 2 MB, and, where max_pages allows sequences of more than 4096 tokens (blocks of
+ * many rows are then cut along them), 50 / 101 / 101 MB for heads of 64 / 128 /
+ * 256; not with force_path MLD_KV4_PATH_FEW_ROWS.  A plan may be used from one
+ * stream at a time; calls may be captured. */
 MLD_API int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out);
 MLD_API int mld_kv4_attn_plan_destroy(mld_kv4_attn_plan* plan);
 MLD_API size_t mld_kv4_attn_plan_workspace_bytes(const mld_kv4_attn_plan* plan);

@@ -25,6 +25,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 
 #include "common.cuh"
@@ -35,7 +36,7 @@
 namespace mld {
 namespace {
 
-constexpr int kMaxGrid = 256;
+constexpr int kMaxGrid = 256, kTickets = kMaxGrid * kKv4Slots;
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm(
@@ -895,18 +896,24 @@ bool countable(const mld_kv4_attn_desc& d, int batch, int64_t rows) {
   return tiles * batch * d.cache.kv_heads * div_up64(rows, 8) <= 2147483647.0;
 }
 
-// Whether a call's rows are worked on here or in blocks of 256 on the tensor cores.  64 tokens cost this kernel a time in
-// proportion to heads x blocks of 16 rows (8 for heads of 256), spread over all SMs; the other one a fixed time per wave of its
-// blocks, of which one walks all tokens.  Both sides, us, 4096 cached tokens: 8 heads of 128, 512 rows 70 / 85, 1024 rows 119 / 85
-// (16384 tokens: 211 / 303, 403 / 304); 32 heads, 128 rows 58 / 83, 256 rows 96 / 85; 128 heads, 32 rows 62 / 85, 64 rows 93 / 86;
-// 64 heads of 64, 128 rows 57 / 75, 256 rows 85 / 76; 16 heads of 64, 512 rows 59 / 75, 1024 rows 96 / 75; 8 heads of 256, 256 rows
-// 67 / 127, 1024 rows 213 / 128.
-bool few_rows(const mld_kv4_attn_desc& d, int batch, int64_t rows, int sms) {
-  const int64_t units = static_cast<int64_t>(batch) * d.cache.kv_heads;
-  const bool wide = d.cache.head_dim == 256;
-  const int64_t blocks = div_up64(rows, wide ? 8 : 16), waves = div_up64(units * div_up64(rows, wide ? 128 : 256), sms);
+// Whether a call's rows are worked on here or in blocks of 256 (128 for heads of 256) on the tensor cores.  64 tokens cost this
+// kernel a time in proportion to `small`, heads x blocks of 16 rows (8 for heads of 256), spread over all SMs.
+// The other kernel takes a time in proportion to `large`, heads x its blocks, and about 40 us for cutting and joining them, which
+// are worth more or less of `small` with the tokens that a sequence has; the host does not know them, and 8192 are assumed.  Both
+// sides, us, for 4608 and 16384 cached tokens: 8 heads of 128, 64 rows 24 / 44 and 42 / 65, 128 rows 34 / 45 and 69 / 66, 256 rows 47
+// / 49 and 116 / 69, 512 rows 76 / 50 and 211 / 82; 32 heads of 128 (8 x 4 sequences), 64 rows 39 / 54 and 86 / 151, 128 rows 57 / 55
+// and 152 / 151; 8 heads of 64, 256 rows 34 / 36 and 68 / 53, 512 rows 48 / 39 and 113 / 68; 2 heads of 256, 256 rows 36 / 52 and 84 /
+// 83, 512 rows 54 / 55 and 151 / 88.
+// Where sequences are too short to be cut, that kernel's time is a fixed one per wave of its blocks, of which one walks all tokens.
+// Both sides, us, 4096 tokens: 8 heads of 128, 512 rows 70 / 85, 1024 rows 119 / 85; 32 heads, 128 rows 58 / 83, 256 rows 96 / 85; 64
+// heads of 64, 128 rows 57 / 75, 256 rows 85 / 76; 8 heads of 256, 256 rows 67 / 127, 1024 rows 213 / 128.
+bool few_rows(const mld_kv4_attn_desc& d, int batch, int64_t rows, int sms, bool cut) {
   if (!countable(d, batch, rows)) return false;
-  return units * blocks <= (d.cache.head_dim == 64 ? 1000 : wide ? 500 : 450) * waves;
+  const int64_t units = static_cast<int64_t>(batch) * d.cache.kv_heads;
+  const int dim = d.cache.head_dim;
+  const int64_t small = units * div_up64(rows, dim == 256 ? 8 : 16), large = units * div_up64(rows, dim == 256 ? 128 : 256);
+  if (cut) return dim == 64 ? small <= 4.5 * large + 150 : dim == 128 ? small <= 2.6 * large + 104 : small <= 2.7 * large + 75;
+  return small <= (dim == 64 ? 1000 : dim == 128 ? 450 : 500) * div_up64(large, sms);
 }
 
 }  // namespace
@@ -916,11 +923,12 @@ using namespace mld;
 
 struct mld_kv4_attn_plan {
   mld_kv4_attn_desc d;
-  int device, grid;
+  int device, grid, slots;
   uint8_t* workspace;
   size_t bytes;
   float* part;
   int *tickets, *error;
+  int4* pieces;  // null where no sequence can be long enough to be cut
 };
 
 extern "C" {
@@ -950,14 +958,21 @@ int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out
   if (cudaGetDevice(&before) != cudaSuccess || cudaSetDevice(p->device) != cudaSuccess) return fail("cudaSetDevice");
   p->grid = sm_count(p->device);
   if (p->grid > kMaxGrid) p->grid = kMaxGrid;
-  const size_t part = static_cast<size_t>(p->grid) * 2 * 16 * (d->cache.head_dim + 4) * sizeof(float);
-  p->bytes = part + kMaxGrid * sizeof(int) + sizeof(int);
-  const bool made = cudaMalloc(&p->workspace, p->bytes) == cudaSuccess && zero_now(p->workspace, p->bytes) == cudaSuccess;
+  size_t part = static_cast<size_t>(p->grid) * 2 * 16 * (d->cache.head_dim + 4) * sizeof(float), pieces = 0;
+  if (d->force_path != MLD_KV4_PATH_FEW_ROWS && kv4_can_cut(static_cast<int64_t>(d->max_pages) * d->cache.page_tokens)) {
+    p->slots = p->grid * kKv4Slots;
+    part = std::max(part, p->slots * kv4_slot_bytes(d->cache.head_dim));
+    pieces = (kKv4MaxEntries + p->slots) * sizeof(int4);
+  }
+  const size_t words = (kTickets + 1) * sizeof(int);
+  p->bytes = part + pieces + words;
+  const bool made = cudaMalloc(&p->workspace, p->bytes) == cudaSuccess && zero_now(p->workspace + part + pieces, words) == cudaSuccess;
   cudaSetDevice(before);
   if (!made) return fail("workspace of the attention plan");
   p->part = reinterpret_cast<float*>(p->workspace);
-  p->tickets = reinterpret_cast<int*>(p->workspace + part);
-  p->error = p->tickets + kMaxGrid;
+  p->pieces = pieces > 0 ? reinterpret_cast<int4*>(p->workspace + part) : nullptr;
+  p->tickets = reinterpret_cast<int*>(p->workspace + part + pieces);
+  p->error = p->tickets + kTickets;
   *out = p;
   return MLD_OK;
 }
@@ -976,7 +991,7 @@ int mld_kv4_attn_plan_device_status(mld_kv4_attn_plan* plan, int32_t* code) {
   MLD_CUDA_CHECK(cudaDeviceSynchronize());
   MLD_CUDA_CHECK(cudaMemcpy(code, plan->error, sizeof(int), cudaMemcpyDeviceToHost));
   if (*code == 0) return MLD_OK;
-  MLD_CUDA_CHECK(zero_now(plan->tickets, (kMaxGrid + 1) * sizeof(int)));
+  MLD_CUDA_CHECK(zero_now(plan->tickets, (kTickets + 1) * sizeof(int)));
   if (*code == kErrPage) {
     set_last_error_text("a page table names a page that the pool does not have");
     return MLD_OUT_OF_RANGE;
@@ -1029,11 +1044,15 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = plan->part;
   a.tickets = plan->tickets;
+  a.pieces = plan->pieces;
+  a.slots = plan->slots;
   a.error = plan->error;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const int64_t rows = static_cast<int64_t>(io->max_queries) * a.group;
-  if (d.force_path == MLD_KV4_PATH_MANY_ROWS || (d.force_path == MLD_KV4_PATH_AUTO && !few_rows(d, io->batch, rows, plan->grid)))
-    return launch_kv4_prefill(a, d.cache.head_dim, stream);
+  const bool cut = plan->pieces != nullptr && kv4_cuts(a, d.cache.head_dim);
+  if (!cut) a.pieces = nullptr;
+  if (d.force_path == MLD_KV4_PATH_MANY_ROWS || (d.force_path == MLD_KV4_PATH_AUTO && !few_rows(d, io->batch, rows, plan->grid, cut)))
+    return launch_kv4_prefill(a, d.cache.head_dim, plan->grid, stream);
   if (!countable(d, io->batch, rows)) {
     set_last_error_text("more work than one call of this path can count: fewer sequences, or a narrower page table");
     return MLD_OUT_OF_RANGE;

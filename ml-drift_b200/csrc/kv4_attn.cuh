@@ -21,12 +21,24 @@ struct Kv4AttnArgs {
   int page_tiles, pages;
   int window;
   float scale_log2;  // log2(e) times the scale of the scores
-  float* part;       // [grid][2][rows][D + 4]
-  int* tickets;      // [grid], zero between launches
+  float* part;       // few rows: [grid][2][rows][D + 4]; many: [slots][D / 4 + 1][rows of a block][4]
+  int* tickets;      // few rows: [grid], many: [slots]; zero between launches
+  int4* pieces;      // many rows: [kKv4MaxEntries + slots], or null
+  int slots;
   int* error;
 };
 
-int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, cudaStream_t stream);
+// Many rows: blocks of rows that may be cut along the cached tokens, in all sequences of a call.
+constexpr int kKv4MaxEntries = 4096;
+// Pieces of cut blocks that a call may have, for each SM (101 MB of workspace for heads of 128 on 148 SMs).  With 2 in place of 5: 8
+// heads of 128, 2048 rows, 65536 tokens 768 us against 635, 4 sequences of 16384 583 against 454.
+constexpr int kKv4Slots = 5;
+size_t kv4_slot_bytes(int head_dim);
+// Whether sequences of so many tokens can be long enough for that; whether a call's blocks may be cut.
+bool kv4_can_cut(int64_t tokens);
+bool kv4_cuts(const Kv4AttnArgs& a, int head_dim);
+
+int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, int sms, cudaStream_t stream);
 
 #ifdef __CUDACC__
 namespace {

@@ -6,10 +6,13 @@
 //   P = 2^(S - ref)  a thread per row; written over S as fp16, where the next product takes it from
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
 // The next step's S is asked for ahead of this step's O, so that the threads that make P find it ready: steps of 128 tokens, of
-// which tensor memory holds one S per tile beside O, had every thread wait for its own products (chunks of 64 sequences 938 us
-// against 902).  Measured: 574 TFLOP/s for a prompt of 2048 (32 heads of 128 over 8), 798 for 552 blocks of chunks, which 148
-// multiprocessors share unevenly (four blocks on most, three on some, of unequal lengths); a step of a pair of tiles takes about
-// 2250 cycles where its products take 1024: exponentials, unpacking and the reads of K and V for 64 columns a product bound it.
+// which tensor memory holds one S per tile beside O, had every thread wait for its own products (ragged chunks 938 us against
+// 902, whole blocks).  A step of a pair of tiles takes about 2250 cycles where its products take 1024: exponentials, unpacking and the
+// reads of K and V for 64 columns a product bound it.
+// Blocks of long sequences are cut along the tokens where that fills the SMs (kv4_prefill_pieces_kernel): a piece leaves its sums
+// and their reference in the plan's workspace, and the last one of a block joins them in the pieces' order.  Whole / cut, us, 8
+// heads of 128: 2048 rows, 16384 tokens 303 / 187; 4 times that 583 / 454; 256 rows, 65536 tokens 1210 / 126.
+// Measured (32 heads of 128 over 8): 576 TFLOP/s for a prompt of 2048 tokens, 811 for ragged chunks behind up to 16384.
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled
@@ -37,6 +40,10 @@ constexpr int kRowWarps = 8, kUnpackWarps = 8, kLoadWarp = 16, kMmaWarp = 17;  /
 constexpr int kRegsRows = 136, kRegsUnpack = 72, kRegsRest = 64;
 constexpr int kRowsPerTile = 128;
 constexpr float kPrefillHeadroom = 5.0f, kPrefillLift = 10.0f, kPrefillFloor = -1e30f;
+// What a block of rows takes beside its steps, a piece of one that is cut, and joining one piece to others, in steps; chosen by
+// sweeps over 9, 14, 20 and 28 for a piece (8 heads of 128: 2048 rows, 16384 tokens 227 / 187 / 187 / 225 us; 4 times that 453 / 454 /
+// 474 / 584; 1024 rows, 32768 tokens 202 / 197 / 233 / 266).
+constexpr float kBlockCost = 4.0f, kCutCost = 14.0f, kJoinCost = 1.5f;
 constexpr int kMaskedBlocks = 24;  // blocks of tokens that only some rows of a block of rows see, at most
 
 template <int D>
@@ -187,6 +194,13 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 // Barrier `id` of 256 threads.  One warp of them waits for a transaction barrier and the others for it here, without polls.
 __device__ __forceinline__ void sync_256(int id) { asm volatile("barrier.cta.sync.aligned %0, 256;" ::"r"(id) : "memory"); }
 
+// The same for the N threads that have rows.
+template <int N>
+__device__ __forceinline__ void sync_rows() {
+  __syncwarp();
+  asm volatile("barrier.cta.sync 4, %0;" ::"n"(N) : "memory");
+}
+
 template <int N>
 __device__ __forceinline__ void more_registers() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -196,7 +210,131 @@ __device__ __forceinline__ void fewer_registers() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// The steps that a block of rows walks.
+struct BlockSteps {
+  int at_lo, at_hi, first_step, steps;  // what the first and the last row see ends at at_lo and at_hi
+};
 template <int D>
+__device__ __forceinline__ BlockSteps block_steps(const Kv4AttnArgs& a, const Kv4Sequence& q, int block) {
+  using S = Prefill<D>;
+  const int row0 = block * S::kRows, row_end = min(q.m * a.group, row0 + S::kRows);
+  BlockSteps s;
+  s.at_lo = q.n - q.m + row0 / a.group;
+  s.at_hi = q.n - q.m + (row_end - 1) / a.group;
+  s.first_step = (a.window > 0 ? max(0, s.at_lo - a.window + 1) : 0) / S::kN;
+  s.steps = s.at_hi < 0 ? 0 : s.at_hi / S::kN + 1 - s.first_step;
+  return s;
+}
+
+// Cuts long blocks of rows along the cached tokens where all SMs are done sooner for it.  One block of 1024 threads; an entry is a
+// block of rows of a sequence, those with the most tokens ahead of them first.  Warp w weighs cutting everything longer than
+// 1 / pieces_of(w) of the longest entry into pieces no longer than that: the time is an SM's share of all pieces and half of the
+// longest one's (or that, if longer), and what the last of a block's pieces takes to join them.  A piece is (sequence, block,
+// piece | pieces << 16, slot of the block's first); one for each key/value head.
+__device__ __forceinline__ int pieces_of(int w) { return w < 16 ? w + 1 : 16 + (w - 15) * 8; }
+
+template <int D>
+__global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks, int sms) {
+  constexpr int kPer = kKv4MaxEntries / 1024;
+  __shared__ int s_steps[kKv4MaxEntries], s_count[32], s_slots[32], s_longest;
+  __shared__ float s_time[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, entries = row_blocks * a.batch;
+  if (threadIdx.x == 0) s_longest = 1;
+  __syncthreads();
+  pdl_wait();
+  const auto place = [&](int e, int& b, int& block) {
+    const int rank = e / a.batch;
+    b = e - rank * a.batch;
+    block = row_blocks - 1 - rank;
+  };
+  int longest = 1;
+  for (int e = threadIdx.x; e < entries; e += 1024) {
+    int b, block, steps = -1;  // no rows
+    place(e, b, block);
+    const Kv4Sequence q = kv4_sequence(a, b);
+    if (static_cast<long long>(block) * Prefill<D>::kRows < q.m * a.group) steps = block_steps<D>(a, q, block).steps;
+    s_steps[e] = steps;
+    longest = max(longest, steps);
+  }
+  longest = __reduce_max_sync(0xFFFFFFFFu, longest);
+  if (lane == 0) atomicMax(&s_longest, longest);
+  __syncthreads();
+  longest = s_longest;
+  const int room = a.slots / a.kv_heads;
+  {
+    const int most = (longest + pieces_of(warp) - 1) / pieces_of(warp);
+    const float inv = 1.0f / static_cast<float>(most);
+    float work = 0.0f;
+    int cut = 0, joined = 1;
+    for (int e = lane; e < entries; e += 32) {
+      const int steps = s_steps[e];
+      if (steps < 0) continue;
+      const int k = steps > most ? static_cast<int>(ceilf(static_cast<float>(steps) * inv)) : 1;
+      work += static_cast<float>(steps) + static_cast<float>(k) * (k > 1 ? kCutCost : kBlockCost);
+      cut += k > 1 ? k + 1 : 0;  // one more than there may be after rounding
+      joined = max(joined, k);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xFFFFFFFFu, work, o);
+    cut = __reduce_add_sync(0xFFFFFFFFu, cut);
+    joined = __reduce_max_sync(0xFFFFFFFFu, joined);
+    const float piece = static_cast<float>(most) + (joined > 1 ? kCutCost : kBlockCost);
+    const float time = fmaxf(piece, work * static_cast<float>(a.kv_heads) / static_cast<float>(sms) + 0.5f * piece) +
+                       (joined > 1 ? kJoinCost * static_cast<float>(joined) : 0.0f);
+    if (lane == 0) s_time[warp] = cut <= room ? time : INFINITY;
+  }
+  __syncthreads();
+  int best = 0;
+  for (int w = 1; w < 32; ++w)
+    if (s_time[w] < s_time[best]) best = w;
+  const int most = (longest + pieces_of(best) - 1) / pieces_of(best);
+  int count = 0, slots = 0;  // of the entries before the thread's, after the scan
+  int pieces[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = threadIdx.x * kPer + i, steps = e < entries ? s_steps[e] : -1;
+    pieces[i] = steps < 0 ? 0 : max(1, (steps + most - 1) / most);
+    count += pieces[i];
+    slots += pieces[i] > 1 ? pieces[i] : 0;
+  }
+  const int own_count = count, own_slots = slots;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int c = __shfl_up_sync(0xFFFFFFFFu, count, o), l = __shfl_up_sync(0xFFFFFFFFu, slots, o);
+    if (lane >= o) {
+      count += c;
+      slots += l;
+    }
+  }
+  if (lane == 31) {
+    s_count[warp] = count;
+    s_slots[warp] = slots;
+  }
+  count -= own_count;
+  slots -= own_slots;
+  __syncthreads();
+  int end = 0;
+  for (int w = 0; w < 32; ++w) {
+    if (w < warp) {
+      count += s_count[w];
+      slots += s_slots[w];
+    }
+    end += s_count[w];
+  }
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    int b, block;
+    place(threadIdx.x * kPer + i, b, block);
+    for (int k = 0; k < pieces[i]; ++k) a.pieces[count + k] = make_int4(b, block, k | pieces[i] << 16, slots);
+    count += pieces[i];
+    slots += pieces[i] > 1 ? pieces[i] : 0;
+  }
+  for (int i = end + threadIdx.x; i < entries + room; i += 1024) a.pieces[i] = make_int4(-1, 0, 0, 0);
+}
+
+// kCut: blocks may be cut, and are listed.  Calls whose sequences are too short for that take the form without the joining, which
+// costs the loop registers (a prompt of 2048 tokens 60 us in its own form, 62 to 65 in the other).
+template <int D, bool kCut>
 __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks) {
   using S = Prefill<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -209,6 +347,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   __shared__ PrefillBars bars;
   __shared__ uint32_t tmem_base;
   __shared__ int any_bad;
+  __shared__ bool is_last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -230,20 +369,33 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   }
   pdl_wait();
   // ---- which rows: the blocks with the most tokens ahead of them first
-  const int units = a.batch * a.kv_heads, rank = blockIdx.x / units, unit = blockIdx.x - rank * units;
-  const int b = unit / a.kv_heads, h = unit - b * a.kv_heads;
-  const int block = row_blocks - 1 - rank;
-  const Kv4Sequence q = kv4_sequence(a, b);
+  const int item = blockIdx.x / a.kv_heads, h = blockIdx.x - item * a.kv_heads;
+  int b, block, piece = 0, pieces = 1, slot = 0;
+  if constexpr (kCut) {
+    const int4 p = __ldcg(a.pieces + item);
+    b = p.x;
+    block = p.y;
+    piece = p.z & 0xFFFF;
+    pieces = p.z >> 16;
+    slot = p.w * a.kv_heads + h;
+  } else {
+    const int rank = item / a.batch;
+    b = item - rank * a.batch;
+    block = row_blocks - 1 - rank;
+  }
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.batch; i += kPrefillThreads)
       if (!kv4_fits(a, i, kv4_sequence(a, i))) atomicExch(a.error, kErrLength);
   }
+  if (kCut && b < 0) return;
+  const Kv4Sequence q = kv4_sequence(a, b);
   const int rows = q.m * a.group, row0 = block * S::kRows;
   if (row0 >= rows) return;
-  const int row_end = min(rows, row0 + S::kRows);
-  const int at_lo = q.n - q.m + row0 / a.group, at_hi = q.n - q.m + (row_end - 1) / a.group;  // what the rows see ends here
-  const int first = a.window > 0 ? max(0, at_lo - a.window + 1) : 0;
-  const int step0 = first / S::kN, steps = at_hi < 0 ? 0 : at_hi / S::kN + 1 - step0;
+  const BlockSteps all_steps = block_steps<D>(a, q, block);
+  const int at_lo = all_steps.at_lo, at_hi = all_steps.at_hi;
+  const int step_from = static_cast<int>(static_cast<long long>(all_steps.steps) * piece / pieces);
+  const int step0 = all_steps.first_step + step_from;
+  const int steps = static_cast<int>(static_cast<long long>(all_steps.steps) * (piece + 1) / pieces) - step_from;
   // whether all rows see all of a step's tokens
   const auto whole = [&](int t0, int lo, int hi) { return t0 + S::kN - 1 <= lo && (a.window == 0 || t0 >= hi - a.window + 1); };
 
@@ -372,9 +524,25 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
           ++k;
         }
       }
-      const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
       const int token = row / a.group, head = h * a.group + row - token * a.group;
       __half* dst = a.out + (q.first_token + token) * a.out_stride + static_cast<long long>(head) * D;
+      const auto put = [&](int c, const float* o, uint32_t bad_groups, float inv) {  // 16 columns
+        const float f = (bad_groups >> (c / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
+        if (row < rows) {
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            // value k of eight lies in column 2 k, value 4 + k in column 2 k + 1
+            const auto x = [&](int k) { return o[e + (k < 4 ? 2 * k : 2 * k - 7)] * f; };
+            *reinterpret_cast<uint4*>(dst + c + e) =
+                make_uint4(half2_bits(x(0), x(1)), half2_bits(x(2), x(3)), half2_bits(x(4), x(5)), half2_bits(x(6), x(7)));
+          }
+        }
+      };
+      const auto inverse = [](float sum) { return sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f; };
+      constexpr int kSlot = (D / 4 + 1) * S::kRows;
+      float4* const parts = reinterpret_cast<float4*>(a.part) + static_cast<long long>(slot) * kSlot + tile * kRowsPerTile + (warp & 3) * 32 + lane;
+      const long long next = static_cast<long long>(a.kv_heads) * kSlot;  // the block's next piece
+      float4* const mine = parts + piece * next;
 #pragma unroll 1
       for (int c = 0; c < D; c += 16) {
         uint32_t o[16];
@@ -385,14 +553,58 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[e] = 0;
         }
-        const float f = (bad >> (c / 32)) & 1 ? __int_as_float(0x7FFFFFFF) : inv;
-        if (row < rows) {
+        float x[16];
 #pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            // value k of eight lies in column 2 k, value 4 + k in column 2 k + 1
-            const auto x = [&](int k) { return __uint_as_float(o[e + (k < 4 ? 2 * k : 2 * k - 7)]) * f; };
-            *reinterpret_cast<uint4*>(dst + c + e) =
-                make_uint4(half2_bits(x(0), x(1)), half2_bits(x(2), x(3)), half2_bits(x(4), x(5)), half2_bits(x(6), x(7)));
+        for (int e = 0; e < 16; ++e) x[e] = __uint_as_float(o[e]);
+        if (!kCut || pieces == 1) {
+          put(c, x, bad, inverse(l));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) __stcg(mine + (c / 4 + e) * S::kRows, make_float4(x[4 * e], x[4 * e + 1], x[4 * e + 2], x[4 * e + 3]));
+        }
+      }
+      if (kCut && pieces > 1) {
+        // ---- the last of the block's pieces joins them, in their order
+        __stcg(mine + D / 4 * S::kRows, make_float4(-minus_ref, l, __uint_as_float(bad), 0.0f));
+        __threadfence();
+        sync_rows<S::kTilesM * kRowsPerTile>();
+        if (threadIdx.x == 0) {
+          const bool last = atomicAdd(a.tickets + slot, 1) == pieces - 1;
+          if (last) a.tickets[slot] = 0;
+          is_last = last;
+          __threadfence();
+        }
+        sync_rows<S::kTilesM * kRowsPerTile>();
+        if (is_last) {
+          __threadfence();
+          float ref = kPrefillFloor, sum = 0.0f;
+          bad = 0;
+          const float4* const states = parts + D / 4 * S::kRows;
+          for (int p = 0; p < pieces; ++p) ref = fmaxf(ref, __ldcg(states + p * next).x);
+          for (int p = 0; p < pieces; ++p) {
+            const float4 state = __ldcg(states + p * next);
+            sum += exp2_hw(state.x - ref) * state.y;
+            bad |= __float_as_uint(state.z);
+          }
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            float x[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) x[e] = 0.0f;
+#pragma unroll 2
+            for (int p = 0; p < pieces; ++p) {
+              const float f = exp2_hw(__ldcg(states + p * next).x - ref);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const float4 y = __ldcg(parts + p * next + (c / 4 + e) * S::kRows);
+                x[4 * e] = fmaf(f, y.x, x[4 * e]);
+                x[4 * e + 1] = fmaf(f, y.y, x[4 * e + 1]);
+                x[4 * e + 2] = fmaf(f, y.z, x[4 * e + 2]);
+                x[4 * e + 3] = fmaf(f, y.w, x[4 * e + 3]);
+              }
+            }
+            put(c, x, bad, inverse(sum));
+            put(c + 16, x + 16, bad, inverse(sum));
           }
         }
       }
@@ -563,31 +775,55 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   if (warp == kMmaWarp) tmem_dealloc_512(tmem_base);
 }
 
-template <int D>
-int launch_prefill_t(const Kv4AttnArgs& a, cudaStream_t stream) {
+template <int D, bool kCut>
+int launch_prefill_t(const Kv4AttnArgs& a, int sms, cudaStream_t stream) {
   using S = Prefill<D>;
   static bool configured[kMaxDevices];
   int dev;
   if (needs_configure(configured, &dev)) {
-    MLD_CUDA_CHECK(cudaFuncSetAttribute(kv4_prefill_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
+    MLD_CUDA_CHECK(cudaFuncSetAttribute(kv4_prefill_kernel<D, kCut>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(S::kSmem)));
     if (dev >= 0) configured[dev] = true;
   }
   const int64_t row_blocks = div_up64(static_cast<int64_t>(a.max_queries) * a.group, S::kRows);
-  const int64_t grid = row_blocks * a.batch * a.kv_heads;
+  const int64_t grid = (row_blocks * a.batch + (kCut ? a.slots / a.kv_heads : 0)) * a.kv_heads;
   if (grid > 0x7FFFFFFF) {
     set_last_error_text("more work than one call can count: fewer sequences or queries");
     return MLD_OUT_OF_RANGE;
   }
-  MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_kernel<D>, dim3(static_cast<unsigned>(grid)), dim3(kPrefillThreads), S::kSmem, stream, a,
+  if constexpr (kCut) {
+    MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_pieces_kernel<D>, dim3(1), dim3(1024), 0, stream, a, static_cast<int>(row_blocks), sms));
+    MLD_LAUNCH_CHECK();
+  }
+  MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_kernel<D, kCut>, dim3(static_cast<unsigned>(grid)), dim3(kPrefillThreads), S::kSmem, stream, a,
                                    static_cast<int>(row_blocks)));
   MLD_LAUNCH_CHECK();
   return MLD_OK;
 }
 
+template <int D>
+int launch_prefill_d(const Kv4AttnArgs& a, int sms, cudaStream_t stream) {
+  return a.pieces != nullptr ? launch_prefill_t<D, true>(a, sms, stream) : launch_prefill_t<D, false>(a, sms, stream);
+}
+
+template <int D>
+constexpr size_t kSlotBytes = static_cast<size_t>(Prefill<D>::kRows) * (D + 4) * sizeof(float);
+
 }  // namespace
 
-int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, cudaStream_t stream) {
-  return head_dim == 64 ? launch_prefill_t<64>(a, stream) : head_dim == 128 ? launch_prefill_t<128>(a, stream) : launch_prefill_t<256>(a, stream);
+size_t kv4_slot_bytes(int head_dim) { return head_dim == 64 ? kSlotBytes<64> : head_dim == 128 ? kSlotBytes<128> : kSlotBytes<256>; }
+
+// Up to 4096 tokens the pieces are hardly worth what they cost (8 heads of 128, 2048 rows, 4096 tokens: 85 us whole, 86 cut), and
+// the list takes a launch more (a prompt of 2048 tokens 60 us without, 63 with it).
+bool kv4_can_cut(int64_t tokens) { return tokens > 4096; }
+
+bool kv4_cuts(const Kv4AttnArgs& a, int head_dim) {
+  const int64_t blocks = div_up64(static_cast<int64_t>(a.max_queries) * a.group, head_dim == 256 ? Prefill<256>::kRows : Prefill<128>::kRows);
+  return blocks * a.batch <= kKv4MaxEntries && (a.window == 0 || kv4_can_cut(a.window));
+}
+
+int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, int sms, cudaStream_t stream) {
+  return head_dim == 64 ? launch_prefill_d<64>(a, sms, stream)
+                        : head_dim == 128 ? launch_prefill_d<128>(a, sms, stream) : launch_prefill_d<256>(a, sms, stream);
 }
 
 }  // namespace mld

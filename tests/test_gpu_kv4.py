@@ -158,14 +158,14 @@ def test_keys_and_values_written_in_the_same_pass_are_those_written_after_it(mld
 
 
 # --------------------------------------------------------------------------------------------------------- attention
-def _attention_case(mld, seed, head_dim, kv_heads, group, page, lens, news, window=0, scale=0.0, spread=1.5, v_size=1.0, split=None):
+def _attention_case(mld, seed, head_dim, kv_heads, group, page, lens, news, window=0, scale=0.0, spread=1.5, v_size=1.0, wide=0):
     """Runs a batch and compares every row with the restatement on what the cache holds."""
     rng = np.random.default_rng(seed)
     heads, batch = kv_heads * group, len(lens)
     per = [-(-n // page) for n in lens]
     pages = sum(per) + 3
     order = rng.permutation(pages)
-    table = np.full((batch, max(max(per), 1) + 1), -7, np.int32)  # entries that nobody may read
+    table = np.full((batch, max(max(per), wide, 1) + 1), -7, np.int32)  # entries that nobody may read
     cache = mld.Kv4Cache(kv_heads, head_dim, page, pages)
     cache.pool.fill_(0x7E)                                        # NaN scales wherever nothing is written
     kept, at = [], 0
@@ -302,9 +302,43 @@ def test_nan_and_infinities_at_places_that_a_row_does_not_see_stay_out_of_it(mld
         assert (np.abs(got - want)[~nan] <= tol[~nan]).all()
 
 
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,news,group,window", [([9000], [1], 1, 0), ([4097], [70], 4, 0), ([20011, 0, 333, 6000], [33, 4, 65, 1], 4, 0),
+                                                    ([9001, 5000], [50, 130], 3, 4500), ([70], [9], 2, 0)])
+def test_long_sequences_are_cut_and_joined(mld, head_dim, lens, news, group, window):
+    _attention_case(mld, 41, head_dim, 2, group, 48, lens, news, window=window, wide=100)
+
+
+def test_more_heads_than_places_for_cut_blocks(mld):
+    _attention_case(mld, 42, 64, 800, 1, 16, [40, 17], [3, 2], wide=260)
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_what_is_not_finite_stays_in_its_groups_when_a_sequence_is_cut(mld, head_dim):
+    rng = np.random.default_rng(head_dim)
+    n, m, page = 12000, 90, 64
+    pages = -(-n // page)
+    cache = mld.Kv4Cache(1, head_dim, page, pages)
+    k, v = (rng.standard_normal((n, 1, head_dim)).astype(np.float16) for _ in range(2))
+    v[11950, 0, 33] = np.nan  # seen by the last 50 rows
+    cache.write(_dev(k), _dev(v), torch.arange(n, dtype=torch.int32, device="cuda"))
+    q = rng.standard_normal((m, 1, head_dim)).astype(np.float16)
+    nan = np.zeros((m, 1, head_dim), bool)
+    nan[np.arange(n - m, n) >= 11950, 0, 32:64] = True
+    want, size = ref.attention(q, ref.quantise(k), np.nan_to_num(ref.quantise(v)), m, head_dim ** -0.5, 0)
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    for path in (mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+        out = torch.zeros(m, 1, head_dim, dtype=torch.float16, device="cuda")
+        plan = mld.Kv4Attention(cache, 1, 1, pages, force_path=path)
+        plan.run(_dev(q), table, _dev(np.int32([n])), out, q_starts=_dev(np.int32([0, m])), max_queries=m)
+        got = out.cpu().numpy().astype(np.float64)
+        assert np.array_equal(np.isnan(got), nan), path
+        assert (np.abs(got - want)[~nan] <= (1.1 * 2.0 ** -11 * (np.abs(want) + size) + 2.0 ** -25)[~nan]).all()
+
+
 @pytest.mark.parametrize("head_dim,kv_heads,page", [(64, 2, 64), (128, 2, 16), (256, 1, 64)])
 def test_a_hundred_runs_give_the_same_bits(mld, head_dim, kv_heads, page):
-    n, m, g = 2500, 70, 4
+    n, m, g = 5000, 70, 4  # long enough to be cut
     cache = mld.Kv4Cache(kv_heads, head_dim, page, -(-n // page))
     k, v = (torch.randn(n, kv_heads, head_dim, device="cuda").half() for _ in range(2))
     cache.write(k, v, torch.arange(n, dtype=torch.int32, device="cuda"))
