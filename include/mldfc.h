@@ -754,9 +754,9 @@ typedef struct mld_kv4_attn_io {
 } mld_kv4_attn_io;
 
 typedef struct mld_kv4_attn_plan mld_kv4_attn_plan;
-/* All workspace is allocated here and is clear when the call returns: about
- * 2 MB, and, where max_pages allows sequences of more than 4096 tokens (blocks of
- * many rows are then cut along them), 50 / 101 / 101 MB for heads of 64 / 128 /
+/* All workspace is allocated here and is clear when the call returns: up to
+ * 5 MB, and, where max_pages allows sequences of more than 4096 tokens (blocks of
+ * many rows are then cut along them), 52 / 100 / 99 MB for heads of 64 / 128 /
  * 256; not with force_path MLD_KV4_PATH_FEW_ROWS.  A plan may be used from one
  * stream at a time; calls may be captured. */
 MLD_API int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out);
