@@ -309,6 +309,32 @@ def test_long_sequences_are_cut_and_joined(mld, head_dim, lens, news, group, win
     _attention_case(mld, 41, head_dim, 2, group, 48, lens, news, window=window, wide=100)
 
 
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_a_captured_call_cuts_anew_for_new_lengths(mld, head_dim):
+    page, pages, m = 64, 160, 100
+    cache = mld.Kv4Cache(1, head_dim, page, pages)
+    k, v = (torch.randn(pages * page, 1, head_dim, device="cuda").half() for _ in range(2))
+    cache.write(k, v, torch.arange(pages * page, dtype=torch.int32, device="cuda"))
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None].contiguous()
+    q = torch.randn(m, 4, head_dim, device="cuda").half()
+    starts, lens, out = _dev(np.int32([0, m])), _dev(np.int32([9000])), torch.zeros_like(q)
+    plan = mld.Kv4Attention(cache, 4, 1, pages, force_path=mld.KV4_PATH_MANY_ROWS)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan.run(q, table, lens, out, q_starts=starts, max_queries=m)
+        plan.run(q, table, lens, out, q_starts=starts, max_queries=m)
+    for n in (9000, 150, 10240, 100):
+        lens.fill_(n)
+        out.fill_(float("nan"))
+        graph.replay()
+        want = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        plan.run(q, table, lens, want, q_starts=starts, max_queries=m)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+    assert plan.device_status() == 0
+
+
 def test_more_heads_than_places_for_cut_blocks(mld):
     _attention_case(mld, 42, 64, 800, 1, 16, [40, 17], [3, 2], wide=260)
 
