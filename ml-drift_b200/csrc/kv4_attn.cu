@@ -75,6 +75,11 @@ __device__ __forceinline__ uint32_t fma_half2(uint32_t x, float scale, float off
 __device__ __forceinline__ uint32_t code_lo(uint32_t x) { return fma_half2(x & 0x000F000Fu, 32768.0f, -0.015625f); }
 __device__ __forceinline__ uint32_t code_hi(uint32_t x) { return fma_half2(x & 0x00F000F0u, 2048.0f, -0.015625f); }
 
+// Two halves, each zero where it is an infinity or a NaN.
+__device__ __forceinline__ uint32_t finite_halves(uint32_t x) {
+  return ((x & 0x7C00u) == 0x7C00u ? 0u : x & 0xFFFFu) | ((x & 0x7C000000u) == 0x7C000000u ? 0u : x & 0xFFFF0000u);
+}
+
 constexpr float kFloor = -1e30f;   // reference of a row that has seen nothing
 constexpr float kHeadroom = 2.0f;  // how far weights may exceed the reference, as a power of two
 constexpr float kLift = 13.0f;
@@ -370,8 +375,17 @@ __device__ __forceinline__ void step(const uint8_t* tiles, const LaneAt<D>& at, 
       over = over || m > w.limit[i][c];
     }
   if (__any_sync(0xFFFFFFFFu, over)) {
+    wild = __any_sync(0xFFFFFFFFu, most >= 0x7C00u);
+    if (wild) {
+      // What is not finite stays that whatever it is multiplied by; rows that do not see it keep their weights' decimals.
+      most = 0;
+#pragma unroll
+      for (int k = 0; k < TILES; ++k)
+#pragma unroll
+        for (int e = 0; e < kG / 2; ++e) most = __vmaxu2(most, __vmaxu2(finite_halves(v0[k][e]), finite_halves(v1[k][e])));
+      most = max(most & 0xFFFFu, most >> 16);
+    }
     most = __reduce_max_sync(0xFFFFFFFFu, most);
-    wild = most >= 0x7C00u;
     if (most > w.scale_limit) {
       w.scale_limit = most | 0x3FFu;  // the end of its binade
       w.e = static_cast<float>(static_cast<int>(most >> 10) - 14);
