@@ -291,7 +291,9 @@ __global__ void __launch_bounds__(kThreads, 16) qk_rope_kernel(const __grid_cons
       }
 #pragma unroll
       for (int c = 0; c < 8; c += 2) {
-        const float2 z = mul2(make_float2(r, r), fma2(pair(x, c), pair(mine, c), mul2(pair(y, c), pair(other, c))));
+        // a value that is not turned has no partner: an infinity there, times zero, would be a NaN
+        const float2 z = mul2(make_float2(r, r), turns ? fma2(pair(x, c), pair(mine, c), mul2(pair(y, c), pair(other, c)))
+                                                       : mul2(pair(x, c), pair(mine, c)));
         x[c] = z.x;
         x[c + 1] = z.y;
       }

@@ -18,6 +18,35 @@ def mld():
     return g.import_package()
 
 
+@pytest.mark.parametrize("f16", [True, False])
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("weighted", [False, True])
+@pytest.mark.parametrize("head_dim,rotary", [(64, 16), (128, 64), (256, 240), (64, 0), (128, 128)])
+def test_what_is_not_finite_in_a_head_changes_only_what_the_formula_says(mld, head_dim, rotary, neighbours, weighted, f16):
+    rng = np.random.default_rng(head_dim + rotary)
+    dt, tt = (np.float16, torch.float16) if f16 else (np.float32, torch.float32)
+    n, h = 12, 3
+    x = rng.standard_normal((n, h, head_dim)).astype(dt)
+    places = [0, 1, rotary // 2, max(rotary - 1, 0), rotary % head_dim, (rotary + 1) % head_dim, (rotary + 6) % head_dim, head_dim - 1]
+    for i, (at, value) in enumerate(zip(places + places[:2], [np.inf, -np.inf, np.nan] * 4)):
+        x[i, 1, at] = value
+    pos = rng.integers(1, 1000, (1, n)).astype(np.int32)
+    w = (1 + 0.1 * rng.standard_normal(head_dim)).astype(dt) if weighted else None
+    plan = mld.QkNormRope(h, h, head_dim, rotary, mld.ROPE_NEIGHBOURS if neighbours else mld.ROPE_HALVES, rms_eps=1e-5, f16=f16)
+    qo, ko = (torch.zeros(n, h, head_dim, dtype=tt, device="cuda") for _ in range(2))
+    wd = None if w is None else _dev(w)
+    plan.run(_dev(x), _dev(x), _dev(pos[0]), qo, ko, q_weight=wd, k_weight=wd)
+    with np.errstate(invalid="ignore"):
+        want = ref.norm_rope(x, w, 1e-5, pos, rotary, neighbours, [rotary // 2], 1.0, 1e6)
+    size = np.where(np.isfinite(want), np.abs(want), 0).max(-1, keepdims=True)
+    for got in (qo.cpu().numpy().astype(np.float64), ko.cpu().numpy().astype(np.float64)):
+        finite = np.isfinite(want)
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        assert np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+        tol = 16 * 2.0 ** -24 * size + (2.0 ** -11 * np.abs(want) + 2.0 ** -25 if f16 else 0 * want)
+        assert (np.abs(got[finite] - want[finite]) <= tol[finite]).all()
+
+
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 def test_small_values_beside_nan_that_a_row_does_not_see(mld, head_dim):
     """A window that has left a NaN behind: the rows after it are as exact as without it."""
