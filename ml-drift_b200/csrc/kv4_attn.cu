@@ -113,7 +113,7 @@ __device__ __forceinline__ Span span_of(const Kv4AttnArgs& a, int b) {
   s.first_row_token = q.first_token;
   const int first = a.window > 0 ? max(0, s.n - s.m + 1 - a.window) : 0;
   s.c0 = first / S::kChunk;
-  s.chunks = max(1, (s.n + S::kChunk - 1) / S::kChunk - s.c0);
+  s.chunks = max(1, (s.n - 1) / S::kChunk + 1 - s.c0);  // no sum here may pass 2^31 - 1, which n comes close to
   s.blocks = (s.m * a.group + S::kRows - 1) / S::kRows;
   return s;
 }
@@ -1056,7 +1056,8 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   a.group = d.heads / d.cache.kv_heads;
   a.page_tiles = d.cache.page_tokens / kv4::kTile;
   a.pages = d.cache.pages;
-  a.window = d.window;
+  // A window that no sequence is longer than hides nothing; differences with the others stay within 32 bits.
+  a.window = d.window < static_cast<int64_t>(d.max_pages) * d.cache.page_tokens ? d.window : 0;
   const float scale = d.scale > 0.0f ? d.scale : 1.0f / sqrtf(static_cast<float>(d.cache.head_dim));
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = plan->part;

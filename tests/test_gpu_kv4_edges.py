@@ -75,3 +75,32 @@ def test_small_values_beside_nan_that_a_row_does_not_see(mld, head_dim):
         tol = 1.1 * 2.0 ** -11 * (np.abs(want) + size) + 2.0 ** -25
         worst = (np.abs(got - want) / tol)[~nan].max()
         assert worst <= 1, (path, worst)
+
+
+def test_a_sequence_of_almost_2_31_tokens(mld):
+    """One page of keys and values 2^26 times over, then another one as often."""
+    rng = np.random.default_rng(7)
+    d, page, entries = 64, 16, (1 << 27) - 1
+    cache = mld.Kv4Cache(1, d, page, 2)
+    k, v = (rng.standard_normal((2 * page, 1, d)).astype(np.float16) for _ in range(2))
+    v[page:] += np.float16(2)
+    cache.write(_dev(k), _dev(v), torch.arange(2 * page, dtype=torch.int32, device="cuda"))
+    table = torch.zeros(1, entries, dtype=torch.int32, device="cuda")
+    table[:, entries // 2:] = 1
+    q = rng.standard_normal((1, 1, d)).astype(np.float16)
+    out = torch.zeros(1, 1, d, dtype=torch.float16, device="cuda")
+    plan = mld.Kv4Attention(cache, 1, 1, entries, force_path=mld.KV4_PATH_FEW_ROWS)
+    plan.run(_dev(q), table, _dev(np.int32([entries * page])), out)
+    assert plan.device_status() == 0
+    want, size = ref.attention(q, ref.quantise(k), ref.quantise(v), 1, d ** -0.5, 0)
+    # A warp adds 2^27 / (148 * 12) products of 16 tokens up in 32 bits: 2^-23 of the sum each, if all err to one side.
+    tol = 2 ** 27 / (148 * 12) * 2.0 ** -23 * size + 2.0 ** -10
+    assert (np.abs(out.cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 60, 1 << 20])
+def test_a_window_wider_than_any_sequence_hides_nothing(mld, head_dim, window):
+    # the queries outnumber the tokens of the first sequence: the first of them see nothing
+    _attention_case(mld, 61, head_dim, 2, 4, 32, [3, 300, 0], [70, 5, 2], window=window)
+    _attention_case(mld, 62, head_dim, 1, 2, 16, [100, 5000], [120, 40], window=window, wide=400)
