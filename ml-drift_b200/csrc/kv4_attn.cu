@@ -745,8 +745,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       // branches meet.
 #pragma unroll 1
       while (item < end && token >= whole_lo && token <= whole_hi) {
-        if (alive) alive = mbar_wait(bars + stage, phase);
-        if (!alive) break;
+        // the warp gives up together, and goes on without waiting or asking
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bars + stage, phase));
 #pragma unroll
         for (int k = 0; k < S::kTiles; k += S::kStep)
           step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, 0, 0, 0);
@@ -755,11 +755,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
         ask_ahead(item);
       }
       if (item < end) {
-        if (alive) alive = mbar_wait(bars + stage, phase);
+        if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bars + stage, phase));
 #pragma unroll 1
         for (int k = 0; k < S::kTiles; k += S::kStep) {
           const int from = token + k * kv4::kTile;
-          if (!alive || from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
+          if (from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
           step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, a.window, from, p.s.n);
         }
         release();
@@ -779,8 +779,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     }
     if (!alive && lane == 0) {
       atomicExch(a.error, kErrWait);
-      for (int s = 0; s < S::kStages; ++s)  // copies in flight end before the shared memory does
-        for (int ph = 0; ph < 2; ++ph) mbar_wait(bars + s, ph);
+      const int n = ii - wlo;  // copies in flight end before the shared memory does
+      for (int s = 0; s < S::kStages; ++s) mbar_wait(bars + s, ring_last_phase(s, n % S::kStages, n / S::kStages & 1));
     }
   }
   __syncthreads();
@@ -860,20 +860,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
           bulk_load_1d(ring_all + lane * S::kSlotBytes,
                        a.part + (static_cast<long long>(c0 + part) * 2 + (part == 0 ? 1 : 0)) * S::kRows * S::kRecord, S::kSlotBytes, &join_bar);
       }
-      if (!mbar_wait(&join_bar, phase)) {
-        if (lane == 0) atomicExch(a.error, kErrWait);
+      const bool there = __all_sync(0xFFFFFFFFu, mbar_wait(&join_bar, phase));
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int row = warp + k * WARPS;
+        if (row >= S::kRows || !there) break;
+        const float* from = reinterpret_cast<const float*>(ring_all) + row * S::kRecord;
+        join<D>(r[k], from, from + S::kRows * S::kRecord, S::kRows * S::kRecord, n, lane);
+      }
+      if (!__syncthreads_and(there)) {
+        if (!there && lane == 0) atomicExch(a.error, kErrWait);
         mbar_wait(&join_bar, phase);  // copies in flight end before the shared memory does
         return;
       }
       phase ^= 1;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int row = warp + k * WARPS;
-        if (row >= S::kRows) break;
-        const float* from = reinterpret_cast<const float*>(ring_all) + row * S::kRecord;
-        join<D>(r[k], from, from + S::kRows * S::kRecord, S::kRows * S::kRecord, n, lane);
-      }
-      __syncthreads();
       asm volatile("fence.proxy.async;" ::: "memory");
     }
 #pragma unroll

@@ -5,6 +5,7 @@
 
 #include "common.cuh"
 #include "kv4.cuh"
+#include "ring_order.h"
 
 namespace mld {
 

@@ -66,6 +66,7 @@ struct PrefillBars {
   // What is numbered by steps has as many barriers as there are buffers of K and V: a step's products are also what its buffers
   // become free by.
   uint64_t pack_full[3], pack_empty[3], k_full[4], v_full[4], s_full[2][4], p_full[2][4], pv_done[2][4];
+  uint64_t gave_up[2];  // all products of a tile, when the block gives up
 };
 
 // mbar_wait that looks at the clock only now and then: a waiting warp's polls take issue slots from the others.
@@ -87,6 +88,8 @@ __device__ __forceinline__ bool wait_quietly(uint64_t* bar, uint32_t parity) {
     if (t - t0 > kWaitLimitNs) return false;
   }
 }
+// The same for a warp, which gives up together: what follows needs all of its lanes.
+__device__ __forceinline__ bool wait_all(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_quietly(bar, parity)) != 0; }
 // Products are issued by one elected lane, predicated inside a block without branches: the warp stays together, so that the
 // operands can live in uniform registers, which the instruction takes them from.  Descriptors come as their low words, the high
 // word is the same for all operands here (1024 bytes from eight rows to the next, 128-byte swizzle).
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   __shared__ uint32_t tmem_base;
   __shared__ int any_bad;
   __shared__ bool is_last;
+  __shared__ int2 last_asked;  // stage and phase of the packed tiles that would be asked for next
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
@@ -355,6 +359,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       mbar_init(&bars.pack_full[i], 1);
       mbar_init(&bars.pack_empty[i], kUnpackWarps);
     }
+    for (int t = 0; t < S::kTilesM; ++t) mbar_init(&bars.gave_up[t], 1);
     for (int i = 0; i < S::kBuffers; ++i) {
       mbar_init(&bars.k_full[i], kUnpackWarps);
       mbar_init(&bars.v_full[i], kUnpackWarps);
@@ -435,8 +440,9 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       float limit = kPrefillFloor * inv_scale;  // scores that may not be exceeded
 #pragma unroll 1
       for (int j = 0; j < steps; ++j) {
-        ok = wait_quietly(&bars.s_full[tile][j % kB], j / kB & 1);
-        if (!ok) break;
+        // who gives up goes on without waiting: the warp's lanes are needed together
+        ok = ok && wait_quietly(&bars.s_full[tile][j % kB], j / kB & 1);
+        __syncwarp();
         tc_after();
         const uint32_t t_s = t_s0 + (j & 1) * S::kN;
         const int t0 = (step0 + j) * S::kN;
@@ -468,8 +474,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
             sums[i].y *= f;
           }
           if (j > 0) {
-            ok = wait_quietly(&bars.pv_done[tile][(j - 1) % kB], (j - 1) / kB & 1);
-            if (!ok) break;
+            ok = ok && wait_quietly(&bars.pv_done[tile][(j - 1) % kB], (j - 1) / kB & 1);
+            __syncwarp();
             tc_after();
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -626,8 +632,8 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       const bool all = whole(t0, at_lo, at_hi);
       if (!all) masked = min(masked + 1, kMaskedBlocks - 1);
       if (w == 0) {
-        ok = ok && wait_quietly(&bars.pack_full[stage], phase);
-        for (int i = 0; i < S::kTilesM; ++i) ok = ok && wait_quietly(&bars.pv_done[i][buf], use ^ 1);  // then K is free as well
+        ok = ok && wait_all(&bars.pack_full[stage], phase);
+        for (int i = 0; i < S::kTilesM; ++i) ok = ok && wait_all(&bars.pv_done[i][buf], use ^ 1);  // then K is free as well
       }
       sync_256(3);
       // all of the lane's words of K and V are asked for before the first is turned into values
@@ -699,7 +705,7 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------------ packed tiles
     // Lane l looks up every 32nd tile and brings it when its stage's turn comes, with the tiles behind it that lie in the same page.
-    int stage = 0, phase = 0;
+    int asked = 0, asked_phase = 0;
     const int tiles = (min(at_hi, q.n - 1) >> 4) + 1, tile0 = step0 * (S::kN / 16);
 #pragma unroll 1
     for (int from = tile0; from < tile0 + steps * (S::kN / 16) && ok; from += 32) {
@@ -717,23 +723,20 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       }
 #pragma unroll 1
       for (int l = 0; l < 32 && from + l < tile0 + steps * (S::kN / 16); l += S::kPackTiles) {
-        ok = wait_quietly(&bars.pack_empty[stage], phase ^ 1);
+        ok = wait_all(&bars.pack_empty[asked], asked_phase ^ 1);
         if (!ok) break;
         const int there = min(S::kPackTiles, max(0, tiles - from - l));
-        if (lane == 0) mbar_arrive_expect_tx(&bars.pack_full[stage], there * S::kTileBytes);
+        if (lane == 0) mbar_arrive_expect_tx(&bars.pack_full[asked], there * S::kTileBytes);
         __syncwarp();
         if (run > 0 && lane >= l && lane < l + S::kPackTiles)
-          bulk_load_1d(s_pack + stage * S::kPackBytes + (lane - l) * S::kTileBytes, src, run * S::kTileBytes, &bars.pack_full[stage]);
-        if (++stage == S::kRing) {
-          stage = 0;
-          phase ^= 1;
+          bulk_load_1d(s_pack + asked * S::kPackBytes + (lane - l) * S::kTileBytes, src, run * S::kTileBytes, &bars.pack_full[asked]);
+        if (++asked == S::kRing) {
+          asked = 0;
+          asked_phase ^= 1;
         }
       }
     }
-    if (!ok) {  // copies in flight end before the shared memory does
-      for (int i = 0; i < S::kRing; ++i)
-        for (int ph = 0; ph < 2; ++ph) wait_quietly(&bars.pack_full[i], ph);
-    }
+    if (lane == 0) last_asked = make_int2(asked, asked_phase);
   } else if (warp >= kMmaWarp && warp < kMmaWarp + S::kTilesM) {
     // ------------------------------------------------------------------ products of a tile
     const int tile = warp - kMmaWarp;
@@ -741,7 +744,6 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     const uint32_t idesc_o = 1u << 4 | 1u << 16 | static_cast<uint32_t>(D >> 3) << 17 | 8u << 24;
     const uint32_t q_low = desc_low(s_q + tile * S::kQBytes, 16), k_low = desc_low(s_k, 16), v_low = desc_low(s_v, S::kN * 128);
     const uint32_t t_s = tmem + tile * 2 * S::kN, t_o = tmem + S::kO + tile * D, me = elected();
-    const auto wait_all = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, wait_quietly(bar, parity)) != 0; };
     const auto scores = [&](int j) {  // of step j, into the tile's j % 2nd place
       ok = wait_all(&bars.k_full[j % kB], j / kB & 1);
       if (j > 1) ok = ok && wait_all(&bars.pv_done[tile][(j - 2) % kB], (j - 2) / kB & 1);  // whose weights lie there
@@ -768,9 +770,18 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
       umma_commit(me, &bars.pv_done[tile][j % kB]);
     }
   }
-  if (!ok && lane == 0) atomicExch(a.error, kErrWait);
   tc_before();
-  __syncthreads();
+  if (__syncthreads_or(!ok)) {
+    // Some role gave up: the copies and products that others have in flight end before the memory that they use does.
+    if (threadIdx.x == 0) atomicExch(a.error, kErrWait);
+    if (warp == kLoadWarp) {
+      for (int i = 0; i < S::kRing; ++i) wait_all(&bars.pack_full[i], ring_last_phase(i, last_asked.x, last_asked.y));
+    } else if (warp >= kMmaWarp && warp < kMmaWarp + S::kTilesM) {
+      umma_commit(elected(), &bars.gave_up[warp - kMmaWarp]);
+      wait_all(&bars.gave_up[warp - kMmaWarp], 0);
+    }
+    __syncthreads();
+  }
   tc_after();
   if (warp == kMmaWarp) tmem_dealloc_512(tmem_base);
 }

@@ -33,4 +33,9 @@ MLD_HOST_DEVICE unsigned ring_lanes_before(int lane, int distance) {
   return lane < distance ? 0u : (2u << (lane - distance)) - 1u;
 }
 
+// For a kernel that gives up and waits for its copies in flight: the parity of the phase that the last copy into stage `i` ends,
+// when `next` is the stage to be asked for next and `phase` the parity of that pass through the ring (0 in the first).  A stage that
+// has not been asked for in the first pass gives 1, which a wait on a new barrier passes at once.
+MLD_HOST_DEVICE int ring_last_phase(int i, int next, int phase) { return i < next ? phase : phase ^ 1; }
+
 }  // namespace mld
