@@ -683,8 +683,9 @@ typedef struct mld_qk_rope_desc {
 } mld_qk_rope_desc;
 
 /* Tensors of a call: rows of heads * head_dim values, `stride` elements from
- * token to token, 16-byte aligned.  q_out may be q and k_out may be k (with the
- * same stride); otherwise outputs must not overlap inputs. */
+ * token to token, 16-byte aligned; an input's may be 0 (one row for all tokens),
+ * an output's not.  q_out may be q and k_out may be k (with the same stride);
+ * otherwise outputs must not overlap inputs. */
 typedef struct mld_qk_rope_io {
   const void* q;
   int64_t q_stride;

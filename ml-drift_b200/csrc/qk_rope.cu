@@ -478,13 +478,23 @@ int mld_qk_rope_run(mld_qk_rope_plan* plan, const mld_qk_rope_io* io, int32_t to
   const int per16 = d.f16 ? 8 : 4;
   const void* const tensors[] = {io->q, io->k, io->v, io->q_out, io->k_out, io->q_weight, io->k_weight};
   for (const void* p : tensors) MLD_REQUIRE(aligned16(p), "tensors must be 16-byte aligned");
-  const int64_t strides[] = {d.heads ? io->q_stride : 0, d.kv_heads ? io->k_stride : 0, cached ? io->v_stride : 0,
-                             d.heads ? io->q_out_stride : 0, io->k_out != nullptr ? io->k_out_stride : 0};
-  const int64_t widths[] = {d.heads, d.kv_heads, d.kv_heads, d.heads, d.kv_heads};
-  for (int i = 0; i < 5; ++i) {
-    MLD_REQUIRE(strides[i] % per16 == 0, "token strides must be multiples of 16 bytes");
-    MLD_REQUIRE(strides[i] == 0 || strides[i] >= widths[i] * d.head_dim || tokens == 1, "token strides must not be shorter than a token");
+  const bool keys = d.kv_heads > 0, keys_out = keys && io->k_out != nullptr;
+  const struct {
+    bool there, out;
+    int64_t stride, heads;
+  } rows[] = {{d.heads > 0, false, io->q_stride, d.heads},
+              {keys, false, io->k_stride, d.kv_heads},
+              {cached, false, io->v_stride, d.kv_heads},
+              {d.heads > 0, true, io->q_out_stride, d.heads},
+              {keys_out, true, io->k_out_stride, d.kv_heads}};
+  for (const auto& r : rows) {
+    if (!r.there) continue;
+    MLD_REQUIRE(r.stride % per16 == 0, "token strides must be multiples of 16 bytes");
+    // all tokens may read one row, but not write it
+    MLD_REQUIRE(tokens == 1 || r.stride >= r.heads * d.head_dim || (r.stride == 0 && !r.out), "token strides must not be shorter than a token");
   }
+  MLD_REQUIRE(tokens == 1 || d.heads == 0 || io->q_out != io->q || io->q_out_stride == io->q_stride, "in place, queries go out with the stride that they come with");
+  MLD_REQUIRE(tokens == 1 || !keys_out || io->k_out != io->k || io->k_out_stride == io->k_stride, "in place, keys go out with the stride that they come with");
   RopeArgs a = {};
   a.q = io->q;
   a.k = io->k;

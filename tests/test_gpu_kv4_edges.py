@@ -104,3 +104,25 @@ def test_a_window_wider_than_any_sequence_hides_nothing(mld, head_dim, window):
     # the queries outnumber the tokens of the first sequence: the first of them see nothing
     _attention_case(mld, 61, head_dim, 2, 4, 32, [3, 300, 0], [70, 5, 2], window=window)
     _attention_case(mld, 62, head_dim, 1, 2, 16, [100, 5000], [120, 40], window=window, wide=400)
+
+
+def test_one_row_for_all_tokens_may_be_read_and_not_written(mld):
+    rng = np.random.default_rng(1)
+    n, h, hk, d = 9, 4, 2, 64
+    row = rng.standard_normal((1, h + 2 * hk, d)).astype(np.float16)
+    x = _dev(row).expand(n, -1, -1)
+    pos, slots = torch.arange(n, dtype=torch.int32, device="cuda"), torch.arange(n, dtype=torch.int32, device="cuda")
+    plan, outs = mld.QkNormRope(h, hk, d), []
+    for rows in (x, x.contiguous()):
+        cache = mld.Kv4Cache(hk, d, 16, 1)
+        q, k = torch.zeros(n, h, d, dtype=torch.float16, device="cuda"), torch.zeros(n, hk, d, dtype=torch.float16, device="cuda")
+        plan.run(rows[:, :h], rows[:, h:h + hk], pos, q, k, v=rows[:, h + hk:], cache=cache, slots=slots)
+        again = mld.Kv4Cache(hk, d, 16, 1)
+        again.write(rows[:, h:h + hk], rows[:, h + hk:], slots)
+        outs.append((q, k, cache.pool, again.pool))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    for q, k in ((torch.zeros(1, h, d, dtype=torch.float16, device="cuda").expand(n, -1, -1), outs[0][1]),
+                 (outs[0][0], torch.zeros(1, hk, d, dtype=torch.float16, device="cuda").expand(n, -1, -1))):
+        with pytest.raises(mld.MldError) as e:
+            plan.run(x[:, :h], x[:, h:h + hk], pos, q, k)
+        assert e.value.status == mld.INVALID_ARGUMENT

@@ -1,0 +1,31 @@
+"""Calls around the 4-bit cache that the host refuses, without a GPU: nothing of them reaches a kernel."""
+import ctypes
+
+import pytest
+
+
+@pytest.fixture(scope="module")
+def mld():
+    import __graft_entry__ as g
+    g.build()
+    return g.import_package()
+
+
+def _io(mld, **change):
+    io = mld.binding.QkRopeIo()
+    io.q, io.k, io.q_out, io.k_out, io.positions = 1 << 20, 2 << 20, 3 << 20, 4 << 20, 5 << 20
+    io.q_stride = io.q_out_stride = 512
+    io.k_stride = io.k_out_stride = 256
+    for name, value in change.items():
+        setattr(io, name, value)
+    return io
+
+
+@pytest.mark.parametrize("change", [dict(q_out_stride=0), dict(k_out_stride=0), dict(q_stride=0, q_out=1 << 20, q_out_stride=0),
+                                    dict(q_out=1 << 20, q_out_stride=1024), dict(k_out=2 << 20, k_stride=512), dict(q_stride=-512),
+                                    dict(k_out_stride=-256), dict(q_stride=256), dict(k_stride=8)])
+def test_tokens_that_would_write_one_row_or_read_what_another_wrote_are_refused(mld, change):
+    plan = mld.QkNormRope(4, 2, 128)
+    io = _io(mld, **change)
+    assert mld.lib().mld_qk_rope_run(plan._h, ctypes.byref(io), 2, None) == mld.INVALID_ARGUMENT
+    assert b"stride" in mld.lib().mld_last_error()
