@@ -497,8 +497,22 @@ class Kv4AttnIo(C.Structure):
                 ("max_queries", C.c_int32), ("out", C.c_void_p), ("out_stride", C.c_int64)]
 
 
-def _rows(t, tokens, heads, head_dim, dtype, what):
+def _here(stream):
+    """The current GPU's number (-2, which no tensor has, while CUDA has not been started) and the stream's handle."""
+    if not torch.cuda.is_initialized():
+        return -2, None
+    gpu = torch._C._cuda_getDevice()
+    return gpu, torch._C._cuda_getCurrentRawStream(gpu) if stream is None else stream.cuda_stream
+
+
+def _elsewhere(t, what):
+    return ValueError(f"{what}: expected a tensor on the current GPU, got one on {t.device}")
+
+
+def _rows(t, tokens, heads, head_dim, dtype, what, gpu):
     """Elements from token to token of a [tokens][heads][head_dim] tensor whose rows are contiguous."""
+    if t.get_device() != gpu:
+        raise _elsewhere(t, what)
     n, h, d = t.shape
     stride = t.stride()
     if n != tokens or t.dtype is not dtype or h != heads or d != head_dim or stride[2] != 1 or \
@@ -508,7 +522,9 @@ def _rows(t, tokens, heads, head_dim, dtype, what):
     return stride[0]
 
 
-def _ints(t, shape, what):
+def _ints(t, shape, what, gpu):
+    if t.get_device() != gpu:
+        raise _elsewhere(t, what)
     if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{what}: expected contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
@@ -528,7 +544,13 @@ class Kv4Cache:
             pool = torch.zeros(shape, dtype=torch.uint8, device=device)
         if pool.dtype != torch.uint8 or tuple(pool.shape) != shape or not pool.is_contiguous():
             raise ValueError(f"pool: expected contiguous uint8 {shape}, got {pool.dtype} {tuple(pool.shape)}")
-        self.pool, self.head_dim, self._base = pool, head_dim, pool.data_ptr()
+        if not pool.is_cuda:
+            raise ValueError(f"pool: expected a tensor on a GPU, got one on {pool.device}")
+        self.pool, self.head_dim, self._base, self._gpu = pool, head_dim, pool.data_ptr(), pool.get_device()
+
+    def _check_gpu(self, gpu):
+        if self._gpu != gpu:
+            raise _elsewhere(self.pool, "pool")
 
     def address(self, layer=0):
         if not 0 <= layer < self.layers:
@@ -539,18 +561,22 @@ class Kv4Cache:
         """k, v: [tokens][kv_heads][head_dim] fp16 or fp32; slots: int32 [tokens] on the device (-1: passed over)."""
         d = self.desc
         n = k.shape[0]
-        ks, vs = (_rows(t, n, d.kv_heads, d.head_dim, k.dtype, what) for t, what in ((k, "k"), (v, "v")))
+        gpu, queue = _here(stream)
+        self._check_gpu(gpu)
+        ks, vs = (_rows(t, n, d.kv_heads, d.head_dim, k.dtype, what, gpu) for t, what in ((k, "k"), (v, "v")))
         _check(lib().mld_kv4_write(C.byref(d), self.address(layer), k.data_ptr(), ks, v.data_ptr(), vs, _f16(k),
-                                   _ints(slots, (n,), "slots"), n, _stream_addr(stream)), "mld_kv4_write")
+                                   _ints(slots, (n,), "slots", gpu), n, queue), "mld_kv4_write")
 
     def read(self, slots, k, v, layer=0, stream=None):
         """The cache's values at `slots` into k and v, fp16 [tokens][kv_heads][head_dim]."""
         d = self.desc
         hk, hd = d.kv_heads, d.head_dim
         n = k.shape[0]
-        ks, vs = _rows(k, n, hk, hd, torch.float16, "k"), _rows(v, n, hk, hd, torch.float16, "v")
-        rc = _lib.mld_kv4_read(C.byref(d), self.address(layer), _ints(slots, (n,), "slots"), n, k.data_ptr(), ks, v.data_ptr(), vs,
-                               _stream_addr(stream))
+        gpu, queue = _here(stream)
+        self._check_gpu(gpu)
+        ks, vs = _rows(k, n, hk, hd, torch.float16, "k", gpu), _rows(v, n, hk, hd, torch.float16, "v", gpu)
+        rc = _lib.mld_kv4_read(C.byref(d), self.address(layer), _ints(slots, (n,), "slots", gpu), n, k.data_ptr(), ks, v.data_ptr(), vs,
+                               queue)
         if rc != OK:
             _check(rc, "mld_kv4_read")
 
@@ -559,9 +585,11 @@ class Kv4Cache:
         n = len(src)
         if len(dst) != n:
             raise ValueError("src and dst differ in length")
+        gpu, queue = _here(stream)
+        self._check_gpu(gpu)
         ints = C.c_int32 * n
         _check(lib().mld_kv4_copy_pages(C.byref(self.desc), self.pool.data_ptr(), self.layers, self.layer_bytes, ints(*src),
-                                        ints(*dst), n, _stream_addr(stream)), "mld_kv4_copy_pages")
+                                        ints(*dst), n, queue), "mld_kv4_copy_pages")
 
 
 def _f16(t):
@@ -655,29 +683,33 @@ class QkNormRope:
         """q, k, v: [tokens][heads][head_dim] (rows may be strided); positions: int32 [tokens] or [axes][tokens] on the device."""
         h, hk, d, dt = self.heads, self.kv_heads, self.head_dim, self.dtype
         n = (q if h else k).shape[0]
+        gpu, queue = _here(stream)
         io = QkRopeIo()
         if h:
-            io.q, io.q_stride = q.data_ptr(), _rows(q, n, h, d, dt, "q")
-            io.q_out, io.q_out_stride = q_out.data_ptr(), _rows(q_out, n, h, d, dt, "q_out")
+            io.q, io.q_stride = q.data_ptr(), _rows(q, n, h, d, dt, "q", gpu)
+            io.q_out, io.q_out_stride = q_out.data_ptr(), _rows(q_out, n, h, d, dt, "q_out", gpu)
         if hk:
-            io.k, io.k_stride = k.data_ptr(), _rows(k, n, hk, d, dt, "k")
+            io.k, io.k_stride = k.data_ptr(), _rows(k, n, hk, d, dt, "k", gpu)
             if k_out is not None:
-                io.k_out, io.k_out_stride = k_out.data_ptr(), _rows(k_out, n, hk, d, dt, "k_out")
+                io.k_out, io.k_out_stride = k_out.data_ptr(), _rows(k_out, n, hk, d, dt, "k_out", gpu)
         for w in (q_weight, k_weight):
             if w is not None and (w.dtype is not dt or w.numel() != d or not w.is_contiguous()):
                 raise ValueError(f"norm weights: expected contiguous {dt} [{d}]")
+            if w is not None and w.get_device() != gpu:
+                raise _elsewhere(w, "norm weights")
         if q_weight is not None:
             io.q_weight = q_weight.data_ptr()
         if k_weight is not None:
             io.k_weight = k_weight.data_ptr()
         if positions is not None:
-            io.positions = _ints(positions, (n,) if self.axes == 1 and positions.dim() == 1 else (self.axes, n), "positions")
+            io.positions = _ints(positions, (n,) if self.axes == 1 and positions.dim() == 1 else (self.axes, n), "positions", gpu)
         if cache is not None:
             if v is None or slots is None:
                 raise ValueError("a cache needs v and slots")
-            io.v, io.v_stride = v.data_ptr(), _rows(v, n, hk, d, dt, "v")
-            io.cache, io.pool, io.slots = C.addressof(cache.desc), cache.address(layer), _ints(slots, (n,), "slots")
-        rc = _lib.mld_qk_rope_run(self._h, C.byref(io), n, _stream_addr(stream))
+            cache._check_gpu(gpu)
+            io.v, io.v_stride = v.data_ptr(), _rows(v, n, hk, d, dt, "v", gpu)
+            io.cache, io.pool, io.slots = C.addressof(cache.desc), cache.address(layer), _ints(slots, (n,), "slots", gpu)
+        rc = _lib.mld_qk_rope_run(self._h, C.byref(io), n, queue)
         if rc != OK:
             _check(rc, "mld_qk_rope_run")
 
@@ -707,11 +739,13 @@ class Kv4Attention:
         [batch + 1], the rows of each sequence, of which none has more than max_queries (None: one row each)."""
         d, h = self.cache.head_dim, self.heads
         batch, n = lens.shape[0], q.shape[0]
-        io = Kv4AttnIo(q.data_ptr(), _rows(q, n, h, d, torch.float16, "q"), self.cache.address(layer),
-                       _ints(page_table, (batch, self.max_pages), "page_table"), _ints(lens, (batch,), "lens"),
-                       None if q_starts is None else _ints(q_starts, (batch + 1,), "q_starts"), batch, n, max_queries,
-                       out.data_ptr(), _rows(out, n, h, d, torch.float16, "out"))
-        rc = _lib.mld_kv4_attn_run(self._h, C.byref(io), _stream_addr(stream))
+        gpu, queue = _here(stream)
+        self.cache._check_gpu(gpu)
+        io = Kv4AttnIo(q.data_ptr(), _rows(q, n, h, d, torch.float16, "q", gpu), self.cache.address(layer),
+                       _ints(page_table, (batch, self.max_pages), "page_table", gpu), _ints(lens, (batch,), "lens", gpu),
+                       None if q_starts is None else _ints(q_starts, (batch + 1,), "q_starts", gpu), batch, n, max_queries,
+                       out.data_ptr(), _rows(out, n, h, d, torch.float16, "out", gpu))
+        rc = _lib.mld_kv4_attn_run(self._h, C.byref(io), queue)
         if rc != OK:
             _check(rc, "mld_kv4_attn_run")
 

@@ -126,3 +126,24 @@ def test_one_row_for_all_tokens_may_be_read_and_not_written(mld):
         with pytest.raises(mld.MldError) as e:
             plan.run(x[:, :h], x[:, h:h + hk], pos, q, k)
         assert e.value.status == mld.INVALID_ARGUMENT
+
+
+def test_any_tensor_in_host_memory_is_refused(mld):
+    """What a pager answers is easily made a tensor without a device."""
+    n, h, hk, d = 3, 4, 2, 64
+    cache = mld.Kv4Cache(hk, d, 16, 4)
+    rope, attention = mld.QkNormRope(h, hk, d), mld.Kv4Attention(cache, h, 1, 4)
+    q, k = (torch.zeros(n, heads, d, dtype=torch.float16, device="cuda") for heads in (h, hk))
+    ints, w = torch.arange(n, dtype=torch.int32, device="cuda"), torch.ones(d, dtype=torch.float16, device="cuda")
+    calls = [(cache.write, dict(k=k, v=k, slots=ints)), (cache.read, dict(slots=ints, k=k.clone(), v=k.clone())),
+             (rope.run, dict(q=q, k=k, positions=ints, q_out=q.clone(), k_out=k.clone(), q_weight=w, k_weight=w, v=k, cache=cache,
+                             slots=ints)),
+             (attention.run, dict(q=q, page_table=torch.zeros(1, 4, dtype=torch.int32, device="cuda"), lens=ints[:1], out=q.clone(),
+                                  q_starts=_dev(np.int32([0, n])), max_queries=n))]
+    for call, args in calls:
+        for name, t in args.items():
+            if isinstance(t, torch.Tensor):
+                with pytest.raises(ValueError, match="GPU"):
+                    call(**{**args, name: t.cpu()})
+        call(**args)
+    assert attention.device_status() == 0

@@ -29,3 +29,14 @@ def test_tokens_that_would_write_one_row_or_read_what_another_wrote_are_refused(
     io = _io(mld, **change)
     assert mld.lib().mld_qk_rope_run(plan._h, ctypes.byref(io), 2, None) == mld.INVALID_ARGUMENT
     assert b"stride" in mld.lib().mld_last_error()
+
+
+def test_tensors_in_host_memory_are_refused(mld):
+    import torch
+    with pytest.raises(ValueError, match="GPU"):
+        mld.Kv4Cache(2, 64, 16, 4, device="cpu")
+    with pytest.raises(ValueError, match="GPU"):
+        mld.Kv4Cache(2, 64, 16, 4, pool=torch.zeros(1, 4, 2, 1, 18 * 64, dtype=torch.uint8))
+    q, k = torch.zeros(3, 4, 64, dtype=torch.float16), torch.zeros(3, 2, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="q: expected a tensor on the current GPU, got one on cpu"):
+        mld.QkNormRope(4, 2, 64).run(q, k, torch.zeros(3, dtype=torch.int32), torch.empty_like(q), torch.empty_like(k))
