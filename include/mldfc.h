@@ -759,16 +759,16 @@ typedef struct mld_kv4_attn_plan mld_kv4_attn_plan;
  * 5 MB, and, where max_pages allows sequences of more than 4096 tokens (blocks of
  * many rows are then cut along them), 52 / 100 / 99 MB for heads of 64 / 128 /
  * 256; not with force_path MLD_KV4_PATH_FEW_ROWS.  A plan may be used from one
- * stream at a time; calls may be captured. */
+ * stream at a time, with its device current; calls may be captured. */
 MLD_API int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out);
 MLD_API int mld_kv4_attn_plan_destroy(mld_kv4_attn_plan* plan);
 MLD_API size_t mld_kv4_attn_plan_workspace_bytes(const mld_kv4_attn_plan* plan);
 MLD_API int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* stream);
-/* Synchronous: *code = 0, or what a kernel found since the last call (then
- * cleared): MLD_OUT_OF_RANGE for a page, length or row range on the device that
- * does not fit (pages outside the pool are read as page 0, lengths and ranges
- * are cut, nothing is accessed out of range), MLD_TIMEOUT for a bounded wait
- * that gave up. */
+/* Waits for the plan's device, whichever is current: *code = 0, or what a
+ * kernel found since the last call (then cleared): MLD_OUT_OF_RANGE for a page,
+ * length or row range on the device that does not fit (pages outside the pool
+ * are read as page 0, lengths and ranges are cut, nothing is accessed out of
+ * range), MLD_TIMEOUT for a bounded wait that gave up. */
 MLD_API int mld_kv4_attn_plan_device_status(mld_kv4_attn_plan* plan, int32_t* code);
 
 #ifdef __cplusplus

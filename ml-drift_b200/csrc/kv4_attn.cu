@@ -972,7 +972,11 @@ int mld_kv4_attn_plan_create(const mld_kv4_attn_desc* d, mld_kv4_attn_plan** out
     return MLD_CUDA_ERROR;
   };
   int before = -1;
-  if (cudaGetDevice(&before) != cudaSuccess || cudaSetDevice(p->device) != cudaSuccess) return fail("cudaSetDevice");
+  if (cudaGetDevice(&before) != cudaSuccess) return fail("cudaGetDevice");
+  if (cudaSetDevice(p->device) != cudaSuccess) {
+    cudaSetDevice(before);
+    return fail("cudaSetDevice");
+  }
   p->grid = sm_count(p->device);
   if (p->grid > kMaxGrid) p->grid = kMaxGrid;
   size_t part = static_cast<size_t>(p->grid) * 2 * 16 * (d->cache.head_dim + 4) * sizeof(float), pieces = 0;
@@ -1005,10 +1009,16 @@ size_t mld_kv4_attn_plan_workspace_bytes(const mld_kv4_attn_plan* plan) { return
 int mld_kv4_attn_plan_device_status(mld_kv4_attn_plan* plan, int32_t* code) {
   MLD_REQUIRE(plan != nullptr && code != nullptr, "null argument");
   *code = 0;
-  MLD_CUDA_CHECK(cudaDeviceSynchronize());
-  MLD_CUDA_CHECK(cudaMemcpy(code, plan->error, sizeof(int), cudaMemcpyDeviceToHost));
+  // The plan's device, which need not be the current one, is what has to be idle while its words are read and cleared.
+  int before = -1;
+  MLD_CUDA_CHECK(cudaGetDevice(&before));
+  MLD_CUDA_CHECK(cudaSetDevice(plan->device));
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(code, plan->error, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && *code != 0) e = zero_now(plan->tickets, (kTickets + 1) * sizeof(int));
+  cudaSetDevice(before);
+  MLD_CUDA_CHECK(e);
   if (*code == 0) return MLD_OK;
-  MLD_CUDA_CHECK(zero_now(plan->tickets, (kTickets + 1) * sizeof(int)));
   if (*code == kErrPage) {
     set_last_error_text("a page table names a page that the pool does not have");
     return MLD_OUT_OF_RANGE;
@@ -1024,6 +1034,9 @@ int mld_kv4_attn_plan_device_status(mld_kv4_attn_plan* plan, int32_t* code) {
 int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* stream_v) {
   MLD_REQUIRE(plan != nullptr && io != nullptr, "null argument");
   const mld_kv4_attn_desc& d = plan->d;
+  int device = -1;
+  MLD_CUDA_CHECK(cudaGetDevice(&device));
+  MLD_REQUIRE(device == plan->device, "the plan belongs to another device than the current one");
   MLD_REQUIRE(io->batch >= 0 && io->batch <= d.max_batch, "batch exceeds the plan's max_batch");
   MLD_REQUIRE(io->q_tokens >= 0 && io->max_queries >= 0, "bad query count");
   if (io->batch == 0 || io->q_tokens == 0 || io->max_queries == 0) return MLD_OK;

@@ -2,6 +2,8 @@
 
 Tolerances are those of the operators' other tests: attention 2^-11 of the output and of sum(p |v|), a tenth on top; rotation a
 handful of roundings of 2^-24 of a row's size and of the output's type."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -147,3 +149,18 @@ def test_any_tensor_in_host_memory_is_refused(mld):
                     call(**{**args, name: t.cpu()})
         call(**args)
     assert attention.device_status() == 0
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_a_plan_is_run_on_its_own_device_and_asked_from_any(mld):
+    with torch.cuda.device(1):
+        cache = mld.Kv4Cache(1, 64, 16, 4, device="cuda:1")
+        plan = mld.Kv4Attention(cache, 1, 1, 4)
+        q = torch.zeros(1, 1, 64, dtype=torch.float16, device="cuda:1")
+        table, lens = torch.full((1, 4), 9, dtype=torch.int32, device="cuda:1"), torch.full((1,), 40, dtype=torch.int32, device="cuda:1")
+        plan.run(q, table, lens, torch.empty_like(q), stream=torch.cuda.Stream())
+    with torch.cuda.device(0):
+        assert plan.device_status() != 0 and plan.device_status() == 0
+        assert torch.cuda.current_device() == 0
+        io = mld.binding.Kv4AttnIo(q.data_ptr(), 64, cache.address(), table.data_ptr(), lens.data_ptr(), None, 1, 1, 1, q.data_ptr(), 64)
+        assert mld.lib().mld_kv4_attn_run(plan._h, ctypes.byref(io), None) == mld.INVALID_ARGUMENT
