@@ -597,15 +597,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
   pdl_wait();
   // ---- how many items lie ahead of each sequence
   int items = 0, segments = 0;
+  bool deal;  // evenly over all CTAs
   {
     const int per = (a.batch + WARPS * 32 - 1) / (WARPS * 32);
     const int b0 = threadIdx.x * per, b1 = min(a.batch, b0 + per);
     int mine = 0, mine_segs = 0;
+    bool mine_long = false;
     for (int b = b0; b < b1; ++b) {
       const Span s = span_of<D, NT>(a, b);
       if (blockIdx.x == 0 && !kv4_fits(a, b, {s.n, s.m, s.first_row_token})) atomicExch(a.error, kErrLength);
       mine += a.kv_heads * s.blocks * s.chunks;
       mine_segs += a.kv_heads * s.blocks;
+      mine_long = mine_long || (s.blocks > 0 && s.chunks > 3 * WARPS);
     }
     int incl = mine;
 #pragma unroll
@@ -618,7 +621,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       warp_items[warp] = incl;
       warp_segs[warp] = mine_segs;
     }
-    __syncthreads();
+    deal = __syncthreads_or(mine_long);
     int ahead = incl - mine;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) {
@@ -636,9 +639,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
     __syncthreads();
   }
   if (items == 0) return;
-  // Segments of two chunks a warp at most on average: a CTA takes whole ones, as joining parts through the workspace costs more
-  // than the work that is dealt out unevenly.  Else a CTA's warps have a chunk each at least.
-  const bool snap = items <= 2 * WARPS * segments && segments <= static_cast<int>(gridDim.x);
+  // Where no segment has more than three chunks a warp, a CTA takes whole ones: joining parts through the workspace takes longer than
+  // the chunks that are dealt out unevenly.  Whole / dealt, us, 8 heads of 128, one sequence of 36 chunks among 17 of one: 12.3 / 13.2,
+  // of 48: 14.0 / 13.4, of 144: 27 / 15; 18 sequences of 25: 11.3 / 17.2; one alone of 36: 12.3 / 12.5.  Else a CTA's warps have a
+  // chunk each at least.
+  const bool snap = !deal && segments <= static_cast<int>(gridDim.x);
   const int ctas = min(static_cast<int>(gridDim.x), snap ? segments : (items + WARPS - 1) / WARPS);
   const int cta = blockIdx.x;
   if (cta >= ctas) return;

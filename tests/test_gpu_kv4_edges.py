@@ -100,6 +100,50 @@ def test_a_sequence_of_almost_2_31_tokens(mld):
     assert (np.abs(out.cpu().numpy() - want) <= tol).all()
 
 
+def _time(call):
+    """Microseconds of a call, the smallest of five means of ten."""
+    for _ in range(3):
+        call()
+    best = float("inf")
+    for _ in range(5):
+        begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        begin.record()
+        for _ in range(10):
+            call()
+        end.record()
+        end.synchronize()
+        best = min(best, begin.elapsed_time(end) * 100)
+    return best
+
+
+def _timed_batch(mld, kv_heads, lens, news, pages=0):
+    """A batch over one pool of random codes, page tables that share its pages; the call."""
+    page, d, g = 64, 128, 4
+    cache = mld.Kv4Cache(kv_heads, d, page, 512)
+    k = torch.randn(512 * page, kv_heads, d, device="cuda").half()
+    cache.write(k, k, torch.arange(512 * page, dtype=torch.int32, device="cuda"))
+    pages = max(pages, -(-max(lens) // page))
+    table = torch.randint(0, 512, (len(lens), pages), dtype=torch.int32, device="cuda")
+    starts = np.concatenate(([0], np.cumsum(news))).astype(np.int32)
+    q = torch.randn(int(starts[-1]), kv_heads * g, d, device="cuda").half()
+    plan, out = mld.Kv4Attention(cache, kv_heads * g, len(lens), pages), torch.empty_like(q)
+    lens, starts, longest = _dev(np.int32(lens)), _dev(starts), max(news)
+    return lambda: plan.run(q, table, lens, out, q_starts=starts, max_queries=longest)
+
+
+def test_one_long_sequence_among_many_short_ones(mld):
+    lens = [int(n) for n in np.random.default_rng(3).integers(1, 33, 147)]
+    lens.insert(70, 108000)
+    _attention_case(mld, 51, 128, 1, 4, 64, lens, [1] * 148)
+
+
+@pytest.mark.parametrize("kv_heads,shorter,longest", [(1, 147, 108000), (8, 17, 13000)])
+def test_a_long_sequence_takes_no_longer_for_short_ones_beside_it(mld, kv_heads, shorter, longest):
+    alone = _time(_timed_batch(mld, kv_heads, [longest], [1]))
+    beside = _time(_timed_batch(mld, kv_heads, [20] * (shorter // 2) + [longest] + [20] * (shorter - shorter // 2), [1] * (shorter + 1)))
+    assert beside < 3 * alone + 20, (alone, beside)
+
+
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 @pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 60, 1 << 20])
 def test_a_window_wider_than_any_sequence_hides_nothing(mld, head_dim, window):
