@@ -912,10 +912,11 @@ int launch_attn_t(const Kv4AttnArgs& a, int grid, cudaStream_t stream) {
   return MLD_OK;
 }
 
-// The pieces of work of a call are counted in 32 bits in this kernel.
-bool countable(const mld_kv4_attn_desc& d, int batch, int64_t rows) {
+// The pieces of work of a call are counted in 32 bits in this kernel, whatever row ranges the device holds: every sequence may have as
+// many rows as any.
+bool countable(const mld_kv4_attn_desc& d, const Kv4AttnArgs& a) {
   const double tiles = static_cast<double>(d.max_pages) * (d.cache.page_tokens / kv4::kTile);
-  return tiles * batch * d.cache.kv_heads * div_up64(rows, 8) <= 2147483647.0;
+  return tiles * a.batch * d.cache.kv_heads * div_up64(static_cast<int64_t>(a.max_queries) * a.group, 8) <= 2147483647.0;
 }
 
 // Whether a call's rows are worked on here or in blocks of 256 (128 for heads of 256) on the tensor cores.  64 tokens cost this
@@ -929,11 +930,11 @@ bool countable(const mld_kv4_attn_desc& d, int batch, int64_t rows) {
 // Where sequences are too short to be cut, that kernel's time is a fixed one per wave of its blocks, of which one walks all tokens.
 // Both sides, us, 4096 tokens: 8 heads of 128, 512 rows 70 / 85, 1024 rows 119 / 85; 32 heads, 128 rows 58 / 83, 256 rows 96 / 85; 64
 // heads of 64, 128 rows 57 / 75, 256 rows 85 / 76; 8 heads of 256, 256 rows 67 / 127, 1024 rows 213 / 128.
-bool few_rows(const mld_kv4_attn_desc& d, int batch, int64_t rows, int sms, bool cut) {
-  if (!countable(d, batch, rows)) return false;
-  const int64_t units = static_cast<int64_t>(batch) * d.cache.kv_heads;
+bool few_rows(const mld_kv4_attn_desc& d, const Kv4AttnArgs& a, int sms, bool cut) {
+  if (!countable(d, a)) return false;
   const int dim = d.cache.head_dim;
-  const int64_t small = units * div_up64(rows, dim == 256 ? 8 : 16), large = units * div_up64(rows, dim == 256 ? 128 : 256);
+  const auto heads_blocks = [&](int rows) { return a.kv_heads * kv4_blocks(a.batch, a.max_queries, a.q_tokens, a.group, rows); };
+  const int64_t small = heads_blocks(dim == 256 ? 8 : 16), large = heads_blocks(dim == 256 ? 128 : 256);
   if (cut) return dim == 64 ? small <= 4.5 * large + 150 : dim == 128 ? small <= 2.6 * large + 104 : small <= 2.7 * large + 75;
   return small <= (dim == 64 ? 1000 : dim == 128 ? 450 : 500) * div_up64(large, sms);
 }
@@ -1084,16 +1085,15 @@ int mld_kv4_attn_run(mld_kv4_attn_plan* plan, const mld_kv4_attn_io* io, void* s
   a.slots = plan->slots;
   a.error = plan->error;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
-  const int64_t rows = static_cast<int64_t>(io->max_queries) * a.group;
   const bool cut = plan->pieces != nullptr && kv4_cuts(a, d.cache.head_dim);
   if (!cut) a.pieces = nullptr;
-  if (d.force_path == MLD_KV4_PATH_MANY_ROWS || (d.force_path == MLD_KV4_PATH_AUTO && !few_rows(d, io->batch, rows, plan->grid, cut)))
+  if (d.force_path == MLD_KV4_PATH_MANY_ROWS || (d.force_path == MLD_KV4_PATH_AUTO && !few_rows(d, a, plan->grid, cut)))
     return launch_kv4_prefill(a, d.cache.head_dim, plan->grid, stream);
-  if (!countable(d, io->batch, rows)) {
+  if (!countable(d, a)) {
     set_last_error_text("more work than one call of this path can count: fewer sequences, or a narrower page table");
     return MLD_OUT_OF_RANGE;
   }
-  const bool few = rows <= 8;
+  const bool few = static_cast<int64_t>(io->max_queries) * a.group <= 8;
   switch (d.cache.head_dim) {
     case 64:
       return few ? launch_attn_t<64, 1, 12>(a, plan->grid, stream) : launch_attn_t<64, 2, 12>(a, plan->grid, stream);

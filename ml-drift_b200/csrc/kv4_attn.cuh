@@ -35,6 +35,12 @@ constexpr int kKv4MaxEntries = 4096;
 // heads of 128, 2048 rows, 65536 tokens 768 us against 635, 4 sequences of 16384 583 against 454.
 constexpr int kKv4Slots = 5;
 size_t kv4_slot_bytes(int head_dim);
+// Blocks of `rows` rows that the sequences of a call have at most, for each key/value head: none has more than `max_queries` tokens, all
+// together have `q_tokens`.  (A chunk of a prompt beside single tokens: counted by its own rows, not by them times the batch.)
+inline int64_t kv4_blocks(int64_t batch, int64_t max_queries, int64_t q_tokens, int64_t group, int64_t rows) {
+  const int64_t alike = batch * div_up64(max_queries * group, rows), together = batch + q_tokens * group / rows;
+  return alike < together ? alike : together;
+}
 // Whether sequences of so many tokens can be long enough for that; whether a call's blocks may be cut.
 bool kv4_can_cut(int64_t tokens);
 bool kv4_cuts(const Kv4AttnArgs& a, int head_dim);

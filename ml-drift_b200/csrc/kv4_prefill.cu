@@ -229,33 +229,95 @@ __device__ __forceinline__ BlockSteps block_steps(const Kv4AttnArgs& a, const Kv
   return s;
 }
 
+// Blocks of rows that a sequence has.
+template <int D>
+__device__ __forceinline__ int blocks_of(const Kv4AttnArgs& a, const Kv4Sequence& q) {
+  return static_cast<int>((static_cast<long long>(q.m) * a.group + Prefill<D>::kRows - 1) / Prefill<D>::kRows);
+}
+
 // Cuts long blocks of rows along the cached tokens where all SMs are done sooner for it.  One block of 1024 threads; an entry is a
-// block of rows of a sequence, those with the most tokens ahead of them first.  Warp w weighs cutting everything longer than
+// block of rows of a sequence, those with the most blocks of their sequence ahead of them first (every sequence's last block, if it has
+// as many as the one with the most, and so on).  Warp w weighs cutting everything longer than
 // 1 / pieces_of(w) of the longest entry into pieces no longer than that: the time is an SM's share of all pieces and half of the
 // longest one's (or that, if longer), and what the last of a block's pieces takes to join them.  A piece is (sequence, block,
 // piece | pieces << 16, slot of the block's first); one for each key/value head.
 __device__ __forceinline__ int pieces_of(int w) { return w < 16 ? w + 1 : 16 + (w - 15) * 8; }
 
-template <int D>
-__global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks, int sms) {
-  constexpr int kPer = kKv4MaxEntries / 1024;
-  __shared__ int s_steps[kKv4MaxEntries], s_count[32], s_slots[32], s_longest;
-  __shared__ float s_time[32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, entries = row_blocks * a.batch;
-  if (threadIdx.x == 0) s_longest = 1;
+// Ahead of the thread in the block of 1024, and in all; every thread calls it.
+__device__ __forceinline__ int sum_before(int mine, int (&warps)[32], int& all) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xFFFFFFFFu, incl, o);
+    if (lane >= o) incl += v;
+  }
+  if (lane == 31) warps[warp] = incl;
   __syncthreads();
+  int before = incl - mine;
+  all = 0;
+  for (int w = 0; w < 32; ++w) {
+    if (w < warp) before += warps[w];
+    all += warps[w];
+  }
+  return before;
+}
+
+template <int D>
+__global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __grid_constant__ Kv4AttnArgs a, int entries, int sms) {
+  constexpr int kPer = kKv4MaxEntries / 1024;
+  // sequences in the order of their blocks, most first: key, number; end[c]: entries of the blocks that more than c sequences have
+  __shared__ __align__(16) int s_key[kKv4MaxBatch];
+  __shared__ int s_blocks[kKv4MaxBatch + 1], s_sequence[kKv4MaxBatch], s_end[kKv4MaxBatch];
+  __shared__ int s_steps[kKv4MaxEntries], s_scan[3][32], s_longest;
+  __shared__ float s_time[32];
+  static_assert(kKv4MaxBatch == 1024, "a thread to a sequence");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int own = threadIdx.x;  // a sequence, then a place in their order
+  if (threadIdx.x == 0) s_longest = 1;
   pdl_wait();
+  int blocks = 0;
+  if (own < a.batch) blocks = min(blocks_of<D>(a, kv4_sequence(a, own)), entries);
+  const int key = own < a.batch ? blocks << 10 | (1023 - own) : -1;
+  s_key[own] = key;
+  __syncthreads();
+  if (own < a.batch) {
+    int place = 0;
+    for (int i = 0; i < a.batch; i += 4) {
+      const int4 others = *reinterpret_cast<const int4*>(s_key + i);
+      place += (others.x > key ? 1 : 0) + (others.y > key ? 1 : 0) + (others.z > key ? 1 : 0) + (others.w > key ? 1 : 0);
+    }
+    s_blocks[place] = blocks;
+    s_sequence[place] = own;
+  }
+  if (own == 0) s_blocks[a.batch] = 0;
+  __syncthreads();
+  {
+    int all;
+    blocks = own < a.batch ? s_blocks[own] : 0;
+    const int before = sum_before(blocks, s_scan[0], all);
+    // the first own + 1 sequences' blocks from the number on that the next sequence has
+    if (own < a.batch) s_end[own] = before + blocks - (own + 1) * s_blocks[own + 1];
+  }
+  __syncthreads();
+  const int there = min(s_end[a.batch - 1], entries);
   const auto place = [&](int e, int& b, int& block) {
-    const int rank = e / a.batch;
-    b = e - rank * a.batch;
-    block = row_blocks - 1 - rank;
+    int lo = 0, hi = a.batch - 1;
+    while (lo < hi) {  // the first group of blocks that ends behind the entry
+      const int mid = (lo + hi) >> 1;
+      if (s_end[mid] > e) hi = mid; else lo = mid + 1;
+    }
+    const int in = lo > 0 ? e - s_end[lo - 1] : e, row = in / (lo + 1);
+    b = s_sequence[in - row * (lo + 1)];
+    block = s_blocks[lo] - 1 - row;
   };
   int longest = 1;
   for (int e = threadIdx.x; e < entries; e += 1024) {
     int b, block, steps = -1;  // no rows
-    place(e, b, block);
-    const Kv4Sequence q = kv4_sequence(a, b);
-    if (static_cast<long long>(block) * Prefill<D>::kRows < q.m * a.group) steps = block_steps<D>(a, q, block).steps;
+    if (e < there) {
+      place(e, b, block);
+      steps = block_steps<D>(a, kv4_sequence(a, b), block).steps;
+    }
     s_steps[e] = steps;
     longest = max(longest, steps);
   }
@@ -300,34 +362,13 @@ __global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __gri
     count += pieces[i];
     slots += pieces[i] > 1 ? pieces[i] : 0;
   }
-  const int own_count = count, own_slots = slots;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int c = __shfl_up_sync(0xFFFFFFFFu, count, o), l = __shfl_up_sync(0xFFFFFFFFu, slots, o);
-    if (lane >= o) {
-      count += c;
-      slots += l;
-    }
-  }
-  if (lane == 31) {
-    s_count[warp] = count;
-    s_slots[warp] = slots;
-  }
-  count -= own_count;
-  slots -= own_slots;
-  __syncthreads();
-  int end = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w < warp) {
-      count += s_count[w];
-      slots += s_slots[w];
-    }
-    end += s_count[w];
-  }
+  int end, all_slots;
+  count = sum_before(count, s_scan[1], end);
+  slots = sum_before(slots, s_scan[2], all_slots);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    int b, block;
-    place(threadIdx.x * kPer + i, b, block);
+    int b = 0, block = 0;
+    if (pieces[i] > 0) place(threadIdx.x * kPer + i, b, block);
     for (int k = 0; k < pieces[i]; ++k) a.pieces[count + k] = make_int4(b, block, k | pieces[i] << 16, slots);
     count += pieces[i];
     slots += pieces[i] > 1 ? pieces[i] : 0;
@@ -335,10 +376,39 @@ __global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __gri
   for (int i = end + threadIdx.x; i < entries + room; i += 1024) a.pieces[i] = make_int4(-1, 0, 0, 0);
 }
 
+// The item-th block of rows of a call without a list, in the list's order; a warp together, which gets the same as any other.  `counts`:
+// blocks of each sequence, none more than `most`.  False: there are not so many.
+__device__ __forceinline__ bool find_block(const int* counts, int batch, int most, int item, int& b, int& block) {
+  const int lane = threadIdx.x & 31, first = lane < batch ? counts[lane] : 0;
+  const auto from = [&](int k) {  // blocks of all sequences from number k on
+    unsigned sum = max(0, first - k);
+    for (int i = lane + 32; i < batch; i += 32) sum += max(0, counts[i] - k);
+    return __reduce_add_sync(0xFFFFFFFFu, min(sum, 1u << 26));  // no 32 bits overflow, whatever row ranges a call has
+  };
+  if (from(0) <= static_cast<unsigned>(item)) return false;
+  int lo = 0, hi = most;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > static_cast<unsigned>(item)) lo = mid; else hi = mid;
+  }
+  block = lo;
+  int left = item - static_cast<int>(from(lo + 1));
+  for (int i = 0; i < batch; i += 32) {
+    const bool mine = i + lane < batch && counts[i + lane] > lo;
+    const unsigned has = __ballot_sync(0xFFFFFFFFu, mine);
+    if (left < __popc(has)) {
+      b = i + __ffs(__ballot_sync(0xFFFFFFFFu, mine && __popc(has & ((1u << lane) - 1u)) == left)) - 1;
+      return true;
+    }
+    left -= __popc(has);
+  }
+  return false;
+}
+
 // kCut: blocks may be cut, and are listed.  Calls whose sequences are too short for that take the form without the joining, which
 // costs the loop registers (a prompt of 2048 tokens 60 us in its own form, 62 to 65 in the other).
 template <int D, bool kCut>
-__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks) {
+__global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const __grid_constant__ Kv4AttnArgs a, int row_blocks, bool alike) {
   using S = Prefill<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -383,16 +453,22 @@ __global__ void __launch_bounds__(kPrefillThreads, 1) kv4_prefill_kernel(const _
     piece = p.z & 0xFFFF;
     pieces = p.z >> 16;
     slot = p.w * a.kv_heads + h;
-  } else {
+  } else if (alike) {
     const int rank = item / a.batch;
     b = item - rank * a.batch;
     block = row_blocks - 1 - rank;
+  } else {
+    int* const counts = reinterpret_cast<int*>(s_pack);
+    static_assert(kKv4MaxBatch * sizeof(int) <= S::kRing * S::kPackBytes, "a count for each sequence");
+    for (int i = threadIdx.x; i < a.batch; i += kPrefillThreads) counts[i] = blocks_of<D>(a, kv4_sequence(a, i));
+    __syncthreads();
+    if (!find_block(counts, a.batch, row_blocks, item, b, block)) b = -1;
   }
   if (blockIdx.x == 0) {
     for (int i = threadIdx.x; i < a.batch; i += kPrefillThreads)
       if (!kv4_fits(a, i, kv4_sequence(a, i))) atomicExch(a.error, kErrLength);
   }
-  if (kCut && b < 0) return;
+  if (b < 0) return;
   const Kv4Sequence q = kv4_sequence(a, b);
   const int rows = q.m * a.group, row0 = block * S::kRows;
   if (row0 >= rows) return;
@@ -796,17 +872,18 @@ int launch_prefill_t(const Kv4AttnArgs& a, int sms, cudaStream_t stream) {
     if (dev >= 0) configured[dev] = true;
   }
   const int64_t row_blocks = div_up64(static_cast<int64_t>(a.max_queries) * a.group, S::kRows);
-  const int64_t grid = (row_blocks * a.batch + (kCut ? a.slots / a.kv_heads : 0)) * a.kv_heads;
+  const int64_t blocks = kv4_blocks(a.batch, a.max_queries, a.q_tokens, a.group, S::kRows);
+  const int64_t grid = (blocks + (kCut ? a.slots / a.kv_heads : 0)) * a.kv_heads;
   if (grid > 0x7FFFFFFF) {
     set_last_error_text("more work than one call can count: fewer sequences or queries");
     return MLD_OUT_OF_RANGE;
   }
   if constexpr (kCut) {
-    MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_pieces_kernel<D>, dim3(1), dim3(1024), 0, stream, a, static_cast<int>(row_blocks), sms));
+    MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_pieces_kernel<D>, dim3(1), dim3(1024), 0, stream, a, static_cast<int>(blocks), sms));
     MLD_LAUNCH_CHECK();
   }
   MLD_CUDA_CHECK(launch_overlapped(kv4_prefill_kernel<D, kCut>, dim3(static_cast<unsigned>(grid)), dim3(kPrefillThreads), S::kSmem, stream, a,
-                                   static_cast<int>(row_blocks)));
+                                   static_cast<int>(row_blocks), blocks == row_blocks * a.batch));
   MLD_LAUNCH_CHECK();
   return MLD_OK;
 }
@@ -828,8 +905,8 @@ size_t kv4_slot_bytes(int head_dim) { return head_dim == 64 ? kSlotBytes<64> : h
 bool kv4_can_cut(int64_t tokens) { return tokens > 4096; }
 
 bool kv4_cuts(const Kv4AttnArgs& a, int head_dim) {
-  const int64_t blocks = div_up64(static_cast<int64_t>(a.max_queries) * a.group, head_dim == 256 ? Prefill<256>::kRows : Prefill<128>::kRows);
-  return blocks * a.batch <= kKv4MaxEntries && (a.window == 0 || kv4_can_cut(a.window));
+  const int rows = head_dim == 256 ? Prefill<256>::kRows : Prefill<128>::kRows;
+  return kv4_blocks(a.batch, a.max_queries, a.q_tokens, a.group, rows) <= kKv4MaxEntries && (a.window == 0 || kv4_can_cut(a.window));
 }
 
 int launch_kv4_prefill(const Kv4AttnArgs& a, int head_dim, int sms, cudaStream_t stream) {

@@ -144,6 +144,15 @@ def test_a_long_sequence_takes_no_longer_for_short_ones_beside_it(mld, kv_heads,
     assert beside < 3 * alone + 20, (alone, beside)
 
 
+@pytest.mark.parametrize("history,times", [(131072, 4), (1000, 3)])
+def test_a_chunk_of_a_prompt_beside_many_single_tokens(mld, history, times):
+    """The rows of a call are counted as they are, not as if every sequence had as many as the one with the most."""
+    chunk = _time(_timed_batch(mld, 8, [4000], [2048]))
+    tokens = _time(_timed_batch(mld, 8, [1000] * 127 + [history], [1] * 128))
+    both = _time(_timed_batch(mld, 8, [1000] * 127 + [history, 4000], [1] * 128 + [2048]))
+    assert both < times * (chunk + tokens), (chunk, tokens, both)
+
+
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
 @pytest.mark.parametrize("window", [2**31 - 1, 2**31 - 60, 1 << 20])
 def test_a_window_wider_than_any_sequence_hides_nothing(mld, head_dim, window):
@@ -208,3 +217,41 @@ def test_a_plan_is_run_on_its_own_device_and_asked_from_any(mld):
         assert torch.cuda.current_device() == 0
         io = mld.binding.Kv4AttnIo(q.data_ptr(), 64, cache.address(), table.data_ptr(), lens.data_ptr(), None, 1, 1, 1, q.data_ptr(), 64)
         assert mld.lib().mld_kv4_attn_run(plan._h, ctypes.byref(io), None) == mld.INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("wide", [0, 400])
+def test_batches_of_sequences_with_very_different_rows(mld, head_dim, wide):
+    """Blocks of rows are found by their number: short and long sequences, some without rows, in any order; cut or not."""
+    rng = np.random.default_rng(head_dim)
+    news = [0, 1, 300, 1, 0, 0, 700, 2, 300, 1] + [1] * 60 + [0, 257, 256, 255, 0]
+    lens = [int(n + rng.integers(0, 200)) for n in news]
+    _attention_case(mld, 71, head_dim, 2, 3, 16, lens, news, wide=wide)
+    order = rng.permutation(len(news))
+    _attention_case(mld, 72, head_dim, 1, 1, 32, [lens[i] for i in order], [news[i] for i in order], wide=wide // 2)
+
+
+def test_row_ranges_that_overlap_or_descend_are_reported_and_write_nothing_beside_the_output(mld):
+    cache = mld.Kv4Cache(1, 64, 64, 80)
+    k = torch.randn(80 * 64, 1, 64, device="cuda").half()
+    cache.write(k, k, torch.arange(80 * 64, dtype=torch.int32, device="cuda"))
+    n, batch = 600, 40
+    q = torch.randn(n, 1, 64, device="cuda").half()
+    good = _dev(np.linspace(0, n, batch + 1).astype(np.int32))
+    for pages in (40, 80):  # whole blocks, and blocks that may be cut
+        table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1).contiguous()
+        lens = torch.full((batch,), pages * 64, dtype=torch.int32, device="cuda")
+        for path in (mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+            plan = mld.Kv4Attention(cache, 1, batch, pages, force_path=path)
+            want = torch.full((n + 2, 1, 64), 7.0, dtype=torch.float16, device="cuda")
+            plan.run(q, table, lens, want[1:-1], q_starts=good, max_queries=n)
+            assert plan.device_status() == 0
+            for bad in (np.arange(batch + 1) % 2 * n, np.where(np.arange(batch + 1) % 2, 2**31 - 1, -2**31), np.arange(batch + 1)[::-1] * 15,
+                        np.arange(batch + 1) % 2 * 300):
+                out = torch.full((n + 2, 1, 64), 7.0, dtype=torch.float16, device="cuda")
+                plan.run(q, table, lens, out[1:-1], q_starts=_dev(bad.astype(np.int32)), max_queries=n)
+                assert plan.device_status() != 0
+                assert bool((out[[0, -1]] == 7).all())
+            out = torch.full_like(want, 7.0)
+            plan.run(q, table, lens, out[1:-1], q_starts=good, max_queries=n)
+            assert plan.device_status() == 0 and torch.equal(out, want)
