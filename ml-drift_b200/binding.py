@@ -511,21 +511,20 @@ def _elsewhere(t, what):
 
 def _rows(t, tokens, heads, head_dim, dtype, what, gpu):
     """Elements from token to token of a [tokens][heads][head_dim] tensor whose rows are contiguous."""
-    if t.get_device() != gpu:
-        raise _elsewhere(t, what)
-    n, h, d = t.shape
     stride = t.stride()
-    if n != tokens or t.dtype is not dtype or h != heads or d != head_dim or stride[2] != 1 or \
+    if t.get_device() != gpu or t.dtype is not dtype or t.shape != (tokens, heads, head_dim) or stride[2] != 1 or \
             (stride[1] != head_dim and heads > 1):
+        if t.get_device() != gpu:
+            raise _elsewhere(t, what)
         raise ValueError(f"{what}: expected {dtype} [{tokens}][{heads}][{head_dim}] with contiguous heads, "
                          f"got {t.dtype} {tuple(t.shape)} strides {stride}")
     return stride[0]
 
 
 def _ints(t, shape, what, gpu):
-    if t.get_device() != gpu:
-        raise _elsewhere(t, what)
-    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.get_device() != gpu or t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
+        if t.get_device() != gpu:
+            raise _elsewhere(t, what)
         raise ValueError(f"{what}: expected contiguous int32 {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
