@@ -27,6 +27,7 @@ namespace mld {
 namespace {
 
 constexpr int kThreads = 64;  // few lanes to a token: each works out its cosines and weights once for all its heads
+constexpr int kBlocksPerSm = 16;
 constexpr int kMaxPairs = 128;
 
 struct RopeArgs {
@@ -198,7 +199,7 @@ __device__ __forceinline__ void put_eight(uint8_t* tile, bool is_v, int tau, int
 
 // Blocks: tokens along x; along y, parts of a token's heads (each takes every gridDim.y-th of the groups of kHeads heads).
 template <typename T, int D, bool NEIGHBOURS>
-__global__ void __launch_bounds__(kThreads, 16) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) qk_rope_kernel(const __grid_constant__ RopeArgs a) {
   constexpr int kLanes = D / 8;
   constexpr int kHeads = kThreads / kLanes;
   __shared__ float2 turned[8][kMaxPairs / 8];  // cosine, sine of pair 8 j + i at [i][j]
@@ -363,8 +364,13 @@ __global__ void __launch_bounds__(kThreads) kv4_read_kernel(ReadArgs a) {
   }
 }
 
-// Blocks of a token: as many as it has groups of heads while the GPU has room for them at once, else one.
-int parts_of_token(int tokens, int groups) { return groups < 1 ? 1 : static_cast<int64_t>(tokens) * groups <= 4 * 148 ? groups : 1; }
+// Blocks of a token: as many as it has groups of heads while the GPU has room for them at once, else one, which works a token's cosines
+// and weights out once.  One / a group each, us, 32 + 8 + 8 heads of 128 into the cache: 74 tokens 8.8 / 5.1, 148 9.3 / 5.5, 296 (2368
+// blocks) 9.3 / 6.6, 600 (4800) 10.1 / 11; 8 + 1 heads of 256 in fp32: 148 tokens 5.7 / 5.3, 296 5.9 / 6.2, 600 (2400) 6.7 / 8.4.
+// (148 SMs: asking the runtime for them takes 0.3 us of a call's 4.)
+int parts_of_token(int tokens, int groups) {
+  return groups > 1 && static_cast<int64_t>(tokens) * groups <= kBlocksPerSm * 148 ? groups : 1;
+}
 
 template <typename T, int D>
 int launch_rope_t(const RopeArgs& a, cudaStream_t stream) {

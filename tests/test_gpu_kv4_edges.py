@@ -255,3 +255,25 @@ def test_row_ranges_that_overlap_or_descend_are_reported_and_write_nothing_besid
             out = torch.full_like(want, 7.0)
             plan.run(q, table, lens, out[1:-1], q_starts=good, max_queries=n)
             assert plan.device_status() == 0 and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("head_dim,heads,kv_heads", [(128, 32, 8), (64, 6, 3), (256, 8, 1)])
+def test_how_many_tokens_a_call_has_changes_no_token(mld, head_dim, heads, kv_heads):
+    """Few tokens are spread over blocks by their heads, many are not."""
+    n, page = 1400, 64
+    x = torch.randn(n, heads + 2 * kv_heads, head_dim, device="cuda").half()
+    w = (1 + 0.1 * torch.randn(head_dim, device="cuda")).half()
+    pos = torch.arange(n, dtype=torch.int32, device="cuda")
+    plan, outs = mld.QkNormRope(heads, kv_heads, head_dim), []
+    for some in (n, 600, 290, 75, 1):
+        cache = mld.Kv4Cache(kv_heads, head_dim, page, -(-n // page))
+        q, k, v = (torch.zeros(n, h, head_dim, dtype=torch.float16, device="cuda") for h in (heads, kv_heads, kv_heads))
+        for at in range(0, n, some):
+            part = slice(at, min(n, at + some))
+            y = x[part]
+            plan.run(y[:, :heads], y[:, heads:heads + kv_heads], pos[part], q[part], q_weight=w, k_weight=w, v=y[:, heads + kv_heads:],
+                     cache=cache, slots=pos[part])
+            cache.read(pos[part], k[part], v[part])
+        outs.append((q, k, v, cache.pool))
+    for out in outs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
