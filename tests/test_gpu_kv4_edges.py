@@ -277,3 +277,82 @@ def test_how_many_tokens_a_call_has_changes_no_token(mld, head_dim, heads, kv_he
         outs.append((q, k, v, cache.pool))
     for out in outs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(out, outs[0]))
+
+
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("head_dim,rotary", [(64, 64), (128, 32), (256, 256)])
+@pytest.mark.parametrize("tokens", [1, 90, 700])
+def test_queries_and_keys_of_one_projection_in_place(mld, tokens, head_dim, rotary, neighbours):
+    h, hk = 6, 2
+    x = torch.randn(tokens, h + 2 * hk, head_dim, device="cuda").half()
+    wq, wk = ((1 + 0.2 * torch.randn(head_dim, device="cuda")).half() for _ in range(2))
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda") + 77
+    slots = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    plan = mld.QkNormRope(h, hk, head_dim, rotary, mld.ROPE_NEIGHBOURS if neighbours else mld.ROPE_HALVES)
+    q, k = torch.empty(tokens, h, head_dim, dtype=torch.float16, device="cuda"), torch.empty(tokens, hk, head_dim, dtype=torch.float16, device="cuda")
+    caches = [mld.Kv4Cache(hk, head_dim, 16, -(-tokens // 16)) for _ in range(2)]
+    y = x.clone()
+    plan.run(x[:, :h], x[:, h:h + hk], pos, q, k, q_weight=wq, k_weight=wk, v=x[:, h + hk:], cache=caches[0], slots=slots)
+    plan.run(y[:, :h], y[:, h:h + hk], pos, y[:, :h], y[:, h:h + hk], q_weight=wq, k_weight=wk, v=y[:, h + hk:], cache=caches[1], slots=slots)
+    assert torch.equal(y[:, :h], q) and torch.equal(y[:, h:h + hk], k) and torch.equal(y[:, h + hk:], x[:, h + hk:])
+    assert torch.equal(caches[0].pool, caches[1].pool)
+    want = ref.norm_rope(x[:, :h].cpu().numpy(), wq.cpu().numpy(), 1e-6, pos.cpu().numpy()[None], rotary, neighbours, [rotary // 2], 1.0, 1e6)
+    tol = 16 * 2.0 ** -24 * np.abs(want).max(-1, keepdims=True) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    assert (np.abs(y[:, :h].cpu().numpy() - want) <= tol).all()
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+def test_fp32_keys_of_neighbouring_pairs_in_the_cache(mld, head_dim):
+    n, h, hk = 53, 4, 2
+    rng = np.random.default_rng(head_dim)
+    x = rng.standard_normal((n, h + 2 * hk, head_dim)).astype(np.float32)
+    w = (1 + 0.2 * rng.standard_normal(head_dim)).astype(np.float32)
+    pos = np.arange(n, dtype=np.int32) + 500
+    plan = mld.QkNormRope(h, hk, head_dim, head_dim // 2, mld.ROPE_NEIGHBOURS, f16=False)
+    cache, slots, xd = mld.Kv4Cache(hk, head_dim, 16, 5), torch.arange(n, dtype=torch.int32, device="cuda") + 9, _dev(x)
+    q, k = torch.empty(n, h, head_dim, device="cuda"), torch.empty(n, hk, head_dim, device="cuda")
+    plan.run(xd[:, :h], xd[:, h:h + hk], _dev(pos), q, k, q_weight=_dev(w), k_weight=_dev(w), v=xd[:, h + hk:], cache=cache, slots=slots)
+    want = ref.norm_rope(x[:, h:h + hk], w, 1e-6, pos[None], head_dim // 2, True, [head_dim // 4], 1.0, 1e6)
+    got = k.cpu().numpy()
+    assert (np.abs(got - want) <= 16 * 2.0 ** -24 * np.abs(want).max(-1, keepdims=True)).all()
+    gk, gv = (torch.empty(n, hk, head_dim, dtype=torch.float16, device="cuda") for _ in range(2))
+    cache.read(slots, gk, gv)
+    assert np.array_equal(gk.cpu().numpy().astype(np.float64), ref.quantise(got))
+    assert np.array_equal(gv.cpu().numpy().astype(np.float64), ref.quantise(x[:, h + hk:]))
+
+
+@pytest.mark.parametrize("head_dim,kv_heads,page", [(128, 8, 64), (64, 4, 16), (256, 2, 128)])
+def test_pages_behind_the_first_gigabytes(mld, head_dim, kv_heads, page):
+    """The last pages of the second layer of a cache of 10 GB against the first ones of a small one."""
+    page_bytes = kv_heads * page * head_dim * 18 // 16
+    pages, n, m = (5 << 30) // page_bytes, 700, 150
+    large, small = mld.Kv4Cache(kv_heads, head_dim, page, pages, layers=2), mld.Kv4Cache(kv_heads, head_dim, page, 60)
+    k, v = (torch.randn(n, kv_heads, head_dim, device="cuda").half() for _ in range(2))
+    there = -(-n // page)
+    last = pages - 1 - torch.arange(there, dtype=torch.int32, device="cuda")
+    at = torch.arange(n, dtype=torch.int32, device="cuda")
+    far = last[(at // page).long()] * page + at % page
+    large.write(k, v, far, layer=1)
+    small.write(k, v, at)
+    q = torch.randn(m, kv_heads * 4, head_dim, device="cuda").half()
+    table = torch.zeros(1, 60, dtype=torch.int32, device="cuda")
+    outs, first = [], torch.arange(there, dtype=torch.int32, device="cuda")
+
+    def attend(cache, layer, pages_of):
+        table[0, :there] = pages_of
+        for path in (mld.KV4_PATH_FEW_ROWS, mld.KV4_PATH_MANY_ROWS):
+            out = torch.zeros_like(q)
+            mld.Kv4Attention(cache, kv_heads * 4, 1, 60, force_path=path).run(q, table, _dev(np.int32([n])), out,
+                                                                              q_starts=_dev(np.int32([0, m])), max_queries=m, layer=layer)
+            outs.append(out)
+
+    attend(small, 0, first)
+    attend(large, 1, last)
+    large.copy_pages(last.tolist(), (last - 100).tolist())
+    attend(large, 1, last - 100)
+    assert torch.equal(outs[0], outs[2]) and torch.equal(outs[1], outs[3]) and torch.equal(outs[0], outs[4]) and torch.equal(outs[1], outs[5])
+    assert int(large.pool[0].view(torch.int64).count_nonzero()) == 0
+    read = [torch.empty_like(k) for _ in range(4)]
+    large.read(far, *read[:2], layer=1)
+    small.read(at, *read[2:])
+    assert torch.equal(read[0], read[2]) and torch.equal(read[1], read[3])
