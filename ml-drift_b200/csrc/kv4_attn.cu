@@ -750,8 +750,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
       // branches meet.
 #pragma unroll 1
       while (item < end && token >= whole_lo && token <= whole_hi) {
-        // the warp gives up together, and goes on without waiting or asking
+        // the warp gives up together: what follows needs all of its lanes
         if (alive) alive = __all_sync(0xFFFFFFFFu, mbar_wait(bars + stage, phase));
+        if (!alive) break;
 #pragma unroll
         for (int k = 0; k < S::kTiles; k += S::kStep)
           step<D, NT, S::kStep, false>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, 0, 0, 0);
@@ -764,7 +765,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) kv4_attn_kernel(const __grid_co
 #pragma unroll 1
         for (int k = 0; k < S::kTiles; k += S::kStep) {
           const int from = token + k * kv4::kTile;
-          if (from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
+          if (!alive || from > sees_hi || from + S::kStep * kv4::kTile <= first_lo) continue;
           step<D, NT, S::kStep, true>(ring + stage * S::kStageBytes + k * S::kTileBytes, at, w, sees, a.window, from, p.s.n);
         }
         release();

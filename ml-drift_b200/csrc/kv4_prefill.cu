@@ -267,9 +267,10 @@ template <int D>
 __global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __grid_constant__ Kv4AttnArgs a, int entries, int sms) {
   constexpr int kPer = kKv4MaxEntries / 1024;
   // sequences in the order of their blocks, most first: key, number; end[c]: entries of the blocks that more than c sequences have
-  __shared__ __align__(16) int s_key[kKv4MaxBatch];
+  __shared__ __align__(16) int s_place[kKv4MaxEntries];  // of the entries: number of the block, sequence
+  int* const s_key = s_place;                            // ahead of that
   __shared__ int s_blocks[kKv4MaxBatch + 1], s_sequence[kKv4MaxBatch], s_end[kKv4MaxBatch];
-  __shared__ int s_steps[kKv4MaxEntries], s_scan[3][32], s_longest;
+  __shared__ int s_steps[kKv4MaxEntries], s_scan[2][32], s_longest;
   __shared__ float s_time[32];
   static_assert(kKv4MaxBatch == 1024, "a thread to a sequence");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -301,21 +302,18 @@ __global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __gri
   }
   __syncthreads();
   const int there = min(s_end[a.batch - 1], entries);
-  const auto place = [&](int e, int& b, int& block) {
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {  // the first group of blocks that ends behind the entry
-      const int mid = (lo + hi) >> 1;
-      if (s_end[mid] > e) hi = mid; else lo = mid + 1;
-    }
-    const int in = lo > 0 ? e - s_end[lo - 1] : e, row = in / (lo + 1);
-    b = s_sequence[in - row * (lo + 1)];
-    block = s_blocks[lo] - 1 - row;
-  };
   int longest = 1;
   for (int e = threadIdx.x; e < entries; e += 1024) {
-    int b, block, steps = -1;  // no rows
+    int steps = -1;  // no rows
     if (e < there) {
-      place(e, b, block);
+      int lo = 0, hi = a.batch - 1;
+      while (lo < hi) {  // the first group of blocks that ends behind the entry
+        const int mid = (lo + hi) >> 1;
+        if (s_end[mid] > e) hi = mid; else lo = mid + 1;
+      }
+      const int in = lo > 0 ? e - s_end[lo - 1] : e, row = in / (lo + 1);
+      const int b = s_sequence[in - row * (lo + 1)], block = s_blocks[lo] - 1 - row;
+      s_place[e] = block << 10 | b;
       steps = block_steps<D>(a, kv4_sequence(a, b), block).steps;
     }
     s_steps[e] = steps;
@@ -362,13 +360,16 @@ __global__ void __launch_bounds__(1024, 1) kv4_prefill_pieces_kernel(const __gri
     count += pieces[i];
     slots += pieces[i] > 1 ? pieces[i] : 0;
   }
-  int end, all_slots;
-  count = sum_before(count, s_scan[1], end);
-  slots = sum_before(slots, s_scan[2], all_slots);
+  // both sums in one number: fewer than 2^13 pieces in all, fewer than 2^12 slots
+  static_assert(kKv4MaxEntries + 256 * kKv4Slots < 1 << 13, "a list's pieces");
+  int both;
+  const int before = sum_before(count << 12 | slots, s_scan[1], both), end = both >> 12;
+  count = before >> 12;
+  slots = before & 0xFFF;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    int b = 0, block = 0;
-    if (pieces[i] > 0) place(threadIdx.x * kPer + i, b, block);
+    if (pieces[i] == 0) continue;
+    const int at = s_place[threadIdx.x * kPer + i], b = at & 1023, block = at >> 10;
     for (int k = 0; k < pieces[i]; ++k) a.pieces[count + k] = make_int4(b, block, k | pieces[i] << 16, slots);
     count += pieces[i];
     slots += pieces[i] > 1 ? pieces[i] : 0;
