@@ -719,7 +719,10 @@ MLD_API int mld_qk_rope_run(mld_qk_rope_plan* plan, const mld_qk_rope_io* io, in
  * qwen3_model_builder.cc:983-1017).  Head h reads key/value head
  * h / (heads / kv_heads).  Query token i of m of a sequence of n cached tokens
  * stands at n - m + i and sees the tokens at or before it, with a window only
- * the last `window` of those; a query that sees none gives zeros. */
+ * the last `window` of those; a query that sees none gives zeros.  Rows of q that
+ * no sequence has are not written.  Scores, maxima, sums and outputs are held in
+ * 32 bits; exponentials are good to 2^-20, and the weights are rounded to fp16
+ * (11 bits, times the scale of V with few rows) for the product with the values. */
 typedef enum mld_kv4_path {
   MLD_KV4_PATH_AUTO = 0,
   MLD_KV4_PATH_FEW_ROWS = 1, /* cut over all SMs without regard to sequences:

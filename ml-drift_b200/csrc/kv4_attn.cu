@@ -3,8 +3,10 @@
 //   o_i = sum_t softmax_t(scale q_i.k_t) v_t over the tokens t that row i sees; nothing seen gives zeros.
 //
 // What it cannot do without is reading the cache once: 18 D / 16 bytes per token and head (144 for D = 128, 3.6 times fewer than
-// fp16).  What bounds it is unpacking: one token over 131071 of 8 heads of 128 takes 48 us, 3.15 TB/s, where copies into the same
-// rings without the arithmetic take 22; 64 ragged sequences of up to 8191 tokens 95 us, 2.9 TB/s; 300 tokens 8 us, all latencies.
+// fp16).  One token over 131071 of 8 heads of 128 takes 48 us, 3.1 TB/s, where copies into the same rings without the arithmetic take
+// 22; 64 ragged sequences of up to 8191 tokens 97 us, 2.9 TB/s; 300 tokens 8 us, all latencies.  What bounds the long ones is a warp's
+// chain of instructions (scores, vote, exponentials, transposition, values), of which three to a scheduler fill 2.2 of 4 issue slots:
+// 390 for a tile of 16 tokens, 120 of them unpacking; then about 8 us of joining.
 // The queries of all heads that share a key/value head, and of all new tokens of a sequence, are the columns of the products,
 // so a code is unpacked once for all of them:
 //   S^T[token][row] = K q:  A = codes of K as they lie, masked into fp16 subnormals u 2^-24 (and 16 u 2^-24 for the odd nibbles,
@@ -65,8 +67,8 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t x) { return __half22floa
 
 // (u - 8) 2^-9 of the codes in bits 0..3 (lo), 4..7 (hi) of both halves: what the mask leaves is an fp16 subnormal, u 2^-24 or
 // u 2^-20, which one fused multiply-add turns into that, exactly.  Masks, shifts and these multiply-adds share a pipe that takes one
-// in two cycles, which is what bounds the kernel's arithmetic: 64 masks, 24 shifts and permutations and 32 multiply-adds to 16
-// tokens of 128 values.
+// in two cycles: 64 masks, 24 shifts and permutations and 32 multiply-adds to 16 tokens of 128 values, 13.5 us for 131071 tokens of
+// 8 heads.
 constexpr float kCodeUnit = 512.0f;
 __device__ __forceinline__ uint32_t fma_half2(uint32_t x, float scale, float offset) {
   const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&x), __float2half2_rn(scale), __float2half2_rn(offset));

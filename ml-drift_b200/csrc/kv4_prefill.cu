@@ -7,12 +7,15 @@
 //   O += P V         V from shared memory, 128 x D fp32 in tensor memory
 // The next step's S is asked for ahead of this step's O, so that the threads that make P find it ready: steps of 128 tokens, of
 // which tensor memory holds one S per tile beside O, had every thread wait for its own products (ragged chunks 938 us against
-// 902, whole blocks).  A step of a pair of tiles takes about 2250 cycles where its products take 1024: exponentials, unpacking and the
-// reads of K and V for 64 columns a product bound it.
+// 902, whole blocks).  A step of a pair of tiles takes about 2200 cycles where its products take 1024.  No one pipe is full (tensor 29 %,
+// exponentials 31 %, 1.7 of 4 issue slots), and forms of an earlier stage without the exponentials, the maxima or the unpacking took
+// as long as the whole.  A score product of 128 x 64 x 16 reads 6 KB of shared memory, 48 cycles at 128 bytes, for 32 of tensor work:
+// the likeliest bound, beside the chain from scores to weights.
 // Blocks of long sequences are cut along the tokens where that fills the SMs (kv4_prefill_pieces_kernel): a piece leaves its sums
 // and their reference in the plan's workspace, and the last one of a block joins them in the pieces' order.  Whole / cut, us, 8
 // heads of 128: 2048 rows, 16384 tokens 303 / 187; 4 times that 583 / 454; 256 rows, 65536 tokens 1210 / 126.
-// Measured (32 heads of 128 over 8): 576 TFLOP/s for a prompt of 2048 tokens, 811 for ragged chunks behind up to 16384.
+// Measured (32 heads of 128 over 8): 588 TFLOP/s for a prompt of 2048 tokens, 802 for ragged chunks behind up to 16384; a prompt of
+// 2048 with heads of 64 45 us, with heads of 256 136, 386 and 504 TFLOP/s.
 // The cache's values are fp16 numbers exactly, so unpacking rounds nothing; V's rows lie with the head's values contiguous, as the
 // cache has them (the product takes them transposed), four of eight neighbours interleaved, which the output undoes for nothing.
 // ref is a row's running maximum, which moves only when a step exceeds it by 2^5: then the row's sums in tensor memory are scaled

@@ -6,13 +6,17 @@
 //   y = x * w / sqrt(mean(x^2) + eps);   pair i of a head: (a, b) -> (a cos - b sin, b cos + a sin),
 //   angle = position[axis of i] / (min_timescale * (max_timescale / min_timescale)^(2 i / rotary_dim))
 // The angle is taken in turns, as a product of 32 x 64-bit integers modulo one turn (2^64), since a 32-bit float loses the
-// decimals of position * frequency for long contexts (position 131071: 0.008 rad); what is left is exact to 2^-31 turns.
+// decimals of position * frequency for long contexts (position 131071: 0.008 rad).  What is left is off by 2^-26 turns at most, when
+// half a turn becomes a 32-bit float; a table of 64-bit floats adds 2^-31 turns at position 2^24 and 2^-24.4 at 2^31.
 //
 // D / 8 lanes hold a head, eight neighbouring values each (16 bytes of fp16), and go through heads of one token.  With x' a value's
 // partner in its pair, a turned value is r (x A + x' B), r = 1 / sqrt(...): A = w cos and B = -+ w' sin are worked out once per token
-// and lane, so that a head costs an exchange of the raw values and three operations per value.  Blocks of two warps, 16 to an SM:
-// 8192 tokens of 32 + 8 + 8 heads of 128 into the cache take 66 us with the read behind it, 71 with 12 blocks of more registers to an
-// SM, 73 to 81 in blocks of four warps; it is bound by instructions (conversions, exchanges, quantisation), not by memory.
+// and lane, so that a head costs an exchange of the raw values and three operations per value.  Blocks of two warps, 16 to an SM (64
+// registers: 8 to 28 bytes of a lane's lie in local memory): 8192 tokens of 32 + 8 + 8 heads of 128 into the cache take 67 us with the
+// read behind it (71 with 12 blocks of more registers to an SM, 73 to 81 in blocks of four warps), 56 without, 2.6 TB/s.  Three
+// quarters of the issue slots are taken (225 instructions to a warp's two heads, of which rounding K and V to codes, 26 us for them
+// alone, is about half and sines and cosines a twentieth); behind a full scheduler ("not selected") warps wait for their own results,
+// then for loads.
 #include <cuda_fp16.h>
 #include <math.h>
 #include <string.h>
