@@ -366,6 +366,174 @@ MLD_API int mld_fc_run(mld_fc_plan* plan, const void* src, const void* weights,
                        const void* bias, void* dst, int32_t tokens,
                        void* stream);
 
+/* The same product on activations that are quantised already, by mld_add_rms_norm
+ * for instance: codes int8 [tokens] rows of k values rounded up to a multiple of
+ * 16 (zeros behind a row), 16-byte aligned; params fp32 [tokens][3]: the scale
+ * and the zero point of a token's codes, value = code * scale + zero point, and
+ * a third that is not read.  For operators with prefill_act_quant: 1 takes no
+ * notice of zero points, 2 needs mld_fc_plan_set_weights_sum.  Runs the prefill
+ * GEMM for any number of tokens; the weights, scales and sums must not be
+ * written by launches of this library that may still be running (the
+ * conversion functions above are not such launches). */
+MLD_API int mld_fc_run_codes(mld_fc_plan* plan, const int8_t* codes, const float* params, const void* weights,
+                             const void* scale, const void* bias, void* dst, int32_t tokens, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Residual and RMS norm ahead of a projection                               */
+/* ------------------------------------------------------------------------ */
+
+/* What the reference builds from Add and RMSNorm nodes between the halves of a
+ * layer (samples/llm/qwen3_model_builder.cc:426-508, 947-1038) and, for 8-bit
+ * products, the quantisation of their input (common/kernels/
+ * quantize_and_dequantize.cc:355-441), in one pass:
+ *   h = x + residual, rounded to the tensors' type;
+ *   y = h (weight_offset + weight) / sqrt(mean(h^2) + eps);
+ *   codes of v = h (weight_offset + weight), which y is a multiple of:
+ *     symmetric:  scale = max|y| / 127, zero point 0,
+ *                 code = floor(127 v / max|v| + 1/2)
+ *     asymmetric: scale = (max y - min y) / 255, zero point = min y + 128 scale,
+ *                 code = floor(255 (v - min v) / (max v - min v) + 1/2) - 128
+ * in 32 bits, codes that lie next to a border in 64.  A row of equal v (of
+ * zeros, symmetric) has codes 0 and scale 0.  The sum of a row's squares has to
+ * be a 32-bit float: a row where it, or a product with a weight, is infinite or
+ * NaN has NaN parameters and codes 0. */
+typedef struct mld_add_norm_desc {
+  int32_t width;             /* values of a row, 1 to 16384 */
+  float eps;
+  float weight_offset;       /* 0, or 1 for weights that are stored less one */
+  int32_t f16;               /* 1: tensors and weights are fp16, 0: fp32 */
+  int32_t asymmetric;        /* the rule for codes */
+} mld_add_norm_desc;
+
+/* Rows of `width` values, `stride` elements from token to token; rows that are
+ * 16-byte aligned, of a multiple of 8 values, are read and written in wide
+ * accesses.  An input's stride may be 0.  sum_out and out may be x or residual
+ * (with the same stride, and not both the same); otherwise outputs must not
+ * overlap inputs or one another. */
+typedef struct mld_add_norm_io {
+  const void* x;
+  int64_t x_stride;
+  const void* residual;      /* NULL: none */
+  int64_t residual_stride;
+  const void* weight;        /* [width]; NULL: no weights (and no offset) */
+  void* sum_out;             /* h; may be NULL */
+  int64_t sum_stride;
+  void* out;                 /* y; may be NULL with codes */
+  int64_t out_stride;
+  int8_t* codes;             /* may be NULL; what mld_fc_run_codes takes */
+  int64_t codes_stride;      /* a multiple of 16, at least width; the columns up
+                                to width rounded up to 16 are written */
+  float* params;             /* [tokens][3]: scale, zero point, 0 */
+} mld_add_norm_io;
+
+MLD_API int mld_add_rms_norm(const mld_add_norm_desc* d, const mld_add_norm_io* io, int32_t tokens, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Experts                                                                   */
+/* ------------------------------------------------------------------------ */
+
+/* Mixture-of-experts feed-forward networks: which experts a token goes to, and
+ * their products.  The reference builds the products from FullyConnected nodes
+ * with batched weights and per-token batch ids
+ * (common/gpu_model_builder_moe_util.cc:200-270). */
+typedef enum mld_moe_score {
+  MLD_MOE_SOFTMAX = 0,
+  MLD_MOE_SIGMOID = 1
+} mld_moe_score;
+
+/* score_e = softmax over the experts, or sigmoid, of the logits; an expert is
+ * chosen by value_e = score_e + bias_e.  Experts lie in `groups` groups of
+ * neighbours; the top_groups groups with the largest sum of their group_best
+ * largest values are kept, and of their experts the top_k with the largest
+ * values, in that order.  Of equal values the one with the larger logit comes
+ * first (values round to 0 and 1, logits do not), of equal experts or groups
+ * the one with the lower number.  A chosen expert's weight is factor * score_e,
+ * with renormalise factor * score_e / the sum of the chosen ones' scores.
+ * Values and groups' sums are compared in 64 bits.
+ * An expert whose logit is -infinity or NaN, or whose value is, is not to be
+ * had and counts as -infinity in a group's sum; a logit of +infinity is the
+ * largest 32-bit float.  Places that no expert is left for get id -1 and weight
+ * 0. */
+typedef struct mld_moe_route_desc {
+  int32_t experts;           /* 1 to 1024 */
+  int32_t top_k;             /* 1 to 32 */
+  int32_t score;             /* mld_moe_score */
+  int32_t groups;            /* 1 to 32, divides experts */
+  int32_t top_groups;        /* top_groups * experts / groups >= top_k */
+  int32_t group_best;        /* 1 or 2; of groups of one expert: 1 */
+  int32_t renormalise;
+  float factor;
+  int32_t f16;               /* the logits: 1 fp16, 0 fp32 */
+} mld_moe_route_desc;
+
+/* logits: [tokens] rows of `experts`, `stride` elements apart; bias: fp32
+ * [experts] or NULL; ids: int32, weights: fp32, both [tokens][top_k]. */
+MLD_API int mld_moe_route(const mld_moe_route_desc* d, const void* logits, int64_t stride, const float* bias,
+                          int32_t* ids, float* weights, int32_t tokens, void* stream);
+
+typedef enum mld_moe_activation {
+  MLD_MOE_SILU = 0,          /* g / (1 + exp(-g)) */
+  MLD_MOE_GELU_TANH = 1      /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+} mld_moe_activation;
+
+typedef enum mld_moe_path {
+  MLD_MOE_PATH_AUTO = 0,
+  MLD_MOE_PATH_FEW_ROWS = 1, /* bound by the weights: decoding, small batches */
+  MLD_MOE_PATH_MANY_ROWS = 2 /* tiles on the tensor cores: prompts */
+} mld_moe_path;
+
+/* out_t = residual_t + sum_j weights_tj down_e (act(gate_e x_t) * (up_e x_t)), e = ids_tj.
+ * An id outside 0 .. experts - 1 is no expert: its place is passed over (-1
+ * marks padding); an expert may appear twice in a row.  Weight matrices are
+ * FullyConnected weights (kOSpatialIOGroupI4O4), those of expert e + 1 right
+ * behind those of expert e: gate_up has 2 ffn outputs gate_0, up_0, gate_1, ...
+ * and d_model inputs, down d_model outputs and ffn inputs; scales fp16
+ * [experts][inputs / block][outputs].
+ * Products are summed in 32 bits.  act(..) * (..) is rounded to fp16 for the
+ * second product; with many rows, weights are rounded to fp16 as
+ * FullyConnected's prefill does and down_e(..) is, too, ahead of the sum over j,
+ * which is in 32 bits and in the order of j: the same call gives the same bits. */
+typedef struct mld_moe_desc {
+  int32_t experts;           /* 1 to 1024 */
+  int32_t top_k;             /* places of a token in ids, 1 to 32 */
+  int32_t d_model, ffn;      /* multiples of 32, up to 32768 */
+  int32_t weight_bits;       /* 4 or 8 */
+  int32_t block;             /* inputs that share a scale: 32, 64, 128 or 256, and
+                                a divisor of d_model and ffn; 0: all of them */
+  int32_t activation;        /* mld_moe_activation */
+  int32_t max_tokens;        /* 1 to 65536 */
+  int32_t device;            /* -1 = current */
+  int32_t force_path;        /* mld_moe_path; 0 = by the measured rule on tokens,
+                                top_k and experts */
+} mld_moe_desc;
+
+typedef struct mld_moe_io {
+  const void* x;             /* fp16 [tokens] rows of d_model */
+  int64_t x_stride;          /* elements from token to token, a multiple of 8;
+                                16-byte aligned, as all rows here */
+  const int32_t* ids;        /* device, [tokens][top_k] */
+  const float* weights;      /* device, [tokens][top_k] */
+  const void *gate_up, *gate_up_scale, *down, *down_scale;
+  const void* residual;      /* fp16 [tokens] rows of d_model; NULL: none */
+  int64_t residual_stride;
+  void* out;                 /* fp16 [tokens] rows; may be the residual, with the
+                                same stride, or x */
+  int64_t out_stride;
+} mld_moe_io;
+
+typedef struct mld_moe_plan mld_moe_plan;
+/* All workspace is allocated here; the call waits for its clearing.  A plan may
+ * be used from one stream at a time, with its device current; calls may be
+ * captured. */
+MLD_API int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out);
+MLD_API int mld_moe_plan_destroy(mld_moe_plan* plan);
+MLD_API size_t mld_moe_plan_workspace_bytes(const mld_moe_plan* plan);
+MLD_API int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* stream);
+/* Waits for the plan's device, whichever is current: *code = 0, or MLD_TIMEOUT
+ * for a bounded device-side wait of an earlier call that gave up (then cleared;
+ * the function returns MLD_TIMEOUT then). */
+MLD_API int mld_moe_plan_device_status(mld_moe_plan* plan, int32_t* code);
+
 /* ------------------------------------------------------------------------ */
 /* Embedding lookup over the same packed table                               */
 /* ------------------------------------------------------------------------ */

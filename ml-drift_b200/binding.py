@@ -91,6 +91,11 @@ def lib() -> C.CDLL:
         L.mld_kv4_copy_pages.argtypes = [p, p, i, l, p, p, i, p]
         L.mld_qk_rope_run.argtypes = [p, p, i, p]
         L.mld_kv4_attn_run.argtypes = [p, p, p]
+        L.mld_fc_run_codes.argtypes = [p, p, p, p, p, p, p, i, p]
+        L.mld_add_rms_norm.argtypes = [p, p, i, p]
+        L.mld_moe_route.argtypes = [p, p, l, p, p, p, i, p]
+        L.mld_moe_run.argtypes = [p, p, i, p]
+        L.mld_moe_plan_workspace_bytes.restype = C.c_size_t
         _lib = L
     return _lib
 
@@ -232,6 +237,18 @@ class FullyConnectedPlan:
                                         _addr(dst), tokens, _stream_addr(stream))
         if rc != OK:
             _check(rc, "mld_fc_run")
+
+    def run_codes(self, codes, params, weights, scale, dst, tokens, bias=None, stream=None):
+        """The product on activations that are quantised already: codes int8 [tokens][k rounded up to 16], params fp32 [tokens][3],
+        as add_rms_norm makes them."""
+        gpu, queue = _here(stream)
+        _codes(codes, params, tokens, self.desc.k, gpu)
+        if tokens > 1 and codes.stride(0) != div_up(self.desc.k, 16) * 16:
+            raise ValueError(f"codes: rows have to be {div_up(self.desc.k, 16) * 16} apart, these are {codes.stride(0)}")
+        rc = _lib.mld_fc_run_codes(self._h, codes.data_ptr(), params.data_ptr(), _addr(weights), _addr(scale), _addr(bias), _addr(dst),
+                                   tokens, queue)
+        if rc != OK:
+            _check(rc, "mld_fc_run_codes")
 
     def close(self):
         if self._h:
@@ -762,6 +779,163 @@ class Kv4Attention:
     def close(self):
         if self._h:
             lib().mld_kv4_attn_plan_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+# -------------------------------------------- residual, norm and codes; experts
+class AddNormDesc(C.Structure):
+    _fields_ = [("width", C.c_int32), ("eps", C.c_float), ("weight_offset", C.c_float), ("f16", C.c_int32), ("asymmetric", C.c_int32)]
+
+
+class AddNormIo(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("residual", C.c_void_p), ("residual_stride", C.c_int64),
+                ("weight", C.c_void_p), ("sum_out", C.c_void_p), ("sum_stride", C.c_int64), ("out", C.c_void_p),
+                ("out_stride", C.c_int64), ("codes", C.c_void_p), ("codes_stride", C.c_int64), ("params", C.c_void_p)]
+
+
+class MoeRouteDesc(C.Structure):
+    _fields_ = [("experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32), ("groups", C.c_int32), ("top_groups", C.c_int32),
+                ("group_best", C.c_int32), ("renormalise", C.c_int32), ("factor", C.c_float), ("f16", C.c_int32)]
+
+
+class MoeDesc(C.Structure):
+    _fields_ = [("experts", C.c_int32), ("top_k", C.c_int32), ("d_model", C.c_int32), ("ffn", C.c_int32), ("weight_bits", C.c_int32),
+                ("block", C.c_int32), ("activation", C.c_int32), ("max_tokens", C.c_int32), ("device", C.c_int32),
+                ("force_path", C.c_int32)]
+
+
+class MoeIo(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("x_stride", C.c_int64), ("ids", C.c_void_p), ("weights", C.c_void_p), ("gate_up", C.c_void_p),
+                ("gate_up_scale", C.c_void_p), ("down", C.c_void_p), ("down_scale", C.c_void_p), ("residual", C.c_void_p),
+                ("residual_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+def _table(t, rows, columns, dtype, what, gpu):
+    """Elements from row to row of a [rows][columns] tensor whose rows are contiguous."""
+    stride = t.stride()
+    if t.get_device() != gpu or t.dtype is not dtype or t.shape != (rows, columns) or (stride[1] != 1 and columns > 1):
+        if t.get_device() != gpu:
+            raise _elsewhere(t, what)
+        raise ValueError(f"{what}: expected {dtype} [{rows}][{columns}] with contiguous rows, got {t.dtype} {tuple(t.shape)} "
+                         f"strides {stride}")
+    return stride[0]
+
+
+def _whole(t, elements, dtype, what, gpu):
+    if t.get_device() != gpu or t.dtype is not dtype or t.numel() != elements or not t.is_contiguous():
+        if t.get_device() != gpu:
+            raise _elsewhere(t, what)
+        raise ValueError(f"{what}: expected {elements} contiguous values of {dtype}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _codes(codes, params, tokens, width, gpu):
+    stride = _table(codes, tokens, div_up(width, 16) * 16, torch.int8, "codes", gpu)
+    _whole(params, 3 * tokens, torch.float32, "params", gpu)
+    return stride
+
+
+def add_rms_norm(x, weight=None, residual=None, sum_out=None, out=None, codes=None, params=None, eps=1e-6, weight_offset=0.0,
+                 symmetric=True, stream=None):
+    """h = x + residual (into sum_out), y = h (weight_offset + weight) / sqrt(mean h^2 + eps) into out, and / or its codes (int8
+    [tokens][width rounded up to 16]) with scale and zero point (params, fp32 [tokens][3]); x, residual, sum_out, out: [tokens][width]
+    fp16 or fp32, rows may be strided."""
+    n, w = x.shape
+    dt = x.dtype
+    gpu, queue = _here(stream)
+    d = AddNormDesc(w, eps, weight_offset, _f16(x), int(not symmetric))
+    io = AddNormIo()
+    io.x, io.x_stride = x.data_ptr(), _table(x, n, w, dt, "x", gpu)
+    if residual is not None:
+        io.residual, io.residual_stride = residual.data_ptr(), _table(residual, n, w, dt, "residual", gpu)
+    if weight is not None:
+        io.weight = _whole(weight, w, dt, "weight", gpu)
+    if sum_out is not None:
+        io.sum_out, io.sum_stride = sum_out.data_ptr(), _table(sum_out, n, w, dt, "sum_out", gpu)
+    if out is not None:
+        io.out, io.out_stride = out.data_ptr(), _table(out, n, w, dt, "out", gpu)
+    if codes is not None:
+        if params is None:
+            raise ValueError("codes and params go together")
+        io.codes, io.codes_stride, io.params = codes.data_ptr(), _codes(codes, params, n, w, gpu), params.data_ptr()
+    rc = lib().mld_add_rms_norm(C.byref(d), C.byref(io), n, queue)
+    if rc != OK:
+        _check(rc, "mld_add_rms_norm")
+
+
+MOE_SOFTMAX, MOE_SIGMOID = 0, 1
+MOE_SILU, MOE_GELU_TANH = 0, 1
+MOE_PATH_AUTO, MOE_PATH_FEW_ROWS, MOE_PATH_MANY_ROWS = 0, 1, 2
+
+
+class MoeRouter:
+    """Which experts tokens go to, and with what weights (see mldfc.h)."""
+
+    def __init__(self, experts, top_k, score=MOE_SOFTMAX, groups=1, top_groups=1, group_best=1, renormalise=True, factor=1.0, f16=True):
+        self.desc = MoeRouteDesc(experts, top_k, score, groups, top_groups, group_best, int(renormalise), factor, int(f16))
+        self.experts, self.top_k, self.dtype = experts, top_k, torch.float16 if f16 else torch.float32
+
+    def run(self, logits, ids, weights, bias=None, stream=None):
+        """logits: [tokens][experts] (rows may be strided); ids int32, weights fp32, [tokens][top_k]; bias: fp32 [experts]."""
+        n = logits.shape[0]
+        gpu, queue = _here(stream)
+        stride = _table(logits, n, self.experts, self.dtype, "logits", gpu)
+        rc = lib().mld_moe_route(C.byref(self.desc), logits.data_ptr(), stride,
+                                 None if bias is None else _whole(bias, self.experts, torch.float32, "bias", gpu),
+                                 _ints(ids, (n, self.top_k), "ids", gpu), _whole(weights, n * self.top_k, torch.float32, "weights", gpu), n, queue)
+        if rc != OK:
+            _check(rc, "mld_moe_route")
+
+
+class MoeExperts:
+    """Gated feed-forward networks of experts over FullyConnected weights (see mldfc.h)."""
+
+    def __init__(self, experts, top_k, d_model, ffn, weight_bits=4, block=32, activation=MOE_SILU, max_tokens=1, device=-1,
+                 force_path=MOE_PATH_AUTO):
+        self.desc = MoeDesc(experts, top_k, d_model, ffn, weight_bits, block, activation, max_tokens, device, force_path)
+        self._h = C.c_void_p()
+        _check(lib().mld_moe_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_moe_plan_create")
+        per = [d_model // block if block else 1, ffn // block if block else 1]
+        self._sizes = [experts * 2 * ffn * d_model * weight_bits // 8, experts * per[0] * 2 * ffn,
+                       experts * d_model * ffn * weight_bits // 8, experts * per[1] * d_model]
+
+    def run(self, x, ids, weights, gate_up, gate_up_scale, down, down_scale, out, residual=None, stream=None):
+        """x, out, residual: fp16 [tokens][d_model] (rows may be strided); ids int32, weights fp32, [tokens][top_k]; the experts' packed
+        matrices (uint8) one behind the other, scales fp16 [experts][groups][outputs]."""
+        n, d, k = x.shape[0], self.desc.d_model, self.desc.top_k
+        gpu, queue = _here(stream)
+        z = self._sizes
+        io = MoeIo(x.data_ptr(), _table(x, n, d, torch.float16, "x", gpu), _ints(ids, (n, k), "ids", gpu),
+                   _whole(weights, n * k, torch.float32, "weights", gpu), _whole(gate_up, z[0], torch.uint8, "gate_up", gpu),
+                   _whole(gate_up_scale, z[1], torch.float16, "gate_up_scale", gpu), _whole(down, z[2], torch.uint8, "down", gpu),
+                   _whole(down_scale, z[3], torch.float16, "down_scale", gpu))
+        if residual is not None:
+            io.residual, io.residual_stride = residual.data_ptr(), _table(residual, n, d, torch.float16, "residual", gpu)
+        io.out, io.out_stride = out.data_ptr(), _table(out, n, d, torch.float16, "out", gpu)
+        rc = _lib.mld_moe_run(self._h, C.byref(io), n, queue)
+        if rc != OK:
+            _check(rc, "mld_moe_run")
+
+    def workspace_bytes(self) -> int:
+        return int(lib().mld_moe_plan_workspace_bytes(self._h))
+
+    def device_status(self) -> int:
+        """0, or TIMEOUT when a bounded device-side wait gave up (then cleared)."""
+        code = C.c_int32(0)
+        rc = lib().mld_moe_plan_device_status(self._h, C.byref(code))
+        if rc not in (OK, TIMEOUT):
+            raise MldError(rc, "mld_moe_plan_device_status")
+        return code.value
+
+    def close(self):
+        if self._h:
+            lib().mld_moe_plan_destroy(self._h)
             self._h = C.c_void_p()
 
     def __del__(self):

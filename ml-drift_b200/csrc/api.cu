@@ -567,8 +567,10 @@ static int run_stream(mld_fc_plan* p, const StripGeometry& gm, const void* src, 
 // bytes, into tensor memory (gemm_wtmem_kernel); with cache_prepared_weights, where convert_pays says so, or for a weight
 // matrix whose row pitch a tensor map cannot express, the weights are first expanded to a K-major copy (kept between calls
 // when cached) and a plain GEMM runs on that.
+// codes, params != null: the activations quantised already, rows of K rounded up to 16 bytes (then src is not read).
 static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const void* scale, const void* bias,
-                    void* dst, int tokens, cudaStream_t stream, const PeerOutputs* outs, bool* outs_used) {
+                    void* dst, int tokens, cudaStream_t stream, const PeerOutputs* outs, bool* outs_used,
+                    const int8_t* codes = nullptr, const float* params = nullptr) {
   const mld_fc_desc& d = p->d;
   const bool i8 = d.prefill_act_quant != 0;
   int* err = p->error_shared != nullptr ? p->error_shared : p->error;
@@ -581,7 +583,9 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     set_last_error_text("asymmetric int8 activations need the weights' per-output sums (mld_fc_plan_set_weights_sum)");
     return MLD_INVALID_ARGUMENT;
   }
-  int rc;
+  int rc = MLD_OK;
+  const void* const x_kmajor = codes != nullptr ? codes : p->x_kmajor;
+  const float* const a_params = codes != nullptr ? params : p->a_params;
   const bool convert = d.cache_prepared_weights != 0 || !p->pair_ok || d.prefill_route == MLD_PREFILL_ROUTE_CONVERT ||
                        (d.prefill_route == MLD_PREFILL_ROUTE_AUTO && convert_pays(d, tokens));  // (routes 1 and 3: inside)
   if (!convert && d.prefill_route != MLD_PREFILL_ROUTE_INLINE_SMEM) {
@@ -590,15 +594,17 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     const int mode = i8 ? 2 : d.weight_bits == 4 ? 0 : 1;
     const WtGeometry wg = wtmem_geometry(tokens, d.n, d.k, mode, p->sms, true);
     if (++p->split.epoch == 0) p->split.epoch = 1;
-    if (i8)
+    if (codes != nullptr)
+      rc = MLD_OK;
+    else if (i8)
       rc = launch_quantize_act(src, d.src_layout, tokens, d.k, wg.kp, d.prefill_act_quant == 1, p->x_kmajor, p->a_params,
                                stream);
     else
       rc = launch_transpose_x(src, d.src_layout, tokens, d.k, wg.kp, p->x_kmajor, stream);
     if (rc != MLD_OK) return rc;
-    return launch_gemm_wtmem(mode, p->x_kmajor, weights, wg, tokens, d.n, d.k, scale, d.scale_mode,
+    return launch_gemm_wtmem(mode, x_kmajor, weights, wg, tokens, d.n, d.k, scale, d.scale_mode,
                              d.scale_mode == MLD_SCALE_BLOCK ? d.groups : 1, p->group_slices, d.scalar_scale, bias,
-                             p->a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream, outs,
+                             a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream, outs,
                              &p->split);
   }
   if (!convert) {
@@ -606,15 +612,17 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     const int mode = i8 ? 2 : (d.weight_bits == 4 ? 0 : 1);
     const PairGeometry pg = pair_geometry(tokens, d.n, d.k, mode, p->sms, true);
     if (++p->split.epoch == 0) p->split.epoch = 1;
-    if (i8)
+    if (codes != nullptr)
+      rc = MLD_OK;
+    else if (i8)
       rc = launch_quantize_act(src, d.src_layout, tokens, d.k, pg.kp, d.prefill_act_quant == 1, p->x_kmajor, p->a_params,
                                stream);
     else
       rc = launch_transpose_x(src, d.src_layout, tokens, d.k, pg.kp, p->x_kmajor, stream);
     if (rc != MLD_OK) return rc;
-    return launch_gemm_pair(mode, p->x_kmajor, weights, pg, tokens, d.n, d.k, scale, d.scale_mode,
+    return launch_gemm_pair(mode, x_kmajor, weights, pg, tokens, d.n, d.k, scale, d.scale_mode,
                             d.scale_mode == MLD_SCALE_BLOCK ? d.groups : 1, p->group_slices, d.scalar_scale, bias,
-                            p->a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream,
+                            a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream,
                             outs, &p->split);
   }
 
@@ -633,7 +641,7 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     p->prepared_s = scale;
     x_done = ride;
   }
-  if (x_done) {
+  if (x_done || codes != nullptr) {
     rc = MLD_OK;
   } else if (i8)
     rc = launch_quantize_act(src, d.src_layout, tokens, d.k, g.kp, d.prefill_act_quant == 1, p->x_kmajor, p->a_params,
@@ -647,8 +655,8 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     const PairGeometry pg = pair_geometry(tokens, d.n, d.k, mode, p->sms, true);
     if (++p->split.epoch == 0) p->split.epoch = 1;
     if (pg.kp == g.kp)
-      return launch_gemm_pair(mode, p->x_kmajor, p->w_kmajor, pg, tokens, d.n, d.k, scale, d.scale_mode, 1, 1, 0.0f,
-                              bias, p->a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err,
+      return launch_gemm_pair(mode, x_kmajor, p->w_kmajor, pg, tokens, d.n, d.k, scale, d.scale_mode, 1, 1, 0.0f,
+                              bias, a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err,
                               stream, outs, &p->split);
   }
   if (d.prefill_act_quant == 2) {
@@ -656,13 +664,34 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     return MLD_UNIMPLEMENTED;
   }
   if (outs_used != nullptr) *outs_used = false;  // this kernel writes dst only
-  return launch_gemm_umma(i8, p->x_kmajor, p->w_kmajor, g, tokens, d.n, d.k, bias, scale, p->a_params, dst,
+  return launch_gemm_umma(i8, x_kmajor, p->w_kmajor, g, tokens, d.n, d.k, bias, scale, a_params, dst,
                           d.dst_layout, err, stream);
 }
 
 int mld_fc_run(mld_fc_plan* plan, const void* src, const void* weights, const void* scale, const void* zero_point,
                const void* bias, void* dst, int32_t tokens, void* stream_v) {
   return mld::fc_run_internal(plan, src, weights, scale, zero_point, bias, dst, tokens, stream_v, nullptr, nullptr);
+}
+
+int mld_fc_run_codes(mld_fc_plan* plan, const int8_t* codes, const float* params, const void* weights, const void* scale,
+                     const void* bias, void* dst, int32_t tokens, void* stream_v) {
+  MLD_REQUIRE(plan != nullptr, "null plan");
+  const mld_fc_desc& d = plan->d;
+  MLD_REQUIRE(d.prefill_act_quant != 0, "codes need an operator with prefill_act_quant");
+  MLD_REQUIRE(tokens >= 0 && tokens <= d.max_tokens, "tokens exceeds the plan's max_tokens");
+  if (tokens == 0) return MLD_OK;
+  MLD_REQUIRE(codes != nullptr && params != nullptr && weights != nullptr && scale != nullptr && dst != nullptr, "null tensor");
+  MLD_REQUIRE(!d.has_bias || bias != nullptr, "biases tensor missing");
+  MLD_REQUIRE((reinterpret_cast<uintptr_t>(weights) & 15) == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0,
+              "weights and codes must be 16-byte aligned");
+  MLD_REQUIRE((reinterpret_cast<uintptr_t>(params) & 3) == 0, "params must be aligned to their type");
+  MLD_REQUIRE(d.epilogue == MLD_EPILOGUE_NONE, "codes are multiplied by the prefill GEMM, which has no fused SiLU*mul write");
+  if (d.precision == MLD_PRECISION_F32 || get_encode_tiled() == nullptr) {
+    set_last_error_text("quantised-activation prefill needs fp16 tensors and no zero points");
+    return MLD_UNIMPLEMENTED;
+  }
+  return run_gemm(plan, nullptr, weights, scale, d.has_bias ? bias : nullptr, dst, tokens, static_cast<cudaStream_t>(stream_v),
+                  nullptr, nullptr, codes, params);
 }
 
 }  // extern "C"

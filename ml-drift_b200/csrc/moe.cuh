@@ -1,0 +1,41 @@
+// What the kernels of the experts' networks share.
+#pragma once
+#include "common.cuh"
+#include "kernels.h"
+
+namespace mld {
+
+// Rows of one expert that are worked on together: positions row0 .. row0 + rows - 1 of the order by experts.
+struct MoeTile {
+  int expert, row0, rows, unused;
+};
+
+// Device memory of a plan.
+struct MoeBuffers {
+  int* order;        // [pairs]: position -> pair (token * top_k + place)
+  int* position;     // [pairs]: pair -> position, -1: no expert
+  MoeTile* tiles;    // [most tiles]
+  int* n_tiles;
+  void* hidden;      // fp16 [pairs][ffn], by position
+  void* part;        // [pairs][d_model], by position: fp32 with few rows, fp16 with many
+  void* sorted;      // fp16 [pairs][d_model]: x by position (many rows)
+  int* error;
+};
+
+struct MoeShape {
+  int experts, top_k, d_model, ffn, bits, block, activation;
+};
+
+#ifdef __CUDACC__
+// act(gate) * up
+__device__ __forceinline__ float moe_gated(float gate, float up, int activation) {
+  const float u = activation == MLD_MOE_SILU ? gate : 1.5957691216057308f * (gate + 0.044715f * gate * gate * gate);
+  return gate / (1.0f + __expf(-u)) * up;  // (GELU's (1 + tanh(u / 2)) / 2 is 1 / (1 + exp(-u)))
+}
+#endif
+
+// The products of tiles of rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16).
+int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs,
+                    int tile_rows, int sms, cudaStream_t stream);
+
+}  // namespace mld

@@ -1,0 +1,163 @@
+"""Experts' gated networks over packed weights against the formulas in 64 bits, on both paths."""
+import functools
+
+import numpy as np
+import pytest
+import torch
+
+from tests import ffn_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def mld():
+    import __graft_entry__ as g
+    return g.import_package()
+
+
+def _dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+@functools.lru_cache(4)
+def _weights(e, d, f, bits, block):
+    rng = np.random.default_rng(e * d + f)
+    first, second = [ref.matrix(rng, 2 * f, d, bits, block) for _ in range(e)], [ref.matrix(rng, d, f, bits, block) for _ in range(e)]
+    host = [np.stack([m[2] for m in ms]) for ms in (first, second)]
+    dev = [_dev(np.stack([m[i] for m in ms])) for ms in (first, second) for i in range(2)]
+    return host, dev
+
+
+def _bound(want, size, many):
+    """fp16 roundings (2^-11 of the value): of the gated product (act, up: `size` holds second |h|) and of the result; with many
+    rows of each weight (the rest of `size`) and of each expert's output; 32-bit sums, exp and divisions beside them are 2^-17
+    of size at most (512 roundings of partial sums).  Below 2^-14 fp16 is spaced 2^-24."""
+    return 2.0 ** -11 * np.abs(want) + size * ((3.1 if many else 1.1) * 2.0 ** -11 + 2.0 ** -17) + 2.0 ** -16
+
+
+def _run(mld, n, e, k, d, f, bits, block, gelu, path, ids, residual=True, seed=0):
+    rng = np.random.default_rng(seed + n)
+    (first, second), (w1, s1, w2, s2) = _weights(e, d, f, bits, block)
+    x = rng.standard_normal((n, d)).astype(np.float16)
+    weights = rng.random((n, k)).astype(np.float32)
+    res = (2 * rng.standard_normal((n, d))).astype(np.float16) if residual else None
+    plan = mld.MoeExperts(e, k, d, f, weight_bits=bits, block=block, activation=mld.MOE_GELU_TANH if gelu else mld.MOE_SILU, max_tokens=n,
+                          force_path=path)
+    out = torch.full((n, d), 7.0, dtype=torch.float16, device="cuda")
+    xd, idd, wd, rd = _dev(x), _dev(ids.astype(np.int32)), _dev(weights), _dev(res) if residual else None
+    plan.run(xd, idd, wd, w1, s1, w2, s2, out, residual=rd)
+    torch.cuda.synchronize()
+    assert plan.device_status() == 0
+    want, size = ref.experts(x, ids, weights, first, second, res, gelu)
+    got = out.cpu().numpy().astype(np.float64)
+    bound = _bound(want, size, path == mld.MOE_PATH_MANY_ROWS)
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
+    again = torch.empty_like(out)
+    plan.run(xd, idd, wd, w1, s1, w2, s2, again, residual=rd)
+    assert torch.equal(out, again)  # the same bits
+    return got
+
+
+def _ids(rng, n, e, k, skew=0.0):
+    ids = np.argsort(-(rng.standard_normal((n, e)) + skew * rng.standard_normal(e)), 1)[:, :k]
+    return ids
+
+
+SHAPES = [  # experts, top_k, d, f, bits, block
+    (4, 2, 256, 128, 4, 32), (8, 3, 160, 96, 4, 32), (5, 1, 96, 352, 8, 0), (6, 2, 128, 64, 8, 64), (3, 3, 384, 256, 4, 128), (4, 2, 64, 32, 4, 0)]
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 33, 100])
+@pytest.mark.parametrize("e,k,d,f,bits,block", SHAPES)
+@pytest.mark.parametrize("path", ["few", "many"])
+def test_experts(mld, n, e, k, d, f, bits, block, path):
+    rng = np.random.default_rng(n * d + f)
+    _run(mld, n, e, k, d, f, bits, block, n % 2 == 1, mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS,
+         _ids(rng, n, e, k, 1.0), residual=n % 3 != 0)
+
+
+@pytest.mark.parametrize("path", ["few", "many"])
+@pytest.mark.parametrize("n", [1, 3, 40])
+def test_no_expert_the_same_expert_twice_and_all_on_one(mld, n, path):
+    path = mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS
+    e, k, d, f = 4, 3, 128, 64
+    rng = np.random.default_rng(n)
+    ids = _ids(rng, n, e, k)
+    ids[0] = (2, 2, 2)
+    _run(mld, n, e, k, d, f, 4, 32, False, path, ids)
+    ids[n // 2:] = -1
+    ids[-1, 0], ids[0, 1] = 4, 1 << 30
+    _run(mld, n, e, k, d, f, 4, 32, False, path, ids)
+    got = _run(mld, n, e, k, d, f, 4, 32, False, path, np.full((n, k), -5), residual=False)
+    assert not got.any()
+    _run(mld, n, e, k, d, f, 4, 32, True, path, np.full((n, k), 3))
+
+
+@pytest.mark.parametrize("n", [300, 700])
+def test_many_rows_ragged(mld, n):
+    rng = np.random.default_rng(n)
+    ids = _ids(rng, n, 4, 2, 1.5)
+    ids[5::17] = -1
+    _run(mld, n, 4, 2, 256, 128, 4, 32, False, mld.MOE_PATH_MANY_ROWS, ids)
+    _run(mld, n, 5, 1, 96, 352, 8, 0, True, mld.MOE_PATH_MANY_ROWS, _ids(rng, n, 5, 1, 2.0))
+
+
+@pytest.mark.parametrize("path", ["few", "many"])
+def test_strides_in_place_capture_and_a_smaller_call(mld, path):
+    path = mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS
+    e, k, d, f, n = 4, 2, 256, 128, 50
+    rng = np.random.default_rng(1)
+    (first, second), (w1, s1, w2, s2) = _weights(e, d, f, 4, 32)
+    wide = torch.from_numpy(rng.standard_normal((n, d + 40)).astype(np.float16)).cuda()
+    x = wide[:, 8:8 + d]
+    stream = torch.from_numpy(rng.standard_normal((n, d + 16)).astype(np.float16)).cuda()
+    res = stream[:, 16:]
+    start = stream.clone()
+    ids, weights = _dev(_ids(rng, n, e, k).astype(np.int32)), _dev(rng.random((n, k)).astype(np.float32))
+    plan = mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=path)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        plan.run(x, ids, weights, w1, s1, w2, s2, res, residual=res)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            plan.run(x, ids, weights, w1, s1, w2, s2, res, residual=res)
+        for rows in (n, 13):  # replayed, and a call of fewer tokens in between
+            stream.copy_(start)
+            if rows == n:
+                graph.replay()
+            else:
+                plan.run(x[:rows], ids[:rows], weights[:rows], w1, s1, w2, s2, res[:rows], residual=res[:rows])
+            s.synchronize()
+            want, size = ref.experts(x.cpu().numpy()[:rows], ids.cpu().numpy()[:rows], weights.cpu().numpy()[:rows], first, second,
+                                     start.cpu().numpy()[:rows, 16:], False)
+            got = res.cpu().numpy().astype(np.float64)
+            assert (np.abs(got[:rows] - want) <= _bound(want, size, path == mld.MOE_PATH_MANY_ROWS)).all()
+            assert torch.equal(stream[:, :16], start[:, :16]) and torch.equal(stream[rows:], start[rows:])
+        stream.copy_(start)
+        graph.replay()
+        s.synchronize()
+    assert plan.device_status() == 0
+
+
+def test_values_that_are_not_numbers_stay_with_their_token(mld):
+    e, k, d, f, n = 4, 2, 128, 64, 20
+    rng = np.random.default_rng(2)
+    (_, _), (w1, s1, w2, s2) = _weights(e, d, f, 4, 32)
+    x = rng.standard_normal((n, d)).astype(np.float16)
+    ids = _ids(rng, n, e, k).astype(np.int32)
+    weights = rng.random((n, k)).astype(np.float32)
+    for path in (mld.MOE_PATH_FEW_ROWS, mld.MOE_PATH_MANY_ROWS):
+        plan = mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=path)
+        outs = []
+        for bad in (False, True):
+            y = x.copy()
+            if bad:
+                y[7, 5], y[11] = np.nan, np.inf
+            out = torch.empty(n, d, dtype=torch.float16, device="cuda")
+            plan.run(_dev(y), _dev(ids), _dev(weights), w1, s1, w2, s2, out)
+            outs.append(out.cpu().numpy())
+        assert np.isnan(outs[1][7]).all() and np.isnan(outs[1][11]).all()
+        rest = [t for t in range(n) if t not in (7, 11)]
+        assert np.array_equal(outs[0][rest], outs[1][rest])
