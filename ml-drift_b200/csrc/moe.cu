@@ -24,7 +24,7 @@ constexpr int kMaxExperts = 1024;
 // it.  The blocks of a cluster take a part of the pairs each and read one another's counts.  (Rows of an expert come in any
 // order; no row's results depend on where it stands.)
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* __restrict__ ids, int pairs, int experts, int tile_rows,
-                                                                 MoeBuffers b) {
+                                                                 bool even, MoeBuffers b) {
   pdl_wait();
   pdl_launch_dependents();
   __shared__ int count[kMaxExperts], next[kMaxExperts];
@@ -77,8 +77,13 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* _
   }
   next[me] = row0 + before;
   if (rank == 0) {
-    for (int i = 0; i < tiles; ++i) b.tiles[tile0 + i] = {me, row0 + i * tile_rows, min(tile_rows, all - i * tile_rows), 0};
-    if (me == kSortThreads - 1) *b.n_tiles = tile0 + tiles;
+    // (even: an expert's tiles alike, in steps of 64 rows: one costs its dequantised weights, however few its rows)
+    const int rows = even && tiles > 0 ? ((all + tiles - 1) / tiles + 63) / 64 * 64 : tile_rows;
+    for (int i = 0; i < tiles; ++i) b.tiles[tile0 + i] = {me, row0 + i * rows, min(rows, all - i * rows), 0};
+    if (me == kSortThreads - 1) {
+      b.n_tiles[0] = tile0 + tiles;
+      b.n_tiles[1] = row0 + all;
+    }
   }
   __syncthreads();
   for (int p = from + me; p < to; p += kSortThreads) {
@@ -92,6 +97,18 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* _
   }
   // (nobody leaves while another may still read its counts)
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Rows of x in the order of positions, a warp to a row.
+__global__ void __launch_bounds__(256) moe_gather_kernel(const __half* __restrict__ x, int64_t x_stride, int top_k, int width, MoeBuffers b) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int at = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (at >= b.n_tiles[1]) return;
+  const uint4* from = reinterpret_cast<const uint4*>(x + b.order[at] / top_k * x_stride);
+  uint4* to = reinterpret_cast<uint4*>(static_cast<__half*>(b.sorted) + static_cast<int64_t>(at) * width);
+#pragma unroll 4
+  for (int c = lane; c < width / 8; c += 32) to[c] = from[c];
 }
 
 // ---------------------------------------------------------------------------------------------------- few rows
@@ -339,7 +356,7 @@ __global__ void __launch_bounds__(256) moe_sum_kernel(SumArgs a) {
   }
 }
 
-int launch_sort(const int32_t* ids, int pairs, int experts, int tile_rows, const MoeBuffers& b, cudaStream_t stream) {
+int launch_sort(const int32_t* ids, int pairs, int experts, int tile_rows, bool even, const MoeBuffers& b, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
   const int ctas = pairs <= kSortAlone ? 1 : kSortCtas;
   cfg.gridDim = dim3(ctas);
@@ -353,7 +370,7 @@ int launch_sort(const int32_t* ids, int pairs, int experts, int tile_rows, const
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  MLD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, moe_sort_kernel, ids, pairs, experts, tile_rows, b));
+  MLD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, moe_sort_kernel, ids, pairs, experts, tile_rows, even, b));
   MLD_LAUNCH_CHECK();
   return MLD_OK;
 }
@@ -410,8 +427,8 @@ int few_eights(int pairs, int experts) { return pairs <= 6 * experts ? 1 : pairs
 int most_tiles(int pairs, int experts, int rows) { return pairs < experts + pairs / rows ? pairs : experts + pairs / rows; }
 
 bool takes_many(const mld_moe_desc& d, int tokens) {
-  (void)tokens;
-  return d.force_path == MLD_MOE_PATH_MANY_ROWS;
+  if (d.force_path != MLD_MOE_PATH_AUTO) return d.force_path == MLD_MOE_PATH_MANY_ROWS;
+  return static_cast<int64_t>(tokens) * d.top_k >= 24ll * d.experts;
 }
 
 }  // namespace
@@ -532,10 +549,35 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
   const bool one = tokens == 1, many = takes_many(d, tokens);
   const int eights = one ? 1 : few_eights(pairs, d.experts);
   int rc = MLD_OK;
-  if (many) return MLD_UNIMPLEMENTED;
+  const MoeShape shape = {d.experts, d.top_k, d.d_model, d.ffn, d.weight_bits, d.block, d.activation};
+  SumArgs s = {};
+  s.b = plan->b;
+  s.ids = one && !many ? io->ids : nullptr;
+  s.weights = io->weights;
+  s.residual = static_cast<const __half*>(io->residual);
+  s.out = static_cast<__half*>(io->out);
+  s.residual_stride = io->residual_stride;
+  s.out_stride = io->out_stride;
+  s.experts = d.experts;
+  s.top_k = d.top_k;
+  s.width = d.d_model;
+  if (many) {
+    const int rows = pairs > 64 * d.experts ? 256 : 128;
+    rc = launch_sort(io->ids, pairs, d.experts, rows, true, plan->b, stream);
+    if (rc != MLD_OK) return rc;
+    MLD_CUDA_CHECK(launch_overlapped(moe_gather_kernel, dim3(div_up(pairs, 8)), dim3(256), 0, stream, static_cast<const __half*>(io->x),
+                                     io->x_stride, d.top_k, d.d_model, plan->b));
+    MLD_LAUNCH_CHECK();
+    rc = launch_moe_gemm(true, shape, plan->b, io->gate_up, io->gate_up_scale, pairs, rows, plan->sms, stream);
+    if (rc == MLD_OK) rc = launch_moe_gemm(false, shape, plan->b, io->down, io->down_scale, pairs, rows, plan->sms, stream);
+    if (rc != MLD_OK) return rc;
+    MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<__half>, dim3(tokens), dim3(256), 0, stream, s));
+    MLD_LAUNCH_CHECK();
+    return MLD_OK;
+  }
   int tiles = pairs;
   if (!one) {
-    rc = launch_sort(io->ids, pairs, d.experts, 8 * eights, plan->b, stream);
+    rc = launch_sort(io->ids, pairs, d.experts, 8 * eights, false, plan->b, stream);
     if (rc != MLD_OK) return rc;
     tiles = most_tiles(pairs, d.experts, 8 * eights);
   }
@@ -563,17 +605,6 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
   matrix(io->down, io->down_scale, d.d_model, d.ffn);
   rc = launch_few<false>(f, d.weight_bits, eights, tiles, stream);
   if (rc != MLD_OK) return rc;
-  SumArgs s = {};
-  s.b = plan->b;
-  s.ids = f.ids;
-  s.weights = io->weights;
-  s.residual = static_cast<const __half*>(io->residual);
-  s.out = static_cast<__half*>(io->out);
-  s.residual_stride = io->residual_stride;
-  s.out_stride = io->out_stride;
-  s.experts = d.experts;
-  s.top_k = d.top_k;
-  s.width = d.d_model;
   MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<float>, dim3(tokens), dim3(256), 0, stream, s));
   MLD_LAUNCH_CHECK();
   return MLD_OK;

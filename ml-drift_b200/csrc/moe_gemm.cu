@@ -1,0 +1,505 @@
+// The experts' products for many rows: tiles of one expert's rows on pairs of SMs, the dequantised weights in tensor memory.
+//
+// The form is gemm_wtmem_kernel's (Y^T = W X^T, tcgen05 cta_group::2, weights as the A operand in tensor memory, rows as the B
+// operand in shared memory), with what a grouped product needs in place of what a single one does:
+//   - a tile is 256 outputs of one expert x up to kTok of its rows; which expert and which rows stands in a list that the
+//     ordering kernel left in device memory.  Every role reads the list for itself and goes through the same tiles.
+//   - rows of an expert follow one another, so a tile's rows are one box after another of 32; as many are fetched as the tile has
+//     rows, and the MMA's N is that many, too (in steps of 64).  Columns behind the tile's rows belong to other experts, or are
+//     zeros, and are not written.
+//   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
+//     and an up channel, exchange half of their tokens; of the second the expert's output.
+// Per CTA: warp 0 fetches rows, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first CTA), warps 6..21 dequantise
+// (four to a stage of 64 inputs), warps 2..5 write the results; with tiles of up to 256 rows the sixteen help them, since all
+// 256 columns are one tile's, with up to 128 there are two sets of accumulators and the next tile goes on meanwhile.
+// Bound by the tensor cores for tiles of 256 rows, by the dequantisation (four instructions for two weights) for smaller ones.
+// Every wait is bounded.
+#include <cuda_fp16.h>
+
+#include <cstring>
+
+#include "common.cuh"
+#include "moe.cuh"
+#include "pair_common.cuh"
+#include "wtmem.cuh"
+
+namespace mld {
+namespace {
+
+constexpr int kStages = 8;              // rows in shared memory + weights in tensor memory
+constexpr int kWStages = 8;             // packed weights
+constexpr int kChannels = 128;          // outputs per CTA
+constexpr int kBoxRows = 32;
+constexpr int kBoxBytes = kBoxRows * kKBytes;
+constexpr int kSlices = 16;             // packed rows of a stage: 64 inputs
+constexpr uint32_t kRingCol = 256;      // first tensor-memory column of the weights
+constexpr int kThreads = 23 * 32;
+constexpr int kReaders = 5;             // warps that can read a lane quarter's accumulators
+constexpr int kErrMoeBase = 70;
+
+struct GemmArgs {
+  const MoeTile* tiles;
+  const int* n_tiles;
+  int n_channel_tiles, k_blocks;
+  int n, k;                             // outputs, inputs
+  const __half* scale;
+  int64_t expert_scales;
+  int groups, group_shift;              // log2 of a group's input slices
+  __half* out;                          // rows by position: act(gate) * up [n / 2], or [n]
+  int activation;
+  int* error;
+};
+
+struct Work {
+  int t, total, step, n_channel_tiles;
+  const MoeTile* tiles;
+  __device__ __forceinline__ bool next(MoeTile& tile, int& n0) {
+    if (t >= total) return false;
+    const int4 v = *reinterpret_cast<const int4*>(tiles + t / n_channel_tiles);
+    tile.expert = v.x;
+    tile.row0 = v.y;
+    tile.rows = v.z;
+    n0 = t % n_channel_tiles * (2 * kChannels);
+    t += step;
+    return true;
+  }
+  __device__ __forceinline__ bool done() const { return t >= total; }
+};
+__device__ __forceinline__ int columns_of(const MoeTile& t) { return (t.rows + 63) & ~63; }
+
+// x0..x3: a lane's four pairs of tokens -> pair q of the tokens of four lanes' channels.  A: lane bits that number the four.
+template <int LOW>
+__device__ __forceinline__ void turn_pairs(uint32_t& x0, uint32_t& x1, uint32_t& x2, uint32_t& x3, int q) {
+  {
+    const bool up = (q & 2) != 0;
+    const uint32_t s0 = up ? x0 : x2, s1 = up ? x1 : x3;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, s0, 2 * LOW), r1 = __shfl_xor_sync(0xffffffffu, s1, 2 * LOW);
+    if (up) {
+      x0 = r0;
+      x1 = r1;
+    } else {
+      x2 = r0;
+      x3 = r1;
+    }
+  }
+  {
+    const bool up = (q & 1) != 0;
+    const uint32_t s0 = up ? x0 : x1, s1 = up ? x2 : x3;
+    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, s0, LOW), r1 = __shfl_xor_sync(0xffffffffu, s1, LOW);
+    if (up) {
+      x0 = r0;
+      x2 = r1;
+    } else {
+      x1 = r0;
+      x3 = r1;
+    }
+  }
+}
+// The four channels of a token pair, after turn_pairs, to two rows of the output.
+__device__ __forceinline__ void store_pair(__half* first, int64_t pitch, bool one, bool two, uint32_t x0, uint32_t x1, uint32_t x2,
+                                           uint32_t x3) {
+  if (one) *reinterpret_cast<uint2*>(first) = make_uint2(__byte_perm(x0, x1, 0x5410), __byte_perm(x2, x3, 0x5410));
+  if (two) *reinterpret_cast<uint2*>(first + pitch) = make_uint2(__byte_perm(x0, x1, 0x7632), __byte_perm(x2, x3, 0x7632));
+}
+
+template <int BITS, bool FIRST, int TOK>
+__global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
+    moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, GemmArgs a) {
+  constexpr int kBlk = BITS == 4 ? 8 : 16;
+  constexpr int kPitch = kChannels / 4 * kBlk;        // bytes of a packed row of the box
+  constexpr int kWBytes = kSlices * kPitch;
+  constexpr int kSets = 256 / TOK;                    // sets of accumulators
+  constexpr int kXBytes = TOK / 2 * kKBytes;          // a CTA's rows of a stage
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sX = smem;
+  uint8_t* sW = sX + kStages * kXBytes;
+  uint64_t* full_w = reinterpret_cast<uint64_t*>(sW + kWStages * kWBytes);
+  uint64_t* w_empty = full_w + kWStages;       // the dequantising warps have read the box
+  uint64_t* full_ab = w_empty + kWStages;      // first CTA: rows and weights of both CTAs are there
+  uint64_t* empty = full_ab + kStages;         // the stage's MMAs are done (arrives in both CTAs)
+  uint64_t* tmem_full = empty + kStages;       // [3]: sets that the writing warp reads alone, then those that all read
+  uint64_t* tmem_empty = tmem_full + 3;        // [2], first CTA
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  // (the ordering kernel's list, and for the first product its rows, come from launches ahead; for the second the list is older
+  // than the launch ahead, which began only when it was complete)
+  if constexpr (FIRST) {
+    pdl_wait();
+  }
+  pdl_launch_dependents();
+  Work work0;
+  work0.n_channel_tiles = a.n_channel_tiles;
+  work0.t = static_cast<int>(blockIdx.x) / 2;
+  work0.step = static_cast<int>(gridDim.x) / 2;
+  work0.total = *a.n_tiles * a.n_channel_tiles;
+  work0.tiles = a.tiles;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kWStages; ++s) {
+      mbar_init(&full_w[s], 1);
+      mbar_init(&w_empty[s], 4);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&full_ab[s], 1 + 2 * 4);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 3; ++b) mbar_init(&tmem_full[b], 1);
+    for (int b = 0; b < 2; ++b) mbar_init(&tmem_empty[b], kSets == 1 ? 2 * 4 * kReaders : 2 * 4);
+    fence_barrier_init();
+  }
+  if (warp == 1) tmem_alloc_all<true>(tmem_slot);
+  tc_before();
+  __syncthreads();
+  cluster_sync_all();
+  tc_after();
+  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t full_ab_lead = map_shared(smem_u32(full_ab), 0), tmem_empty_lead = map_shared(smem_u32(tmem_empty), 0);
+  // With one set of accumulators all warps of a quarter read it; with two the last tile's only.
+  const auto read_by_all = [&](bool last) { return kSets == 1 || last; };
+
+  const auto drain = [&](const MoeTile& tile, int n0, int part, int parts, int set) {
+    const int quad = warp & 3;
+    const uint32_t base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(set * TOK);
+    const int n = n0 + static_cast<int>(rank) * kChannels + quad * 32;  // the warp's first channel
+    const bool has_n = n < a.n;                                         // (a.n is a multiple of 32)
+    const int pieces = (tile.rows + 15) >> 4;
+    for (int pc = part; pc < pieces; pc += parts) {
+      uint32_t r[16];
+      tmem_ld16(base + static_cast<uint32_t>(16 * pc), r);
+      tmem_ld_wait();
+      if constexpr (FIRST) {
+        const bool odd = (lane & 1) != 0;
+        uint32_t x[4];
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+          float v[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int j = 2 * p + i;
+            const float got = __uint_as_float(__shfl_xor_sync(0xffffffffu, odd ? r[j] : r[8 + j], 1));
+            const float gate = odd ? got : __uint_as_float(r[j]), up = odd ? __uint_as_float(r[8 + j]) : got;
+            v[i] = moe_gated(gate, up, a.activation);
+          }
+          const __half2 h = __floats2half2_rn(v[0], v[1]);
+          x[p] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        const int q = (lane >> 1) & 3;
+        turn_pairs<2>(x[0], x[1], x[2], x[3], q);
+        const int m = 16 * pc + (odd ? 8 : 0) + 2 * q;
+        __half* to = a.out + static_cast<int64_t>(tile.row0 + m) * (a.n >> 1) + (n >> 1) + (lane >> 3) * 4;
+        store_pair(to, a.n >> 1, has_n && m < tile.rows, has_n && m + 1 < tile.rows, x[0], x[1], x[2], x[3]);
+      } else {
+        uint32_t x[8];
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const __half2 h = __floats2half2_rn(__uint_as_float(r[2 * p]), __uint_as_float(r[2 * p + 1]));
+          x[p] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        const int q = lane & 3;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          turn_pairs<1>(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3], q);
+          const int m = 16 * pc + 8 * h + 2 * q;
+          __half* to = a.out + static_cast<int64_t>(tile.row0 + m) * a.n + n + (lane >> 2) * 4;
+          store_pair(to, a.n, has_n && m < tile.rows, has_n && m + 1 < tile.rows, x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
+        }
+      }
+    }
+    tc_before();
+    __syncwarp();
+    if (lane == 0 && (kSets == 1 || part == 0)) arrive_in_pair(tmem_empty_lead + set * 8);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ rows
+    if (lane == 0) prefetch_tmap(&tmap_x);
+    if constexpr (!FIRST) pdl_wait();
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    Work work = work0;
+    MoeTile tile;
+    int n0;
+    while (ok && work.next(tile, n0)) {
+      const int cols = columns_of(tile), row = tile.row0 + static_cast<int>(rank) * (cols >> 1);
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1))) {
+          if (lane == 0) atomicExch(a.error, kErrMoeBase + 1);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          if (rank == 0) mbar_arrive_expect_tx(&full_ab[stage], static_cast<uint32_t>(cols) * kKBytes);
+          for (int i = 0; i < cols >> 6; ++i)
+            tma_load_2d_pair(sX + stage * kXBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row + i * kBoxRows);
+        }
+        __syncwarp();
+        if (++stage == kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------- MMAs
+    if (rank == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      Work work = work0;
+      MoeTile tile;
+      int n0;
+      for (int nth = 0; ok && work.next(tile, n0); ++nth) {
+        const int set = kSets == 1 ? 0 : nth & 1;
+        const uint32_t set_phase = static_cast<uint32_t>(kSets == 1 ? nth : nth >> 1) & 1u;
+        const uint32_t idesc = 1u << 4 | static_cast<uint32_t>(columns_of(tile) >> 3) << 17 | 16u << 24;
+        const uint32_t d = tmem_base + static_cast<uint32_t>(set * TOK);
+        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[set], set_phase ^ 1))) {
+          if (lane == 0) atomicExch(a.error, kErrMoeBase + 2);
+          break;
+        }
+        tc_after();
+        for (int kb = 0; kb < a.k_blocks; ++kb) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&full_ab[stage], phase))) {
+            if (lane == 0) atomicExch(a.error, kErrMoeBase + 3);
+            ok = false;
+            break;
+          }
+          tc_after();
+          const uint64_t db = make_desc(smem_u32(sX + stage * kXBytes));
+          const uint32_t ta = tmem_base + kRingCol + static_cast<uint32_t>(stage * 32);
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              umma_ts<true, false>(d, ta + 8u * i, db + static_cast<uint64_t>((i * 32) >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
+            commit<true>(&empty[stage]);
+          }
+          __syncwarp();
+          if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok && elect_one()) commit<true>(&tmem_full[read_by_all(work.done()) ? 2 : set]);
+        __syncwarp();
+      }
+    }
+  } else if (warp < 6) {
+    // ---------------------------------------------------------------- results
+    if constexpr (!FIRST) pdl_wait();  // (what is written here may still be read by launches ahead of the one ahead)
+    Work work = work0;
+    MoeTile tile;
+    int n0, together = 0;
+    for (int nth = 0; work.next(tile, n0); ++nth) {
+      const int set = kSets == 1 ? 0 : nth & 1;
+      const bool all = read_by_all(work.done());
+      const int use = all ? together++ : nth >> 1;
+      if (!mbar_wait(&tmem_full[all ? 2 : set], static_cast<uint32_t>(use) & 1u)) {
+        atomicExch(a.error, kErrMoeBase + 4);
+        break;
+      }
+      tc_after();
+      drain(tile, n0, 0, all ? kReaders : 1, set);
+    }
+  } else if (warp == 22) {
+    // --------------------------------------------------------- packed weights
+    if (lane == 0) prefetch_tmap(&tmap_w);
+    int ws = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    Work work = work0;
+    MoeTile tile;
+    int n0;
+    while (ok && work.next(tile, n0)) {
+      const int column = (n0 + static_cast<int>(rank) * kChannels) / 4 * kBlk / 4;  // in 32-bit elements
+      const int row = tile.expert * (a.k >> 2);
+      for (int kb = 0; kb < a.k_blocks; ++kb) {
+        if (!__all_sync(0xffffffffu, mbar_wait(&w_empty[ws], phase ^ 1))) {
+          if (lane == 0) atomicExch(a.error, kErrMoeBase + 5);
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
+          mbar_arrive_expect_tx(&full_w[ws], kWBytes);
+          tma_load_2d(sW + ws * kWBytes, &tmap_w, &full_w[ws], column, row + kb * kSlices);
+        }
+        __syncwarp();
+        if (++ws == kWStages) {
+          ws = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // -------------------------------------------------------- dequantisation
+    const int group = (warp - 6) >> 2;  // this group of four warps takes every fourth stage
+    const int quad = warp & 3;
+    const int row = quad * 32 + lane;   // output channel of the CTA's 128 = tensor-memory lane
+    const int col4 = row & 3;
+    const uint32_t sel8 = static_cast<uint32_t>(col4) | static_cast<uint32_t>(4 + col4) << 8;
+    const __half2 offset = __float2half2_rn(BITS == 4 ? 1032.0f : 1152.0f);
+    bool ok = true;
+    int before = 0;  // stages before the tile
+    int stored = -1;
+    const auto announce = [&]() {
+      if (stored < 0) return;
+      tmem_st_wait();
+      tc_before();
+      __syncwarp();
+      if (lane == 0) arrive_in_pair(full_ab_lead + stored * 8);
+      stored = -1;
+    };
+    if constexpr (!FIRST && kSets == 1) pdl_wait();  // (it writes results, too)
+    Work work = work0;
+    MoeTile tile;
+    int n0, together = 0;
+    for (int nth = 0; ok && work.next(tile, n0); ++nth) {
+      const int n = n0 + static_cast<int>(rank) * kChannels + row;
+      const bool has_n = n < a.n;
+      const __half* const scale = a.scale + tile.expert * a.expert_scales + n;
+      // the scale of 32 inputs, asked for four stages ahead (by hand, so that nothing looks at it before)
+      const auto ask = [&](unsigned short& v, int slice) {
+        const int g = min(slice >> a.group_shift, a.groups - 1);
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.nc.u16 %0, [%1];\n\t}"
+                     : "+h"(v)
+                     : "l"(scale + static_cast<int64_t>(g) * a.n), "r"(has_n ? 1u : 0u));
+      };
+      int kb = (group - before) & 3;
+      unsigned short next0 = 0, next1 = 0;
+      if (kb < a.k_blocks) {
+        ask(next0, kb * kSlices);
+        ask(next1, kb * kSlices + 8);
+      }
+      for (; kb < a.k_blocks; kb += 4) {
+        const int iter = before + kb, stage = iter & (kStages - 1), ws = iter & (kWStages - 1);
+        const unsigned short cur0 = next0, cur1 = next1;
+        if (kb + 4 < a.k_blocks) {
+          ask(next0, (kb + 4) * kSlices);
+          ask(next1, (kb + 4) * kSlices + 8);
+        }
+        if (!mbar_wait(&full_w[ws], static_cast<uint32_t>(iter / kWStages) & 1u)) {
+          atomicExch(a.error, kErrMoeBase + 6);
+          ok = false;
+          break;
+        }
+        const uint8_t* wp = sW + ws * kWBytes + (row >> 2) * kBlk;
+        const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kRingCol + static_cast<uint32_t>(stage * 32);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          using Block = typename std::conditional<BITS == 4, uint2, uint4>::type;
+          Block blk[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (8 * half + i) * kPitch);
+          if (half == 0) {
+            announce();
+            if (!mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u)) {
+              atomicExch(a.error, kErrMoeBase + 6);
+              ok = false;
+              break;
+            }
+            tc_after();
+          }
+          uint32_t o[16];
+          const __half2 s2 = __half2half2(__ushort_as_half(half == 0 ? cur0 : cur1));
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const Block v = blk[i];
+            if constexpr (BITS == 4) {
+              o[2 * i] = dq_once(((v.x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+              o[2 * i + 1] = dq_once(((v.y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+            } else {
+              o[2 * i] = dq_once((__byte_perm(v.x, v.y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+              o[2 * i + 1] = dq_once((__byte_perm(v.z, v.w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+            }
+          }
+          tmem_st16(columns + static_cast<uint32_t>(16 * half), o);
+        }
+        if (!ok) break;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&w_empty[ws]);
+        stored = stage;
+      }
+      announce();
+      before += a.k_blocks;
+      if (!ok) break;
+      if (!read_by_all(work.done())) continue;
+      if constexpr (!FIRST && kSets == 2) pdl_wait();
+      if (!mbar_wait(&tmem_full[2], static_cast<uint32_t>(together++) & 1u)) {
+        atomicExch(a.error, kErrMoeBase + 7);
+        break;
+      }
+      tc_after();
+      drain(tile, n0, 1 + group, kReaders, kSets == 1 ? 0 : nth & 1);
+    }
+  }
+  // Nobody leaves while the partner may still arrive on this CTA's barriers or the pair's MMAs write its tensor memory.
+  tc_before();
+  __syncthreads();
+  cluster_sync_all();
+  if (*reinterpret_cast<volatile int*>(a.error) != 0) {
+    // a wait ran out somewhere: copies may still be in flight towards this CTA's shared memory
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+  }
+  if (warp == 1) {
+    tc_after();
+    tmem_dealloc_all<true>(tmem_base);
+  }
+}
+
+template <int BITS, bool FIRST, int TOK>
+int launch_of(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int grid, cudaStream_t stream) {
+  constexpr size_t smem = 1024 + kStages * (TOK / 2) * kKBytes + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
+                          (2 * kWStages + 2 * kStages + 5) * 8 + 64;
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kern = moe_gemm_kernel<BITS, FIRST, TOK>;
+  static bool done[kMaxDevices];
+  int dev;
+  if (needs_configure(done, &dev)) {
+    MLD_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    if (dev >= 0) done[dev] = true;
+  }
+  MLD_CUDA_CHECK(launch_overlapped(kern, dim3(grid), dim3(kThreads), smem, stream, tx, tw, a));
+  MLD_LAUNCH_CHECK();
+  return MLD_OK;
+}
+
+}  // namespace
+
+int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs,
+                    int tile_rows, int sms, cudaStream_t stream) {
+  const int n = first ? 2 * s.ffn : s.d_model, k = first ? s.d_model : s.ffn, blk = s.bits == 4 ? 8 : 16;
+  CUtensorMap tx, tw;
+  int rc = make_tmap_2d(&tx, first ? b.sorted : b.hidden, static_cast<uint64_t>(k) * 2, pairs, static_cast<uint64_t>(k) * 2, kKBytes,
+                        kBoxRows, 2, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, true);
+  if (rc != MLD_OK) return rc;
+  rc = make_tmap_2d(&tw, weights, static_cast<uint64_t>(n / 4) * blk, static_cast<uint64_t>(s.experts) * (k / 4),
+                    static_cast<uint64_t>(n / 4) * blk, kChannels / 4 * blk, kSlices, 4, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc != MLD_OK) return rc;
+  GemmArgs a = {};
+  a.tiles = b.tiles;
+  a.n_tiles = b.n_tiles;
+  a.n_channel_tiles = div_up(n, 2 * kChannels);
+  a.k_blocks = div_up(k, 64);
+  a.n = n;
+  a.k = k;
+  a.scale = static_cast<const __half*>(scale);
+  a.groups = s.block != 0 ? k / s.block : 1;
+  a.group_shift = 30;
+  if (s.block != 0)
+    for (a.group_shift = 3; (4 << a.group_shift) < s.block;) ++a.group_shift;
+  a.expert_scales = static_cast<int64_t>(a.groups) * n;
+  a.out = static_cast<__half*>(first ? b.hidden : b.part);
+  a.activation = s.activation;
+  a.error = b.error;
+  const int grid = sms / 2 * 2;
+#define MLD_MOE_GEMM(BITS, FIRST) \
+  (tile_rows > 128 ? launch_of<BITS, FIRST, 256>(tx, tw, a, grid, stream) : launch_of<BITS, FIRST, 128>(tx, tw, a, grid, stream))
+  if (s.bits == 4) return first ? MLD_MOE_GEMM(4, true) : MLD_MOE_GEMM(4, false);
+  return first ? MLD_MOE_GEMM(8, true) : MLD_MOE_GEMM(8, false);
+#undef MLD_MOE_GEMM
+}
+
+}  // namespace mld
