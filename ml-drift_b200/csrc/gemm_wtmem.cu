@@ -265,6 +265,8 @@ __global__ void __launch_bounds__(kWtThreads, 1)
       }
     }
     const int q = lane & 3;  // place among the four channels of the output slice n >> 2
+    // row-major outputs whose four channels lie on 8 bytes go the same way, a token's four at a time
+    const bool rows_of_4 = a.dst_layout != MLD_LAYOUT_SLICED && a.N % 4 == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7) == 0;
     for (int pc = kUnit * part; pc < n_pieces; pc = next_piece(pc, kUnit, parts)) {
       const int c0 = 16 * pc;
       uint32_t r[16];
@@ -308,7 +310,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
         if (a.bias != nullptr) v = __hadd2(v, __half2half2(bias_h));
         h2[i] = *reinterpret_cast<const uint32_t*>(&v);
       }
-      if (a.dst_layout == MLD_LAYOUT_SLICED) {
+      if (a.dst_layout == MLD_LAYOUT_SLICED || rows_of_4) {
         // Eight tokens at a time: the four lanes of a slice exchange token pairs so that lane q holds tokens
         // 2q, 2q + 1 (of the eight) of all four channels, 16 contiguous bytes of [slice][token][4 channels].
 #pragma unroll
@@ -346,7 +348,13 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           pk.y = __byte_perm(x2, x3, 0x5410);  //          channels 2, 3
           pk.z = __byte_perm(x0, x1, 0x7632);  // token m + 1
           pk.w = __byte_perm(x2, x3, 0x7632);
-          if (has_n && m < a.M) {
+          if (rows_of_4) {
+            if (has_n && m < a.M) {
+              __half* const base = static_cast<__half*>(a.y) + (size_t)m * a.N + (n & ~3);
+              *reinterpret_cast<uint2*>(base) = make_uint2(pk.x, pk.y);
+              if (m + 1 < a.M) *reinterpret_cast<uint2*>(base + a.N) = make_uint2(pk.z, pk.w);
+            }
+          } else if (has_n && m < a.M) {
             const size_t at = ((size_t)(n >> 2) * a.M + m) * 4;  // in halves
             const bool both = m + 1 < a.M && ((at * 2) & 15) == 0;
             const int world = a.outs.world > 1 ? a.outs.world : 1;
