@@ -816,13 +816,13 @@ class MoeIo(C.Structure):
                 ("residual_stride", C.c_int64), ("out", C.c_void_p), ("out_stride", C.c_int64)]
 
 
-def _table(t, rows, columns, dtype, what, gpu):
+def _table(t, shape, dtype, what, gpu):
     """Elements from row to row of a [rows][columns] tensor whose rows are contiguous."""
     stride = t.stride()
-    if t.get_device() != gpu or t.dtype is not dtype or t.shape != (rows, columns) or (stride[1] != 1 and columns > 1):
+    if t.get_device() != gpu or t.dtype is not dtype or t.shape != shape or (stride[1] != 1 and shape[1] > 1):
         if t.get_device() != gpu:
             raise _elsewhere(t, what)
-        raise ValueError(f"{what}: expected {dtype} [{rows}][{columns}] with contiguous rows, got {t.dtype} {tuple(t.shape)} "
+        raise ValueError(f"{what}: expected {dtype} [{shape[0]}][{shape[1]}] with contiguous rows, got {t.dtype} {tuple(t.shape)} "
                          f"strides {stride}")
     return stride[0]
 
@@ -836,7 +836,7 @@ def _whole(t, elements, dtype, what, gpu):
 
 
 def _codes(codes, params, tokens, width, gpu):
-    stride = _table(codes, tokens, div_up(width, 16) * 16, torch.int8, "codes", gpu)
+    stride = _table(codes, (tokens, (width + 15) // 16 * 16), torch.int8, "codes", gpu)
     _whole(params, 3 * tokens, torch.float32, "params", gpu)
     return stride
 
@@ -846,27 +846,34 @@ def add_rms_norm(x, weight=None, residual=None, sum_out=None, out=None, codes=No
     """h = x + residual (into sum_out), y = h (weight_offset + weight) / sqrt(mean h^2 + eps) into out, and / or its codes (int8
     [tokens][width rounded up to 16]) with scale and zero point (params, fp32 [tokens][3]); x, residual, sum_out, out: [tokens][width]
     fp16 or fp32, rows may be strided."""
-    n, w = x.shape
-    dt = x.dtype
+    shape, dt = x.shape, x.dtype
+    n, w = shape
     gpu, queue = _here(stream)
-    d = AddNormDesc(w, eps, weight_offset, _f16(x), int(not symmetric))
-    io = AddNormIo()
-    io.x, io.x_stride = x.data_ptr(), _table(x, n, w, dt, "x", gpu)
+    what = (w, eps, weight_offset, dt, symmetric)
+    d = _norm_descs.get(what)
+    if d is None:
+        d = _norm_descs[what] = AddNormDesc(w, eps, weight_offset, _f16(x), int(not symmetric))
+    xs = _table(x, shape, dt, "x", gpu)
+    r = s = o = q = p = g = None
+    rs = ss = os_ = qs = 0
     if residual is not None:
-        io.residual, io.residual_stride = residual.data_ptr(), _table(residual, n, w, dt, "residual", gpu)
+        r, rs = residual.data_ptr(), _table(residual, shape, dt, "residual", gpu)
     if weight is not None:
-        io.weight = _whole(weight, w, dt, "weight", gpu)
+        g = _whole(weight, w, dt, "weight", gpu)
     if sum_out is not None:
-        io.sum_out, io.sum_stride = sum_out.data_ptr(), _table(sum_out, n, w, dt, "sum_out", gpu)
+        s, ss = sum_out.data_ptr(), _table(sum_out, shape, dt, "sum_out", gpu)
     if out is not None:
-        io.out, io.out_stride = out.data_ptr(), _table(out, n, w, dt, "out", gpu)
+        o, os_ = out.data_ptr(), _table(out, shape, dt, "out", gpu)
     if codes is not None:
         if params is None:
             raise ValueError("codes and params go together")
-        io.codes, io.codes_stride, io.params = codes.data_ptr(), _codes(codes, params, n, w, gpu), params.data_ptr()
-    rc = lib().mld_add_rms_norm(C.byref(d), C.byref(io), n, queue)
+        q, qs, p = codes.data_ptr(), _codes(codes, params, n, w, gpu), params.data_ptr()
+    rc = (_lib or lib()).mld_add_rms_norm(C.byref(d), C.byref(AddNormIo(x.data_ptr(), xs, r, rs, g, s, ss, o, os_, q, qs, p)), n, queue)
     if rc != OK:
         _check(rc, "mld_add_rms_norm")
+
+
+_norm_descs = {}  # descriptors by what they say
 
 
 MOE_SOFTMAX, MOE_SIGMOID = 0, 1
@@ -880,15 +887,16 @@ class MoeRouter:
     def __init__(self, experts, top_k, score=MOE_SOFTMAX, groups=1, top_groups=1, group_best=1, renormalise=True, factor=1.0, f16=True):
         self.desc = MoeRouteDesc(experts, top_k, score, groups, top_groups, group_best, int(renormalise), factor, int(f16))
         self.experts, self.top_k, self.dtype = experts, top_k, torch.float16 if f16 else torch.float32
+        self._d = C.byref(self.desc)
 
     def run(self, logits, ids, weights, bias=None, stream=None):
         """logits: [tokens][experts] (rows may be strided); ids int32, weights fp32, [tokens][top_k]; bias: fp32 [experts]."""
-        n = logits.shape[0]
+        n, k = logits.shape[0], self.top_k
         gpu, queue = _here(stream)
-        stride = _table(logits, n, self.experts, self.dtype, "logits", gpu)
-        rc = lib().mld_moe_route(C.byref(self.desc), logits.data_ptr(), stride,
-                                 None if bias is None else _whole(bias, self.experts, torch.float32, "bias", gpu),
-                                 _ints(ids, (n, self.top_k), "ids", gpu), _whole(weights, n * self.top_k, torch.float32, "weights", gpu), n, queue)
+        stride = _table(logits, (n, self.experts), self.dtype, "logits", gpu)
+        rc = (_lib or lib()).mld_moe_route(self._d, logits.data_ptr(), stride,
+                                None if bias is None else _whole(bias, self.experts, torch.float32, "bias", gpu),
+                                _ints(ids, (n, k), "ids", gpu), _whole(weights, n * k, torch.float32, "weights", gpu), n, queue)
         if rc != OK:
             _check(rc, "mld_moe_route")
 
@@ -899,6 +907,7 @@ class MoeExperts:
     def __init__(self, experts, top_k, d_model, ffn, weight_bits=4, block=32, activation=MOE_SILU, max_tokens=1, device=-1,
                  force_path=MOE_PATH_AUTO):
         self.desc = MoeDesc(experts, top_k, d_model, ffn, weight_bits, block, activation, max_tokens, device, force_path)
+        self._k, self._d = top_k, d_model
         self._h = C.c_void_p()
         _check(lib().mld_moe_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_moe_plan_create")
         per = [d_model // block if block else 1, ffn // block if block else 1]
@@ -908,16 +917,18 @@ class MoeExperts:
     def run(self, x, ids, weights, gate_up, gate_up_scale, down, down_scale, out, residual=None, stream=None):
         """x, out, residual: fp16 [tokens][d_model] (rows may be strided); ids int32, weights fp32, [tokens][top_k]; the experts' packed
         matrices (uint8) one behind the other, scales fp16 [experts][groups][outputs]."""
-        n, d, k = x.shape[0], self.desc.d_model, self.desc.top_k
+        n, shape, k = x.shape[0], x.shape, self._k
+        if shape[1] != self._d:
+            raise ValueError(f"x: expected rows of {self._d}, got {tuple(shape)}")
         gpu, queue = _here(stream)
-        z = self._sizes
-        io = MoeIo(x.data_ptr(), _table(x, n, d, torch.float16, "x", gpu), _ints(ids, (n, k), "ids", gpu),
-                   _whole(weights, n * k, torch.float32, "weights", gpu), _whole(gate_up, z[0], torch.uint8, "gate_up", gpu),
-                   _whole(gate_up_scale, z[1], torch.float16, "gate_up_scale", gpu), _whole(down, z[2], torch.uint8, "down", gpu),
-                   _whole(down_scale, z[3], torch.float16, "down_scale", gpu))
+        z, half, byte = self._sizes, torch.float16, torch.uint8
+        r, rs = None, 0
         if residual is not None:
-            io.residual, io.residual_stride = residual.data_ptr(), _table(residual, n, d, torch.float16, "residual", gpu)
-        io.out, io.out_stride = out.data_ptr(), _table(out, n, d, torch.float16, "out", gpu)
+            r, rs = residual.data_ptr(), _table(residual, shape, half, "residual", gpu)
+        io = MoeIo(x.data_ptr(), _table(x, shape, half, "x", gpu), _ints(ids, (n, k), "ids", gpu),
+                   _whole(weights, n * k, torch.float32, "weights", gpu), _whole(gate_up, z[0], byte, "gate_up", gpu),
+                   _whole(gate_up_scale, z[1], half, "gate_up_scale", gpu), _whole(down, z[2], byte, "down", gpu),
+                   _whole(down_scale, z[3], half, "down_scale", gpu), r, rs, out.data_ptr(), _table(out, shape, half, "out", gpu))
         rc = _lib.mld_moe_run(self._h, C.byref(io), n, queue)
         if rc != OK:
             _check(rc, "mld_moe_run")

@@ -26,8 +26,11 @@ void set_last_error_text(const char* what) { g_last_error = what; }
 void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
 
 int sm_count(int device) {
-  int n = 0;
+  static std::atomic<int> known[kMaxDevices];  // (asking takes as long as a tenth of a launch)
+  int n = device >= 0 && device < kMaxDevices ? known[device].load(std::memory_order_relaxed) : 0;
+  if (n > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) return 0;
+  if (device >= 0 && device < kMaxDevices) known[device].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -1,5 +1,5 @@
 // Experts' gated feed-forward networks over INT4 / INT8 FullyConnected weights: the plan, the order of rows by experts, the
-// products for few rows, the weighted sum.  (Products for many rows: moe_gemm.cu.)
+// weighted sum.  (Products: moe_few.cu, moe_gemm.cu.)
 #include <cuda_fp16.h>
 
 #include <cstring>
@@ -15,9 +15,8 @@ namespace {
 constexpr int kSortThreads = 1024;
 constexpr int kSortCtas = 8;            // of a cluster, where one block would take long
 constexpr int kSortAlone = 8192;        // pairs that one block sorts
-constexpr int kFewWarps = 8;
-constexpr int kFewOutputs = 64;         // outputs of a block with few rows
 constexpr int kMaxExperts = 1024;
+constexpr size_t kControlBytes = 256;   // of a plan's memory: the error, numbers of tiles and rows
 
 // ------------------------------------------------------------------------------------------------ order by experts
 // Pairs (token, place) counted by expert, the counts summed up, and every pair put behind those of its expert that came before
@@ -111,195 +110,10 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const __half* __restric
   for (int c = lane; c < width / 8; c += 32) to[c] = from[c];
 }
 
-// ---------------------------------------------------------------------------------------------------- few rows
-struct FewArgs {
-  MoeBuffers b;
-  const int32_t* ids;      // one token: its experts, no order was made
-  const __half* x;         // the first product: rows by token
-  int64_t x_stride;
-  const uint8_t* weights;
-  const __half* scale;
-  int64_t expert_bytes, expert_scales;
-  int experts, top_k, n, k, groups, block_shift;  // block_shift: log2 of the inputs of a scale
-  int activation;
-};
-
-__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint4 load_stream(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint32_t less(uint32_t biased, __half2 zero) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&biased), zero);
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
-
-// 32 inputs x 64 outputs as a lane (g = lane / 4, t = lane % 4) holds them: the 4x4 blocks of output slices 2 g and 2 g + 1, input
-// slices t and t + 4, and the scales of its eight outputs.
-template <int BITS>
-struct FewGroup {
-  uint4 w[BITS == 4 ? 2 : 4];
-  uint4 s;
-};
-
-// FIRST: x -> hidden, else hidden -> part.  NT: eights of rows.
-template <int BITS, int NT, bool FIRST>
-__global__ void __launch_bounds__(kFewWarps * 32) moe_few_kernel(FewArgs a) {
-  constexpr int kAhead = BITS == 4 ? 4 : 3;  // groups of a lane under way
-  constexpr int kBlk = BITS == 4 ? 8 : 16;
-  constexpr int kCols = 8 * NT;
-  extern __shared__ float red[];  // [warps][kCols][kFewOutputs + 4]
-  constexpr int kPitch = kFewOutputs + 4;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  if constexpr (FIRST) pdl_wait();
-  // (The second product's tiles and weights were complete before the launch ahead let this one begin; its rows were not.)
-  const int nth = static_cast<int>(blockIdx.z * gridDim.y + blockIdx.y);
-  MoeTile tile = {0, nth, 1, 0};
-  if (a.ids != nullptr) {
-    tile.expert = a.ids[nth];
-    if (static_cast<unsigned>(tile.expert) >= static_cast<unsigned>(a.experts)) return;
-  } else {
-    if (nth >= *a.b.n_tiles) return;
-    tile = a.b.tiles[nth];
-  }
-  const int n0 = static_cast<int>(blockIdx.x) * kFewOutputs;
-  const bool has_n = n0 + 8 * g < a.n;
-  const int64_t pitch = static_cast<int64_t>(a.n >> 2) * kBlk;  // bytes of an input slice
-  const uint8_t* const wp = a.weights + tile.expert * a.expert_bytes + t * pitch + ((n0 >> 2) + 2 * g) * kBlk;
-  const __half* const sp = a.scale + tile.expert * a.expert_scales + n0 + 8 * g;
-  const int groups = a.k >> 5;
-  FewGroup<BITS> ring[kAhead];
-  const auto fetch = [&](FewGroup<BITS>& r, int group) {
-    if (has_n && group < groups) {
-      const uint8_t* p = wp + static_cast<int64_t>(group) * 8 * pitch;
-      r.w[0] = load_stream(p);
-      if constexpr (BITS == 4) {
-        r.w[1] = load_stream(p + 4 * pitch);
-      } else {
-        r.w[1] = load_stream(p + 16);
-        r.w[2] = load_stream(p + 4 * pitch);
-        r.w[3] = load_stream(p + 4 * pitch + 16);
-      }
-      r.s = *reinterpret_cast<const uint4*>(sp + static_cast<int64_t>(min((group << 5) >> a.block_shift, a.groups - 1)) * a.n);
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) {
-    ring[i] = {};
-    fetch(ring[i], warp + i * kFewWarps);
-  }
-  if constexpr (!FIRST) pdl_wait();
-  pdl_launch_dependents();
-  const uint2* row[NT];  // this lane's row of every eight: its input slices t, t + 4, ...
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    row[nt] = nullptr;
-    if (8 * nt + g < tile.rows) {
-      const int at = tile.row0 + 8 * nt + g;
-      if constexpr (FIRST) {
-        const int token = a.ids != nullptr ? 0 : a.b.order[at] / a.top_k;
-        row[nt] = reinterpret_cast<const uint2*>(a.x + token * a.x_stride) + t;
-      } else {
-        row[nt] = reinterpret_cast<const uint2*>(static_cast<const __half*>(a.b.hidden) + static_cast<int64_t>(at) * a.k) + t;
-      }
-    }
-  }
-  float acc[2][2][NT][4];  // [output slice of the pair][outputs 0, 1 / 2, 3][eight of rows]
-#pragma unroll
-  for (int i = 0; i < 2 * 2 * NT * 4; ++i) (&acc[0][0][0][0])[i] = 0.0f;
-  const __half2 zero = __float2half2_rn(BITS == 4 ? 1032.0f : 1152.0f);
-  for (int base = warp; base < groups; base += kAhead * kFewWarps) {
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int group = base + i * kFewWarps;
-      if (group < groups) {
-        uint2 xb[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) xb[nt][h] = row[nt] != nullptr ? row[nt][group * 8 + 4 * h] : make_uint2(0u, 0u);
-        const FewGroup<BITS> cur = ring[i];
-        fetch(ring[i], group + kAhead * kFewWarps);
-        const __half2* const s2 = reinterpret_cast<const __half2*>(&cur.s);
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float sum[NT][4];
-#pragma unroll
-            for (int i4 = 0; i4 < NT * 4; ++i4) (&sum[0][0])[i4] = 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              uint32_t a0, a1, a2, a3;
-              if constexpr (BITS == 4) {
-                const uint32_t lo = b == 0 ? cur.w[h].x : cur.w[h].z, hi = b == 0 ? cur.w[h].y : cur.w[h].w;
-                a0 = less(((lo >> (8 * r)) & 0x000F000Fu) | 0x64006400u, zero);
-                a1 = less(((lo >> (8 * r + 4)) & 0x000F000Fu) | 0x64006400u, zero);
-                a2 = less(((hi >> (8 * r)) & 0x000F000Fu) | 0x64006400u, zero);
-                a3 = less(((hi >> (8 * r + 4)) & 0x000F000Fu) | 0x64006400u, zero);
-              } else {
-                // a word per input channel, a byte per output
-                const uint4 v = cur.w[2 * h + b];
-                a0 = less((__byte_perm(v.x, v.y, 0x0400u + (2 * r) * 0x0101u) & 0x00FF00FFu) | 0x64006400u, zero);
-                a1 = less((__byte_perm(v.x, v.y, 0x0400u + (2 * r + 1) * 0x0101u) & 0x00FF00FFu) | 0x64006400u, zero);
-                a2 = less((__byte_perm(v.z, v.w, 0x0400u + (2 * r) * 0x0101u) & 0x00FF00FFu) | 0x64006400u, zero);
-                a3 = less((__byte_perm(v.z, v.w, 0x0400u + (2 * r + 1) * 0x0101u) & 0x00FF00FFu) | 0x64006400u, zero);
-              }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) mma_f16(sum[nt], a0, a1, a2, a3, xb[nt][h].x, xb[nt][h].y);
-            }
-            const float2 s = __half22float2(s2[2 * b + r]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              acc[b][r][nt][0] += sum[nt][0] * s.x;
-              acc[b][r][nt][1] += sum[nt][1] * s.x;
-              acc[b][r][nt][2] += sum[nt][2] * s.y;
-              acc[b][r][nt][3] += sum[nt][3] * s.y;
-            }
-          }
-      }
-    }
-  }
-  // the warps' sums meet in shared memory
-#pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int r = 0; r < 2; ++r)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-          *reinterpret_cast<float2*>(&red[(warp * kCols + 8 * nt + 2 * t + c) * kPitch + 8 * g + 4 * b + 2 * r]) =
-              make_float2(acc[b][r][nt][c], acc[b][r][nt][2 + c]);
-  __syncthreads();
-  for (int i = threadIdx.x; i < kCols * (kFewOutputs / 2); i += kFewWarps * 32) {
-    const int col = i / (kFewOutputs / 2), pair = i % (kFewOutputs / 2);
-    if (col >= tile.rows || n0 + 2 * pair >= a.n) continue;
-    float2 v = make_float2(0.0f, 0.0f);
-#pragma unroll
-    for (int w = 0; w < kFewWarps; ++w) {
-      const float2 p = *reinterpret_cast<const float2*>(&red[(w * kCols + col) * kPitch + 2 * pair]);
-      v.x += p.x;
-      v.y += p.y;
-    }
-    const int64_t at = tile.row0 + col;
-    if constexpr (FIRST)
-      static_cast<__half*>(a.b.hidden)[at * (a.n >> 1) + (n0 >> 1) + pair] = __float2half_rn(moe_gated(v.x, v.y, a.activation));
-    else
-      *reinterpret_cast<float2*>(static_cast<float*>(a.b.part) + at * a.n + n0 + 2 * pair) = v;
-  }
-}
-
 // ------------------------------------------------------------------------------------------------- weighted sum
 struct SumArgs {
   MoeBuffers b;
-  const int32_t* ids;  // one token: as FewArgs
+  const int32_t* ids;  // one token: its experts, no order was made
   const float* weights;
   const __half* residual;
   __half* out;
@@ -327,11 +141,7 @@ __global__ void __launch_bounds__(256) moe_sum_kernel(SumArgs a) {
 #pragma unroll 4
     for (int j = 0; j < a.top_k; ++j) {
       const int pair = token * a.top_k + j;
-      int at;
-      if (a.ids != nullptr)
-        at = static_cast<unsigned>(a.ids[j]) < static_cast<unsigned>(a.experts) ? j : -1;
-      else
-        at = a.b.position[pair];
+      const int at = a.ids == nullptr ? a.b.position[pair] : static_cast<unsigned>(a.ids[j]) < static_cast<unsigned>(a.experts) ? j : -1;
       if (at < 0) continue;
       const float w = a.weights[pair];
       const P* p = static_cast<const P*>(a.b.part) + static_cast<int64_t>(at) * a.width + c;
@@ -375,38 +185,6 @@ int launch_sort(const int32_t* ids, int pairs, int experts, int tile_rows, bool 
   return MLD_OK;
 }
 
-template <int BITS, int NT, bool FIRST>
-int launch_few_of(const FewArgs& a, int tiles, cudaStream_t stream) {
-  constexpr size_t smem = static_cast<size_t>(kFewWarps) * 8 * NT * (kFewOutputs + 4) * sizeof(float);
-  auto kern = moe_few_kernel<BITS, NT, FIRST>;
-  static bool done[kMaxDevices];
-  int dev;
-  if (needs_configure(done, &dev)) {
-    MLD_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
-    if (dev >= 0) done[dev] = true;
-  }
-  MLD_CUDA_CHECK(launch_overlapped(kern, dim3(div_up(a.n, kFewOutputs), tiles < 32768 ? tiles : 32768, div_up(tiles, 32768)),
-                                   dim3(kFewWarps * 32), smem, stream, a));
-  MLD_LAUNCH_CHECK();
-  return MLD_OK;
-}
-template <bool FIRST>
-int launch_few(const FewArgs& a, int bits, int eights, int tiles, cudaStream_t stream) {
-  if (bits == 4)
-    return eights == 1   ? launch_few_of<4, 1, FIRST>(a, tiles, stream)
-           : eights == 2 ? launch_few_of<4, 2, FIRST>(a, tiles, stream)
-                         : launch_few_of<4, 4, FIRST>(a, tiles, stream);
-  return eights == 1   ? launch_few_of<8, 1, FIRST>(a, tiles, stream)
-         : eights == 2 ? launch_few_of<8, 2, FIRST>(a, tiles, stream)
-                       : launch_few_of<8, 4, FIRST>(a, tiles, stream);
-}
-
-int log2_of(int v) {
-  int s = 0;
-  while ((1 << s) < v) ++s;
-  return s;
-}
-
 }  // namespace
 }  // namespace mld
 
@@ -422,8 +200,8 @@ struct mld_moe_plan {
 
 namespace {
 
-// With many rows, tiles of up to 256 (two SMs) or 128; with few, of 8 to 32: enough for a usual expert's share.
-int few_eights(int pairs, int experts) { return pairs <= 6 * experts ? 1 : pairs <= 12 * experts ? 2 : 4; }
+// With many rows, tiles of up to 256 (two SMs) or 128; with few, of 8 or 16: enough for a usual expert's share.
+int few_eights(int pairs, int experts) { return pairs <= 6 * experts ? 1 : 2; }
 int most_tiles(int pairs, int experts, int rows) { return pairs < experts + pairs / rows ? pairs : experts + pairs / rows; }
 
 bool takes_many(const mld_moe_desc& d, int tokens) {
@@ -465,14 +243,14 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
     at += (bytes + 255) / 256 * 256;
     return here;
   };
-  const size_t error = room(256), order = room(pairs * 4), position = room(pairs * 4),
+  const size_t control = room(kControlBytes), order = room(pairs * 4), position = room(pairs * 4),
                tiles = room(most_tiles(static_cast<int>(pairs), d->experts, 8) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2),
                part = room(pairs * d->d_model * 4), sorted = room(pairs * d->d_model * 2);
   int before = -1;
   cudaError_t e = cudaGetDevice(&before);
   if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
   if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&p->memory), at);
-  if (e == cudaSuccess) e = zero_now(p->memory, 256);
+  if (e == cudaSuccess) e = zero_now(p->memory, kControlBytes);
   if (before >= 0 && before != device) cudaSetDevice(before);
   if (e != cudaSuccess) {
     set_last_error("experts' workspace", e);
@@ -481,8 +259,8 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
     return MLD_CUDA_ERROR;
   }
   p->bytes = at;
-  p->b.error = reinterpret_cast<int*>(p->memory + error);
-  p->b.n_tiles = reinterpret_cast<int*>(p->memory + error) + 1;
+  p->b.error = reinterpret_cast<int*>(p->memory + control);
+  p->b.n_tiles = p->b.error + 1;
   p->b.order = reinterpret_cast<int*>(p->memory + order);
   p->b.position = reinterpret_cast<int*>(p->memory + position);
   p->b.tiles = reinterpret_cast<MoeTile*>(p->memory + tiles);
@@ -509,7 +287,7 @@ int mld_moe_plan_device_status(mld_moe_plan* plan, int32_t* code) {
   if (before != plan->device) MLD_CUDA_CHECK(cudaSetDevice(plan->device));
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpy(&c, plan->b.error, sizeof c, cudaMemcpyDeviceToHost);
-  if (e == cudaSuccess && c != 0) e = zero_now(plan->b.error, sizeof c);
+  if (e == cudaSuccess && c != 0) e = zero_now(plan->memory, kControlBytes);
   if (before != plan->device) cudaSetDevice(before);
   MLD_CUDA_CHECK(e);
   *code = c != 0 ? MLD_TIMEOUT : 0;
@@ -581,29 +359,9 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
     if (rc != MLD_OK) return rc;
     tiles = most_tiles(pairs, d.experts, 8 * eights);
   }
-  FewArgs f = {};
-  f.b = plan->b;
-  f.ids = one ? io->ids : nullptr;
-  f.x = static_cast<const __half*>(io->x);
-  f.x_stride = io->x_stride;
-  f.experts = d.experts;
-  f.top_k = d.top_k;
-  f.activation = d.activation;
-  const auto matrix = [&](const void* w, const void* s, int n, int k) {
-    f.weights = static_cast<const uint8_t*>(w);
-    f.scale = static_cast<const __half*>(s);
-    f.n = n;
-    f.k = k;
-    f.groups = d.block != 0 ? k / d.block : 1;
-    f.block_shift = d.block != 0 ? log2_of(d.block) : 30;
-    f.expert_bytes = static_cast<int64_t>(n) * k * d.weight_bits / 8;
-    f.expert_scales = static_cast<int64_t>(f.groups) * n;
-  };
-  matrix(io->gate_up, io->gate_up_scale, 2 * d.ffn, d.d_model);
-  rc = launch_few<true>(f, d.weight_bits, eights, tiles, stream);
-  if (rc != MLD_OK) return rc;
-  matrix(io->down, io->down_scale, d.d_model, d.ffn);
-  rc = launch_few<false>(f, d.weight_bits, eights, tiles, stream);
+  rc = launch_moe_few(true, shape, plan->b, s.ids, io->x, io->x_stride, io->gate_up, io->gate_up_scale, eights, tiles, plan->sms, stream);
+  if (rc == MLD_OK)
+    rc = launch_moe_few(false, shape, plan->b, s.ids, nullptr, 0, io->down, io->down_scale, eights, tiles, plan->sms, stream);
   if (rc != MLD_OK) return rc;
   MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<float>, dim3(tokens), dim3(256), 0, stream, s));
   MLD_LAUNCH_CHECK();

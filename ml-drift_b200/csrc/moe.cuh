@@ -1,5 +1,7 @@
 // What the kernels of the experts' networks share.
 #pragma once
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -37,5 +39,10 @@ __device__ __forceinline__ float moe_gated(float gate, float up, int activation)
 // The products of tiles of rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16).
 int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs,
                     int tile_rows, int sms, cudaStream_t stream);
+
+// The products of tiles of 8 or 16 rows, bound by the weights.  first: x (rows by token) -> hidden; else hidden -> part (fp32).
+// ids: one token's experts, without an order, or null; tiles: how many there may be.
+int launch_moe_few(bool first, const MoeShape& s, const MoeBuffers& b, const int32_t* ids, const void* x, int64_t x_stride,
+                   const void* weights, const void* scale, int eights, int tiles, int sms, cudaStream_t stream);
 
 }  // namespace mld
