@@ -16,6 +16,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortCtas = 8;            // of a cluster, where one block would take long
 constexpr int kSortAlone = 8192;        // pairs that one block sorts
 constexpr int kMaxExperts = 1024;
+constexpr int kTileSizes = 7;           // of tiles, in steps of 64 rows
 constexpr size_t kControlBytes = 256;   // of a plan's memory: the error, numbers of tiles and rows
 
 // ------------------------------------------------------------------------------------------------ order by experts
@@ -28,9 +29,11 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* _
   pdl_launch_dependents();
   __shared__ int count[kMaxExperts], next[kMaxExperts];
   __shared__ int sums[2][32];
+  __shared__ int of_size[kTileSizes];  // tiles by size, the largest first
   const int me = threadIdx.x, lane = me & 31, warp = me >> 5;
   const int ctas = static_cast<int>(gridDim.x), rank = static_cast<int>(blockIdx.x);  // (one cluster)
   count[me] = 0;
+  if (me < kTileSizes) of_size[me] = 0;
   __syncthreads();
   const int per = (pairs + ctas - 1) / ctas, from = min(pairs, rank * per), to = min(pairs, from + per);
   for (int p = from + me; p < to; p += kSortThreads) {
@@ -74,13 +77,30 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* _
     row0 += sums[0][w];
     tile0 += sums[1][w];
   }
+  const int all_tiles = tile0 + tiles;  // (the last expert's)
   next[me] = row0 + before;
+  // (even: an expert's tiles alike, in steps of 64 rows, since a tile costs its dequantised weights, however few its rows; and
+  // large tiles first, so that what is left for the end is small)
+  const int rows = even && tiles > 0 ? ((all + tiles - 1) / tiles + 63) / 64 * 64 : tile_rows;
+  const int size = kTileSizes - 1 - min(kTileSizes - 1, rows / 64);
+  if (even && rank == 0) {
+    if (tiles > 0) atomicAdd(&of_size[size], tiles);
+    __syncthreads();
+    if (me == 0) {
+      int at = 0;
+      for (int i = 0; i < kTileSizes; ++i) {
+        const int n = of_size[i];
+        of_size[i] = at;
+        at += n;
+      }
+    }
+    __syncthreads();
+    if (tiles > 0) tile0 = atomicAdd(&of_size[size], tiles);
+  }
   if (rank == 0) {
-    // (even: an expert's tiles alike, in steps of 64 rows: one costs its dequantised weights, however few its rows)
-    const int rows = even && tiles > 0 ? ((all + tiles - 1) / tiles + 63) / 64 * 64 : tile_rows;
     for (int i = 0; i < tiles; ++i) b.tiles[tile0 + i] = {me, row0 + i * rows, min(rows, all - i * rows), 0};
     if (me == kSortThreads - 1) {
-      b.n_tiles[0] = tile0 + tiles;
+      b.n_tiles[0] = all_tiles;
       b.n_tiles[1] = row0 + all;
     }
   }
@@ -200,7 +220,7 @@ struct mld_moe_plan {
 
 namespace {
 
-// With many rows, tiles of up to 256 (two SMs) or 128; with few, of 8 or 16: enough for a usual expert's share.
+// With few rows, tiles of 8 or 16: enough for a usual expert's share.
 int few_eights(int pairs, int experts) { return pairs <= 6 * experts ? 1 : 2; }
 int most_tiles(int pairs, int experts, int rows) { return pairs < experts + pairs / rows ? pairs : experts + pairs / rows; }
 
@@ -340,14 +360,14 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
   s.top_k = d.top_k;
   s.width = d.d_model;
   if (many) {
-    const int rows = pairs > 64 * d.experts ? 256 : 128;
+    const int rows = kMoeTileRows;
     rc = launch_sort(io->ids, pairs, d.experts, rows, true, plan->b, stream);
     if (rc != MLD_OK) return rc;
     MLD_CUDA_CHECK(launch_overlapped(moe_gather_kernel, dim3(div_up(pairs, 8)), dim3(256), 0, stream, static_cast<const __half*>(io->x),
                                      io->x_stride, d.top_k, d.d_model, plan->b));
     MLD_LAUNCH_CHECK();
-    rc = launch_moe_gemm(true, shape, plan->b, io->gate_up, io->gate_up_scale, pairs, rows, plan->sms, stream);
-    if (rc == MLD_OK) rc = launch_moe_gemm(false, shape, plan->b, io->down, io->down_scale, pairs, rows, plan->sms, stream);
+    rc = launch_moe_gemm(true, shape, plan->b, io->gate_up, io->gate_up_scale, pairs, plan->sms, stream);
+    if (rc == MLD_OK) rc = launch_moe_gemm(false, shape, plan->b, io->down, io->down_scale, pairs, plan->sms, stream);
     if (rc != MLD_OK) return rc;
     MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<__half>, dim3(tokens), dim3(256), 0, stream, s));
     MLD_LAUNCH_CHECK();

@@ -32,13 +32,16 @@ struct MoeShape {
 // act(gate) * up
 __device__ __forceinline__ float moe_gated(float gate, float up, int activation) {
   const float u = activation == MLD_MOE_SILU ? gate : 1.5957691216057308f * (gate + 0.044715f * gate * gate * gate);
-  return gate / (1.0f + __expf(-u)) * up;  // (GELU's (1 + tanh(u / 2)) / 2 is 1 / (1 + exp(-u)))
+  // (GELU's (1 + tanh(u / 2)) / 2 is 1 / (1 + exp(-u)).  A quotient good to 2 ulp: the exact one took the products' results longer
+  // than their sums, and what is rounded to fp16 next does not show the difference.)
+  return __fdividef(gate, 1.0f + __expf(-u)) * up;
 }
 #endif
 
-// The products of tiles of rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16).
-int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs,
-                    int tile_rows, int sms, cudaStream_t stream);
+// The products of tiles of up to kMoeTileRows rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16).
+constexpr int kMoeTileRows = 384;
+int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs, int sms,
+                    cudaStream_t stream);
 
 // The products of tiles of 8 or 16 rows, bound by the weights.  first: x (rows by token) -> hidden; else hidden -> part (fp32).
 // ids: one token's experts, without an order, or null; tiles: how many there may be.

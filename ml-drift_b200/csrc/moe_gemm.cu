@@ -2,17 +2,19 @@
 //
 // The form is gemm_wtmem_kernel's (Y^T = W X^T, tcgen05 cta_group::2, weights as the A operand in tensor memory, rows as the B
 // operand in shared memory), with what a grouped product needs in place of what a single one does:
-//   - a tile is 256 outputs of one expert x up to kTok of its rows; which expert and which rows stands in a list that the
+//   - a tile is 256 outputs of one expert x up to 384 of its rows; which expert and which rows stands in a list that the
 //     ordering kernel left in device memory.  Every role reads the list for itself and goes through the same tiles.
 //   - rows of an expert follow one another, so a tile's rows are one box after another of 32; as many are fetched as the tile has
-//     rows, and the MMA's N is that many, too (in steps of 64).  Columns behind the tile's rows belong to other experts, or are
-//     zeros, and are not written.
+//     rows, and the MMAs' N is that many, too (in steps of 64; beyond 256 in two MMAs of the same weights).  Columns behind the
+//     tile's rows belong to other experts, or are zeros, and are not written.
 //   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
 //     and an up channel, exchange half of their tokens; of the second the expert's output.
 // Per CTA: warp 0 fetches rows, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first CTA), warps 6..21 dequantise
-// (four to a stage of 64 inputs), warps 2..5 write the results; with tiles of up to 256 rows the sixteen help them, since all
-// 256 columns are one tile's, with up to 128 there are two sets of accumulators and the next tile goes on meanwhile.
-// Bound by the tensor cores for tiles of 256 rows, by the dequantisation (four instructions for two weights) for smaller ones.
+// (four to a stage of 64 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights and two halves of 192 columns
+// of accumulators.  A tile of up to 192 rows takes the half that is free, and the next tile goes on while it is written; a larger
+// one takes both, so the sixteen help writing.
+// A stage's weights take about 550 cycles to dequantise, whatever the rows, its MMAs 2 per row: an expert's rows go in as few tiles
+// as hold them, all alike.  (With tiles of 256 rows, 8 stages of weights and 375 rows to an expert: XXX.)
 // Every wait is bounded.
 #include <cuda_fp16.h>
 
@@ -26,13 +28,15 @@
 namespace mld {
 namespace {
 
-constexpr int kStages = 8;              // rows in shared memory + weights in tensor memory
+constexpr int kStages = 4;              // rows in shared memory + weights in tensor memory
 constexpr int kWStages = 8;             // packed weights
 constexpr int kChannels = 128;          // outputs per CTA
 constexpr int kBoxRows = 32;
 constexpr int kBoxBytes = kBoxRows * kKBytes;
 constexpr int kSlices = 16;             // packed rows of a stage: 64 inputs
-constexpr uint32_t kRingCol = 256;      // first tensor-memory column of the weights
+constexpr int kHalf = 192;               // columns of one of two halves of accumulators
+constexpr int kColumns = 2 * kHalf;      // the weights' follow
+static_assert(kColumns == kMoeTileRows, "a tile's rows");
 constexpr int kThreads = 23 * 32;
 constexpr int kReaders = 5;             // warps that can read a lane quarter's accumulators
 constexpr int kErrMoeBase = 70;
@@ -66,6 +70,30 @@ struct Work {
   __device__ __forceinline__ bool done() const { return t >= total; }
 };
 __device__ __forceinline__ int columns_of(const MoeTile& t) { return (t.rows + 63) & ~63; }
+
+// Which accumulators a tile has, and which barriers: worked out alike by every role that goes through the tiles.
+struct Turns {
+  uint32_t half = 0;              // the next small tile's
+  uint32_t uses = 0;              // of each half so far, odd or even, a bit each
+  uint32_t read = 0;              // tiles so far, odd or even: read by the writing warps alone in each half (bits 0, 1), by all (bit 2)
+  uint32_t at = 0;                // the tile's half (its first, of a large one)
+  bool large = false, all = false;
+  __device__ __forceinline__ void take(const MoeTile& t, bool last) {
+    large = t.rows > kHalf;
+    all = large || last;
+    at = large ? 0 : half;
+  }
+  // barrier of the finished MMAs: [0], [1] of halves that the writing warps read alone, [2] of what all read.  (A wait tells one use
+  // of a barrier from the one before and no more, so nobody may miss a use of one that it waits on.)
+  __device__ __forceinline__ uint32_t full() const { return all ? 2 : at; }
+  __device__ __forceinline__ uint32_t full_phase() const { return read >> full() & 1u; }
+  __device__ __forceinline__ uint32_t uses_of(uint32_t h) const { return uses >> h & 1u; }
+  __device__ __forceinline__ void next() {
+    read ^= 1u << full();
+    uses ^= large ? 3u : 1u << at;
+    half ^= large ? 0u : 1u;
+  }
+};
 
 // x0..x3: a lane's four pairs of tokens -> pair q of the tokens of four lanes' channels.  A: lane bits that number the four.
 template <int LOW>
@@ -102,14 +130,13 @@ __device__ __forceinline__ void store_pair(__half* first, int64_t pitch, bool on
   if (two) *reinterpret_cast<uint2*>(first + pitch) = make_uint2(__byte_perm(x0, x1, 0x7632), __byte_perm(x2, x3, 0x7632));
 }
 
-template <int BITS, bool FIRST, int TOK>
+template <int BITS, bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, GemmArgs a) {
   constexpr int kBlk = BITS == 4 ? 8 : 16;
   constexpr int kPitch = kChannels / 4 * kBlk;        // bytes of a packed row of the box
   constexpr int kWBytes = kSlices * kPitch;
-  constexpr int kSets = 256 / TOK;                    // sets of accumulators
-  constexpr int kXBytes = TOK / 2 * kKBytes;          // a CTA's rows of a stage
+  constexpr int kXBytes = kColumns / 2 * kKBytes;     // a CTA's rows of a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
@@ -118,8 +145,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* w_empty = full_w + kWStages;       // the dequantising warps have read the box
   uint64_t* full_ab = w_empty + kWStages;      // first CTA: rows and weights of both CTAs are there
   uint64_t* empty = full_ab + kStages;         // the stage's MMAs are done (arrives in both CTAs)
-  uint64_t* tmem_full = empty + kStages;       // [3]: sets that the writing warp reads alone, then those that all read
-  uint64_t* tmem_empty = tmem_full + 3;        // [2], first CTA
+  uint64_t* tmem_full = empty + kStages;       // [3], see Turns
+  uint64_t* tmem_empty = tmem_full + 3;        // [2], first CTA: a half has been read (by a quarter's five warps, or by one for all)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tmem_empty + 2);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -146,7 +173,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 3; ++b) mbar_init(&tmem_full[b], 1);
-    for (int b = 0; b < 2; ++b) mbar_init(&tmem_empty[b], kSets == 1 ? 2 * 4 * kReaders : 2 * 4);
+    for (int b = 0; b < 2; ++b) mbar_init(&tmem_empty[b], 2 * 4 * kReaders);
     fence_barrier_init();
   }
   if (warp == 1) tmem_alloc_all<true>(tmem_slot);
@@ -156,12 +183,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   tc_after();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t full_ab_lead = map_shared(smem_u32(full_ab), 0), tmem_empty_lead = map_shared(smem_u32(tmem_empty), 0);
-  // With one set of accumulators all warps of a quarter read it; with two the last tile's only.
-  const auto read_by_all = [&](bool last) { return kSets == 1 || last; };
 
-  const auto drain = [&](const MoeTile& tile, int n0, int part, int parts, int set) {
+  const auto drain = [&](const MoeTile& tile, int n0, int part, const Turns& turn) {
+    const int parts = turn.all ? kReaders : 1;
     const int quad = warp & 3;
-    const uint32_t base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(set * TOK);
+    const uint32_t base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(turn.at * kHalf);
     const int n = n0 + static_cast<int>(rank) * kChannels + quad * 32;  // the warp's first channel
     const bool has_n = n < a.n;                                         // (a.n is a multiple of 32)
     const int pieces = (tile.rows + 15) >> 4;
@@ -209,7 +235,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     }
     tc_before();
     __syncwarp();
-    if (lane == 0 && (kSets == 1 || part == 0)) arrive_in_pair(tmem_empty_lead + set * 8);
+    if (lane == 0) {
+      arrive_in_pair(tmem_empty_lead + turn.at * 8, kReaders / parts);
+      if (turn.large) arrive_in_pair(tmem_empty_lead + 8, kReaders / parts);
+    }
   };
 
   if (warp == 0) {
@@ -223,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     MoeTile tile;
     int n0;
     while (ok && work.next(tile, n0)) {
-      const int cols = columns_of(tile), row = tile.row0 + static_cast<int>(rank) * (cols >> 1);
+      const int cols = columns_of(tile), low = min(cols, 256);  // (of the first MMA; a CTA has half of each one's rows)
       for (int kb = 0; kb < a.k_blocks; ++kb) {
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1))) {
           if (lane == 0) atomicExch(a.error, kErrMoeBase + 1);
@@ -232,8 +261,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full_ab[stage], static_cast<uint32_t>(cols) * kKBytes);
-          for (int i = 0; i < cols >> 6; ++i)
-            tma_load_2d_pair(sX + stage * kXBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row + i * kBoxRows);
+          for (int i = 0; i < low >> 6; ++i)
+            tma_load_2d_pair(sX + stage * kXBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64,
+                             tile.row0 + static_cast<int>(rank) * (low >> 1) + i * kBoxRows);
+          if (cols > 256) {
+            for (int i = 0; i < (cols - low) >> 6; ++i)
+              tma_load_2d_pair(sX + stage * kXBytes + 128 * kKBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64,
+                               tile.row0 + 256 + static_cast<int>(rank) * ((cols - low) >> 1) + i * kBoxRows);
+          }
         }
         __syncwarp();
         if (++stage == kStages) {
@@ -251,12 +286,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       Work work = work0;
       MoeTile tile;
       int n0;
-      for (int nth = 0; ok && work.next(tile, n0); ++nth) {
-        const int set = kSets == 1 ? 0 : nth & 1;
-        const uint32_t set_phase = static_cast<uint32_t>(kSets == 1 ? nth : nth >> 1) & 1u;
-        const uint32_t idesc = 1u << 4 | static_cast<uint32_t>(columns_of(tile) >> 3) << 17 | 16u << 24;
-        const uint32_t d = tmem_base + static_cast<uint32_t>(set * TOK);
-        if (!__all_sync(0xffffffffu, mbar_wait(&tmem_empty[set], set_phase ^ 1))) {
+      for (Turns turn; ok && work.next(tile, n0); turn.next()) {
+        turn.take(tile, work.done());
+        const int cols = columns_of(tile), low = min(cols, 256);
+        const auto idesc_of = [](int n) { return 1u << 4 | static_cast<uint32_t>(n >> 3) << 17 | 16u << 24; };
+        const uint32_t idesc = idesc_of(low), idesc_high = idesc_of(cols - low);
+        const uint32_t d = tmem_base + static_cast<uint32_t>(turn.at * kHalf);
+        bool free = mbar_wait(&tmem_empty[turn.at], turn.uses_of(turn.at) ^ 1u);
+        if (turn.large) free = mbar_wait(&tmem_empty[1], turn.uses_of(1) ^ 1u) && free;
+        if (!__all_sync(0xffffffffu, free)) {
           if (lane == 0) atomicExch(a.error, kErrMoeBase + 2);
           break;
         }
@@ -269,11 +307,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
           tc_after();
           const uint64_t db = make_desc(smem_u32(sX + stage * kXBytes));
-          const uint32_t ta = tmem_base + kRingCol + static_cast<uint32_t>(stage * 32);
+          const uint32_t ta = tmem_base + kColumns + static_cast<uint32_t>(stage * 32);
           if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
               umma_ts<true, false>(d, ta + 8u * i, db + static_cast<uint64_t>((i * 32) >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
+              if (cols > 256)
+                umma_ts<true, false>(d + 256, ta + 8u * i, db + static_cast<uint64_t>((128 * kKBytes + i * 32) >> 4), idesc_high,
+                                     (kb > 0 || i > 0) ? 1u : 0u);
+            }
             commit<true>(&empty[stage]);
           }
           __syncwarp();
@@ -282,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             phase ^= 1;
           }
         }
-        if (ok && elect_one()) commit<true>(&tmem_full[read_by_all(work.done()) ? 2 : set]);
+        if (ok && elect_one()) commit<true>(&tmem_full[turn.full()]);
         __syncwarp();
       }
     }
@@ -291,17 +333,15 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     if constexpr (!FIRST) pdl_wait();  // (what is written here may still be read by launches ahead of the one ahead)
     Work work = work0;
     MoeTile tile;
-    int n0, together = 0;
-    for (int nth = 0; work.next(tile, n0); ++nth) {
-      const int set = kSets == 1 ? 0 : nth & 1;
-      const bool all = read_by_all(work.done());
-      const int use = all ? together++ : nth >> 1;
-      if (!mbar_wait(&tmem_full[all ? 2 : set], static_cast<uint32_t>(use) & 1u)) {
+    int n0;
+    for (Turns turn; work.next(tile, n0); turn.next()) {
+      turn.take(tile, work.done());
+      if (!mbar_wait(&tmem_full[turn.full()], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 4);
         break;
       }
       tc_after();
-      drain(tile, n0, 0, all ? kReaders : 1, set);
+      drain(tile, n0, 0, turn);
     }
   } else if (warp == 22) {
     // --------------------------------------------------------- packed weights
@@ -351,11 +391,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       if (lane == 0) arrive_in_pair(full_ab_lead + stored * 8);
       stored = -1;
     };
-    if constexpr (!FIRST && kSets == 1) pdl_wait();  // (it writes results, too)
+    if constexpr (!FIRST) pdl_wait();  // (it writes results, too)
     Work work = work0;
     MoeTile tile;
-    int n0, together = 0;
-    for (int nth = 0; ok && work.next(tile, n0); ++nth) {
+    int n0;
+    for (Turns turn; ok && work.next(tile, n0); turn.next()) {
+      turn.take(tile, work.done());
       const int n = n0 + static_cast<int>(rank) * kChannels + row;
       const bool has_n = n < a.n;
       const __half* const scale = a.scale + tile.expert * a.expert_scales + n;
@@ -385,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           break;
         }
         const uint8_t* wp = sW + ws * kWBytes + (row >> 2) * kBlk;
-        const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kRingCol + static_cast<uint32_t>(stage * 32);
+        const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kColumns + static_cast<uint32_t>(stage * 32);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           using Block = typename std::conditional<BITS == 4, uint2, uint4>::type;
@@ -424,14 +465,13 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       announce();
       before += a.k_blocks;
       if (!ok) break;
-      if (!read_by_all(work.done())) continue;
-      if constexpr (!FIRST && kSets == 2) pdl_wait();
-      if (!mbar_wait(&tmem_full[2], static_cast<uint32_t>(together++) & 1u)) {
+      if (!turn.all) continue;
+      if (!mbar_wait(&tmem_full[2], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 7);
         break;
       }
       tc_after();
-      drain(tile, n0, 1 + group, kReaders, kSets == 1 ? 0 : nth & 1);
+      drain(tile, n0, 1 + group, turn);
     }
   }
   // Nobody leaves while the partner may still arrive on this CTA's barriers or the pair's MMAs write its tensor memory.
@@ -449,12 +489,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   }
 }
 
-template <int BITS, bool FIRST, int TOK>
+template <int BITS, bool FIRST>
 int launch_of(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int grid, cudaStream_t stream) {
-  constexpr size_t smem = 1024 + kStages * (TOK / 2) * kKBytes + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
+  constexpr size_t smem = 1024 + kStages * (kColumns / 2) * kKBytes + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
                           (2 * kWStages + 2 * kStages + 5) * 8 + 64;
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kern = moe_gemm_kernel<BITS, FIRST, TOK>;
+  auto kern = moe_gemm_kernel<BITS, FIRST>;
   static bool done[kMaxDevices];
   int dev;
   if (needs_configure(done, &dev)) {
@@ -468,8 +508,8 @@ int launch_of(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, i
 
 }  // namespace
 
-int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs,
-                    int tile_rows, int sms, cudaStream_t stream) {
+int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs, int sms,
+                    cudaStream_t stream) {
   const int n = first ? 2 * s.ffn : s.d_model, k = first ? s.d_model : s.ffn, blk = s.bits == 4 ? 8 : 16;
   CUtensorMap tx, tw;
   int rc = make_tmap_2d(&tx, first ? b.sorted : b.hidden, static_cast<uint64_t>(k) * 2, pairs, static_cast<uint64_t>(k) * 2, kKBytes,
@@ -495,11 +535,8 @@ int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const vo
   a.activation = s.activation;
   a.error = b.error;
   const int grid = sms / 2 * 2;
-#define MLD_MOE_GEMM(BITS, FIRST) \
-  (tile_rows > 128 ? launch_of<BITS, FIRST, 256>(tx, tw, a, grid, stream) : launch_of<BITS, FIRST, 128>(tx, tw, a, grid, stream))
-  if (s.bits == 4) return first ? MLD_MOE_GEMM(4, true) : MLD_MOE_GEMM(4, false);
-  return first ? MLD_MOE_GEMM(8, true) : MLD_MOE_GEMM(8, false);
-#undef MLD_MOE_GEMM
+  if (s.bits == 4) return first ? launch_of<4, true>(tx, tw, a, grid, stream) : launch_of<4, false>(tx, tw, a, grid, stream);
+  return first ? launch_of<8, true>(tx, tw, a, grid, stream) : launch_of<8, false>(tx, tw, a, grid, stream);
 }
 
 }  // namespace mld
