@@ -382,15 +382,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     const __half2 offset = __float2half2_rn(BITS == 4 ? 1032.0f : 1152.0f);
     bool ok = true;
     int before = 0;  // stages before the tile
-    int stored = -1;
-    const auto announce = [&]() {
-      if (stored < 0) return;
-      tmem_st_wait();
-      tc_before();
-      __syncwarp();
-      if (lane == 0) arrive_in_pair(full_ab_lead + stored * 8);
-      stored = -1;
-    };
     if constexpr (!FIRST) pdl_wait();  // (it writes results, too)
     Work work = work0;
     MoeTile tile;
@@ -427,42 +418,41 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         }
         const uint8_t* wp = sW + ws * kWBytes + (row >> 2) * kBlk;
         const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kColumns + static_cast<uint32_t>(stage * 32);
+        using Block = typename std::conditional<BITS == 4, uint2, uint4>::type;
+        uint32_t o[32];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          using Block = typename std::conditional<BITS == 4, uint2, uint4>::type;
           Block blk[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (8 * half + i) * kPitch);
-          if (half == 0) {
-            announce();
-            if (!mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u)) {
-              atomicExch(a.error, kErrMoeBase + 6);
-              ok = false;
-              break;
-            }
-            tc_after();
-          }
-          uint32_t o[16];
           const __half2 s2 = __half2half2(__ushort_as_half(half == 0 ? cur0 : cur1));
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const Block v = blk[i];
             if constexpr (BITS == 4) {
-              o[2 * i] = dq_once(((v.x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
-              o[2 * i + 1] = dq_once(((v.y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+              o[16 * half + 2 * i] = dq_once(((v.x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+              o[16 * half + 2 * i + 1] = dq_once(((v.y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
             } else {
-              o[2 * i] = dq_once((__byte_perm(v.x, v.y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
-              o[2 * i + 1] = dq_once((__byte_perm(v.z, v.w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+              o[16 * half + 2 * i] = dq_once((__byte_perm(v.x, v.y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+              o[16 * half + 2 * i + 1] = dq_once((__byte_perm(v.z, v.w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
             }
           }
-          tmem_st16(columns + static_cast<uint32_t>(16 * half), o);
         }
-        if (!ok) break;
         __syncwarp();
         if (lane == 0) mbar_arrive(&w_empty[ws]);
-        stored = stage;
+        // (the weights are ready in registers when the stage's last MMAs are done with its columns)
+        if (!mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u)) {
+          atomicExch(a.error, kErrMoeBase + 6);
+          ok = false;
+          break;
+        }
+        tc_after();
+        tmem_st32(columns, o);
+        tmem_st_wait();
+        tc_before();
+        __syncwarp();
+        if (lane == 0) arrive_in_pair(full_ab_lead + stage * 8);
       }
-      announce();
       before += a.k_blocks;
       if (!ok) break;
       if (!turn.all) continue;

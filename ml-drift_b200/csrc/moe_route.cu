@@ -1,10 +1,10 @@
 // Routing of tokens to experts: scores, a bias for balance, groups, the k best, their weights.
 //
-// A warp takes a token, a lane every 32nd expert.  Values (score + bias) become integers that are ordered as they are, so that the
-// largest of a warp's is two reductions of 32 bits and the lowest number among equals one more.  Without a bias and with groups
-// that go by one expert the order is that of the logits, whatever the score: nothing is computed but the chosen ones' scores
-// (and, without renormalising, the softmax's sum).  With them values are compared in 64 bits: in 32 some token of a long prompt
-// has two within a rounding of one another.
+// A warp takes a token, a lane a run of neighbouring experts.  Without a bias and with groups that go by one expert the order is that
+// of the logits, whatever the score: nothing is computed but the chosen ones' scores (and, without renormalising, the softmax's
+// sum).  Else experts are compared by values in 32 bits first; where two that the choice hangs on lie closer to one another
+// than the error of those (some token of a long prompt always has such), the token is gone through again in 64.
+// Bound by instructions: k rounds of the largest of each lane's, the warp's largest (one instruction), its lane and place.
 #include <cuda_fp16.h>
 
 #include <cfloat>
@@ -25,156 +25,258 @@ struct RouteArgs {
   int32_t* ids;
   float* weights;
   int tokens, experts, top_k, sigmoid, groups, per_group, top_groups, group_best, renormalise, f16;
+  int wide;  // rows may be read in pieces
   float factor;
 };
 
-// Numbers in the order of the values; every value that is one (not NaN) has a number above 0.
-__device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t u = __float_as_uint(v);
-  return u ^ ((u >> 31) != 0 ? 0xffffffffu : 0x80000000u);
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ uint64_t ordered(double v) {
-  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v));
-  return u ^ ((u >> 63) != 0 ? ~0ull : 1ull << 63);
+__device__ __forceinline__ float warp_min(float v) {
+  float r;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
 }
-__device__ __forceinline__ uint32_t warp_max(uint32_t k) { return __reduce_max_sync(kAll, k); }
-__device__ __forceinline__ uint64_t warp_max(uint64_t k) {
-  const uint32_t hi = static_cast<uint32_t>(k >> 32), top = warp_max(hi);
-  const uint32_t lo = warp_max(hi == top ? static_cast<uint32_t>(k) : 0u);
-  return static_cast<uint64_t>(top) << 32 | lo;
+__device__ __forceinline__ double warp_max(double v) {
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, off));
+  return v;
 }
-__device__ __forceinline__ double value_of(uint64_t key) {
-  return __longlong_as_double(static_cast<long long>(key ^ ((key >> 63) != 0 ? 1ull << 63 : ~0ull)));
+__device__ __forceinline__ double warp_min(double v) { return -warp_max(-v); }
+
+// The k best of keys (-infinity: not to be had), into lane j the j-th: its expert (-1: none) and its logit.  Of equal keys (64 bits)
+// the larger logit, then the lower number.  False: something that the choice hangs on is closer than `tolerance` (0: never).
+template <typename Key, int N>
+__device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const float (&x)[N], int lane, float tolerance, int& id,
+                                       float& logit) {
+  constexpr bool kWide = sizeof(Key) == 8;
+  constexpr Key kNone = static_cast<Key>(-INFINITY);
+  bool clear = true;
+  const auto close = [&](Key upper, Key lower, float tol) {  // (an infinite value is close to nothing but its like)
+    return !(upper - lower > static_cast<Key>(tol) * (1 + (upper < 0 ? -upper : upper)));
+  };
+  if (a.top_groups < a.groups) {
+    const auto better = [](Key p, Key q) { return p > q ? p : q; };
+    const auto worse = [](Key p, Key q) { return p < q ? p : q; };
+    const int run = a.per_group / N;  // lanes of a group, if it is whole lanes
+    const bool whole = a.per_group % N == 0 && (run & (run - 1)) == 0;
+    Key sum = kNone;      // of this lane's group (whole), or of group `lane`
+    int group = lane;
+    if (whole) {
+      Key first = kNone, second = kNone;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        second = better(second, worse(first, key[i]));
+        first = better(first, key[i]);
+      }
+      for (int off = 1; off < run; off <<= 1) {
+        const Key f = __shfl_xor_sync(kAll, first, off), s = __shfl_xor_sync(kAll, second, off);
+        second = better(better(second, s), worse(first, f));
+        first = better(first, f);
+      }
+      sum = a.group_best == 2 ? first + second : first;
+      group = lane / run;
+    } else {
+      for (int g = 0; g < a.groups; ++g) {
+        const int from = g * a.per_group - lane * N, to = from + a.per_group;
+        Key first = kNone, second = kNone;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const Key k = i >= from && i < to ? key[i] : kNone;
+          second = better(second, worse(first, k));
+          first = better(first, k);
+        }
+        const Key best = warp_max(first);
+        Key s = best;
+        if (a.group_best == 2) {
+          // the largest once out of the way, of the first lane that has it
+          const int holder = __ffs(__ballot_sync(kAll, first == best)) - 1;
+          s += warp_max(lane == holder ? second : first);
+        }
+        if (lane == g) sum = s;
+      }
+    }
+    if (!(sum > kNone)) sum = kNone;  // (a NaN, too)
+    int ahead = 0;  // groups before this one in the order
+    for (int g = 0; g < a.groups; ++g) {
+      const Key s = __shfl_sync(kAll, sum, whole ? g * run : g);
+      ahead += s > sum || (s == sum && g < group) ? 1 : 0;
+    }
+    const bool exists = group < a.groups, kept = exists && ahead < a.top_groups;
+    if (tolerance > 0) {
+      const Key least = warp_min(kept ? sum : static_cast<Key>(INFINITY)), most = warp_max(exists && !kept ? sum : kNone);
+      clear = clear && !(most > kNone && close(least, most, 2 * tolerance));
+    }
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (!kept) key[i] = kNone;
+    } else {
+      const uint32_t mask = __ballot_sync(kAll, kept);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int e = lane * N + i;
+        if (e >= a.experts || (mask >> (e / a.per_group) & 1u) == 0) key[i] = kNone;
+      }
+    }
+  }
+  Key before = static_cast<Key>(INFINITY);
+  for (int j = 0; j < a.top_k + (tolerance > 0 ? 1 : 0); ++j) {
+    Key best = key[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) best = key[i] > best ? key[i] : best;
+    const Key top = warp_max(best);
+    if (!(top > kNone)) break;  // none left
+    if (tolerance > 0) {
+      if (j > 0 && close(before, top, tolerance)) clear = false;
+      before = top;
+      if (j == a.top_k) break;
+    }
+    // the lane's first place with it; of equal values, the one with the larger logit
+    int place = -1;
+    float its = -INFINITY;
+#pragma unroll
+    for (int i = N - 1; i >= 0; --i)
+      if (key[i] == top && (!kWide || x[i] >= its)) {
+        place = i;
+        its = x[i];
+      }
+    bool here = place >= 0;
+    if constexpr (kWide) {
+      const float most = warp_max(its);
+      here = here && its == most;
+    }
+    const int holder = __ffs(__ballot_sync(kAll, here)) - 1;
+    const int e = __shfl_sync(kAll, lane * N + place, holder);
+    const float l = __shfl_sync(kAll, its, holder);
+    if (lane == j) {
+      id = e;
+      logit = l;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane == holder && i == place) key[i] = kNone;
+  }
+  return clear;
 }
 
-// VALUES: the order goes by values in 64 bits, else by logits.  N: experts of a lane.
+// The same by values in 64 bits.
+template <int N>
+__device__ __noinline__ void choose_in_64(const RouteArgs& a, const float* logits, float top, int lane, int& id, float& logit) {
+  float x[N];
+  double v[N], sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    x[i] = logits[i];
+    v[i] = 0.0;
+    if (x[i] > -INFINITY) {
+      v[i] = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x[i]))) : exp(static_cast<double>(x[i]) - static_cast<double>(top));
+      sum += v[i];
+    }
+  }
+  if (!a.sigmoid) {
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (!a.sigmoid) v[i] /= sum;
+    if (a.bias != nullptr && lane * N + i < a.experts) v[i] += static_cast<double>(a.bias[lane * N + i]);
+    if (!(x[i] > -INFINITY && v[i] > -INFINITY)) v[i] = -INFINITY;
+  }
+  id = -1;
+  logit = -INFINITY;
+  choose<double, N>(a, v, x, lane, 0.0f, id, logit);
+}
+
+// VALUES: the order goes by values, else by logits.  N: experts of a lane.
 template <bool VALUES, int N>
 __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a) {
-  using Key = typename std::conditional<VALUES, uint64_t, uint32_t>::type;
   pdl_wait();
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, token = static_cast<int>(blockIdx.x) * kRouteWarps + (threadIdx.x >> 5);
   if (token >= a.tokens) return;
   float x[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int e = 32 * i + lane;
-    x[i] = -INFINITY;
-    if (e < a.experts) {
-      const int64_t at = token * a.stride + e;
-      x[i] = a.f16 ? __half2float(static_cast<const __half*>(a.logits)[at]) : static_cast<const float*>(a.logits)[at];
-      x[i] = x[i] == x[i] ? fminf(x[i], FLT_MAX) + 0.0f : -INFINITY;  // (+ 0: -0 is ordered as 0)
-    }
-  }
-  float top = -INFINITY;  // the largest logit
-#pragma unroll
-  for (int i = 0; i < N; ++i) top = fmaxf(top, x[i]);
   {
-    const uint32_t k = warp_max(ordered(top));
-    top = __uint_as_float(k ^ ((k >> 31) != 0 ? 0x80000000u : 0xffffffffu));
+    const int64_t at = token * a.stride + lane * N;
+    if (a.wide) {  // (whole lanes, 16-byte pieces of 32-bit logits, 2 N bytes of halves)
+      if (lane * N < a.experts) {
+        if (a.f16) {
+          __half h[N];
+          constexpr int kPiece = N * 2 < 16 ? N * 2 : 16;
+#pragma unroll
+          for (int i = 0; i < N * 2 / kPiece; ++i) {
+            const __half* p = static_cast<const __half*>(a.logits) + at + i * (kPiece / 2);
+            if constexpr (kPiece == 16)
+              reinterpret_cast<uint4*>(h)[i] = *reinterpret_cast<const uint4*>(p);
+            else if constexpr (kPiece == 8)
+              reinterpret_cast<uint2*>(h)[i] = *reinterpret_cast<const uint2*>(p);
+            else
+              reinterpret_cast<uint32_t*>(h)[i] = *reinterpret_cast<const uint32_t*>(p);
+          }
+#pragma unroll
+          for (int i = 0; i < N; ++i) x[i] = __half2float(h[i]);
+        } else {
+          constexpr int kPiece = N < 4 ? N : 4;
+#pragma unroll
+          for (int i = 0; i < N / kPiece; ++i) {
+            const float* p = static_cast<const float*>(a.logits) + at + i * kPiece;
+            if constexpr (kPiece == 4)
+              reinterpret_cast<float4*>(x)[i] = *reinterpret_cast<const float4*>(p);
+            else
+              reinterpret_cast<float2*>(x)[i] = *reinterpret_cast<const float2*>(p);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (lane * N + i < a.experts)
+          x[i] = a.f16 ? __half2float(static_cast<const __half*>(a.logits)[at + i]) : static_cast<const float*>(a.logits)[at + i];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)  // (+ 0: -0 is 0)
+      x[i] = lane * N + i < a.experts && x[i] == x[i] ? fminf(x[i], FLT_MAX) + 0.0f : -INFINITY;
   }
-  // keys: 0 for an expert that is not to be had
-  Key key[N];
+  float top = x[0];  // the largest logit
+#pragma unroll
+  for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  top = warp_max(top);
+  int id = -1;
+  float chosen = -INFINITY;  // lane j: the logit of the j-th
   if constexpr (VALUES) {
-    double v[N], sum = 0.0;
+    float v[N], sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      v[i] = 0.0;
-      if (x[i] > -INFINITY) {
-        v[i] = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x[i]))) : exp(static_cast<double>(x[i]) - static_cast<double>(top));
-        sum += v[i];
-      }
+      v[i] = x[i] > -INFINITY ? (a.sigmoid ? 1.0f / (1.0f + expf(-x[i])) : expf(x[i] - top)) : 0.0f;
+      sum += v[i];
     }
     if (!a.sigmoid) {
 #pragma unroll
       for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(kAll, sum, off);
+      sum = 1.0f / sum;
     }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      if (!a.sigmoid) v[i] /= sum;
-      if (a.bias != nullptr && 32 * i + lane < a.experts) v[i] += static_cast<double>(a.bias[32 * i + lane]);
-      key[i] = x[i] > -INFINITY && v[i] > -INFINITY ? ordered(v[i]) : 0;
+      if (!a.sigmoid) v[i] *= sum;
+      if (a.bias != nullptr && lane * N + i < a.experts) v[i] += a.bias[lane * N + i];
+      if (!(x[i] > -INFINITY && v[i] > -INFINITY)) v[i] = -INFINITY;
     }
+    // Errors of two values: 2^-24 times 6 each of a sigmoid's score (exp 2, a sum, a quotient, the bias); N + 5 more of a softmax's
+    // sum, which has 37 at most.
+    const float tolerance = a.sigmoid ? 1.0e-6f : 6.0e-6f;
+    if (!choose<float, N>(a, v, x, lane, tolerance, id, chosen)) choose_in_64<N>(a, x, top, lane, id, chosen);
   } else {
+    float v[N];
 #pragma unroll
-    for (int i = 0; i < N; ++i) key[i] = x[i] > -INFINITY ? ordered(x[i]) : 0;
-  }
-  if (a.groups > 1 && a.top_groups < a.groups) {
-    // lane g gets the key of group g
-    Key mine = 0;
-    for (int g = 0; g < a.groups; ++g) {
-      const int from = g * a.per_group, to = from + a.per_group;
-      Key first = 0, second = 0;  // of this lane's experts in the group
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int e = 32 * i + lane;
-        const Key k = e >= from && e < to ? key[i] : 0;
-        second = k > first ? first : k > second ? k : second;
-        first = k > first ? k : first;
-      }
-      Key best = warp_max(first);
-      if constexpr (VALUES) {
-        if (a.group_best == 2) {
-          // the largest once out of the way, of the one lane that holds it
-          const int holder = __ffs(__ballot_sync(kAll, first == best)) - 1;
-          const Key next = warp_max(lane == holder ? second : first);
-          const double s = (best == 0 ? -INFINITY : value_of(best)) + (next == 0 ? -INFINITY : value_of(next));
-          best = s > -INFINITY ? ordered(s) : 0;
-        }
-      }
-      if (lane == g) mine = best;
-    }
-    uint32_t kept = 0;
-    for (int n = 0; n < a.top_groups; ++n) {
-      const bool open = lane < a.groups && (kept >> lane & 1u) == 0;
-      const Key best = warp_max(open ? mine : static_cast<Key>(0));
-      kept |= 1u << (__ffs(__ballot_sync(kAll, open && mine == best)) - 1);
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int e = 32 * i + lane;
-      if (e >= a.experts || (kept >> (e / a.per_group) & 1u) == 0) key[i] = 0;
-    }
-  }
-  // the k best: each time the largest of the lanes' largest, which its lane then gives up
-  float chosen = -INFINITY;  // lane j: the logit of the j-th
-  int id = -1;
-  for (int j = 0; j < a.top_k; ++j) {
-    Key best = 0;
-    float best_x = -INFINITY;
-    int best_e = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const bool more = VALUES ? key[i] > best || (key[i] == best && x[i] > best_x) : key[i] > best;
-      if (more) {
-        best = key[i];
-        best_x = x[i];
-        best_e = 32 * i + lane;
-      }
-    }
-    const Key top_key = warp_max(best);
-    if (top_key == 0) break;  // none left
-    bool here = best == top_key;
-    if constexpr (VALUES) {
-      const uint32_t k = here ? ordered(best_x) : 0u, top_x = warp_max(k);
-      here = here && k == top_x;
-    }
-    const int e = static_cast<int>(__reduce_min_sync(kAll, here ? static_cast<uint32_t>(best_e) : 0xffffffffu));
-    const float its_x = __shfl_sync(kAll, best_x, e & 31);
-    if (lane == j) {
-      id = e;
-      chosen = its_x;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (32 * i + lane == e) key[i] = 0;
+    for (int i = 0; i < N; ++i) v[i] = x[i];
+    choose<float, N>(a, v, x, lane, 0.0f, id, chosen);
   }
   // Their weights.  Renormalised, a softmax's sum cancels, and what is common to the chosen, too: they are taken against the largest
   // of them (of a sigmoid when all are so small that it is the exponential), so that they never vanish together.
-  const float chosen_top = [&] {
-    const uint32_t k = warp_max(id >= 0 ? ordered(chosen) : 0u);
-    return __uint_as_float(k ^ ((k >> 31) != 0 ? 0x80000000u : 0xffffffffu));
-  }();
+  const float chosen_top = warp_max(chosen);
   float score = 0.0f, by = 1.0f;
   if (id >= 0) {
     if (a.sigmoid && !(a.renormalise && chosen_top < -30.0f))
@@ -198,17 +300,22 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a
   }
 }
 
+template <bool VALUES, int N>
+int launch_of(RouteArgs a, cudaStream_t stream) {
+  const int piece = a.f16 ? (N * 2 < 16 ? N * 2 : 16) : (N < 4 ? N * 4 : 16);
+  a.wide = a.experts % N == 0 && reinterpret_cast<uintptr_t>(a.logits) % piece == 0 && (a.tokens == 1 || a.stride * (a.f16 ? 2 : 4) % piece == 0);
+  MLD_CUDA_CHECK(launch_overlapped(moe_route_kernel<VALUES, N>, dim3(div_up(a.tokens, kRouteWarps)), dim3(kRouteWarps * 32), 0, stream, a));
+  MLD_LAUNCH_CHECK();
+  return MLD_OK;
+}
 template <bool VALUES>
 int launch(const RouteArgs& a, cudaStream_t stream) {
   const int n = div_up(a.experts, 32);
-  void (*kern)(RouteArgs) = n <= 2    ? moe_route_kernel<VALUES, 2>
-                            : n <= 4  ? moe_route_kernel<VALUES, 4>
-                            : n <= 8  ? moe_route_kernel<VALUES, 8>
-                            : n <= 16 ? moe_route_kernel<VALUES, 16>
-                                      : moe_route_kernel<VALUES, 32>;
-  MLD_CUDA_CHECK(launch_overlapped(kern, dim3(div_up(a.tokens, kRouteWarps)), dim3(kRouteWarps * 32), 0, stream, a));
-  MLD_LAUNCH_CHECK();
-  return MLD_OK;
+  return n <= 2    ? launch_of<VALUES, 2>(a, stream)
+         : n <= 4  ? launch_of<VALUES, 4>(a, stream)
+         : n <= 8  ? launch_of<VALUES, 8>(a, stream)
+         : n <= 16 ? launch_of<VALUES, 16>(a, stream)
+                   : launch_of<VALUES, 32>(a, stream);
 }
 
 }  // namespace
