@@ -39,10 +39,13 @@ __device__ __forceinline__ float warp_min(float v) {
   asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
+// (as integers in the order of the values, the upper halves first)
 __device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = fmax(v, __shfl_xor_sync(kAll, v, off));
-  return v;
+  const uint64_t u = static_cast<uint64_t>(__double_as_longlong(v)), k = u ^ ((u >> 63) != 0 ? ~0ull : 1ull << 63);
+  const uint32_t hi = static_cast<uint32_t>(k >> 32), top = __reduce_max_sync(kAll, hi);
+  const uint32_t low = __reduce_max_sync(kAll, hi == top ? static_cast<uint32_t>(k) : 0u);
+  const uint64_t m = static_cast<uint64_t>(top) << 32 | low;
+  return __longlong_as_double(static_cast<long long>(m ^ ((m >> 63) != 0 ? 1ull << 63 : ~0ull)));
 }
 __device__ __forceinline__ double warp_min(double v) { return -warp_max(-v); }
 
@@ -124,10 +127,14 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
   }
   Key before = static_cast<Key>(INFINITY);
   for (int j = 0; j < a.top_k + (tolerance > 0 ? 1 : 0); ++j) {
-    Key best = key[0];
+    Key best[N];
 #pragma unroll
-    for (int i = 1; i < N; ++i) best = key[i] > best ? key[i] : best;
-    const Key top = warp_max(best);
+    for (int i = 0; i < N; ++i) best[i] = key[i];
+#pragma unroll
+    for (int s = N / 2; s > 0; s /= 2)
+#pragma unroll
+      for (int i = 0; i < s; ++i) best[i] = best[i + s] > best[i] ? best[i + s] : best[i];
+    const Key top = warp_max(best[0]);
     if (!(top > kNone)) break;  // none left
     if (tolerance > 0) {
       if (j > 0 && close(before, top, tolerance)) clear = false;
@@ -162,14 +169,22 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
   return clear;
 }
 
-// The same by values in 64 bits.
+// A logit as it counts: NaN as -infinity, +infinity as the largest number, -0 as 0.
+__device__ __forceinline__ float counted(float x) { return x == x ? fminf(x, FLT_MAX) + 0.0f : -INFINITY; }
+
+// The same by values in 64 bits, from the logits on (which then need not lie in memory for it while it is not needed).  The expert
+// in the upper half, the logit in the lower.
 template <int N>
-__device__ __noinline__ void choose_in_64(const RouteArgs& a, const float* logits, float top, int lane, int& id, float& logit) {
+__device__ __noinline__ uint64_t choose_in_64(RouteArgs a, int token, float top) {
+  const int lane = threadIdx.x & 31;
   float x[N];
   double v[N], sum = 0.0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    x[i] = logits[i];
+    const int64_t at = token * a.stride + lane * N + i;
+    x[i] = -INFINITY;
+    if (lane * N + i < a.experts)
+      x[i] = counted(a.f16 ? __half2float(static_cast<const __half*>(a.logits)[at]) : static_cast<const float*>(a.logits)[at]);
     v[i] = 0.0;
     if (x[i] > -INFINITY) {
       v[i] = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x[i]))) : exp(static_cast<double>(x[i]) - static_cast<double>(top));
@@ -186,9 +201,10 @@ __device__ __noinline__ void choose_in_64(const RouteArgs& a, const float* logit
     if (a.bias != nullptr && lane * N + i < a.experts) v[i] += static_cast<double>(a.bias[lane * N + i]);
     if (!(x[i] > -INFINITY && v[i] > -INFINITY)) v[i] = -INFINITY;
   }
-  id = -1;
-  logit = -INFINITY;
+  int id = -1;
+  float logit = -INFINITY;
   choose<double, N>(a, v, x, lane, 0.0f, id, logit);
+  return static_cast<uint64_t>(static_cast<uint32_t>(id)) << 32 | __float_as_uint(logit);
 }
 
 // VALUES: the order goes by values, else by logits.  N: experts of a lane.
@@ -237,8 +253,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a
           x[i] = a.f16 ? __half2float(static_cast<const __half*>(a.logits)[at + i]) : static_cast<const float*>(a.logits)[at + i];
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i)  // (+ 0: -0 is 0)
-      x[i] = lane * N + i < a.experts && x[i] == x[i] ? fminf(x[i], FLT_MAX) + 0.0f : -INFINITY;
+    for (int i = 0; i < N; ++i) x[i] = lane * N + i < a.experts ? counted(x[i]) : -INFINITY;
   }
   float top = x[0];  // the largest logit
 #pragma unroll
@@ -267,7 +282,11 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a
     // Errors of two values: 2^-24 times 6 each of a sigmoid's score (exp 2, a sum, a quotient, the bias); N + 5 more of a softmax's
     // sum, which has 37 at most.
     const float tolerance = a.sigmoid ? 1.0e-6f : 6.0e-6f;
-    if (!choose<float, N>(a, v, x, lane, tolerance, id, chosen)) choose_in_64<N>(a, x, top, lane, id, chosen);
+    if (!choose<float, N>(a, v, x, lane, tolerance, id, chosen)) {
+      const uint64_t again = choose_in_64<N>(a, token, top);
+      id = static_cast<int>(again >> 32);
+      chosen = __uint_as_float(static_cast<uint32_t>(again));
+    }
   } else {
     float v[N];
 #pragma unroll
