@@ -467,7 +467,7 @@ extern "C" int mld_add_rms_norm(const mld_add_norm_desc* d, const mld_add_norm_i
   MLD_REQUIRE(d->width >= 1 && d->width <= 16384, "width must be 1 to 16384");
   MLD_REQUIRE(d->eps >= 0.0f && d->eps < INFINITY && d->weight_offset > -INFINITY && d->weight_offset < INFINITY,
               "eps must be finite and not negative, weight_offset finite");
-  MLD_REQUIRE(tokens >= 0, "negative number of tokens");
+  MLD_REQUIRE(tokens >= 0 && tokens <= 1 << 30, "tokens must be 0 to 2^30");
   MLD_REQUIRE(io->out != nullptr || io->codes != nullptr, "neither out nor codes");
   MLD_REQUIRE((io->codes == nullptr) == (io->params == nullptr), "codes and params go together");
   MLD_REQUIRE(io->sum_out == nullptr || io->residual != nullptr, "sum_out needs a residual");

@@ -16,6 +16,7 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortCtas = 8;            // of a cluster, where one block would take long
 constexpr int kSortAlone = 8192;        // pairs that one block sorts
 constexpr int kMaxExperts = 1024;
+constexpr int kFewShare = 12;           // rows to an expert, on average, that the products for few rows are for
 constexpr int kTileSizes = 7;           // of tiles, in steps of 64 rows
 constexpr size_t kControlBytes = 256;   // of a plan's memory: the error, numbers of tiles and rows
 
@@ -220,13 +221,14 @@ struct mld_moe_plan {
 
 namespace {
 
-// With few rows, tiles of 8 or 16: enough for a usual expert's share.
-int few_eights(int pairs, int experts) { return pairs <= 6 * experts ? 1 : 2; }
 int most_tiles(int pairs, int experts, int rows) { return pairs < experts + pairs / rows ? pairs : experts + pairs / rows; }
 
 bool takes_many(const mld_moe_desc& d, int tokens) {
   if (d.force_path != MLD_MOE_PATH_AUTO) return d.force_path == MLD_MOE_PATH_MANY_ROWS;
-  return static_cast<int64_t>(tokens) * d.top_k >= 24ll * d.experts;
+  // By the rows of an expert, were all alike.  us, few / many, at 8, 12 and 16: 64 experts of 2048 x 1024 in 4 bits 102 / 130, 132 / 131,
+  // 158 / 131; 8 of 4096 x 4096 90 / 143, 116 / 144, 145 / 144, in 8 bits 107 / 142, 135 / 142, 170 / 143; 128 of 2048 x 768 144 / 178,
+  // 192 / 184, 234 / 185.
+  return static_cast<int64_t>(tokens) * d.top_k > kFewShare * static_cast<int64_t>(d.experts);
 }
 
 }  // namespace
@@ -256,7 +258,12 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   p->d = *d;
   p->device = device;
   p->sms = sm_count(device);
+  // The most pairs that either path may get.  The rows of x in order and the experts' outputs share their place: those are read by the
+  // first product, these written by the second.
   const size_t pairs = static_cast<size_t>(d->max_tokens) * d->top_k;
+  const bool may_many = takes_many(*d, d->max_tokens);
+  const size_t few = d->force_path == MLD_MOE_PATH_FEW_ROWS || !may_many ? pairs : d->force_path == MLD_MOE_PATH_AUTO ? kFewShare * static_cast<size_t>(d->experts) : 0;
+  const size_t width = static_cast<size_t>(d->d_model), shared = may_many && pairs * width * 2 > few * width * 4 ? pairs * width * 2 : few * width * 4;
   size_t at = 0;
   const auto room = [&](size_t bytes) {
     const size_t here = at;
@@ -264,8 +271,7 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
     return here;
   };
   const size_t control = room(kControlBytes), order = room(pairs * 4), position = room(pairs * 4),
-               tiles = room(most_tiles(static_cast<int>(pairs), d->experts, 8) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2),
-               part = room(pairs * d->d_model * 4), sorted = room(pairs * d->d_model * 2);
+               tiles = room(most_tiles(static_cast<int>(pairs), d->experts, kMoeFewRows) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2), rows = room(shared);
   int before = -1;
   cudaError_t e = cudaGetDevice(&before);
   if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
@@ -285,8 +291,7 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   p->b.position = reinterpret_cast<int*>(p->memory + position);
   p->b.tiles = reinterpret_cast<MoeTile*>(p->memory + tiles);
   p->b.hidden = p->memory + hidden;
-  p->b.part = p->memory + part;
-  p->b.sorted = p->memory + sorted;
+  p->b.part = p->b.sorted = p->memory + rows;
   *out = p;
   return MLD_OK;
 }
@@ -345,7 +350,6 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_v);
   const int pairs = tokens * d.top_k;
   const bool one = tokens == 1, many = takes_many(d, tokens);
-  const int eights = one ? 1 : few_eights(pairs, d.experts);
   int rc = MLD_OK;
   const MoeShape shape = {d.experts, d.top_k, d.d_model, d.ffn, d.weight_bits, d.block, d.activation};
   SumArgs s = {};
@@ -375,13 +379,13 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
   }
   int tiles = pairs;
   if (!one) {
-    rc = launch_sort(io->ids, pairs, d.experts, 8 * eights, false, plan->b, stream);
+    rc = launch_sort(io->ids, pairs, d.experts, kMoeFewRows, false, plan->b, stream);
     if (rc != MLD_OK) return rc;
-    tiles = most_tiles(pairs, d.experts, 8 * eights);
+    tiles = most_tiles(pairs, d.experts, kMoeFewRows);
   }
-  rc = launch_moe_few(true, shape, plan->b, s.ids, io->x, io->x_stride, io->gate_up, io->gate_up_scale, eights, tiles, plan->sms, stream);
+  rc = launch_moe_few(true, shape, plan->b, s.ids, io->x, io->x_stride, io->gate_up, io->gate_up_scale, tiles, plan->sms, stream);
   if (rc == MLD_OK)
-    rc = launch_moe_few(false, shape, plan->b, s.ids, nullptr, 0, io->down, io->down_scale, eights, tiles, plan->sms, stream);
+    rc = launch_moe_few(false, shape, plan->b, s.ids, nullptr, 0, io->down, io->down_scale, tiles, plan->sms, stream);
   if (rc != MLD_OK) return rc;
   MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<float>, dim3(tokens), dim3(256), 0, stream, s));
   MLD_LAUNCH_CHECK();

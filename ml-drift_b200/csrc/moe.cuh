@@ -20,7 +20,7 @@ struct MoeBuffers {
   int* n_tiles;
   void* hidden;      // fp16 [pairs][ffn], by position
   void* part;        // [pairs][d_model], by position: fp32 with few rows, fp16 with many
-  void* sorted;      // fp16 [pairs][d_model]: x by position (many rows)
+  void* sorted;      // fp16 [pairs][d_model]: x by position (many rows); in the place of `part`, which is written later
   int* error;
 };
 
@@ -43,9 +43,10 @@ constexpr int kMoeTileRows = 384;
 int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs, int sms,
                     cudaStream_t stream);
 
-// The products of tiles of 8 or 16 rows, bound by the weights.  first: x (rows by token) -> hidden; else hidden -> part (fp32).
+// The products of tiles of up to kMoeFewRows rows, bound by the weights.  first: x (rows by token) -> hidden; else hidden -> part (fp32).
 // ids: one token's experts, without an order, or null; tiles: how many there may be.
+constexpr int kMoeFewRows = 8;
 int launch_moe_few(bool first, const MoeShape& s, const MoeBuffers& b, const int32_t* ids, const void* x, int64_t x_stride,
-                   const void* weights, const void* scale, int eights, int tiles, int sms, cudaStream_t stream);
+                   const void* weights, const void* scale, int tiles, int sms, cudaStream_t stream);
 
 }  // namespace mld

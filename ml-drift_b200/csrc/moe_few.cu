@@ -1,4 +1,4 @@
-// The experts' products for few rows: weights streamed once past tiles of 8 or 16 rows.
+// The experts' products for few rows: weights streamed once past tiles of up to eight rows.
 //
 // Bound by HBM: a weight is read once for all rows of a tile, and there are too few of those to fill the tensor cores.  An item is 64
 // outputs of one tile over all inputs; a persistent block takes every grid-th item.
@@ -18,8 +18,8 @@
 //   and four warps that add up the warps' parts of an item, in the order of the inputs, and write act(gate) * up or the expert's
 //                output.
 // Columns behind a tile's rows hold whatever was there: no column sees another, and they are not written.
-// Each side waits for the other through barriers in shared memory, every wait bounded.  Parts have two places per warp (one
-// with 16 rows), so that multiplying goes on meanwhile.
+// Each side waits for the other through barriers in shared memory, every wait bounded.  Parts have two places per warp, so that
+// multiplying goes on meanwhile.
 #include <cuda_fp16.h>
 
 #include <cstring>
@@ -31,6 +31,7 @@ namespace mld {
 namespace {
 
 constexpr int kOutputs = 64;        // of an item
+constexpr int kRows = kMoeFewRows;  // of a tile at most: the columns of a fragment
 constexpr int kInputs = 128;        // of a box
 constexpr int kCopyWarps = 4;
 constexpr int kSumWarps = 4;
@@ -42,17 +43,17 @@ constexpr int kRoom = 226 * 1024;              // shared memory
 // The block's shape.  Places of the ring are a multiple of the multiplying warps, so that a place is always the same warp's, which
 // then waits for each of the place's boxes in turn.  (A wait tells a box from the one before it and no more: a warp that took
 // another one's place could take an old box for its own.)
-template <int BITS, int NT>
+template <int BITS>
 struct Shape {
   static constexpr int kWarps = 8;
   static constexpr int kThreads = 32 * (kCopyWarps + kWarps + kSumWarps);
   static constexpr int kWBytes = kBoxBytes * (BITS == 4 ? 1 : 2);
   static constexpr int kScaleBytes = 4 * kOutputs * 2;           // four rows at most
   static constexpr int kStage = kWBytes + kScaleBytes;
-  static constexpr int kPart = 8 * NT * 32;                      // float2s of a part
-  static constexpr int kPlaces = NT == 1 ? 2 : 1;                // for a warp's parts
+  static constexpr int kPart = 8 * 32;                           // float2s of a part
+  static constexpr int kPlaces = 2;                              // for a warp's parts
   static constexpr int kPartBytes = kWarps * kPlaces * kPart * 8;
-  static constexpr int kRowBytes = kItemBars * 8 * NT * 8;       // where the rows of the items under way are
+  static constexpr int kRowBytes = kItemBars * kRows * 8;        // where the rows of the items under way are
   static constexpr int kStages = (kRoom - 3 * 1024 - kPartBytes - kRowBytes) / kStage / kWarps * kWarps;
   static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + kPartBytes + kRowBytes + (2 * kStages + 2 * kItemBars + kWarps * kPlaces) * 8;
   static_assert(kStages >= kWarps && kStages % kCopyWarps == 0 && kSmem <= 227 * 1024, "shared memory");
@@ -126,19 +127,18 @@ __device__ __forceinline__ MoeTile tile_of(const FewArgs& a, int i) {
   return {v.x, v.y, v.z, 0};
 }
 
-// FIRST: x -> hidden, else hidden -> part.  NT: eights of rows.
-template <int BITS, int NT, bool FIRST>
-__global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
+// FIRST: x -> hidden, else hidden -> part.
+template <int BITS, bool FIRST>
+__global__ void __launch_bounds__(Shape<BITS>::kThreads, 1)
     moe_few_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_s, FewArgs a) {
-  using S = Shape<BITS, NT>;
+  using S = Shape<BITS>;
   constexpr int kWarps = S::kWarps, kStages = S::kStages, kPlaces = S::kPlaces, kPart = S::kPart;
-  constexpr int kHeld = NT == 1 ? 4 : 2;  // groups of 32 inputs whose rows are in registers
   extern __shared__ uint8_t smem_raw[];
   uint8_t* const ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* const scale_ring = ring + kStages * S::kWBytes;
   float2* const parts = reinterpret_cast<float2*>(scale_ring + kStages * S::kScaleBytes);  // [warp][place][kPart]
-  const uint4** const rows = reinterpret_cast<const uint4**>(parts + kWarps * kPlaces * kPart);  // [item % kItemBars][8 NT]
-  uint64_t* const full = reinterpret_cast<uint64_t*>(rows + kItemBars * 8 * NT);
+  const uint4** const rows = reinterpret_cast<const uint4**>(parts + kWarps * kPlaces * kPart);  // [item % kItemBars][kRows]
+  uint64_t* const full = reinterpret_cast<uint64_t*>(rows + kItemBars * kRows);
   uint64_t* const empty = full + kStages;
   uint64_t* const item_full = empty + kStages;          // [kItemBars]: all parts of an item are there
   uint64_t* const item_rows = item_full + kItemBars;    // [kItemBars]: it is known where an item's rows are
@@ -193,13 +193,13 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
       if (warp == 0) {
         next_token = token_of(next_tile);
         // (places behind the tile's rows get one that exists; a slot's last readers are a ring's boxes behind at most)
-        if (lane < 8 * NT) {
+        if (lane < kRows) {
           const __half* p;
           if constexpr (FIRST)
             p = a.x + (a.ids != nullptr ? 0 : (lane < tile.rows ? token / a.top_k : 0) * a.x_stride);
           else
             p = static_cast<const __half*>(a.b.hidden) + static_cast<int64_t>(token) * a.k;
-          rows[nth % kItemBars * (8 * NT) + lane] = reinterpret_cast<const uint4*>(p);
+          rows[nth % kItemBars * kRows + lane] = reinterpret_cast<const uint4*>(p);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_rows[nth % kItemBars]);
@@ -245,9 +245,9 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
     if constexpr (!FIRST) pdl_wait();
     for (; ok && items.there(); items.next(), ++nth) {
       if (first < boxes) {
-        float acc[2][2][NT][4];  // [block of the pair][outputs 0, 1 / 2, 3 of it][eight of rows]
+        float acc[2][2][4];  // [block of the pair][outputs 0, 1 / 2, 3 of it]
 #pragma unroll
-        for (int i = 0; i < 2 * 2 * NT * 4; ++i) (&acc[0][0][0][0])[i] = 0.0f;
+        for (int i = 0; i < 16; ++i) (&acc[0][0][0])[i] = 0.0f;
         if (!wait_asleep(&item_rows[nth % kItemBars], static_cast<uint32_t>(nth / kItemBars) & 1u)) {
           atomicExch(a.b.error, kErrFewBase + 5);
           break;
@@ -261,23 +261,14 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
           }
           const uint8_t* const box = ring + s * S::kWBytes;
           const uint8_t* const scale_box = scale_ring + s * S::kScaleBytes + (BITS == 4 ? 16 : 8) * g;
-          // input slices 2 t (.x, .y) and 2 t + 1 of this lane's rows, of all the box (or, with 16 rows, half of it)
-          uint4 held[kHeld][NT];
-          const auto ask = [&](int from) {
+          uint4 held[4];  // input slices 2 t (.x, .y) and 2 t + 1 of this lane's row, of the box's four groups of 32
+          const uint4* const row = rows[nth % kItemBars * kRows + g] + c * (kInputs / 8) + t;
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4* const p = rows[nth % kItemBars * (8 * NT) + 8 * nt + g] + c * (kInputs / 8) + t;
-#pragma unroll
-              for (int i = 0; i < kHeld; ++i)
-                held[i][nt] = c * kInputs + 32 * (from + i) < a.k ? p[4 * (from + i)] : make_uint4(0u, 0u, 0u, 0u);
-            }
-          };
-          ask(0);
+          for (int i = 0; i < 4; ++i) held[i] = c * kInputs + 32 * i < a.k ? row[4 * i] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             if (c * kInputs + 32 * i >= a.k) break;  // (what lies behind the last input is another expert's)
-            if (i > 0 && i % kHeld == 0) ask(i);
-            const uint4(&x)[NT] = held[i % kHeld];
+            const uint2 x0 = make_uint2(held[i].x, held[i].y), x1 = make_uint2(held[i].z, held[i].w);
             uint4 w[2][BITS == 4 ? 1 : 2];
             uint4 scales;
 #pragma unroll
@@ -296,17 +287,16 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
             const __half2* const s2 = reinterpret_cast<const __half2*>(&scales);
             constexpr uint32_t kOnes = 0x3C003C00u;
             constexpr float kZero = BITS == 4 ? -8.0f * 0x1p-24f : -128.0f * 0x1p-24f, kZeroOdd = BITS == 4 ? -8.0f * 0x1p-20f : kZero;
-            float start[NT][4];
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
+            float start[4];
+            {
               const float none[4] = {0.0f, 0.0f, 0.0f, 0.0f};
               float half[4], sum[4];
-              mma_f16(half, kOnes, kOnes, kOnes, kOnes, make_uint2(x[nt].x, x[nt].y), none);
-              mma_f16(sum, kOnes, kOnes, kOnes, kOnes, make_uint2(x[nt].z, x[nt].w), half);
-              start[nt][0] = kZero * sum[0];
-              start[nt][1] = kZero * sum[1];
-              start[nt][2] = kZeroOdd * sum[0];
-              start[nt][3] = kZeroOdd * sum[1];
+              mma_f16(half, kOnes, kOnes, kOnes, kOnes, x0, none);
+              mma_f16(sum, kOnes, kOnes, kOnes, kOnes, x1, half);
+              start[0] = kZero * sum[0];
+              start[1] = kZero * sum[1];
+              start[2] = kZeroOdd * sum[0];
+              start[3] = kZeroOdd * sum[1];
             }
 #pragma unroll
             for (int b = 0; b < 2; ++b)
@@ -331,16 +321,13 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
                   }
                 }
                 const float2 sc = __half22float2(s2[2 * b + r]);
-#pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                  float half[4], sum[4];
-                  mma_f16(half, m[0][0], m[0][1], m[0][2], m[0][3], make_uint2(x[nt].x, x[nt].y), start[nt]);
-                  mma_f16(sum, m[1][0], m[1][1], m[1][2], m[1][3], make_uint2(x[nt].z, x[nt].w), half);
-                  acc[b][r][nt][0] += sum[0] * sc.x;
-                  acc[b][r][nt][1] += sum[1] * sc.x;
-                  acc[b][r][nt][2] += sum[2] * sc.y;
-                  acc[b][r][nt][3] += sum[3] * sc.y;
-                }
+                float half[4], sum[4];
+                mma_f16(half, m[0][0], m[0][1], m[0][2], m[0][3], x0, start);
+                mma_f16(sum, m[1][0], m[1][1], m[1][2], m[1][3], x1, half);
+                acc[b][r][0] += sum[0] * sc.x;
+                acc[b][r][1] += sum[1] * sc.x;
+                acc[b][r][2] += sum[2] * sc.y;
+                acc[b][r][3] += sum[3] * sc.y;
               }
           }
           __syncwarp();
@@ -353,7 +340,7 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
         }
         if (!ok) break;
         first = c;
-        // the part: pairs of neighbouring outputs, for the lane's two rows of every eight
+        // the part: pairs of neighbouring outputs, for the lane's two rows
         const int place = mine % kPlaces;
         if (!wait_asleep(&part_free[me * kPlaces + place], (static_cast<uint32_t>(mine / kPlaces) & 1u) ^ 1u)) {
           atomicExch(a.b.error, kErrFewBase + 3);
@@ -366,9 +353,7 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) to[(((b * 2 + r) * NT + nt) * 2 + e) * 32] = make_float2(acc[b][r][nt][e], acc[b][r][nt][2 + e]);
+            for (int e = 0; e < 2; ++e) to[((b * 2 + r) * 2 + e) * 32] = make_float2(acc[b][r][e], acc[b][r][2 + e]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&item_full[nth % kItemBars]);
         ++mine;
@@ -414,9 +399,9 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
       odd ^= turned;
 #pragma unroll
       for (int i = 0; i < kShare; ++i) {
-        // float2 number `at` of a part: [block][outputs][eight][row of two][lane]
-        const int at = me + 32 * kSumWarps * i, l = at & 31, e = at >> 5 & 1, nt = (at >> 6) % NT, r = (at >> 6) / NT & 1, b = (at >> 6) / NT >> 1;
-        const int n = n0 + (BITS == 4 ? 8 * (l >> 2) + 4 * b : 4 * (l >> 2) + 32 * b) + 2 * r, col = 8 * nt + 2 * (l & 3) + e;
+        // float2 number `at` of a part: [block][outputs][row of two][lane]
+        const int at = me + 32 * kSumWarps * i, l = at & 31, e = at >> 5 & 1, r = at >> 6 & 1, b = at >> 7;
+        const int n = n0 + (BITS == 4 ? 8 * (l >> 2) + 4 * b : 4 * (l >> 2) + 32 * b) + 2 * r, col = 2 * (l & 3) + e;
         if (col >= tile.rows || n >= a.n) continue;
         const float x = v[i].x * 0x1p24f, y = v[i].y * (BITS == 4 ? 0x1p20f : 0x1p24f);
         const int64_t pos = tile.row0 + col;
@@ -439,10 +424,10 @@ __global__ void __launch_bounds__(Shape<BITS, NT>::kThreads, 1)
   }
 }
 
-template <int BITS, int NT, bool FIRST>
+template <int BITS, bool FIRST>
 int launch_of(const CUtensorMap& tw, const CUtensorMap& ts, const FewArgs& a, int grid, cudaStream_t stream) {
-  using S = Shape<BITS, NT>;
-  auto kern = moe_few_kernel<BITS, NT, FIRST>;
+  using S = Shape<BITS>;
+  auto kern = moe_few_kernel<BITS, FIRST>;
   static bool done[kMaxDevices];
   int dev;
   if (needs_configure(done, &dev)) {
@@ -457,7 +442,7 @@ int launch_of(const CUtensorMap& tw, const CUtensorMap& ts, const FewArgs& a, in
 }  // namespace
 
 int launch_moe_few(bool first, const MoeShape& s, const MoeBuffers& b, const int32_t* ids, const void* x, int64_t x_stride,
-                   const void* weights, const void* scale, int eights, int tiles, int sms, cudaStream_t stream) {
+                   const void* weights, const void* scale, int tiles, int sms, cudaStream_t stream) {
   const int n = first ? 2 * s.ffn : s.d_model, k = first ? s.d_model : s.ffn, blk = s.bits == 4 ? 8 : 16;
   FewArgs a = {};
   a.b = b;
@@ -484,11 +469,8 @@ int launch_moe_few(bool first, const MoeShape& s, const MoeBuffers& b, const int
   if (rc != MLD_OK) return rc;
   const int64_t items = static_cast<int64_t>(tiles) * a.n_items;
   const int grid = items < sms ? static_cast<int>(items) : sms;
-#define MLD_MOE_FEW(BITS, FIRST) \
-  (eights == 1 ? launch_of<BITS, 1, FIRST>(tw, ts, a, grid, stream) : launch_of<BITS, 2, FIRST>(tw, ts, a, grid, stream))
-  if (s.bits == 4) return first ? MLD_MOE_FEW(4, true) : MLD_MOE_FEW(4, false);
-  return first ? MLD_MOE_FEW(8, true) : MLD_MOE_FEW(8, false);
-#undef MLD_MOE_FEW
+  if (s.bits == 4) return first ? launch_of<4, true>(tw, ts, a, grid, stream) : launch_of<4, false>(tw, ts, a, grid, stream);
+  return first ? launch_of<8, true>(tw, ts, a, grid, stream) : launch_of<8, false>(tw, ts, a, grid, stream);
 }
 
 }  // namespace mld

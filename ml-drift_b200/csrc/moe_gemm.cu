@@ -13,8 +13,9 @@
 // (four to a stage of 64 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights and two halves of 192 columns
 // of accumulators.  A tile of up to 192 rows takes the half that is free, and the next tile goes on while it is written; a larger
 // one takes both, so the sixteen help writing.
-// A stage's weights take about 550 cycles to dequantise, whatever the rows, its MMAs 2 per row: an expert's rows go in as few tiles
-// as hold them, all alike.  (With tiles of 256 rows, 8 stages of weights and 375 rows to an expert: XXX.)
+// A stage's weights take about 600 cycles from box to operand, whatever the rows, its MMAs 2 per row: an expert's rows go in as few
+// tiles as hold them, all alike.  (Tiles of 256 rows, one set of accumulators and eight stages of weights: 2048 tokens 298 us against
+// 263, 1531 tokens 1077 against 1024.)
 // Every wait is bounded.
 #include <cuda_fp16.h>
 

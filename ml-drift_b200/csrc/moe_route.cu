@@ -354,7 +354,7 @@ extern "C" int mld_moe_route(const mld_moe_route_desc* d, const void* logits, in
   MLD_REQUIRE(d->group_best == 1 || (d->group_best == 2 && d->experts / d->groups >= 2),
               "group_best must be 1, or 2 with groups of two experts or more");
   MLD_REQUIRE(d->factor > -INFINITY && d->factor < INFINITY, "factor must be finite");
-  MLD_REQUIRE(tokens >= 0, "negative number of tokens");
+  MLD_REQUIRE(tokens >= 0 && tokens <= 1 << 30, "tokens must be 0 to 2^30");
   if (tokens == 0) return MLD_OK;
   MLD_REQUIRE(logits != nullptr && ids != nullptr && weights != nullptr, "null tensor");
   MLD_REQUIRE(stride >= 0, "negative stride");
