@@ -274,7 +274,8 @@ typedef struct mld_fc_desc {
                                 (common/kernels/fully_connected.cc:410-470) */
   int32_t has_batch_ids;     /* per-token weight selection of the mixture-of-
                                 experts builder
-                                (common/gpu_model_builder_moe_util.cc:200-270) */
+                                (common/gpu_model_builder_moe_util.cc:200-270);
+                                experts' networks: mld_moe_plan_create) */
   /* Tuning of the streaming decode kernel; 0 everywhere = the defaults. */
   int32_t exact_operands;    /* 1: dequantise to exact fp16 integers before the MMA.
                                 0: 4-bit weights without zero points and one token

@@ -291,7 +291,7 @@ int mld_fc_plan_create(const mld_fc_desc* d, mld_fc_plan** out) {
     return MLD_UNIMPLEMENTED;
   }
   if (d->has_batch_ids != 0) {
-    set_last_error_text("batch ids (per-token weights of the mixture-of-experts builder) are not implemented");
+    set_last_error_text("batch ids (per-token weights of the mixture-of-experts builder) are not implemented; mld_moe_plan_create serves experts' networks");
     return MLD_UNIMPLEMENTED;
   }
   MLD_REQUIRE(d->weight_bits == 4 || d->weight_bits == 8, "Unsupported WeightsDescription type.");

@@ -147,25 +147,26 @@ __global__ void __launch_bounds__(Shape<BITS>::kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int boxes = (a.k + kInputs - 1) / kInputs;      // of an item
   const int sharing = min(boxes, kWarps);               // warps that have a part of an item
-  if constexpr (FIRST) pdl_wait();
-  // (The second product's tiles, ids and weights were complete before the launch ahead let this one begin; its rows were not.)
-  pdl_launch_dependents();
   if (threadIdx.x == 0) {
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_s);
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+  }
+  for (int i = threadIdx.x; i < kItemBars; i += S::kThreads) {  // (one thread alone would take a microsecond)
+    mbar_init(&item_full[i], sharing);
+    mbar_init(&item_rows[i], 1);
+    if (i < kStages) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < kItemBars; ++i) {
-      mbar_init(&item_full[i], sharing);
-      mbar_init(&item_rows[i], 1);
-    }
-    for (int i = 0; i < kWarps * kPlaces; ++i) mbar_init(&part_free[i], kSumWarps);
+    if (i < kWarps * kPlaces) mbar_init(&part_free[i], kSumWarps);
     fence_barrier_init();
   }
-  const int count = a.ids != nullptr ? a.top_k : *a.b.n_tiles;
+  static_assert(kStages <= kItemBars && kWarps * kPlaces <= kItemBars, "barriers");
   __syncthreads();
+  if constexpr (FIRST) pdl_wait();
+  // (The second product's tiles, ids and weights were complete before the launch ahead let this one begin; its rows were not.)
+  pdl_launch_dependents();
+  const int count = a.ids != nullptr ? a.top_k : *a.b.n_tiles;
   Items items(count, a.n_items);
 
   if (warp < kCopyWarps) {

@@ -152,18 +152,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  // (the ordering kernel's list, and for the first product its rows, come from launches ahead; for the second the list is older
-  // than the launch ahead, which began only when it was complete)
-  if constexpr (FIRST) {
-    pdl_wait();
-  }
-  pdl_launch_dependents();
-  Work work0;
-  work0.n_channel_tiles = a.n_channel_tiles;
-  work0.t = static_cast<int>(blockIdx.x) / 2;
-  work0.step = static_cast<int>(gridDim.x) / 2;
-  work0.total = *a.n_tiles * a.n_channel_tiles;
-  work0.tiles = a.tiles;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kWStages; ++s) {
       mbar_init(&full_w[s], 1);
@@ -182,6 +170,18 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   __syncthreads();
   cluster_sync_all();
   tc_after();
+  // (the ordering kernel's list, and for the first product its rows, come from launches ahead; for the second the list is older
+  // than the launch ahead, which began only when it was complete)
+  if constexpr (FIRST) {
+    pdl_wait();
+  }
+  pdl_launch_dependents();
+  Work work0;
+  work0.n_channel_tiles = a.n_channel_tiles;
+  work0.t = static_cast<int>(blockIdx.x) / 2;
+  work0.step = static_cast<int>(gridDim.x) / 2;
+  work0.total = *a.n_tiles * a.n_channel_tiles;
+  work0.tiles = a.tiles;
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t full_ab_lead = map_shared(smem_u32(full_ab), 0), tmem_empty_lead = map_shared(smem_u32(tmem_empty), 0);
 

@@ -67,23 +67,34 @@ def gated(gate, up, gelu):
 
 
 def experts(x, ids, weights, first, second, residual, gelu):
-    """first [E][2 f][d] (gate, up alternating), second [E][d][f] dequantised.  (out, size): size bounds what roundings act on."""
+    """first [E][2 f][d] (gate, up alternating), second [E][d][f] dequantised.  (out, (carried, before)): what relative errors act on,
+    of the gated values and behind them, and of the weights and sums ahead of the gate (there the worst case, every error one way)."""
     x = x.astype(np.float64)
     out = np.zeros_like(x) if residual is None else residual.astype(np.float64)
-    size = np.abs(out)
+    carried, before = np.abs(out), np.zeros_like(x)
     for t in range(x.shape[0]):
         for j in range(ids.shape[1]):
             e = ids[t, j]
             if not 0 <= e < first.shape[0]:
                 continue
-            gu = first[e] @ x[t]
+            w, gu = abs(float(weights[t, j])), first[e] @ x[t]
             h = gated(gu[0::2], gu[1::2], gelu)
             out[t] += float(weights[t, j]) * (second[e] @ h)
-            # an error of every |product| before the gate, carried through, and of every one behind it
+            carried[t] += w * (np.abs(second[e]) @ np.abs(h))
+            # neither gate is steeper than 1.13
             reach = np.abs(first[e]) @ np.abs(x[t])
             reach = reach[0::2] * (1.13 * np.abs(gu[1::2])) + reach[1::2] * np.abs(gated(gu[0::2], 1.0, gelu))
-            size[t] += abs(float(weights[t, j])) * (np.abs(second[e]) @ (np.abs(h) + reach))
-    return out, size
+            before[t] += w * (np.abs(second[e]) @ reach)
+    return out, (carried, before)
+
+
+def experts_bound(want, size, many):
+    """fp16 roundings (2^-11 of the value): of the gated product and of the result; with many rows also of every weight, and of each
+    expert's output.  32-bit sums, exp and divisions are 2^-17 of what they act on at most (512 roundings of partial sums, halved).
+    Below 2^-14 fp16 is spaced 2^-24."""
+    carried, before = size
+    half, sums = 2.0 ** -11, 2.0 ** -17
+    return half * np.abs(want) + carried * ((3.1 if many else 1.1) * half + sums) + before * ((1.1 * half if many else 0.0) + sums) + 2.0 ** -16
 
 
 def pack(codes_, bits):

@@ -29,11 +29,7 @@ def _weights(e, d, f, bits, block):
     return host, dev
 
 
-def _bound(want, size, many):
-    """fp16 roundings (2^-11 of the value): of the gated product (act, up: `size` holds second |h|) and of the result; with many
-    rows of each weight (the rest of `size`) and of each expert's output; 32-bit sums, exp and divisions beside them are 2^-17
-    of size at most (512 roundings of partial sums).  Below 2^-14 fp16 is spaced 2^-24."""
-    return 2.0 ** -11 * np.abs(want) + size * ((3.1 if many else 1.1) * 2.0 ** -11 + 2.0 ** -17) + 2.0 ** -16
+_bound = ref.experts_bound
 
 
 def _run(mld, n, e, k, d, f, bits, block, gelu, path, ids, residual=True, seed=0):
@@ -161,3 +157,50 @@ def test_values_that_are_not_numbers_stay_with_their_token(mld):
         assert np.isnan(outs[1][7]).all() and np.isnan(outs[1][11]).all()
         rest = [t for t in range(n) if t not in (7, 11)]
         assert np.array_equal(outs[0][rest], outs[1][rest])
+
+
+@pytest.mark.parametrize("path", ["few", "many"])
+@pytest.mark.parametrize("n,e,k,d,f,bits,block", [(3, 1, 1, 16384, 32, 4, 32), (2, 2, 1, 32, 16384, 8, 0), (5, 1024, 32, 32, 32, 4, 32),
+                                                  (2500, 7, 4, 64, 32, 4, 0), (70, 300, 1, 32, 64, 8, 32)])
+def test_the_ends_of_the_ranges(mld, n, e, k, d, f, bits, block, path):
+    """Long rows, many inputs, many experts, more pairs than one block orders."""
+    rng = np.random.default_rng(n + e)
+    ids = _ids(rng, n, e, k, 1.0)
+    ids[n // 2::9] = -1
+    _run(mld, n, e, k, d, f, bits, block, False, mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS, ids)
+
+
+def test_the_path_changes_with_the_tokens_of_a_call(mld):
+    e, k, d, f, n = 4, 2, 128, 64, 60
+    rng = np.random.default_rng(4)
+    (first, second), (w1, s1, w2, s2) = _weights(e, d, f, 4, 32)
+    plan = mld.MoeExperts(e, k, d, f, max_tokens=n)
+    x = rng.standard_normal((n, d)).astype(np.float16)
+    ids, weights = _ids(rng, n, e, k).astype(np.int32), rng.random((n, k)).astype(np.float32)
+    for rows in (n, 1, 24, 25, 2, n, 0):  # 24 tokens are 48 pairs, the most that go the one way
+        out = torch.full((n, d), 3.0, dtype=torch.float16, device="cuda")
+        plan.run(_dev(x[:rows]), _dev(ids[:rows]), _dev(weights[:rows]), w1, s1, w2, s2, out[:rows])
+        got = out.cpu().numpy().astype(np.float64)
+        want, size = ref.experts(x[:rows], ids[:rows], weights[:rows], first, second, None, False)
+        assert (np.abs(got[:rows] - want) <= _bound(want, size, True)).all() and (got[rows:] == 3).all()
+    assert plan.device_status() == 0
+
+
+def test_two_plans_at_once_on_two_streams(mld):
+    e, k, d, f, n = 8, 2, 256, 128, 90
+    rng = np.random.default_rng(6)
+    (first, second), (w1, s1, w2, s2) = _weights(e, d, f, 4, 32)
+    x, ids, weights = rng.standard_normal((n, d)).astype(np.float16), _ids(rng, n, e, k).astype(np.int32), rng.random((n, k)).astype(np.float32)
+    xd, idd, wd = _dev(x), _dev(ids), _dev(weights)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    plans = [mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=p) for p in (mld.MOE_PATH_FEW_ROWS, mld.MOE_PATH_MANY_ROWS)]
+    outs = [torch.empty(20, n, d, dtype=torch.float16, device="cuda") for _ in range(2)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        for s, p, o in zip(streams, plans, outs):
+            p.run(xd, idd, wd, w1, s1, w2, s2, o[i], stream=s)
+    torch.cuda.synchronize()
+    want, size = ref.experts(x, ids, weights, first, second, None, False)
+    for p, o, many in zip(plans, outs, (False, True)):
+        assert p.device_status() == 0 and (o == o[0]).all()
+        assert (np.abs(o[0].cpu().numpy().astype(np.float64) - want) <= _bound(want, size, many)).all()
