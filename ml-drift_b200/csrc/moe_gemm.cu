@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     const int quad = warp & 3;
     const int row = quad * 32 + lane;   // output channel of the CTA's 128 = tensor-memory lane
     const int col4 = row & 3;
+    const uint32_t turn6 = (6u - 4u * static_cast<uint32_t>(col4)) & 31u;
     const uint32_t sel8 = static_cast<uint32_t>(col4) | static_cast<uint32_t>(4 + col4) << 8;
     const __half2 offset = __float2half2_rn(BITS == 4 ? 1032.0f : 1152.0f);
     bool ok = true;
@@ -426,16 +427,35 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           Block blk[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (8 * half + i) * kPitch);
-          const __half2 s2 = __half2half2(__ushort_as_half(half == 0 ? cur0 : cur1));
+          const __half s = __ushort_as_half(half == 0 ? cur0 : cur1);
+          const __half2 s2 = __half2half2(s);
+          if constexpr (BITS == 4) {
+            // A nibble at bits 6..9 is the subnormal half u 2^-18: u 2^-18 (2^18 s) - 8 s is (u - 8) s rounded once, in one
+            // instruction.  2^18 s has to be a half; else from 1024 + u, the zero off exactly first.
+            if (__all_sync(0xffffffffu, __habs(s) < __float2half_rn(0.249f))) {
+              const __half2 up = __hmul2(s2, __float2half2_rn(512.0f)), large = __hmul2(up, __float2half2_rn(512.0f));
+              const __half2 zero = __hmul2(s2, __float2half2_rn(-8.0f));
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const Block v = blk[i];
-            if constexpr (BITS == 4) {
-              o[16 * half + 2 * i] = dq_once(((v.x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
-              o[16 * half + 2 * i + 1] = dq_once(((v.y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t lo = __funnelshift_l(blk[i].x, blk[i].x, turn6) & 0x03C003C0u;
+                const uint32_t hi = __funnelshift_l(blk[i].y, blk[i].y, turn6) & 0x03C003C0u;
+                const __half2 r0 = __hfma2(*reinterpret_cast<const __half2*>(&lo), large, zero);
+                const __half2 r1 = __hfma2(*reinterpret_cast<const __half2*>(&hi), large, zero);
+                o[16 * half + 2 * i] = *reinterpret_cast<const uint32_t*>(&r0);
+                o[16 * half + 2 * i + 1] = *reinterpret_cast<const uint32_t*>(&r1);
+              }
             } else {
-              o[16 * half + 2 * i] = dq_once((__byte_perm(v.x, v.y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
-              o[16 * half + 2 * i + 1] = dq_once((__byte_perm(v.z, v.w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                o[16 * half + 2 * i] = dq_once(((blk[i].x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+                o[16 * half + 2 * i + 1] = dq_once(((blk[i].y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              o[16 * half + 2 * i] = dq_once((__byte_perm(blk[i].x, blk[i].y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+              o[16 * half + 2 * i + 1] = dq_once((__byte_perm(blk[i].z, blk[i].w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
             }
           }
         }
