@@ -9,7 +9,7 @@
 //     tile's rows belong to other experts, or are zeros, and are not written.
 //   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
 //     and an up channel, exchange half of their tokens; of the second the expert's output.
-// Per CTA: warp 0 fetches rows, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first CTA), warps 6..21 dequantise
+// Per CTA: warps 0 and 23 fetch rows, every other stage each (one alone takes 450 to 520 cycles to a stage), warp 22 packed weights, warp 1 issues the MMAs (of the pair's first CTA), warps 6..21 dequantise
 // (four to a stage of 64 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights and two halves of 192 columns
 // of accumulators.  A tile of up to 192 rows takes the half that is free, and the next tile goes on while it is written; a larger
 // one takes both, so the sixteen help writing.
@@ -38,7 +38,7 @@ constexpr int kSlices = 16;             // packed rows of a stage: 64 inputs
 constexpr int kHalf = 192;               // columns of one of two halves of accumulators
 constexpr int kColumns = 2 * kHalf;      // the weights' follow
 static_assert(kColumns == kMoeTileRows, "a tile's rows");
-constexpr int kThreads = 23 * 32;
+constexpr int kThreads = 24 * 32;
 constexpr int kReaders = 5;             // warps that can read a lane quarter's accumulators
 constexpr int kErrMoeBase = 70;
 
@@ -242,41 +242,37 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     }
   };
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 23) {
     // ------------------------------------------------------------------ rows
     if (lane == 0) prefetch_tmap(&tmap_x);
     if constexpr (!FIRST) pdl_wait();
-    int stage = 0;
-    uint32_t phase = 0;
+    const int mine = warp == 0 ? 0 : 1;  // every other stage
+    int before = 0;                      // stages before the tile
     bool ok = true;
     Work work = work0;
     MoeTile tile;
     int n0;
     while (ok && work.next(tile, n0)) {
       const int cols = columns_of(tile), low = min(cols, 256);  // (of the first MMA; a CTA has half of each one's rows)
-      for (int kb = 0; kb < a.k_blocks; ++kb) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], phase ^ 1))) {
+      const int row = tile.row0 + static_cast<int>(rank) * (low >> 1), row_high = tile.row0 + 256 + static_cast<int>(rank) * ((cols - low) >> 1);
+      for (int kb = (mine ^ before) & 1; kb < a.k_blocks; kb += 2) {
+        const int iter = before + kb, stage = iter % kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u))) {
           if (lane == 0) atomicExch(a.error, kErrMoeBase + 1);
           ok = false;
           break;
         }
         if (elect_one()) {
           if (rank == 0) mbar_arrive_expect_tx(&full_ab[stage], static_cast<uint32_t>(cols) * kKBytes);
+          uint8_t* const to = sX + stage * kXBytes;
           for (int i = 0; i < low >> 6; ++i)
-            tma_load_2d_pair(sX + stage * kXBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64,
-                             tile.row0 + static_cast<int>(rank) * (low >> 1) + i * kBoxRows);
-          if (cols > 256) {
-            for (int i = 0; i < (cols - low) >> 6; ++i)
-              tma_load_2d_pair(sX + stage * kXBytes + 128 * kKBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64,
-                               tile.row0 + 256 + static_cast<int>(rank) * ((cols - low) >> 1) + i * kBoxRows);
-          }
+            tma_load_2d_pair(to + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row + i * kBoxRows);
+          for (int i = 0; i < (cols - low) >> 6; ++i)
+            tma_load_2d_pair(to + 128 * kKBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row_high + i * kBoxRows);
         }
         __syncwarp();
-        if (++stage == kStages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
+      before += a.k_blocks;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------- MMAs
