@@ -16,8 +16,8 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortCtas = 8;            // of a cluster, where one block would take long
 constexpr int kSortAlone = 8192;        // pairs that one block sorts
 constexpr int kMaxExperts = 1024;
-constexpr int kFewShare = 12;           // rows to an expert, on average, that the products for few rows are for
-constexpr int kTileSizes = 7;           // of tiles, in steps of 64 rows
+constexpr int kFewShare = 8;            // rows to an expert, on average, that the products for few rows are for
+constexpr int kTileSizes = kMoeTileRows / 64 + 1;  // of tiles, in steps of 64 rows
 constexpr size_t kControlBytes = 256;   // of a plan's memory: the error, numbers of tiles and rows
 
 // ------------------------------------------------------------------------------------------------ order by experts
@@ -225,9 +225,9 @@ int most_tiles(int pairs, int experts, int rows) { return pairs < experts + pair
 
 bool takes_many(const mld_moe_desc& d, int tokens) {
   if (d.force_path != MLD_MOE_PATH_AUTO) return d.force_path == MLD_MOE_PATH_MANY_ROWS;
-  // By the rows of an expert, were all alike.  us, few / many, at 8, 12 and 16: 64 experts of 2048 x 1024 in 4 bits 102 / 130, 132 / 131,
-  // 158 / 131; 8 of 4096 x 4096 90 / 143, 116 / 144, 145 / 144, in 8 bits 107 / 142, 135 / 142, 170 / 143; 128 of 2048 x 768 144 / 178,
-  // 192 / 184, 234 / 185.
+  // By the rows of an expert, were all alike.  us, few / many, at 6, 8 and 10: 64 experts of 2048 x 1024 in 4 bits 86 / 105, 101 / 106,
+  // 115 / 105; 8 of 4096 x 4096 76 / 108, 89 / 109, 113 / 109, in 8 bits 91 / 124, 107 / 124, 134 / 124; 128 of 2048 x 768
+  // 121 / 130, 144 / 141, 166 / 141.
   return static_cast<int64_t>(tokens) * d.top_k > kFewShare * static_cast<int64_t>(d.experts);
 }
 

@@ -39,7 +39,7 @@ __device__ __forceinline__ float moe_gated(float gate, float up, int activation)
 #endif
 
 // The products of tiles of up to kMoeTileRows rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16).
-constexpr int kMoeTileRows = 384;
+constexpr int kMoeTileRows = 256;
 int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs, int sms,
                     cudaStream_t stream);
 

@@ -331,6 +331,7 @@ __global__ void __launch_bounds__(Shape<BITS>::kThreads, 1)
                 acc[b][r][3] += sum[3] * sc.y;
               }
           }
+          fence_proxy_async();  // (what has been asked for is here before a copy may overwrite it)
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[s]);
           s += kWarps;

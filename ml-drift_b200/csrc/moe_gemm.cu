@@ -2,20 +2,21 @@
 //
 // The form is gemm_wtmem_kernel's (Y^T = W X^T, tcgen05 cta_group::2, weights as the A operand in tensor memory, rows as the B
 // operand in shared memory), with what a grouped product needs in place of what a single one does:
-//   - a tile is 256 outputs of one expert x up to 384 of its rows; which expert and which rows stands in a list that the
+//   - a tile is 256 outputs of one expert x up to 256 of its rows; which expert and which rows stands in a list that the
 //     ordering kernel left in device memory.  Every role reads the list for itself and goes through the same tiles.
 //   - rows of an expert follow one another, so a tile's rows are one box after another of 32; as many are fetched as the tile has
-//     rows, and the MMAs' N is that many, too (in steps of 64; beyond 256 in two MMAs of the same weights).  Columns behind the
-//     tile's rows belong to other experts, or are zeros, and are not written.
+//     rows, and the MMAs' N is that many, too (in steps of 64).  Columns behind the tile's rows belong to other experts, or are
+//     zeros, and are not written.
 //   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
 //     and an up channel, exchange half of their tokens; of the second the expert's output.
-// Per CTA: warps 0 and 23 fetch rows, every other stage each (one alone takes 450 to 520 cycles to a stage), warp 22 packed weights, warp 1 issues the MMAs (of the pair's first CTA), warps 6..21 dequantise
-// (four to a stage of 64 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights and two halves of 192 columns
-// of accumulators.  A tile of up to 192 rows takes the half that is free, and the next tile goes on while it is written; a larger
-// one takes both, so the sixteen help writing.
-// A stage's weights take about 600 cycles from box to operand, whatever the rows, its MMAs 2 per row: an expert's rows go in as few
-// tiles as hold them, all alike.  (Tiles of 256 rows, one set of accumulators and eight stages of weights: 2048 tokens 298 us against
-// 263, 1531 tokens 1077 against 1024.)
+// Per CTA: warps 0 and 23 fetch rows, every other stage each, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first
+// CTA), warps 6..21 dequantise (four to a stage of 128 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights
+// and two halves of 128 columns of accumulators.  A tile of up to 128 rows takes the half that is free, and the next tile goes on
+// while it is written; a larger one takes both, so the sixteen help writing.
+// With few rows bound by what a stage costs each role, whatever is in it (the warps that fetch and the one that issues MMAs 300 to
+// 500 cycles, the dequantisation about 1700 for a quarter of the stages): hence 128 inputs to a stage, where 64 took 122 us against
+// 107 (128 tokens through 8 of 64 experts, 2048 x 1024).  With many rows by the MMAs, 4 cycles a row and stage, and by the clock that
+// the power limit leaves: 1531 tokens through 2 of 8 experts of 4096 x 14336 run at 1.02 PFLOP/s.
 // Every wait is bounded.
 #include <cuda_fp16.h>
 
@@ -30,12 +31,14 @@ namespace mld {
 namespace {
 
 constexpr int kStages = 4;              // rows in shared memory + weights in tensor memory
-constexpr int kWStages = 8;             // packed weights
+constexpr int kWStages = 4;             // packed weights
 constexpr int kChannels = 128;          // outputs per CTA
 constexpr int kBoxRows = 32;
 constexpr int kBoxBytes = kBoxRows * kKBytes;
-constexpr int kSlices = 16;             // packed rows of a stage: 64 inputs
-constexpr int kHalf = 192;               // columns of one of two halves of accumulators
+constexpr int kInputs = 128;            // of a stage
+constexpr int kSlices = kInputs / 4;    // packed rows of a stage
+constexpr int kAtom = 128 * kKBytes;    // shared memory of 64 inputs of a CTA's rows
+constexpr int kHalf = 128;               // columns of one of two halves of accumulators
 constexpr int kColumns = 2 * kHalf;      // the weights' follow
 static_assert(kColumns == kMoeTileRows, "a tile's rows");
 constexpr int kThreads = 24 * 32;
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   constexpr int kBlk = BITS == 4 ? 8 : 16;
   constexpr int kPitch = kChannels / 4 * kBlk;        // bytes of a packed row of the box
   constexpr int kWBytes = kSlices * kPitch;
-  constexpr int kXBytes = kColumns / 2 * kKBytes;     // a CTA's rows of a stage
+  constexpr int kXBytes = 2 * kAtom;                  // a CTA's rows of a stage
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sX = smem;
@@ -253,8 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     MoeTile tile;
     int n0;
     while (ok && work.next(tile, n0)) {
-      const int cols = columns_of(tile), low = min(cols, 256);  // (of the first MMA; a CTA has half of each one's rows)
-      const int row = tile.row0 + static_cast<int>(rank) * (low >> 1), row_high = tile.row0 + 256 + static_cast<int>(rank) * ((cols - low) >> 1);
+      const int cols = columns_of(tile), row = tile.row0 + static_cast<int>(rank) * (cols >> 1);
       for (int kb = (mine ^ before) & 1; kb < a.k_blocks; kb += 2) {
         const int iter = before + kb, stage = iter % kStages;
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u))) {
@@ -263,12 +265,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           break;
         }
         if (elect_one()) {
-          if (rank == 0) mbar_arrive_expect_tx(&full_ab[stage], static_cast<uint32_t>(cols) * kKBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full_ab[stage], static_cast<uint32_t>(cols) * (2 * kKBytes));
           uint8_t* const to = sX + stage * kXBytes;
-          for (int i = 0; i < low >> 6; ++i)
-            tma_load_2d_pair(to + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row + i * kBoxRows);
-          for (int i = 0; i < (cols - low) >> 6; ++i)
-            tma_load_2d_pair(to + 128 * kKBytes + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * 64, row_high + i * kBoxRows);
+          for (int i = 0; i < cols >> 6; ++i) {
+            tma_load_2d_pair(to + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * kInputs, row + i * kBoxRows);
+            tma_load_2d_pair(to + kAtom + i * kBoxBytes, &tmap_x, full_ab_lead + stage * 8, kb * kInputs + 64, row + i * kBoxRows);
+          }
         }
         __syncwarp();
       }
@@ -285,9 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       int n0;
       for (Turns turn; ok && work.next(tile, n0); turn.next()) {
         turn.take(tile, work.done());
-        const int cols = columns_of(tile), low = min(cols, 256);
-        const auto idesc_of = [](int n) { return 1u << 4 | static_cast<uint32_t>(n >> 3) << 17 | 16u << 24; };
-        const uint32_t idesc = idesc_of(low), idesc_high = idesc_of(cols - low);
+        const uint32_t idesc = 1u << 4 | static_cast<uint32_t>(columns_of(tile) >> 3) << 17 | 16u << 24;
         const uint32_t d = tmem_base + static_cast<uint32_t>(turn.at * kHalf);
         bool free = mbar_wait(&tmem_empty[turn.at], turn.uses_of(turn.at) ^ 1u);
         if (turn.large) free = mbar_wait(&tmem_empty[1], turn.uses_of(1) ^ 1u) && free;
@@ -304,15 +304,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
           tc_after();
           const uint64_t db = make_desc(smem_u32(sX + stage * kXBytes));
-          const uint32_t ta = tmem_base + kColumns + static_cast<uint32_t>(stage * 32);
+          const uint32_t ta = tmem_base + kColumns + static_cast<uint32_t>(stage * (kInputs / 2));
           if (elect_one()) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              umma_ts<true, false>(d, ta + 8u * i, db + static_cast<uint64_t>((i * 32) >> 4), idesc, (kb > 0 || i > 0) ? 1u : 0u);
-              if (cols > 256)
-                umma_ts<true, false>(d + 256, ta + 8u * i, db + static_cast<uint64_t>((128 * kKBytes + i * 32) >> 4), idesc_high,
-                                     (kb > 0 || i > 0) ? 1u : 0u);
-            }
+            for (int i = 0; i < kInputs / 16; ++i)
+              umma_ts<true, false>(d, ta + 8u * i, db + static_cast<uint64_t>(((i >> 2) * kAtom + (i & 3) * 32) >> 4), idesc,
+                                   (kb > 0 || i > 0) ? 1u : 0u);
             commit<true>(&empty[stage]);
           }
           __syncwarp();
@@ -397,17 +394,19 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
                      : "l"(scale + static_cast<int64_t>(g) * a.n), "r"(has_n ? 1u : 0u));
       };
       int kb = (group - before) & 3;
-      unsigned short next0 = 0, next1 = 0;
+      unsigned short next[4] = {0, 0, 0, 0};
       if (kb < a.k_blocks) {
-        ask(next0, kb * kSlices);
-        ask(next1, kb * kSlices + 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ask(next[i], kb * kSlices + 8 * i);
       }
       for (; kb < a.k_blocks; kb += 4) {
         const int iter = before + kb, stage = iter & (kStages - 1), ws = iter & (kWStages - 1);
-        const unsigned short cur0 = next0, cur1 = next1;
+        unsigned short cur[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cur[i] = next[i];
         if (kb + 4 < a.k_blocks) {
-          ask(next0, (kb + 4) * kSlices);
-          ask(next1, (kb + 4) * kSlices + 8);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ask(next[i], (kb + 4) * kSlices + 8 * i);
         }
         if (!mbar_wait(&full_w[ws], static_cast<uint32_t>(iter / kWStages) & 1u)) {
           atomicExch(a.error, kErrMoeBase + 6);
@@ -415,56 +414,63 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           break;
         }
         const uint8_t* wp = sW + ws * kWBytes + (row >> 2) * kBlk;
-        const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kColumns + static_cast<uint32_t>(stage * 32);
+        const uint32_t columns = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + kColumns + static_cast<uint32_t>(stage * (kInputs / 2));
         using Block = typename std::conditional<BITS == 4, uint2, uint4>::type;
-        uint32_t o[32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          Block blk[8];
+        for (int sixty_four = 0; sixty_four < 2; ++sixty_four) {
+          uint32_t o[32];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (8 * half + i) * kPitch);
-          const __half s = __ushort_as_half(half == 0 ? cur0 : cur1);
-          const __half2 s2 = __half2half2(s);
-          if constexpr (BITS == 4) {
-            // A nibble at bits 6..9 is the subnormal half u 2^-18: u 2^-18 (2^18 s) - 8 s is (u - 8) s rounded once, in one
-            // instruction.  2^18 s has to be a half; else from 1024 + u, the zero off exactly first.
-            if (__all_sync(0xffffffffu, __habs(s) < __float2half_rn(0.249f))) {
-              const __half2 up = __hmul2(s2, __float2half2_rn(512.0f)), large = __hmul2(up, __float2half2_rn(512.0f));
-              const __half2 zero = __hmul2(s2, __float2half2_rn(-8.0f));
+          for (int half = 0; half < 2; ++half) {
+            Block blk[8];
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t lo = __funnelshift_l(blk[i].x, blk[i].x, turn6) & 0x03C003C0u;
-                const uint32_t hi = __funnelshift_l(blk[i].y, blk[i].y, turn6) & 0x03C003C0u;
-                const __half2 r0 = __hfma2(*reinterpret_cast<const __half2*>(&lo), large, zero);
-                const __half2 r1 = __hfma2(*reinterpret_cast<const __half2*>(&hi), large, zero);
-                o[16 * half + 2 * i] = *reinterpret_cast<const uint32_t*>(&r0);
-                o[16 * half + 2 * i + 1] = *reinterpret_cast<const uint32_t*>(&r1);
+            for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (16 * sixty_four + 8 * half + i) * kPitch);
+            const __half s = __ushort_as_half(cur[2 * sixty_four + half]);
+            const __half2 s2 = __half2half2(s);
+            if constexpr (BITS == 4) {
+              // A nibble at bits 6..9 is the subnormal half u 2^-18: u 2^-18 (2^18 s) - 8 s is (u - 8) s rounded once, in one
+              // instruction.  2^18 s has to be a half; else from 1024 + u, the zero off exactly first.
+              if (__all_sync(0xffffffffu, __habs(s) < __float2half_rn(0.249f))) {
+                const __half2 up = __hmul2(s2, __float2half2_rn(512.0f)), large = __hmul2(up, __float2half2_rn(512.0f));
+                const __half2 zero = __hmul2(s2, __float2half2_rn(-8.0f));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const uint32_t lo = __funnelshift_l(blk[i].x, blk[i].x, turn6) & 0x03C003C0u;
+                  const uint32_t hi = __funnelshift_l(blk[i].y, blk[i].y, turn6) & 0x03C003C0u;
+                  const __half2 r0 = __hfma2(*reinterpret_cast<const __half2*>(&lo), large, zero);
+                  const __half2 r1 = __hfma2(*reinterpret_cast<const __half2*>(&hi), large, zero);
+                  o[16 * half + 2 * i] = *reinterpret_cast<const uint32_t*>(&r0);
+                  o[16 * half + 2 * i + 1] = *reinterpret_cast<const uint32_t*>(&r1);
+                }
+              } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  o[16 * half + 2 * i] = dq_once(((blk[i].x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+                  o[16 * half + 2 * i + 1] = dq_once(((blk[i].y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+                }
               }
             } else {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                o[16 * half + 2 * i] = dq_once(((blk[i].x >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
-                o[16 * half + 2 * i + 1] = dq_once(((blk[i].y >> (4 * col4)) & 0x000F000Fu) | 0x64006400u, offset, s2);
+                o[16 * half + 2 * i] = dq_once((__byte_perm(blk[i].x, blk[i].y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
+                o[16 * half + 2 * i + 1] = dq_once((__byte_perm(blk[i].z, blk[i].w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
               }
             }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              o[16 * half + 2 * i] = dq_once((__byte_perm(blk[i].x, blk[i].y, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
-              o[16 * half + 2 * i + 1] = dq_once((__byte_perm(blk[i].z, blk[i].w, sel8) & 0x00FF00FFu) | 0x64006400u, offset, s2);
-            }
           }
+          if (sixty_four == 1) {
+            fence_proxy_async();  // (what has been asked for is here before a copy may overwrite it)
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&w_empty[ws]);
+          } else if (!mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u)) {
+            // (the first weights are ready in registers when the stage's last MMAs are done with its columns)
+            atomicExch(a.error, kErrMoeBase + 6);
+            ok = false;
+            break;
+          } else {
+            tc_after();
+          }
+          tmem_st32(columns + static_cast<uint32_t>(32 * sixty_four), o);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&w_empty[ws]);
-        // (the weights are ready in registers when the stage's last MMAs are done with its columns)
-        if (!mbar_wait(&empty[stage], (static_cast<uint32_t>(iter / kStages) & 1u) ^ 1u)) {
-          atomicExch(a.error, kErrMoeBase + 6);
-          ok = false;
-          break;
-        }
-        tc_after();
-        tmem_st32(columns, o);
+        if (!ok) break;
         tmem_st_wait();
         tc_before();
         __syncwarp();
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 
 template <int BITS, bool FIRST>
 int launch_of(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int grid, cudaStream_t stream) {
-  constexpr size_t smem = 1024 + kStages * (kColumns / 2) * kKBytes + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
+  constexpr size_t smem = 1024 + kStages * 2 * kAtom + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
                           (2 * kWStages + 2 * kStages + 5) * 8 + 64;
   static_assert(smem <= 227 * 1024, "shared memory");
   auto kern = moe_gemm_kernel<BITS, FIRST>;
@@ -529,7 +535,7 @@ int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const vo
   a.tiles = b.tiles;
   a.n_tiles = b.n_tiles;
   a.n_channel_tiles = div_up(n, 2 * kChannels);
-  a.k_blocks = div_up(k, 64);
+  a.k_blocks = div_up(k, kInputs);
   a.n = n;
   a.k = k;
   a.scale = static_cast<const __half*>(scale);

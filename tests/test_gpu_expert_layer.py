@@ -65,7 +65,7 @@ def test_a_layer(mld, n, captured):
     second = np.stack([_matrix(layer.weights[2][j], layer.weights[3][j], d, f, 4) for j in range(e)])
     want, size = ref.experts(y, ids, layer.gates[:n].cpu().numpy(), first, second, h, False)
     got = stream.cpu().numpy().astype(np.float64)
-    bound = ref.experts_bound(want, size, n * k > 12 * e)
+    bound = ref.experts_bound(want, size, n * k > 8 * e)
     assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
 
 

@@ -177,7 +177,7 @@ def test_the_path_changes_with_the_tokens_of_a_call(mld):
     plan = mld.MoeExperts(e, k, d, f, max_tokens=n)
     x = rng.standard_normal((n, d)).astype(np.float16)
     ids, weights = _ids(rng, n, e, k).astype(np.int32), rng.random((n, k)).astype(np.float32)
-    for rows in (n, 1, 24, 25, 2, n, 0):  # 24 tokens are 48 pairs, the most that go the one way
+    for rows in (n, 1, 16, 17, 2, n, 0):  # 16 tokens are 32 pairs, the most that go the one way
         out = torch.full((n, d), 3.0, dtype=torch.float16, device="cuda")
         plan.run(_dev(x[:rows]), _dev(ids[:rows]), _dev(weights[:rows]), w1, s1, w2, s2, out[:rows])
         got = out.cpu().numpy().astype(np.float64)
@@ -204,3 +204,42 @@ def test_two_plans_at_once_on_two_streams(mld):
     for p, o, many in zip(plans, outs, (False, True)):
         assert p.device_status() == 0 and (o == o[0]).all()
         assert (np.abs(o[0].cpu().numpy().astype(np.float64) - want) <= _bound(want, size, many)).all()
+
+
+@pytest.mark.parametrize("large", [0.3, 40.0])
+def test_scales_whose_multiples_leave_fp16(mld, large):
+    """Scales at which the short way from a nibble to a weight is not open, beside some at which it is."""
+    e, k, d, f, n = 3, 1, 128, 64, 50
+    rng = np.random.default_rng(9)
+    (first, second), (w1, s1, w2, s2) = _weights(e, d, f, 4, 32)
+    up = np.ones((e, d // 32, 2 * f))
+    up[:, 1::2] = large / s1.float().max().item()
+    s1 = (s1.double() * torch.from_numpy(up).cuda()).half()
+    codes = first / np.repeat(_weights(e, d, f, 4, 32)[1][1].cpu().numpy().astype(np.float64), 32, 1).transpose(0, 2, 1)
+    first = np.rint(codes) * np.repeat(s1.cpu().numpy().astype(np.float64), 32, 1).transpose(0, 2, 1)
+    x = (rng.standard_normal((n, d)) / (20 * large)).astype(np.float16)
+    ids, weights = _ids(rng, n, e, k).astype(np.int32), rng.random((n, k)).astype(np.float32)
+    for path in (mld.MOE_PATH_FEW_ROWS, mld.MOE_PATH_MANY_ROWS):
+        plan = mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=path)
+        out = torch.empty(n, d, dtype=torch.float16, device="cuda")
+        plan.run(_dev(x), _dev(ids), _dev(weights), w1, s1, w2, s2, out)
+        want, size = ref.experts(x, ids, weights, first, second, None, False)
+        assert (np.abs(out.cpu().numpy() - want) <= _bound(want, size, path == mld.MOE_PATH_MANY_ROWS)).all()
+
+
+@pytest.mark.parametrize("path,n", [("few", 40), ("many", 300)])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_a_hundred_calls_give_the_same_bits(mld, path, n, bits):
+    """More boxes of weights than the rings hold, over and over: nothing is overwritten before it has been read."""
+    e, k, d, f = 16, 4, 1024, 512
+    rng = np.random.default_rng(n)
+    w = [torch.randint(0, 256, (e, 2 * f * d * bits // 8), dtype=torch.uint8, device="cuda"), (0.002 * torch.rand(e, 1, 2 * f, device="cuda")).half(),
+         torch.randint(0, 256, (e, f * d * bits // 8), dtype=torch.uint8, device="cuda"), (0.002 * torch.rand(e, 1, d, device="cuda")).half()]
+    x, ids, weights = _dev(rng.standard_normal((n, d)).astype(np.float16)), _dev(_ids(rng, n, e, k).astype(np.int32)), _dev(rng.random((n, k)).astype(np.float32))
+    plan = mld.MoeExperts(e, k, d, f, weight_bits=bits, block=0, max_tokens=n,
+                          force_path=mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS)
+    first, out = torch.empty(n, d, dtype=torch.float16, device="cuda"), torch.empty(n, d, dtype=torch.float16, device="cuda")
+    plan.run(x, ids, weights, *w, first)
+    for _ in range(100):
+        plan.run(x, ids, weights, *w, out)
+        assert torch.equal(out, first)
