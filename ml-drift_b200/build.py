@@ -16,7 +16,7 @@ SOURCES = ["api.cu", "pack_kernels.cu", "gemv_generic.cu", "gemv_stream.cu", "de
            "gemm_umma.cu", "gemm_pair.cu", "gemm_wtmem.cu", "shard_group.cu", "embedding.cu", "loader.cu",
            "qk_rope.cu", "kv4_attn.cu", "kv4_prefill.cu", "kv4_pages.cu", "add_norm.cu",
            "moe_route.cu", "moe.cu", "moe_few.cu", "moe_gemm.cu"]
-HEADERS = ["common.cuh", "kernels.h", "nccl_lazy.h", "pair_common.cuh", "ring_order.h", "kv4.cuh", "kv4_attn.cuh", "moe.cuh", "wtmem.cuh", os.path.join(ROOT, "include", "mldfc.h")]
+HEADERS = ["common.cuh", "kernels.h", "nccl_lazy.h", "pair_common.cuh", "ring_order.h", "kv4.cuh", "kv4_attn.cuh", "moe.cuh", "few_ring.h", "wtmem.cuh", os.path.join(ROOT, "include", "mldfc.h")]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

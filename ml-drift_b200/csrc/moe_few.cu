@@ -25,39 +25,18 @@
 #include <cstring>
 
 #include "common.cuh"
+#include "few_ring.h"
 #include "moe.cuh"
 
 namespace mld {
 namespace {
 
-constexpr int kOutputs = 64;        // of an item
-constexpr int kRows = kMoeFewRows;  // of a tile at most: the columns of a fragment
-constexpr int kInputs = 128;        // of a box
-constexpr int kCopyWarps = 4;
-constexpr int kSumWarps = 4;
-constexpr int kItemBars = 64;       // items under way, of one box at least: a ring's, and two parts of every warp
+constexpr int kOutputs = kFewOutputs, kRows = kFewRows, kInputs = kFewInputs, kCopyWarps = kFewCopyWarps, kSumWarps = kFewSumWarps;
+constexpr int kItemBars = kFewItemBars, kBoxBytes = kFewBoxBytes;
 constexpr int kErrFewBase = 90;
-constexpr int kBoxBytes = kInputs / 4 * 128;   // 128 bytes of every input slice: 64 outputs in 4 bits, 32 in 8
-constexpr int kRoom = 226 * 1024;              // shared memory
-
-// The block's shape.  Places of the ring are a multiple of the multiplying warps, so that a place is always the same warp's, which
-// then waits for each of the place's boxes in turn.  (A wait tells a box from the one before it and no more: a warp that took
-// another one's place could take an old box for its own.)
+static_assert(kRows == kMoeFewRows, "rows of a tile");
 template <int BITS>
-struct Shape {
-  static constexpr int kWarps = 8;
-  static constexpr int kThreads = 32 * (kCopyWarps + kWarps + kSumWarps);
-  static constexpr int kWBytes = kBoxBytes * (BITS == 4 ? 1 : 2);
-  static constexpr int kScaleBytes = 4 * kOutputs * 2;           // four rows at most
-  static constexpr int kStage = kWBytes + kScaleBytes;
-  static constexpr int kPart = 8 * 32;                           // float2s of a part
-  static constexpr int kPlaces = 2;                              // for a warp's parts
-  static constexpr int kPartBytes = kWarps * kPlaces * kPart * 8;
-  static constexpr int kRowBytes = kItemBars * kRows * 8;        // where the rows of the items under way are
-  static constexpr int kStages = (kRoom - 3 * 1024 - kPartBytes - kRowBytes) / kStage / kWarps * kWarps;
-  static constexpr size_t kSmem = 1024 + static_cast<size_t>(kStages) * kStage + kPartBytes + kRowBytes + (2 * kStages + 2 * kItemBars + kWarps * kPlaces) * 8;
-  static_assert(kStages >= kWarps && kStages % kCopyWarps == 0 && kSmem <= 227 * 1024, "shared memory");
-};
+using Shape = FewShape<BITS>;
 
 struct FewArgs {
   MoeBuffers b;
@@ -193,7 +172,7 @@ __global__ void __launch_bounds__(Shape<BITS>::kThreads, 1)
       int next_token = 0;
       if (warp == 0) {
         next_token = token_of(next_tile);
-        // (places behind the tile's rows get one that exists; a slot's last readers are a ring's boxes behind at most)
+        // (places behind the tile's rows get one that exists; a slot's last readers are done with it, see kFewItemBars)
         if (lane < kRows) {
           const __half* p;
           if constexpr (FIRST)
