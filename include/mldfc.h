@@ -394,7 +394,8 @@ MLD_API int mld_fc_run_codes(mld_fc_plan* plan, const int8_t* codes, const float
  *                 code = floor(127 v / max|v| + 1/2)
  *     asymmetric: scale = (max y - min y) / 255, zero point = min y + 128 scale,
  *                 code = floor(255 (v - min v) / (max v - min v) + 1/2) - 128
- * in 32 bits, codes that lie next to a border in 64.  A row of equal v (of
+ * in 32 bits, codes that lie next to a border, and those of rows whose values
+ * are large against their span, in 64: they are the formula's.  A row of equal v (of
  * zeros, symmetric) has codes 0 and scale 0.  The sum of a row's squares has to
  * be a 32-bit float: a row where it, or a product with a weight, is infinite or
  * NaN has NaN parameters and codes 0. */

@@ -9,9 +9,12 @@
 //
 // Bound by HBM: x and the residual in, the sum, y and the codes out, each once.  A row stays in the registers of the warp or the
 // block that owns it, together with its part of the weights, which serve all of its rows; the sum of squares and the extremes of
-// v go through one exchange.  Sums and products are held in 32 bits.  A code whose value in 32 bits lies within 2^-13 of a border
-// between two codes (the error is below 2^-13: six roundings of 2^-24 at a value of 255 at most) is worked out again in 64, with
-// its seven neighbours, so that codes are those of the formula, whoever works it out.  (One chunk in 500 is.)
+// v go through one exchange.  Sums and products are held in 32 bits.  A code whose value in 32 bits lies near a border between two
+// codes is worked out again in 64, with its seven neighbours, so that codes are those of the formula, whoever works it out.  Near is
+// 2^-13, above six roundings of 2^-24 at a value of 255 at most: of the span, its reciprocal and a value's distance from the row's
+// smallest, and, with an offset or 32-bit tensors, of offset + w, v and that smallest.  The last three are relative to v, so for
+// them near grows with max|v| / span where that is above 1; where it passes a quarter, the whole row is worked out in 64.  (Of rows
+// about zero one chunk in 500 is worked out again.)
 #include <cuda_fp16.h>
 
 #include <atomic>
@@ -314,7 +317,7 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) add_norm_kernel(NormArgs a)
       double low = st.low, high = st.high;
       if constexpr (!EXACT) {
         // the extremes in 64 bits: of the threads whose own come near them in 32
-        const float near = 1.0e-6f * fmaxf(fabsf(st.low), fabsf(st.high));
+        const float near = 1.0e-6f * fmaxf(fabsf(st.low), fabsf(st.high)) + 0x1p-147f;  // (of subnormal v: a few of their steps)
         double lo = INFINITY, hi = -INFINITY;
         if (fine && (my_low <= st.low + near || my_high >= st.high - near)) {
 #pragma unroll
@@ -352,11 +355,15 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) add_norm_kernel(NormArgs a)
       const float top = a.symmetric ? 127.0f : 255.0f, from = static_cast<float>(from64);
       const bool live = fine && span > 0.0;
       const float per = live ? top / static_cast<float>(span) : 0.0f;
-      const bool tiny = !(per < 1.0e36f);  // a span so small that its factor leaves 32 bits: everything in 64
+      constexpr float kBorder = 0x1p-13f;
+      const float error = EXACT ? kBorder : fmaxf(kBorder, fmaxf(fabsf(st.low), fabsf(st.high)) * per * (kBorder / 255.0f));
+      // a span whose factor leaves 32 bits, or that leaves them itself, or is small against v: everything in 64
+      const bool wide = !(per > 0.0f && per < 1.0e36f && error <= 0.25f);
       int8_t* const codes = a.codes + row * a.codes_stride;
       // Rounded by the addition of 1.5 2^23, whose last byte then is the code (of 0 .. 255 less 128: with its top bit turned).
       // A value near the middle between two codes, or on it, is compared with it in 64 bits, and goes up from there.
-      constexpr float kRound = 12582912.0f, kNear = 0.5f - 0x1p-13f;
+      constexpr float kRound = 12582912.0f;
+      const float clear = 0.5f - error;
       const uint32_t turned = a.symmetric ? 0u : 0x80808080u;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
@@ -370,14 +377,14 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) add_norm_kernel(NormArgs a)
             off = fmaxf(off, fabsf(fmaf(d, per, kRound - r)));
             q[i] = __float_as_uint(r);
           }
-          if (!(off < kNear) || tiny || !live) {
+          if (!(off < clear) || wide || !live) {
             Chunk<T> w;
             if constexpr (!EXACT) w = weights_of(j);
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) {
               const double d = (EXACT ? static_cast<double>(v.v[i]) : in64(h[j].v[i], EXACT ? h[j].v[i] : w.v[i])) - from64;
               // the code by 32 bits (or, where that fails, below it) and whether the middles on both sides of it move it
-              double at = tiny ? floor(d * (top / span)) : static_cast<double>(static_cast<int>(q[i] - 0x4B400000u));
+              double at = wide ? floor(d * (top / span)) : static_cast<double>(static_cast<int>(q[i] - 0x4B400000u));
               at = fmin(fmax(at, -128.0), 255.0);
               const double twice = d * (2.0f * top);
               at += twice >= (2.0 * at + 1.0) * span ? 1.0 : twice < (2.0 * at - 1.0) * span ? -1.0 : 0.0;
@@ -395,8 +402,9 @@ __global__ void __launch_bounds__(WARP ? 128 : 1024) add_norm_kernel(NormArgs a)
       if (me == 0 && chunks * kChunk < a.codes_width) *reinterpret_cast<uint2*>(codes + chunks * kChunk) = make_uint2(0u, 0u);
       if (me < 3) {
         // (a row of equal values has scale 0, and each is the zero point)
-        const float value = me == 0 ? static_cast<float>(span) * rstd / top
-                            : me == 2 || a.symmetric ? 0.0f : static_cast<float>(low + span * (128.0 / 255.0)) * rstd;
+        const double by = rstd;
+        const float value = me == 0 ? static_cast<float>(span * by * (a.symmetric ? 1.0 / 127.0 : 1.0 / 255.0))
+                            : me == 2 || a.symmetric ? 0.0f : static_cast<float>((low + span * (128.0 / 255.0)) * by);
         a.params[static_cast<int64_t>(row) * 3 + me] = fine || me == 2 ? value : NAN;
       }
     }

@@ -1,0 +1,75 @@
+"""Codes of rows whose values are large against their spread, and of rows at the ends of 32 bits."""
+import numpy as np
+import pytest
+import torch
+
+from tests import ffn_ref as ref
+
+pytestmark = pytest.mark.gpu
+U32 = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def mld():
+    import __graft_entry__ as g
+    return g.import_package()
+
+
+def _dev(a):
+    return torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def _codes(mld, x, g, offset, symmetric, residual=None):
+    n, w = x.shape
+    codes, params = torch.full((n, -(-w // 16) * 16), 77, dtype=torch.int8, device="cuda"), torch.empty(n, 3, device="cuda")
+    total = torch.empty_like(_dev(x)) if residual is not None else None
+    mld.add_rms_norm(_dev(x), weight=None if g is None else _dev(g), residual=None if residual is None else _dev(residual), sum_out=total,
+                     codes=codes, params=params, symmetric=symmetric, weight_offset=offset)
+    return codes.cpu().numpy()[:, :w], params.cpu().numpy().astype(np.float64)
+
+
+def _check(mld, x, g, offset, symmetric, residual=None):
+    _, v, rstd = ref.add_norm(x, residual, g, 1e-6, offset if g is not None else 0.0)
+    q, scale, zero = ref.codes(v, rstd, symmetric)
+    got, p = _codes(mld, x, g, offset, symmetric, residual)
+    assert np.array_equal(got, q), (got != q).sum()
+    # the parameters: as in the norm's own test, 64 roundings of 32 bits at most, the zero point's relative to its largest term
+    assert (np.abs(p[:, :1] - scale) <= 64 * U32 * scale).all()
+    assert (np.abs(p[:, 1:2] - zero) <= 64 * U32 * (np.abs(zero) + 256 * scale)).all()
+
+
+@pytest.mark.parametrize("n,w", [(40, 200), (300, 2048), (200, 1155), (30, 8192), (3, 4096)])
+@pytest.mark.parametrize("mean,spread", [(100.0, 1.0), (1000.0, 1.0), (-1000.0, 0.01), (3.0e5, 1.0), (1.0e-3, 1.0e-5)])
+@pytest.mark.parametrize("offset", [0.0, 1.0])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_rows_far_from_zero_in_32_bits(mld, n, w, mean, spread, offset, symmetric):
+    """v = h (offset + w) is rounded relative to itself, codes are relative to the row's span."""
+    rng = np.random.default_rng(w)
+    x = (mean + spread * rng.standard_normal((n, w))).astype(np.float32)
+    weights = [((1 - offset) + 1e-6 * rng.standard_normal(w)).astype(np.float32), None if offset == 0 else np.zeros(w, np.float32)]
+    for g in weights:
+        _check(mld, x, g, offset, symmetric)
+
+
+@pytest.mark.parametrize("n,w", [(40, 200), (300, 2048), (200, 1155), (30, 8192), (3, 4096)])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_rows_far_from_zero_in_16_bits(mld, n, w, symmetric):
+    rng = np.random.default_rng(w)
+    x = (1000 + 2 * rng.standard_normal((n, w))).astype(np.float16)
+    r = rng.standard_normal((n, w)).astype(np.float16)
+    _check(mld, x, (0.001 * rng.standard_normal(w)).astype(np.float16), 1.0, symmetric, r)
+    _check(mld, np.full((n, w), 1000, np.float16), (0.001 * rng.standard_normal(w)).astype(np.float16), 1.0, symmetric)
+    _check(mld, x, (1 + 0.001 * rng.standard_normal(w)).astype(np.float16), 0.0, symmetric, r)
+
+
+@pytest.mark.parametrize("w", [256, 1155, 4096])
+def test_spans_that_leave_32_bits_and_subnormal_ones(mld, w):
+    rng = np.random.default_rng(w)
+    x = (1e17 * rng.uniform(-1, 1, (5, w))).astype(np.float32)
+    x[:, 0], x[:, 1] = 1e17, -1e17
+    _check(mld, x, np.full(w, 3.3e21, np.float32), 0.0, False)
+    x = (1e-21 * rng.uniform(0.5, 1, (5, w))).astype(np.float32)
+    g = (1e-21 * rng.uniform(0.5, 1, w)).astype(np.float32)  # products are subnormal in 32 bits
+    _, v, rstd = ref.add_norm(x, None, g, 1e-6, 0.0)
+    for symmetric in (True, False):
+        assert np.array_equal(_codes(mld, x, g, 0.0, symmetric)[0], ref.codes(v, rstd, symmetric)[0])
