@@ -3,7 +3,9 @@
 // A warp takes a token, a lane a run of neighbouring experts.  Without a bias and with groups that go by one expert the order is that
 // of the logits, whatever the score: nothing is computed but the chosen ones' scores (and, without renormalising, the softmax's
 // sum).  Else experts are compared by values in 32 bits first; where two that the choice hangs on lie closer to one another
-// than the error of those (some token of a long prompt always has such), the token is gone through again in 64.
+// than the error of those (some token of a long prompt always has such), the token is gone through again in 64.  So it is where the
+// choice hangs on two groups whose logits differ and whose values in 64 bits might not: of equal groups the first counts, not
+// the one with the larger logit.
 // Bound by instructions: k rounds of the largest of each lane's, the warp's largest (one instruction), its lane and place.
 #include <cuda_fp16.h>
 
@@ -49,10 +51,17 @@ __device__ __forceinline__ double warp_max(double v) {
 }
 __device__ __forceinline__ double warp_min(double v) { return -warp_max(-v); }
 
+// Whether two logits, of which the upper is the larger, surely have different values in 64 bits: apart by more than 2^-16, where
+// neither a sigmoid rounds to 1 (below 16, such differ by 1e-12) nor an exponential vanishes.
+__device__ __forceinline__ bool apart_in_64(const RouteArgs& a, float upper, float lower, float top) {
+  return upper - lower > 0x1p-16f && (a.sigmoid ? lower < 16.0f && lower > -600.0f : lower - top > -600.0f);
+}
+
 // The k best of keys (-infinity: not to be had), into lane j the j-th: its expert (-1: none) and its logit.  Of equal keys (64 bits)
-// the larger logit, then the lower number.  False: something that the choice hangs on is closer than `tolerance` (0: never).
-template <typename Key, int N>
-__device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const float (&x)[N], int lane, float tolerance, int& id,
+// the larger logit, then the lower number.  False: something that the choice hangs on is closer than `tolerance` (0: never), or
+// is not surely the same by values, of keys that are logits (the largest is `top`).
+template <bool LOGITS, typename Key, int N>
+__device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const float (&x)[N], int lane, float tolerance, float top, int& id,
                                        float& logit) {
   constexpr bool kWide = sizeof(Key) == 8;
   constexpr Key kNone = static_cast<Key>(-INFINITY);
@@ -112,6 +121,13 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
       const Key least = warp_min(kept ? sum : static_cast<Key>(INFINITY)), most = warp_max(exists && !kept ? sum : kNone);
       clear = clear && !(most > kNone && close(least, most, 2 * tolerance));
     }
+    if constexpr (LOGITS) {
+      // the best one that is not kept: those above it have to be apart from it, and, where one of its like is kept, those below it
+      const float most = warp_max(exists && !kept ? sum : kNone);
+      const bool like = __any_sync(kAll, kept && sum == most);
+      const bool counts = exists && sum > kNone && sum != most && (kept || like);
+      clear = !__any_sync(kAll, most > kNone && counts && !apart_in_64(a, fmaxf(sum, most), fminf(sum, most), top));
+    }
     if (whole) {
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -134,11 +150,11 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
     for (int s = N / 2; s > 0; s /= 2)
 #pragma unroll
       for (int i = 0; i < s; ++i) best[i] = best[i + s] > best[i] ? best[i + s] : best[i];
-    const Key top = warp_max(best[0]);
-    if (!(top > kNone)) break;  // none left
+    const Key most = warp_max(best[0]);
+    if (!(most > kNone)) break;  // none left
     if (tolerance > 0) {
-      if (j > 0 && close(before, top, tolerance)) clear = false;
-      before = top;
+      if (j > 0 && close(before, most, tolerance)) clear = false;
+      before = most;
       if (j == a.top_k) break;
     }
     // the lane's first place with it; of equal values, the one with the larger logit
@@ -146,14 +162,14 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
     float its = -INFINITY;
 #pragma unroll
     for (int i = N - 1; i >= 0; --i)
-      if (key[i] == top && (!kWide || x[i] >= its)) {
+      if (key[i] == most && (!kWide || x[i] >= its)) {
         place = i;
         its = x[i];
       }
     bool here = place >= 0;
     if constexpr (kWide) {
-      const float most = warp_max(its);
-      here = here && its == most;
+      const float larger = warp_max(its);
+      here = here && its == larger;
     }
     const int holder = __ffs(__ballot_sync(kAll, here)) - 1;
     const int e = __shfl_sync(kAll, lane * N + place, holder);
@@ -187,7 +203,14 @@ __device__ __noinline__ uint64_t choose_in_64(RouteArgs a, int token, float top)
       x[i] = counted(a.f16 ? __half2float(static_cast<const __half*>(a.logits)[at]) : static_cast<const float*>(a.logits)[at]);
     v[i] = 0.0;
     if (x[i] > -INFINITY) {
-      v[i] = a.sigmoid ? 1.0 / (1.0 + exp(-static_cast<double>(x[i]))) : exp(static_cast<double>(x[i]) - static_cast<double>(top));
+      if (a.sigmoid) {
+        v[i] = 1.0 / (1.0 + exp(-static_cast<double>(x[i])));
+      } else {
+        // (below the normal numbers as the square of one, which is rounded once: there exp's error may be all of a value)
+        const double y = static_cast<double>(x[i]) - static_cast<double>(top);
+        const double e = exp(y < -700.0 ? 0.5 * y : y);
+        v[i] = y < -700.0 ? e * e : e;
+      }
       sum += v[i];
     }
   }
@@ -203,7 +226,7 @@ __device__ __noinline__ uint64_t choose_in_64(RouteArgs a, int token, float top)
   }
   int id = -1;
   float logit = -INFINITY;
-  choose<double, N>(a, v, x, lane, 0.0f, id, logit);
+  choose<false, double, N>(a, v, x, lane, 0.0f, top, id, logit);
   return static_cast<uint64_t>(static_cast<uint32_t>(id)) << 32 | __float_as_uint(logit);
 }
 
@@ -261,6 +284,7 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a
   top = warp_max(top);
   int id = -1;
   float chosen = -INFINITY;  // lane j: the logit of the j-th
+  bool clear;
   if constexpr (VALUES) {
     float v[N], sum = 0.0f;
 #pragma unroll
@@ -282,16 +306,17 @@ __global__ void __launch_bounds__(kRouteWarps * 32) moe_route_kernel(RouteArgs a
     // Errors of two values: 2^-24 times 6 each of a sigmoid's score (exp 2, a sum, a quotient, the bias); N + 5 more of a softmax's
     // sum, which has 37 at most.
     const float tolerance = a.sigmoid ? 1.0e-6f : 6.0e-6f;
-    if (!choose<float, N>(a, v, x, lane, tolerance, id, chosen)) {
-      const uint64_t again = choose_in_64<N>(a, token, top);
-      id = static_cast<int>(again >> 32);
-      chosen = __uint_as_float(static_cast<uint32_t>(again));
-    }
+    clear = choose<false, float, N>(a, v, x, lane, tolerance, top, id, chosen);
   } else {
     float v[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = x[i];
-    choose<float, N>(a, v, x, lane, 0.0f, id, chosen);
+    clear = choose<true, float, N>(a, v, x, lane, 0.0f, top, id, chosen);
+  }
+  if (!clear) {
+    const uint64_t again = choose_in_64<N>(a, token, top);
+    id = static_cast<int>(again >> 32);
+    chosen = __uint_as_float(static_cast<uint32_t>(again));
   }
   // Their weights.  Renormalised, a softmax's sum cancels, and what is common to the chosen, too: they are taken against the largest
   // of them (of a sigmoid when all are so small that it is the exponential), so that they never vanish together.
