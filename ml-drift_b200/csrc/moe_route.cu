@@ -74,8 +74,9 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
     const auto worse = [](Key p, Key q) { return p < q ? p : q; };
     const int run = a.per_group / N;  // lanes of a group, if it is whole lanes
     const bool whole = a.per_group % N == 0 && (run & (run - 1)) == 0;
-    Key sum = kNone;      // of this lane's group (whole), or of group `lane`
+    Key sum = kNone, size = 0;  // of this lane's group (whole), or of group `lane`; the sum of its terms without their signs
     int group = lane;
+    const auto no_sign = [](Key v) { return v < 0 ? -v : v; };
     if (whole) {
       Key first = kNone, second = kNone;
 #pragma unroll
@@ -89,6 +90,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
         first = better(first, f);
       }
       sum = a.group_best == 2 ? first + second : first;
+      size = a.group_best == 2 ? no_sign(first) + no_sign(second) : no_sign(first);
       group = lane / run;
     } else {
       for (int g = 0; g < a.groups; ++g) {
@@ -101,13 +103,18 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
           first = better(first, k);
         }
         const Key best = warp_max(first);
-        Key s = best;
+        Key s = best, z = no_sign(best);
         if (a.group_best == 2) {
           // the largest once out of the way, of the first lane that has it
           const int holder = __ffs(__ballot_sync(kAll, first == best)) - 1;
-          s += warp_max(lane == holder ? second : first);
+          const Key next = warp_max(lane == holder ? second : first);
+          s += next;
+          z += no_sign(next);
         }
-        if (lane == g) sum = s;
+        if (lane == g) {
+          sum = s;
+          size = z;
+        }
       }
     }
     if (!(sum > kNone)) sum = kNone;  // (a NaN, too)
@@ -118,8 +125,13 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, Key (&key)[N], const 
     }
     const bool exists = group < a.groups, kept = exists && ahead < a.top_groups;
     if (tolerance > 0) {
-      const Key least = warp_min(kept ? sum : static_cast<Key>(INFINITY)), most = warp_max(exists && !kept ? sum : kNone);
-      clear = clear && !(most > kNone && close(least, most, 2 * tolerance));
+      // A sum is as exact as its terms, not as itself: of two sigmoids with their biases within 2^-24 (10 + 2 size), below the
+      // tolerance of 16.7 2^-24 (1 + size); a softmax's likewise.
+      const Key error = static_cast<Key>(tolerance) * (1 + size), kMost = static_cast<Key>(INFINITY);
+      const bool known = error < kMost;
+      const Key least = warp_min(!kept ? kMost : sum > kNone && !known ? kNone : sum - error);
+      const Key most = warp_max(!exists || kept || !(sum > kNone) ? kNone : known ? sum + error : kMost);
+      clear = !(most > kNone && !(least > most));
     }
     if constexpr (LOGITS) {
       // the best one that is not kept: those above it have to be apart from it, and, where one of its like is kept, those below it

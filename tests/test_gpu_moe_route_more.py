@@ -1,4 +1,4 @@
-"""Routing where values of groups tie, though logits do not: the same groups as in 64 bits."""
+"""Routing where values of groups tie or nearly do: the same groups as in 64 bits."""
 import numpy as np
 import pytest
 import torch
@@ -57,3 +57,16 @@ def test_groups_without_a_bias(mld, e, groups, dtype, sigmoid, values):
     score = mld.MOE_SIGMOID if sigmoid else mld.MOE_SOFTMAX
     for top_groups in (1, 2, groups - 1):
         _ids(mld, x.astype(dtype), None, min(4, top_groups * (e // groups)), score, groups, top_groups, 1)
+
+
+@pytest.mark.parametrize("large", [50.0, 5000.0, 3.0e7])
+def test_sums_of_two_values_of_opposite_signs(mld, large):
+    """A group's sum is small, its terms are not: it is as exact as those, not as itself."""
+    rng = np.random.default_rng(4)
+    n, e, groups = 500, 32, 4
+    spread = 30 * large * 2.0 ** -24
+    logits = (spread * rng.standard_normal((n, e))).astype(np.float32)
+    bias = np.full(e, -large, np.float32)
+    bias[np.arange(groups) * (e // groups) + [3, 0, 7, 5]] = large
+    _ids(mld, logits, bias, 1, mld.MOE_SIGMOID, groups, 1, 2)
+    _ids(mld, logits, bias, 1, mld.MOE_SOFTMAX, groups, 1, 2)
