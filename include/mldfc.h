@@ -373,7 +373,8 @@ MLD_API int mld_fc_run(mld_fc_plan* plan, const void* src, const void* weights,
  * and the zero point of a token's codes, value = code * scale + zero point, and
  * a third that is not read.  For operators with prefill_act_quant: 1 takes no
  * notice of zero points, 2 needs mld_fc_plan_set_weights_sum.  Runs the prefill
- * GEMM for any number of tokens; the weights, scales and sums must not be
+ * GEMM for any number of tokens, one included (not for a plan that force_path
+ * holds to the decode kernel); the weights, scales and sums must not be
  * written by launches of this library that may still be running (the
  * conversion functions above are not such launches). */
 MLD_API int mld_fc_run_codes(mld_fc_plan* plan, const int8_t* codes, const float* params, const void* weights,

@@ -362,12 +362,14 @@ int mld_fc_plan_create(const mld_fc_desc* d, mld_fc_plan** out) {
     }
     p->ws_bytes = sizeof(int);
   }
-  // An operator that may run as the prefill GEMM gets its operand workspace now, so that mld_fc_run never
+  // An operator that may run as the prefill GEMM gets its operand workspace now, so that no call ever
   // allocates: the K-major copy of the weights, the K-major (optionally quantised) activations and the
   // per-token quantisation parameters.
   MLD_REQUIRE(d->prefill_route >= MLD_PREFILL_ROUTE_AUTO && d->prefill_route <= MLD_PREFILL_ROUTE_INLINE_SMEM,
               "prefill_route out of range");
-  const bool may_gemm = d->force_path == 2 || (d->force_path == 0 && !mld_fc_is_gemv_recommended(d->precision, d->max_tokens));
+  // (with 8-bit activations: also what mld_fc_run_codes takes for a few tokens)
+  const bool may_gemm = d->force_path == 2 || (d->force_path == 0 && (d->prefill_act_quant != 0 ||
+                                                                      !mld_fc_is_gemv_recommended(d->precision, d->max_tokens)));
   if (may_gemm && d->precision != MLD_PRECISION_F32 && !d->has_zero_point) {
     const bool i8 = d->prefill_act_quant != 0;
     const size_t esz = i8 ? 1 : 2;

@@ -1,4 +1,4 @@
-"""Codes of rows whose values are large against their spread, and of rows at the ends of 32 bits."""
+"""Codes of rows whose values are large against their spread, and of rows at the ends of 32 bits; products on codes with small plans."""
 import numpy as np
 import pytest
 import torch
@@ -73,3 +73,31 @@ def test_spans_that_leave_32_bits_and_subnormal_ones(mld, w):
     _, v, rstd = ref.add_norm(x, None, g, 1e-6, 0.0)
     for symmetric in (True, False):
         assert np.array_equal(_codes(mld, x, g, 0.0, symmetric)[0], ref.codes(v, rstd, symmetric)[0])
+
+
+@pytest.mark.parametrize("most", [1, 4, 8, 16])
+@pytest.mark.parametrize("symmetric", [True, False])
+def test_products_on_codes_with_plans_of_few_tokens(mld, most, symmetric):
+    """A plan whose calls with fp16 activations all take the decode kernel serves codes, too."""
+    n, k = 264, 272
+    rng = np.random.default_rng(most)
+    wq = rng.integers(-128, 128, (n, k))
+    packed, sums = mld.pack_weights(_dev(wq.astype(np.int8)), (n, 1, 1, k), 8, want_sum=True)
+    scale = np.exp(0.3 * rng.standard_normal(n)).astype(np.float16)
+    for cached in (False, True):
+        plan = mld.FullyConnectedPlan(n, k, 8, max_tokens=most, src_layout=mld.LAYOUT_ROW_MAJOR, dst_layout=mld.LAYOUT_ROW_MAJOR,
+                                      prefill_act_quant=1 if symmetric else 2, cache_prepared_weights=cached)
+        plan.set_weights_sum(sums)
+        for tokens in {1, most}:
+            q = rng.integers(-128, 128, (tokens, k))
+            p = np.stack((rng.uniform(0.001, 0.002, tokens), np.zeros(tokens) if symmetric else rng.uniform(-0.1, 0.1, tokens), np.zeros(tokens)), 1)
+            p = p.astype(np.float32)
+            y = torch.empty(tokens, n, dtype=torch.float16, device="cuda")
+            plan.run_codes(_dev(q.astype(np.int8)), _dev(p), packed, _dev(scale), y, tokens)
+            p, s = p.astype(np.float64), scale.astype(np.float64)
+            want = (q @ wq.T * p[:, :1] + p[:, 1:2] * wq.sum(1)) * s
+            # exact sums of integers; four products and an addition in 32 bits, one rounding to fp16
+            size = (np.abs(q @ wq.T) * p[:, :1] + np.abs(p[:, 1:2] * wq.sum(1))) * s
+            bound = 8 * U32 * size + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+            assert (np.abs(y.cpu().numpy() - want) <= bound).all()
+        assert plan.device_status() == 0
