@@ -209,6 +209,7 @@ class FullyConnectedPlan:
                            max_tokens, force_path, device, prefill_act_quant, int(cache_prepared_weights), epilogue,
                            prefill_route, int(runtime_channel_bounds), int(has_batch_ids), int(exact_operands),
                            int(no_overlap), smem_limit_kb, int(independent_io))
+        self._codes_sizes = _codes_sizes(self.desc)
         self._h = C.c_void_p()
         _check(lib().mld_fc_plan_create(C.byref(self.desc), C.byref(self._h)), "mld_fc_plan_create")
 
@@ -242,11 +243,14 @@ class FullyConnectedPlan:
         """The product on activations that are quantised already: codes int8 [tokens][k rounded up to 16], params fp32 [tokens][3],
         as add_rms_norm makes them."""
         gpu, queue = _here(stream)
-        _codes(codes, params, tokens, self.desc.k, gpu)
-        if tokens > 1 and codes.stride(0) != div_up(self.desc.k, 16) * 16:
-            raise ValueError(f"codes: rows have to be {div_up(self.desc.k, 16) * 16} apart, these are {codes.stride(0)}")
-        rc = _lib.mld_fc_run_codes(self._h, codes.data_ptr(), params.data_ptr(), _addr(weights), _addr(scale), _addr(bias), _addr(dst),
-                                   tokens, queue)
+        k, apart, n_weights, n, n_bias, n_out = self._codes_sizes
+        stride = _codes(codes, params, tokens, k, gpu)
+        if stride != apart and tokens > 1:
+            raise ValueError(f"codes: rows have to be {apart} apart, these are {stride}")
+        rc = _lib.mld_fc_run_codes(self._h, codes.data_ptr(), params.data_ptr(), _room(weights, n_weights, torch.uint8, "weights", gpu),
+                                   _room(scale, n, torch.float16, "scale", gpu),
+                                   None if bias is None or not n_bias else _room(bias, n_bias, torch.float16, "bias", gpu),
+                                   _room(dst, tokens * n_out, torch.float16, "dst", gpu), tokens, queue)
         if rc != OK:
             _check(rc, "mld_fc_run_codes")
 
@@ -832,6 +836,22 @@ def _whole(t, elements, dtype, what, gpu):
         if t.get_device() != gpu:
             raise _elsewhere(t, what)
         raise ValueError(f"{what}: expected {elements} contiguous values of {dtype}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+def _codes_sizes(d):
+    """Of products on codes: inputs, values from row to row, and elements of the weights, scales, biases and a token's outputs."""
+    n4 = (d.n + 3) // 4 * 4
+    return (d.k, (d.k + 15) // 16 * 16, n4 * ((d.k + 3) // 4 * 4), d.n, n4 if d.has_bias else 0,
+            d.n if d.dst_layout == LAYOUT_ROW_MAJOR else n4)
+
+
+def _room(t, elements, dtype, what, gpu):
+    """The address of contiguous memory for that many elements, or more."""
+    if t.get_device() != gpu or t.dtype is not dtype or t.numel() < elements or not t.is_contiguous():
+        if t.get_device() != gpu:
+            raise _elsewhere(t, what)
+        raise ValueError(f"{what}: expected at least {elements} contiguous values of {dtype}, got {t.dtype} {tuple(t.shape)}")
     return t.data_ptr()
 
 

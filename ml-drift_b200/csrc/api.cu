@@ -689,12 +689,18 @@ int mld_fc_run_codes(mld_fc_plan* plan, const int8_t* codes, const float* params
   MLD_REQUIRE(!d.has_bias || bias != nullptr, "biases tensor missing");
   MLD_REQUIRE((reinterpret_cast<uintptr_t>(weights) & 15) == 0 && (reinterpret_cast<uintptr_t>(codes) & 15) == 0,
               "weights and codes must be 16-byte aligned");
-  MLD_REQUIRE((reinterpret_cast<uintptr_t>(params) & 3) == 0, "params must be aligned to their type");
+  MLD_REQUIRE((reinterpret_cast<uintptr_t>(params) & 3) == 0 && (reinterpret_cast<uintptr_t>(scale) & 1) == 0,
+              "params and scales must be aligned to their type");
+  MLD_REQUIRE((reinterpret_cast<uintptr_t>(dst) & (d.dst_layout == MLD_LAYOUT_SLICED ? 15 : 1)) == 0,
+              "dst must be aligned to its type, slices to 16 bytes");
   MLD_REQUIRE(d.epilogue == MLD_EPILOGUE_NONE, "codes are multiplied by the prefill GEMM, which has no fused SiLU*mul write");
   if (d.precision == MLD_PRECISION_F32 || get_encode_tiled() == nullptr) {
     set_last_error_text("quantised-activation prefill needs fp16 tensors and no zero points");
     return MLD_UNIMPLEMENTED;
   }
+  int current = -1;
+  MLD_CUDA_CHECK(cudaGetDevice(&current));
+  MLD_REQUIRE(current == plan->device, "the plan belongs to another device than the current one");
   return run_gemm(plan, nullptr, weights, scale, d.has_bias ? bias : nullptr, dst, tokens, static_cast<cudaStream_t>(stream_v),
                   nullptr, nullptr, codes, params);
 }
