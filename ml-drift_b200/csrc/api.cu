@@ -21,6 +21,7 @@ std::atomic<int64_t> g_launches{0};
 
 void set_last_error(const char* what, cudaError_t err) {
   g_last_error = std::string(what) + ": " + cudaGetErrorString(err);
+  cudaGetLastError();  // reported by this call: the check behind a later launch must not find it again
 }
 void set_last_error_text(const char* what) { g_last_error = what; }
 void count_launch(int n) { g_launches.fetch_add(n, std::memory_order_relaxed); }

@@ -52,3 +52,12 @@ def test_items_of_one_box_and_many_of_them(mld, d, f, bits, block):
     bound = ref.experts_bound(want, size, False)
     got = out.cpu().numpy().astype(np.float64)
     assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
+
+
+def test_a_plan_that_does_not_fit_leaves_no_error_behind(mld):
+    with pytest.raises(mld.MldError, match="experts' workspace"):
+        mld.MoeExperts(1024, 32, 32768, 32768, max_tokens=65536)  # 270 GB
+    logits = torch.zeros(3, 64, dtype=torch.float16, device="cuda")
+    ids, weights = torch.empty(3, 2, dtype=torch.int32, device="cuda"), torch.empty(3, 2, device="cuda")
+    mld.MoeRouter(64, 2).run(logits, ids, weights)
+    assert (ids.cpu() == torch.tensor([0, 1])).all()
