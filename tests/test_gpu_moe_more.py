@@ -54,6 +54,39 @@ def test_items_of_one_box_and_many_of_them(mld, d, f, bits, block):
     assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
 
 
+@pytest.mark.parametrize("path", ["few", "many"])
+@pytest.mark.parametrize("n", [1, 5, 70])
+def test_scales_of_256_inputs(mld, n, path):
+    e, k, d, f = 4, 2, 512, 256
+    (first, second), w = _few_matrices(7, d, f, 4, 256, e, e)
+    rng = np.random.default_rng(n)
+    x, gates = rng.standard_normal((n, d)).astype(np.float16), rng.random((n, k)).astype(np.float32)
+    ids = np.argsort(rng.random((n, e)), 1)[:, :k].astype(np.int32)
+    plan = mld.MoeExperts(e, k, d, f, block=256, max_tokens=n, force_path=mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS)
+    out = torch.empty(n, d, dtype=torch.float16, device="cuda")
+    plan.run(_dev(x), _dev(ids), _dev(gates), *w, out)
+    want, size = ref.experts(x, ids, gates, first, second, None, False)
+    assert (np.abs(out.cpu().numpy() - want) <= ref.experts_bound(want, size, path == "many")).all()
+    assert plan.device_status() == 0
+
+
+def test_a_call_goes_the_way_that_its_rows_to_an_expert_say(mld):
+    """Up to eight rows to an expert, on average, as a plan for few rows; more, as one for many: the same bits."""
+    e, k, d, f, n = 4, 2, 512, 256, 60
+    (first, second), w = _few_matrices(8, d, f, 4, 32, e, e)
+    rng = np.random.default_rng(3)
+    x, gates = _dev(rng.standard_normal((n, d)).astype(np.float16)), _dev(rng.random((n, k)).astype(np.float32))
+    ids = _dev(np.argsort(rng.random((n, e)), 1)[:, :k].astype(np.int32))
+    auto, few, many = (mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=p) for p in (0, mld.MOE_PATH_FEW_ROWS, mld.MOE_PATH_MANY_ROWS))
+    for rows in (1, 2, 15, 16, 17, 40, n):
+        outs = []
+        for plan in (auto, few, many):
+            outs.append(torch.empty(rows, d, dtype=torch.float16, device="cuda"))
+            plan.run(x[:rows], ids[:rows], gates[:rows], *w, outs[-1])
+        assert not torch.equal(outs[1], outs[2])  # (weights in 16 bits, and in their codes)
+        assert torch.equal(outs[0], outs[2 if rows * k > 8 * e else 1])
+
+
 def test_a_plan_that_does_not_fit_leaves_no_error_behind(mld):
     with pytest.raises(mld.MldError, match="experts' workspace"):
         mld.MoeExperts(1024, 32, 32768, 32768, max_tokens=65536)  # 270 GB
