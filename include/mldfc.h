@@ -371,7 +371,8 @@ MLD_API int mld_fc_run(mld_fc_plan* plan, const void* src, const void* weights,
  * for instance: codes int8 [tokens] rows of k values rounded up to a multiple of
  * 16 (zeros behind a row), 16-byte aligned; params fp32 [tokens][3]: the scale
  * and the zero point of a token's codes, value = code * scale + zero point, and
- * a third that is not read.  For operators with prefill_act_quant: 1 takes no
+ * a third that is not read.  Outputs are rounded to fp16 once, behind the bias
+ * (mld_fc_run rounds ahead of it, too).  For operators with prefill_act_quant: 1 takes no
  * notice of zero points, 2 needs mld_fc_plan_set_weights_sum.  Runs the prefill
  * GEMM for any number of tokens, one included (not for a plan that force_path
  * holds to the decode kernel); the weights, scales and sums must not be

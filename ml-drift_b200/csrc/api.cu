@@ -573,7 +573,8 @@ static int run_stream(mld_fc_plan* p, const StripGeometry& gm, const void* src, 
 // bytes, into tensor memory (gemm_wtmem_kernel); with cache_prepared_weights, where convert_pays says so, or for a weight
 // matrix whose row pitch a tensor map cannot express, the weights are first expanded to a K-major copy (kept between calls
 // when cached) and a plain GEMM runs on that.
-// codes, params != null: the activations quantised already, rows of K rounded up to 16 bytes (then src is not read).
+// codes, params != null: the activations quantised already, rows of K rounded up to 16 bytes (then src is not read); the bias is
+// added in 32 bits then.
 static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const void* scale, const void* bias,
                     void* dst, int tokens, cudaStream_t stream, const PeerOutputs* outs, bool* outs_used,
                     const int8_t* codes = nullptr, const float* params = nullptr) {
@@ -611,7 +612,7 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     return launch_gemm_wtmem(mode, x_kmajor, weights, wg, tokens, d.n, d.k, scale, d.scale_mode,
                              d.scale_mode == MLD_SCALE_BLOCK ? d.groups : 1, p->group_slices, d.scalar_scale, bias,
                              a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream, outs,
-                             &p->split);
+                             &p->split, codes != nullptr);
   }
   if (!convert) {
     p->last_route = MLD_ROUTE_PREFILL_INLINE;
@@ -629,7 +630,7 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     return launch_gemm_pair(mode, x_kmajor, weights, pg, tokens, d.n, d.k, scale, d.scale_mode,
                             d.scale_mode == MLD_SCALE_BLOCK ? d.groups : 1, p->group_slices, d.scalar_scale, bias,
                             a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err, stream,
-                            outs, &p->split);
+                            outs, &p->split, codes != nullptr);
   }
 
   const GemmGeometry g = gemm_geometry(tokens, d.n, d.k, i8, p->sms);
@@ -663,7 +664,7 @@ static int run_gemm(mld_fc_plan* p, const void* src, const void* weights, const 
     if (pg.kp == g.kp)
       return launch_gemm_pair(mode, x_kmajor, p->w_kmajor, pg, tokens, d.n, d.k, scale, d.scale_mode, 1, 1, 0.0f,
                               bias, a_params, d.prefill_act_quant == 2 ? p->w_sum : nullptr, dst, d.dst_layout, err,
-                              stream, outs, &p->split);
+                              stream, outs, &p->split, codes != nullptr);
   }
   if (d.prefill_act_quant == 2) {
     set_last_error_text("asymmetric int8 activations are served by the SM-pair GEMM only");

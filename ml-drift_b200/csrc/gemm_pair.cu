@@ -52,7 +52,8 @@
 namespace mld {
 namespace {
 
-template <int MODE>
+// BIAS32: the bias is added ahead of the rounding (int8 activations).
+template <int MODE, bool BIAS32 = false>
 __global__ void __launch_bounds__(kPairThreads, 1)
     gemm_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_w, PairArgs a) {
   constexpr bool I8 = MODE == kModeInt8I8 || MODE == kModePreparedI8;
@@ -359,9 +360,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           for (int j = 0; j < 32; j += 4) {
             const int n = n0 + c0 + j;
             if (c0 + j >= a.tile_n || n >= a.N4) break;
+            if constexpr (BIAS32) {
+              const uint2 bv = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(a.bias) + n));
+              const float2 b01 = __half22float2(*reinterpret_cast<const __half2*>(&bv.x)), b23 = __half22float2(*reinterpret_cast<const __half2*>(&bv.y));
+              r[j] = __float_as_uint(__uint_as_float(r[j]) + b01.x);
+              r[j + 1] = __float_as_uint(__uint_as_float(r[j + 1]) + b01.y);
+              r[j + 2] = __float_as_uint(__uint_as_float(r[j + 2]) + b23.x);
+              r[j + 3] = __float_as_uint(__uint_as_float(r[j + 3]) + b23.y);
+            }
             __half2 h01 = __floats2half2_rn(__uint_as_float(r[j]), __uint_as_float(r[j + 1]));
             __half2 h23 = __floats2half2_rn(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3]));
-            if (a.bias != nullptr) {  // [N4] halves: the four of this column block in one load
+            if (!BIAS32 && a.bias != nullptr) {  // [N4] halves: the four of this column block in one load
               const uint2 bv = __ldg(reinterpret_cast<const uint2*>(static_cast<const __half*>(a.bias) + n));
               h01 = __hadd2(h01, *reinterpret_cast<const __half2*>(&bv.x));
               h23 = __hadd2(h23, *reinterpret_cast<const __half2*>(&bv.y));
@@ -736,7 +745,7 @@ PairGeometry pair_geometry(int M, int N, int K, int mode, int sms, bool may_shar
 int launch_gemm_pair(int mode, const void* a_mat, const void* packed, const PairGeometry& g, int M, int N, int K,
                      const void* scale, int scale_mode, int G, int group_slices, float scalar_scale, const void* bias,
                      const float* a_params, const int32_t* w_sum, void* y, int dst_layout, int* error,
-                     cudaStream_t stream, const PeerOutputs* outs, const PairSplit* split) {
+                     cudaStream_t stream, const PeerOutputs* outs, const PairSplit* split, bool bias_in_32) {
   if (g.shares_tiles && (split == nullptr || split->ws == nullptr || split->flags == nullptr || split->epoch == 0)) {
     set_last_error_text("this GEMM geometry shares tiles between SM pairs and needs a split workspace");
     return MLD_INVALID_ARGUMENT;
@@ -809,11 +818,14 @@ int launch_gemm_pair(int mode, const void* a_mat, const void* packed, const Pair
     case kModePreparedI8: kern = gemm_pair_kernel<kModePreparedI8>; break;
     default: set_last_error_text("bad GEMM mode"); return MLD_INVALID_ARGUMENT;
   }
-  static bool configured[5][kMaxDevices];
+  const bool wide = i8 && bias_in_32 && bias != nullptr;
+  if (wide) kern = prepared ? gemm_pair_kernel<kModePreparedI8, true> : gemm_pair_kernel<kModeInt8I8, true>;
+  static bool configured[10][kMaxDevices];
+  bool(&done)[kMaxDevices] = configured[wide ? 5 + mode : mode];
   int dev;
-  if (needs_configure(configured[mode], &dev)) {
+  if (needs_configure(done, &dev)) {
     MLD_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
-    if (dev >= 0) configured[mode][dev] = true;
+    if (dev >= 0) done[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(g.grid, 1, 1);

@@ -109,7 +109,8 @@ __device__ __forceinline__ void turn_blocks(uint32_t w0, uint32_t w1, const Turn
   o0 = __byte_perm(k1, r1, t.out0) ^ 0x80808080u;
   o1 = __byte_perm(k1, r1, t.out1) ^ 0x80808080u;
 }
-template <int MODE, bool PAIR>
+// BIAS32: the bias is added ahead of the rounding (int8 activations).
+template <int MODE, bool PAIR, bool BIAS32 = false>
 __global__ void __launch_bounds__(kWtThreads, 1)
     gemm_wtmem_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, WtArgs wa) {
   const PairArgs& a = wa.p;
@@ -299,6 +300,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
           const float a_scale = __shfl_sync(0xffffffffu, mine, j), a_off = __shfl_sync(0xffffffffu, mine, 16 + j);
           float v = static_cast<float>(static_cast<int32_t>(r[j])) * (w_scale * a_scale);
           if (a.w_sum != nullptr) v += w_scale * a_off * w_offset;
+          if constexpr (BIAS32) v += __half2float(bias_h);
           r[j] = __float_as_uint(v);
         }
       }
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kWtThreads, 1)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         __half2 v = __floats2half2_rn(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-        if (a.bias != nullptr) v = __hadd2(v, __half2half2(bias_h));
+        if (!BIAS32 && a.bias != nullptr) v = __hadd2(v, __half2half2(bias_h));
         h2[i] = *reinterpret_cast<const uint32_t*>(&v);
       }
       if (a.dst_layout == MLD_LAYOUT_SLICED || rows_of_4) {
@@ -762,7 +764,7 @@ WtGeometry wtmem_geometry(int M, int N, int K, int mode, int sms, bool may_share
 int launch_gemm_wtmem(int mode, const void* x_kmajor, const void* packed, const WtGeometry& g, int M, int N, int K,
                       const void* scale, int scale_mode, int G, int group_slices, float scalar_scale, const void* bias,
                       const float* a_params, const int32_t* w_sum, void* y, int dst_layout, int* error, cudaStream_t stream,
-                      const PeerOutputs* outs, const PairSplit* split) {
+                      const PeerOutputs* outs, const PairSplit* split, bool bias_in_32) {
   if (mode != kModeInt4F16 && mode != kModeInt8F16 && mode != kModeInt8I8) {
     set_last_error_text("bad GEMM mode");
     return MLD_INVALID_ARGUMENT;
@@ -830,8 +832,10 @@ int launch_gemm_wtmem(int mode, const void* x_kmajor, const void* packed, const 
                   : (mode == kModeInt4F16   ? gemm_wtmem_kernel<kModeInt4F16, false>
                      : mode == kModeInt8F16 ? gemm_wtmem_kernel<kModeInt8F16, false>
                                             : gemm_wtmem_kernel<kModeInt8I8, false>);
-  static bool configured[2][3][kMaxDevices];
-  bool(&done)[kMaxDevices] = configured[g.ctas - 1][mode];
+  const bool wide = i8 && bias_in_32 && bias != nullptr;
+  if (wide) kern = g.ctas == 2 ? gemm_wtmem_kernel<kModeInt8I8, true, true> : gemm_wtmem_kernel<kModeInt8I8, false, true>;
+  static bool configured[2][4][kMaxDevices];
+  bool(&done)[kMaxDevices] = configured[g.ctas - 1][wide ? 3 : mode];
   int dev;
   if (needs_configure(done, &dev)) {
     MLD_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));

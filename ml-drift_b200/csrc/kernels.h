@@ -227,12 +227,15 @@ inline size_t pair_split_flags(int sms) { return (size_t)(sms / 2 > 0 ? sms / 2 
 // mode: 0 = INT4 weights -> fp16 MMA, 1 = INT8 weights -> fp16 MMA, 2 = INT8 weights x int8 activations (packed
 // weights, transformed in shared memory); 3 / 4 = weights prepared as K-major fp16 / s8 rows [N4][kp] by
 // launch_dequant_weights (then `packed` is that matrix)
+// bias_in_32 (int8 activations): the bias is added ahead of the one rounding to fp16; else the product is rounded, and the sum again.
+// (A kernel of its own: asked for at run time, the unused way cost a call of 25 us 0.4 us, prepared weights up to 5 of 100.)
 // may_share: a PairSplit workspace will be passed to the launch, so tile waves need not be whole
 PairGeometry pair_geometry(int M, int N, int K, int mode, int sms, bool may_share = false);
 int launch_gemm_pair(int mode, const void* a_mat, const void* packed, const PairGeometry& g, int M, int N, int K,
                      const void* scale, int scale_mode, int G, int group_slices, float scalar_scale, const void* bias,
                      const float* a_params, const int32_t* w_sum, void* y, int dst_layout, int* error,
-                     cudaStream_t stream, const PeerOutputs* outs = nullptr, const PairSplit* split = nullptr);
+                     cudaStream_t stream, const PeerOutputs* outs = nullptr, const PairSplit* split = nullptr,
+                     bool bias_in_32 = false);
 
 // ------------------------------------------- prefill GEMM, dequantised weights in tensor memory (SM pairs)
 struct WtGeometry {
@@ -248,6 +251,6 @@ WtGeometry wtmem_geometry(int M, int N, int K, int mode, int sms, bool may_share
 int launch_gemm_wtmem(int mode, const void* x_kmajor, const void* packed, const WtGeometry& g, int M, int N, int K,
                       const void* scale, int scale_mode, int G, int group_slices, float scalar_scale, const void* bias,
                       const float* a_params, const int32_t* w_sum, void* y, int dst_layout, int* error, cudaStream_t stream,
-                      const PeerOutputs* outs = nullptr, const PairSplit* split = nullptr);
+                      const PeerOutputs* outs = nullptr, const PairSplit* split = nullptr, bool bias_in_32 = false);
 
 }  // namespace mld

@@ -101,3 +101,34 @@ def test_products_on_codes_with_plans_of_few_tokens(mld, most, symmetric):
             bound = 8 * U32 * size + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
             assert (np.abs(y.cpu().numpy() - want) <= bound).all()
         assert plan.device_status() == 0
+
+
+@pytest.mark.parametrize("tokens,k,n", [(1, 256, 64), (77, 272, 568), (130, 1040, 262), (513, 512, 1024)])
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("route", ["tensor memory", "shared memory", "prepared"])
+@pytest.mark.parametrize("row_major", [True, False])
+def test_outputs_are_rounded_once(mld, tokens, k, n, symmetric, route, row_major):
+    rng = np.random.default_rng(tokens + k)
+    wq = rng.integers(-128, 128, (n, k))
+    packed, sums = mld.pack_weights(_dev(wq.astype(np.int8)), (n, 1, 1, k), 8, want_sum=True)
+    n4 = (n + 3) // 4 * 4
+    scale, bias = np.zeros(n4, np.float16), np.zeros(n4, np.float16)
+    scale[:n], bias[:n] = np.exp(0.3 * rng.standard_normal(n)) / (70 * np.sqrt(k)), rng.standard_normal(n)
+    plan = mld.FullyConnectedPlan(n, k, 8, has_bias=True, max_tokens=tokens, src_layout=mld.LAYOUT_ROW_MAJOR, force_path=mld.PATH_GEMM,
+                                  dst_layout=mld.LAYOUT_ROW_MAJOR if row_major else mld.LAYOUT_SLICED, prefill_act_quant=1 if symmetric else 2,
+                                  cache_prepared_weights=route == "prepared", prefill_route=dict(zip(("tensor memory", "prepared", "shared memory"), (1, 0, 3)))[route])
+    plan.set_weights_sum(sums)
+    q = rng.integers(-128, 128, (tokens, (k + 15) // 16 * 16))
+    q[:, k:] = 0
+    p = np.stack((rng.uniform(0.01, 0.02, tokens), np.zeros(tokens) if symmetric else rng.uniform(-1, 1, tokens), np.zeros(tokens)), 1).astype(np.float32)
+    y = torch.full((tokens, n) if row_major else (n4 // 4, tokens, 4), 9.0, dtype=torch.float16, device="cuda")
+    plan.run_codes(_dev(q.astype(np.int8)), _dev(p), packed, _dev(scale), y, tokens, bias=_dev(bias))
+    assert plan.device_status() == 0
+    got = y.cpu().numpy().astype(np.float64) if row_major else y.cpu().numpy().astype(np.float64).transpose(1, 0, 2).reshape(tokens, n4)[:, :n]
+    s, b, p = scale[:n].astype(np.float64), bias[:n].astype(np.float64), p.astype(np.float64)
+    product, zero = q[:, :k] @ wq.T * p[:, :1] * s, p[:, 1:2] * wq.sum(1) * s
+    want = product + zero + b
+    # exact sums of integers below 2^24; at most six roundings of 32 bits of each term (the sums as 32-bit numbers, products, additions),
+    # and one to fp16
+    bound = 6 * U32 * (np.abs(product) + np.abs(zero) + np.abs(b)) + 2.0 ** -11 * np.abs(want) + 2.0 ** -25
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
