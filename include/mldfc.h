@@ -495,8 +495,10 @@ typedef enum mld_moe_path {
  * [experts][inputs / block][outputs].
  * Products are summed in 32 bits.  act(..) * (..) is rounded to fp16 for the
  * second product; with many rows, weights are rounded to fp16 as
- * FullyConnected's prefill does and down_e(..) is, too, ahead of the sum over j,
- * which is in 32 bits and in the order of j: the same call gives the same bits. */
+ * FullyConnected's prefill does and weights_tj down_e(..) is, too, ahead of the
+ * sum over j, which is in 32 bits and in the order of j: the same call gives the
+ * same bits.  (A gated value above 65504 is infinite, and, with many rows, such a
+ * term of the sum.) */
 typedef struct mld_moe_desc {
   int32_t experts;           /* 1 to 1024 */
   int32_t top_k;             /* places of a token in ids, 1 to 32 */

@@ -119,13 +119,16 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const int32_t* _
   if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Rows of x in the order of positions, a warp to a row.
-__global__ void __launch_bounds__(256) moe_gather_kernel(const __half* __restrict__ x, int64_t x_stride, int top_k, int width, MoeBuffers b) {
+// Rows of x and their weights in the order of positions, a warp to a row.
+__global__ void __launch_bounds__(256) moe_gather_kernel(const __half* __restrict__ x, int64_t x_stride, const float* __restrict__ weights,
+                                                          int top_k, int width, MoeBuffers b) {
   pdl_wait();
   pdl_launch_dependents();
   const int at = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (at >= b.n_tiles[1]) return;
-  const uint4* from = reinterpret_cast<const uint4*>(x + b.order[at] / top_k * x_stride);
+  const int pair = b.order[at];
+  if (lane == 0) b.gates[at] = weights[pair];
+  const uint4* from = reinterpret_cast<const uint4*>(x + pair / top_k * x_stride);
   uint4* to = reinterpret_cast<uint4*>(static_cast<__half*>(b.sorted) + static_cast<int64_t>(at) * width);
 #pragma unroll 4
   for (int c = lane; c < width / 8; c += 32) to[c] = from[c];
@@ -142,7 +145,8 @@ struct SumArgs {
   int experts, top_k, width;
 };
 
-// out = residual + sum_j weight_j part_j, in the order of j.  A block takes a token, a thread eight neighbours.
+// out = residual + sum_j weight_j part_j, in the order of j (fp16 parts come weighted).  A block takes a token, a thread eight
+// neighbours.
 template <typename P>
 __global__ void __launch_bounds__(256) moe_sum_kernel(SumArgs a) {
   pdl_wait();
@@ -164,7 +168,7 @@ __global__ void __launch_bounds__(256) moe_sum_kernel(SumArgs a) {
       const int pair = token * a.top_k + j;
       const int at = a.ids == nullptr ? a.b.position[pair] : static_cast<unsigned>(a.ids[j]) < static_cast<unsigned>(a.experts) ? j : -1;
       if (at < 0) continue;
-      const float w = a.weights[pair];
+      const float w = sizeof(P) == 4 ? a.weights[pair] : 1.0f;
       const P* p = static_cast<const P*>(a.b.part) + static_cast<int64_t>(at) * a.width + c;
       if constexpr (sizeof(P) == 4) {
         const float4 lo = *reinterpret_cast<const float4*>(p), hi = *reinterpret_cast<const float4*>(p + 4);
@@ -175,8 +179,8 @@ __global__ void __launch_bounds__(256) moe_sum_kernel(SumArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float2 f = __half22float2(reinterpret_cast<const __half2*>(&h)[i]);
-          v[2 * i] += w * f.x;
-          v[2 * i + 1] += w * f.y;
+          v[2 * i] += f.x;
+          v[2 * i + 1] += f.y;
         }
       }
     }
@@ -271,7 +275,8 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
     return here;
   };
   const size_t control = room(kControlBytes), order = room(pairs * 4), position = room(pairs * 4),
-               tiles = room(most_tiles(static_cast<int>(pairs), d->experts, kMoeFewRows) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2), rows = room(shared);
+               tiles = room(most_tiles(static_cast<int>(pairs), d->experts, kMoeFewRows) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2), rows = room(shared),
+               gates = room(may_many ? pairs * 4 : 0);
   int before = -1;
   cudaError_t e = cudaGetDevice(&before);
   if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
@@ -291,6 +296,7 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   p->b.position = reinterpret_cast<int*>(p->memory + position);
   p->b.tiles = reinterpret_cast<MoeTile*>(p->memory + tiles);
   p->b.hidden = p->memory + hidden;
+  p->b.gates = reinterpret_cast<float*>(p->memory + gates);
   p->b.part = p->b.sorted = p->memory + rows;
   *out = p;
   return MLD_OK;
@@ -368,7 +374,7 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
     rc = launch_sort(io->ids, pairs, d.experts, rows, true, plan->b, stream);
     if (rc != MLD_OK) return rc;
     MLD_CUDA_CHECK(launch_overlapped(moe_gather_kernel, dim3(div_up(pairs, 8)), dim3(256), 0, stream, static_cast<const __half*>(io->x),
-                                     io->x_stride, d.top_k, d.d_model, plan->b));
+                                     io->x_stride, io->weights, d.top_k, d.d_model, plan->b));
     MLD_LAUNCH_CHECK();
     rc = launch_moe_gemm(true, shape, plan->b, io->gate_up, io->gate_up_scale, pairs, plan->sms, stream);
     if (rc == MLD_OK) rc = launch_moe_gemm(false, shape, plan->b, io->down, io->down_scale, pairs, plan->sms, stream);

@@ -8,7 +8,7 @@
 //     rows, and the MMAs' N is that many, too (in steps of 64).  Columns behind the tile's rows belong to other experts, or are
 //     zeros, and are not written.
 //   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
-//     and an up channel, exchange half of their tokens; of the second the expert's output.
+//     and an up channel, exchange half of their tokens; of the second the expert's output times the row's weight.
 // Per CTA: warps 0 and 23 fetch rows, every other stage each, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first
 // CTA), warps 6..21 dequantise (four to a stage of 128 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights
 // and two halves of 128 columns of accumulators.  A tile of up to 128 rows takes the half that is free, and the next tile goes on
@@ -54,7 +54,8 @@ struct GemmArgs {
   const __half* scale;
   int64_t expert_scales;
   int groups, group_shift;              // log2 of a group's input slices
-  __half* out;                          // rows by position: act(gate) * up [n / 2], or [n]
+  __half* out;                          // rows by position: act(gate) * up [n / 2], or, times the row's weight, [n]
+  const float* gates;                   // the rows' weights
   int activation;
   int* error;
 };
@@ -189,13 +190,27 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t full_ab_lead = map_shared(smem_u32(full_ab), 0), tmem_empty_lead = map_shared(smem_u32(tmem_empty), 0);
 
-  const auto drain = [&](const MoeTile& tile, int n0, int part, const Turns& turn) {
+  // The weights of the rows that a warp is going to write, of two pieces of 16 rows to a register: eight pieces at most of a tile that
+  // it writes alone, else four.  Asked for ahead of the wait for the products.  (A load to a piece took 2048 tokens through 8 of 64
+  // experts 2 us longer.)
+  const auto weights_of = [&](const MoeTile& tile, int part, int parts, auto& w) {
+    if constexpr (!FIRST) {
+#pragma unroll
+      for (int i = 0; i < static_cast<int>(sizeof w / 4); ++i) {
+        const int m = 16 * (part + parts * (2 * i + (lane >> 4))) + (lane & 15);
+        w[i] = m < tile.rows ? a.gates[tile.row0 + m] : 0.0f;
+      }
+    }
+  };
+  static_assert(kHalf <= 8 * 16 && kMoeTileRows <= 4 * 16 * kReaders, "rows of a warp");
+  const auto drain = [&](const MoeTile& tile, int n0, int part, const Turns& turn, auto& weights) {
     const int parts = turn.all ? kReaders : 1;
     const int quad = warp & 3;
     const uint32_t base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(turn.at * kHalf);
     const int n = n0 + static_cast<int>(rank) * kChannels + quad * 32;  // the warp's first channel
     const bool has_n = n < a.n;                                         // (a.n is a multiple of 32)
     const int pieces = (tile.rows + 15) >> 4;
+    [[maybe_unused]] int from = 0;  // the lane with the weight of the piece's first row
     for (int pc = part; pc < pieces; pc += parts) {
       uint32_t r[16];
       tmem_ld16(base + static_cast<uint32_t>(16 * pc), r);
@@ -225,7 +240,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         uint32_t x[8];
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-          const __half2 h = __floats2half2_rn(__uint_as_float(r[2 * p]), __uint_as_float(r[2 * p + 1]));
+          const float w0 = __shfl_sync(0xffffffffu, weights[0], from + 2 * p), w1 = __shfl_sync(0xffffffffu, weights[0], from + 2 * p + 1);
+          const __half2 h = __floats2half2_rn(__uint_as_float(r[2 * p]) * w0, __uint_as_float(r[2 * p + 1]) * w1);
           x[p] = *reinterpret_cast<const uint32_t*>(&h);
         }
         const int q = lane & 3;
@@ -235,6 +251,11 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           const int m = 16 * pc + 8 * h + 2 * q;
           __half* to = a.out + static_cast<int64_t>(tile.row0 + m) * a.n + n + (lane >> 2) * 4;
           store_pair(to, a.n, has_n && m < tile.rows, has_n && m + 1 < tile.rows, x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
+        }
+        from ^= 16;
+        if (from == 0) {
+#pragma unroll
+          for (int i = 0; i + 1 < static_cast<int>(sizeof weights / 4); ++i) weights[i] = weights[i + 1];
         }
       }
     }
@@ -331,12 +352,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     int n0;
     for (Turns turn; work.next(tile, n0); turn.next()) {
       turn.take(tile, work.done());
+      float weights[4];
+      weights_of(tile, 0, turn.all ? kReaders : 1, weights);
       if (!mbar_wait(&tmem_full[turn.full()], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 4);
         break;
       }
       tc_after();
-      drain(tile, n0, 0, turn);
+      drain(tile, n0, 0, turn, weights);
     }
   } else if (warp == 22) {
     // --------------------------------------------------------- packed weights
@@ -480,12 +503,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       before += a.k_blocks;
       if (!ok) break;
       if (!turn.all) continue;
+      float weights[2];
+      weights_of(tile, 1 + group, kReaders, weights);
       if (!mbar_wait(&tmem_full[2], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 7);
         break;
       }
       tc_after();
-      drain(tile, n0, 1 + group, turn);
+      drain(tile, n0, 1 + group, turn, weights);
     }
   }
   // Nobody leaves while the partner may still arrive on this CTA's barriers or the pair's MMAs write its tensor memory.
@@ -546,6 +571,7 @@ int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const vo
     for (a.group_shift = 3; (4 << a.group_shift) < s.block;) ++a.group_shift;
   a.expert_scales = static_cast<int64_t>(a.groups) * n;
   a.out = static_cast<__half*>(first ? b.hidden : b.part);
+  a.gates = b.gates;
   a.activation = s.activation;
   a.error = b.error;
   const int grid = sms / 2 * 2;

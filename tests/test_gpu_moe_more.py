@@ -94,3 +94,34 @@ def test_a_plan_that_does_not_fit_leaves_no_error_behind(mld):
     ids, weights = torch.empty(3, 2, dtype=torch.int32, device="cuda"), torch.empty(3, 2, device="cuda")
     mld.MoeRouter(64, 2).run(logits, ids, weights)
     assert (ids.cpu() == torch.tensor([0, 1])).all()
+
+
+@pytest.mark.parametrize("path", ["few", "many"])
+@pytest.mark.parametrize("n", [1, 40, 300])
+@pytest.mark.parametrize("large", [1.0, 3.0e4])
+def test_outputs_of_experts_that_leave_16_bits_ahead_of_their_weights(mld, n, path, large):
+    """Experts' outputs of a few hundred thousands, weights that bring the sums back: the same range, however many tokens come along."""
+    e, k, d, f = 4, 2, 256, 128
+    (first, second), (w1, s1, w2, s2) = _few_matrices(9, d, f, 4, 32, e, e)
+    s2 = (s2.double() * large).half()
+    second = np.rint(second / _spread(_few_matrices(9, d, f, 4, 32, e, e)[1][3], f)) * _spread(s2, f)
+    rng = np.random.default_rng(n)
+    x, gates = rng.standard_normal((n, d)).astype(np.float16), (rng.random((n, k)) / large).astype(np.float32)
+    gates[:, 0] *= -1
+    gates[0] = 0
+    ids = np.argsort(rng.random((n, e)), 1)[:, :k].astype(np.int32)
+    res = rng.standard_normal((n, d)).astype(np.float16)
+    plan = mld.MoeExperts(e, k, d, f, max_tokens=n, force_path=mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS)
+    out = torch.empty(n, d, dtype=torch.float16, device="cuda")
+    plan.run(_dev(x), _dev(ids), _dev(gates), w1, s1, w2, s2, out, residual=_dev(res))
+    want, size = ref.experts(x, ids, gates, first, second, res, False)
+    got = out.cpu().numpy().astype(np.float64)
+    bound = ref.experts_bound(want, size, path == "many")
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
+    assert np.array_equal(got[0], res[0])
+
+
+def _spread(scales, inputs):
+    """Scales [experts][groups][outputs] for each of the inputs, [experts][outputs][inputs]."""
+    s = scales.double().cpu().numpy()
+    return np.repeat(s, inputs // s.shape[1], 1).transpose(0, 2, 1)
