@@ -884,8 +884,8 @@ def add_rms_norm(x, weight=None, residual=None, sum_out=None, out=None, codes=No
         s, ss = sum_out.data_ptr(), _table(sum_out, shape, dt, "sum_out", gpu)
     if out is not None:
         o, os_ = out.data_ptr(), _table(out, shape, dt, "out", gpu)
-    if codes is not None:
-        if params is None:
+    if codes is not None or params is not None:
+        if codes is None or params is None:
             raise ValueError("codes and params go together")
         q, qs, p = codes.data_ptr(), _codes(codes, params, n, w, gpu), params.data_ptr()
     rc = (_lib or lib()).mld_add_rms_norm(C.byref(d), C.byref(AddNormIo(x.data_ptr(), xs, r, rs, g, s, ss, o, os_, q, qs, p)), n, queue)
