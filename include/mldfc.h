@@ -494,11 +494,10 @@ typedef enum mld_moe_path {
  * and d_model inputs, down d_model outputs and ffn inputs; scales fp16
  * [experts][inputs / block][outputs].
  * Products are summed in 32 bits.  act(..) * (..) is rounded to fp16 for the
- * second product; with many rows, weights are rounded to fp16 as
- * FullyConnected's prefill does and weights_tj down_e(..) is, too, ahead of the
- * sum over j, which is in 32 bits and in the order of j: the same call gives the
- * same bits.  (A gated value above 65504 is infinite, and, with many rows, such a
- * term of the sum.) */
+ * second product (one above 65504 is infinite).  With many rows and scales to
+ * blocks of inputs, weights are rounded to fp16 as FullyConnected's prefill does,
+ * and weights_tj down_e(..) is, too, ahead of the sum over j, which is in 32 bits
+ * and in the order of j: the same call gives the same bits. */
 typedef struct mld_moe_desc {
   int32_t experts;           /* 1 to 1024 */
   int32_t top_k;             /* places of a token in ids, 1 to 32 */

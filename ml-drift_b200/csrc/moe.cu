@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(256) moe_gather_kernel(const __half* __restric
   const int at = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (at >= b.n_tiles[1]) return;
   const int pair = b.order[at];
-  if (lane == 0) b.gates[at] = weights[pair];
+  if (lane == 0 && b.gates != nullptr) b.gates[at] = weights[pair];
   const uint4* from = reinterpret_cast<const uint4*>(x + pair / top_k * x_stride);
   uint4* to = reinterpret_cast<uint4*>(static_cast<__half*>(b.sorted) + static_cast<int64_t>(at) * width);
 #pragma unroll 4
@@ -267,7 +267,8 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   const size_t pairs = static_cast<size_t>(d->max_tokens) * d->top_k;
   const bool may_many = takes_many(*d, d->max_tokens);
   const size_t few = d->force_path == MLD_MOE_PATH_FEW_ROWS || !may_many ? pairs : d->force_path == MLD_MOE_PATH_AUTO ? kFewShare * static_cast<size_t>(d->experts) : 0;
-  const size_t width = static_cast<size_t>(d->d_model), shared = may_many && pairs * width * 2 > few * width * 4 ? pairs * width * 2 : few * width * 4;
+  const size_t width = static_cast<size_t>(d->d_model), most = may_many ? pairs * width * (moe_weighted_parts(d->block) ? 2 : 4) : 0, shared = most > few * width * 4 ? most : few * width * 4;
+  const bool weighted = may_many && moe_weighted_parts(d->block);
   size_t at = 0;
   const auto room = [&](size_t bytes) {
     const size_t here = at;
@@ -276,7 +277,7 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   };
   const size_t control = room(kControlBytes), order = room(pairs * 4), position = room(pairs * 4),
                tiles = room(most_tiles(static_cast<int>(pairs), d->experts, kMoeFewRows) * sizeof(MoeTile)), hidden = room(pairs * d->ffn * 2), rows = room(shared),
-               gates = room(may_many ? pairs * 4 : 0);
+               gates = room(weighted ? pairs * 4 : 0);
   int before = -1;
   cudaError_t e = cudaGetDevice(&before);
   if (e == cudaSuccess && before != device) e = cudaSetDevice(device);
@@ -296,7 +297,7 @@ int mld_moe_plan_create(const mld_moe_desc* d, mld_moe_plan** out) {
   p->b.position = reinterpret_cast<int*>(p->memory + position);
   p->b.tiles = reinterpret_cast<MoeTile*>(p->memory + tiles);
   p->b.hidden = p->memory + hidden;
-  p->b.gates = reinterpret_cast<float*>(p->memory + gates);
+  p->b.gates = weighted ? reinterpret_cast<float*>(p->memory + gates) : nullptr;
   p->b.part = p->b.sorted = p->memory + rows;
   *out = p;
   return MLD_OK;
@@ -379,7 +380,8 @@ int mld_moe_run(mld_moe_plan* plan, const mld_moe_io* io, int32_t tokens, void* 
     rc = launch_moe_gemm(true, shape, plan->b, io->gate_up, io->gate_up_scale, pairs, plan->sms, stream);
     if (rc == MLD_OK) rc = launch_moe_gemm(false, shape, plan->b, io->down, io->down_scale, pairs, plan->sms, stream);
     if (rc != MLD_OK) return rc;
-    MLD_CUDA_CHECK(launch_overlapped(moe_sum_kernel<__half>, dim3(tokens), dim3(256), 0, stream, s));
+    MLD_CUDA_CHECK(launch_overlapped(moe_weighted_parts(d.block) ? moe_sum_kernel<__half> : moe_sum_kernel<float>, dim3(tokens), dim3(256), 0,
+                                     stream, s));
     MLD_LAUNCH_CHECK();
     return MLD_OK;
   }

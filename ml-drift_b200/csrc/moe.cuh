@@ -19,8 +19,8 @@ struct MoeBuffers {
   MoeTile* tiles;    // [most tiles]
   int* n_tiles;
   void* hidden;      // fp16 [pairs][ffn], by position
-  float* gates;      // [pairs]: the pairs' weights by position (many rows)
-  void* part;        // [pairs][d_model], by position: fp32 with few rows; with many fp16, times the weights
+  float* gates;      // [pairs]: the pairs' weights by position (where parts are weighted, else null)
+  void* part;        // [pairs][d_model], by position: fp32; with many rows and scales to groups fp16, times the weights
   void* sorted;      // fp16 [pairs][d_model]: x by position (many rows); in the place of `part`, which is written later
   int* error;
 };
@@ -39,8 +39,9 @@ __device__ __forceinline__ float moe_gated(float gate, float up, int activation)
 }
 #endif
 
-// The products of tiles of up to kMoeTileRows rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp16,
-// times the pairs' weights: a part is rounded where its sum is, so that it is finite where that is).
+// The products of tiles of up to kMoeTileRows rows on the tensor cores.  first: x by position -> hidden; else hidden -> part (fp32, or
+// moe_weighted_parts: in fp16, times the pairs' weights, so that a part is finite where their sum is).
+inline bool moe_weighted_parts(int block) { return block != 0; }
 constexpr int kMoeTileRows = 256;
 int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const void* weights, const void* scale, int pairs, int sms,
                     cudaStream_t stream);

@@ -9,6 +9,10 @@
 //     zeros, and are not written.
 //   - the epilogue writes rows (not slices): of the first product act(gate) * up, for which neighbouring lanes, which hold a gate
 //     and an up channel, exchange half of their tokens; of the second the expert's output times the row's weight.
+// Weights with a scale to an output (CHANNEL) are multiplied as the integers that they are, which halves hold, and the sums are scaled;
+// the second product's go out in 32 bits then.  So nothing is rounded but x, the gated values and the result, as with few rows.  Weights
+// with scales to groups of inputs have to be scaled, and rounded to halves, ahead of the product; there outputs are halves, too (in
+// 32 bits 2048 tokens through 8 of 64 experts of 2048 x 1024 took 323 us in place of 301, and were 1.1 times as exact).
 // Per CTA: warps 0 and 23 fetch rows, every other stage each, warp 22 packed weights, warp 1 issues the MMAs (of the pair's first
 // CTA), warps 6..21 dequantise (four to a stage of 128 inputs), warps 2..5 write the results.  Tensor memory: four stages of weights
 // and two halves of 128 columns of accumulators.  A tile of up to 128 rows takes the half that is free, and the next tile goes on
@@ -54,8 +58,8 @@ struct GemmArgs {
   const __half* scale;
   int64_t expert_scales;
   int groups, group_shift;              // log2 of a group's input slices
-  __half* out;                          // rows by position: act(gate) * up [n / 2], or, times the row's weight, [n]
-  const float* gates;                   // the rows' weights
+  void* out;                            // rows by position: fp16 act(gate) * up [n / 2]; fp32 outputs [n], or fp16 times the row's weight
+  const float* gates;                   // the rows' weights (not with a scale to an output)
   int activation;
   int* error;
 };
@@ -136,7 +140,7 @@ __device__ __forceinline__ void store_pair(__half* first, int64_t pitch, bool on
   if (two) *reinterpret_cast<uint2*>(first + pitch) = make_uint2(__byte_perm(x0, x1, 0x7632), __byte_perm(x2, x3, 0x7632));
 }
 
-template <int BITS, bool FIRST>
+template <int BITS, bool CHANNEL, bool FIRST>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     moe_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, GemmArgs a) {
   constexpr int kBlk = BITS == 4 ? 8 : 16;
@@ -193,8 +197,9 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   // The weights of the rows that a warp is going to write, of two pieces of 16 rows to a register: eight pieces at most of a tile that
   // it writes alone, else four.  Asked for ahead of the wait for the products.  (A load to a piece took 2048 tokens through 8 of 64
   // experts 2 us longer.)
+  constexpr bool kWeighted = !FIRST && !CHANNEL;
   const auto weights_of = [&](const MoeTile& tile, int part, int parts, auto& w) {
-    if constexpr (!FIRST) {
+    if constexpr (kWeighted) {
 #pragma unroll
       for (int i = 0; i < static_cast<int>(sizeof w / 4); ++i) {
         const int m = 16 * (part + parts * (2 * i + (lane >> 4))) + (lane & 15);
@@ -203,7 +208,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     }
   };
   static_assert(kHalf <= 8 * 16 && kMoeTileRows <= 4 * 16 * kReaders, "rows of a warp");
-  const auto drain = [&](const MoeTile& tile, int n0, int part, const Turns& turn, auto& weights) {
+  // The scale of a lane's channel.
+  const auto scale_of = [&](const MoeTile& tile, int n0) {
+    const int n = n0 + static_cast<int>(rank) * kChannels + (warp & 3) * 32 + lane;
+    return CHANNEL && n < a.n ? __half2float(a.scale[tile.expert * a.expert_scales + n]) : 0.0f;
+  };
+  const auto drain = [&](const MoeTile& tile, int n0, int part, const Turns& turn, auto& weights, float scale) {
     const int parts = turn.all ? kReaders : 1;
     const int quad = warp & 3;
     const uint32_t base = tmem_base + (static_cast<uint32_t>(quad * 32) << 16) + static_cast<uint32_t>(turn.at * kHalf);
@@ -215,6 +225,10 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       uint32_t r[16];
       tmem_ld16(base + static_cast<uint32_t>(16 * pc), r);
       tmem_ld_wait();
+      if constexpr (CHANNEL) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * scale);
+      }
       if constexpr (FIRST) {
         const bool odd = (lane & 1) != 0;
         uint32_t x[4];
@@ -234,8 +248,14 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         const int q = (lane >> 1) & 3;
         turn_pairs<2>(x[0], x[1], x[2], x[3], q);
         const int m = 16 * pc + (odd ? 8 : 0) + 2 * q;
-        __half* to = a.out + static_cast<int64_t>(tile.row0 + m) * (a.n >> 1) + (n >> 1) + (lane >> 3) * 4;
+        __half* to = static_cast<__half*>(a.out) + static_cast<int64_t>(tile.row0 + m) * (a.n >> 1) + (n >> 1) + (lane >> 3) * 4;
         store_pair(to, a.n >> 1, has_n && m < tile.rows, has_n && m + 1 < tile.rows, x[0], x[1], x[2], x[3]);
+      } else if constexpr (CHANNEL) {
+        // (a warp's 32 channels of a row are 128 bytes)
+        float* const to = static_cast<float*>(a.out) + static_cast<int64_t>(tile.row0 + 16 * pc) * a.n + n + lane;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (has_n && 16 * pc + j < tile.rows) to[j * static_cast<int64_t>(a.n)] = __uint_as_float(r[j]);
       } else {
         uint32_t x[8];
 #pragma unroll
@@ -249,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         for (int h = 0; h < 2; ++h) {
           turn_pairs<1>(x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3], q);
           const int m = 16 * pc + 8 * h + 2 * q;
-          __half* to = a.out + static_cast<int64_t>(tile.row0 + m) * a.n + n + (lane >> 2) * 4;
+          __half* to = static_cast<__half*>(a.out) + static_cast<int64_t>(tile.row0 + m) * a.n + n + (lane >> 2) * 4;
           store_pair(to, a.n, has_n && m < tile.rows, has_n && m + 1 < tile.rows, x[4 * h], x[4 * h + 1], x[4 * h + 2], x[4 * h + 3]);
         }
         from ^= 16;
@@ -354,12 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       turn.take(tile, work.done());
       float weights[4];
       weights_of(tile, 0, turn.all ? kReaders : 1, weights);
+      const float scale = scale_of(tile, n0);
       if (!mbar_wait(&tmem_full[turn.full()], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 4);
         break;
       }
       tc_after();
-      drain(tile, n0, 0, turn, weights);
+      drain(tile, n0, 0, turn, weights, scale);
     }
   } else if (warp == 22) {
     // --------------------------------------------------------- packed weights
@@ -409,17 +430,17 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       turn.take(tile, work.done());
       const int n = n0 + static_cast<int>(rank) * kChannels + row;
       const bool has_n = n < a.n;
-      const __half* const scale = a.scale + tile.expert * a.expert_scales + n;
+      const __half* const scales = a.scale + tile.expert * a.expert_scales + n;
       // the scale of 32 inputs, asked for four stages ahead (by hand, so that nothing looks at it before)
       const auto ask = [&](unsigned short& v, int slice) {
         const int g = min(slice >> a.group_shift, a.groups - 1);
         asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p ld.global.nc.u16 %0, [%1];\n\t}"
                      : "+h"(v)
-                     : "l"(scale + static_cast<int64_t>(g) * a.n), "r"(has_n ? 1u : 0u));
+                     : "l"(scales + static_cast<int64_t>(g) * a.n), "r"(has_n ? 1u : 0u));
       };
       int kb = (group - before) & 3;
       unsigned short next[4] = {0, 0, 0, 0};
-      if (kb < a.k_blocks) {
+      if (!CHANNEL && kb < a.k_blocks) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) ask(next[i], kb * kSlices + 8 * i);
       }
@@ -428,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
         unsigned short cur[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) cur[i] = next[i];
-        if (kb + 4 < a.k_blocks) {
+        if (!CHANNEL && kb + 4 < a.k_blocks) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) ask(next[i], (kb + 4) * kSlices + 8 * i);
         }
@@ -450,7 +471,23 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
             for (int i = 0; i < 8; ++i) blk[i] = *reinterpret_cast<const Block*>(wp + (16 * sixty_four + 8 * half + i) * kPitch);
             const __half s = __ushort_as_half(cur[2 * sixty_four + half]);
             const __half2 s2 = __half2half2(s);
-            if constexpr (BITS == 4) {
+            if constexpr (CHANNEL) {
+              const auto exact = [&](uint32_t codes) {  // (1024 + u less 1024 and the zero)
+                const uint32_t biased = codes | 0x64006400u;
+                const __half2 w = __hsub2(*reinterpret_cast<const __half2*>(&biased), offset);
+                return *reinterpret_cast<const uint32_t*>(&w);
+              };
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                if constexpr (BITS == 4) {
+                  o[16 * half + 2 * i] = exact((blk[i].x >> (4 * col4)) & 0x000F000Fu);
+                  o[16 * half + 2 * i + 1] = exact((blk[i].y >> (4 * col4)) & 0x000F000Fu);
+                } else {
+                  o[16 * half + 2 * i] = exact(__byte_perm(blk[i].x, blk[i].y, sel8) & 0x00FF00FFu);
+                  o[16 * half + 2 * i + 1] = exact(__byte_perm(blk[i].z, blk[i].w, sel8) & 0x00FF00FFu);
+                }
+              }
+            } else if constexpr (BITS == 4) {
               // A nibble at bits 6..9 is the subnormal half u 2^-18: u 2^-18 (2^18 s) - 8 s is (u - 8) s rounded once, in one
               // instruction.  2^18 s has to be a half; else from 1024 + u, the zero off exactly first.
               if (__all_sync(0xffffffffu, __habs(s) < __float2half_rn(0.249f))) {
@@ -505,12 +542,13 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       if (!turn.all) continue;
       float weights[2];
       weights_of(tile, 1 + group, kReaders, weights);
+      const float scale = scale_of(tile, n0);
       if (!mbar_wait(&tmem_full[2], turn.full_phase())) {
         atomicExch(a.error, kErrMoeBase + 7);
         break;
       }
       tc_after();
-      drain(tile, n0, 1 + group, turn, weights);
+      drain(tile, n0, 1 + group, turn, weights, scale);
     }
   }
   // Nobody leaves while the partner may still arrive on this CTA's barriers or the pair's MMAs write its tensor memory.
@@ -528,12 +566,12 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   }
 }
 
-template <int BITS, bool FIRST>
+template <int BITS, bool CHANNEL, bool FIRST>
 int launch_of(const CUtensorMap& tx, const CUtensorMap& tw, const GemmArgs& a, int grid, cudaStream_t stream) {
   constexpr size_t smem = 1024 + kStages * 2 * kAtom + kWStages * kSlices * (kChannels / 4) * (BITS == 4 ? 8 : 16) +
                           (2 * kWStages + 2 * kStages + 5) * 8 + 64;
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kern = moe_gemm_kernel<BITS, FIRST>;
+  auto kern = moe_gemm_kernel<BITS, CHANNEL, FIRST>;
   static bool done[kMaxDevices];
   int dev;
   if (needs_configure(done, &dev)) {
@@ -570,13 +608,16 @@ int launch_moe_gemm(bool first, const MoeShape& s, const MoeBuffers& b, const vo
   if (s.block != 0)
     for (a.group_shift = 3; (4 << a.group_shift) < s.block;) ++a.group_shift;
   a.expert_scales = static_cast<int64_t>(a.groups) * n;
-  a.out = static_cast<__half*>(first ? b.hidden : b.part);
+  a.out = first ? b.hidden : b.part;
   a.gates = b.gates;
   a.activation = s.activation;
   a.error = b.error;
   const int grid = sms / 2 * 2;
-  if (s.bits == 4) return first ? launch_of<4, true>(tx, tw, a, grid, stream) : launch_of<4, false>(tx, tw, a, grid, stream);
-  return first ? launch_of<8, true>(tx, tw, a, grid, stream) : launch_of<8, false>(tx, tw, a, grid, stream);
+  const auto launch = s.bits == 4 ? (s.block == 0 ? (first ? launch_of<4, true, true> : launch_of<4, true, false>)
+                                                  : (first ? launch_of<4, false, true> : launch_of<4, false, false>))
+                                  : (s.block == 0 ? (first ? launch_of<8, true, true> : launch_of<8, true, false>)
+                                                  : (first ? launch_of<8, false, true> : launch_of<8, false, false>));
+  return launch(tx, tw, a, grid, stream);
 }
 
 }  // namespace mld

@@ -125,3 +125,30 @@ def _spread(scales, inputs):
     """Scales [experts][groups][outputs] for each of the inputs, [experts][outputs][inputs]."""
     s = scales.double().cpu().numpy()
     return np.repeat(s, inputs // s.shape[1], 1).transpose(0, 2, 1)
+
+
+@pytest.mark.parametrize("path", ["few", "many"])
+@pytest.mark.parametrize("n", [1, 40, 300, 700])
+@pytest.mark.parametrize("bits,d,f", [(8, 96, 352), (8, 512, 256), (4, 256, 128)])
+@pytest.mark.parametrize("large", [1.0, 200.0])
+def test_weights_with_a_scale_to_an_output_are_not_rounded(mld, n, path, bits, d, f, large):
+    """Both kernels within the errors of gated values and results alone; experts' outputs may leave 16 bits ahead of their weights."""
+    e, k = 5, 2
+    (first, second), (w1, s1, w2, s2) = _few_matrices(d + bits, d, f, bits, 0, e, e)
+    s2, old = (s2.double() * large).half(), _spread(s2, f)
+    second = np.rint(second / old) * _spread(s2, f)
+    rng = np.random.default_rng(n)
+    x, gates = (30 * rng.standard_normal((n, d))).astype(np.float16), (rng.random((n, k)) / (900 * large)).astype(np.float32)
+    ids = np.argsort(rng.random((n, e)), 1)[:, :k].astype(np.int32)
+    ids[3::11, 1] = -1
+    plan = mld.MoeExperts(e, k, d, f, weight_bits=bits, block=0, max_tokens=n, activation=n % 2, force_path=mld.MOE_PATH_FEW_ROWS if path == "few" else mld.MOE_PATH_MANY_ROWS)
+    out = torch.empty(n, d, dtype=torch.float16, device="cuda")
+    plan.run(_dev(x), _dev(ids), _dev(gates), w1, s1, w2, s2, out)
+    want, size = ref.experts(x, ids, gates, first, second, None, n % 2 == 1)
+    got = out.cpu().numpy().astype(np.float64)
+    bound = ref.experts_bound(want, size, False)
+    assert (np.abs(got - want) <= bound).all(), np.max(np.abs(got - want) / bound)
+    assert plan.device_status() == 0
+    signal = np.sqrt((want ** 2).sum())
+    # two roundings to 16 bits, of at most 2^-11 each, uncorrelated; sums in 32 bits are far below
+    assert np.sqrt(((got - want) ** 2).sum()) <= 2.0 ** -11 * np.sqrt(2) / np.sqrt(3) * 1.05 * signal
