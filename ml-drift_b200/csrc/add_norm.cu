@@ -14,7 +14,8 @@
 // 2^-13, above six roundings of 2^-24 at a value of 255 at most: of the span, its reciprocal and a value's distance from the row's
 // smallest, and, with an offset or 32-bit tensors, of offset + w, v and that smallest.  The last three are relative to v, so for
 // them near grows with max|v| / span where that is above 1; where it passes a quarter, the whole row is worked out in 64.  (Of rows
-// about zero one chunk in 500 is worked out again.)
+// about zero one chunk in 500 is worked out again: 2048 rows of 4096 in fp32, asymmetric, take 33 us; of a mean of 10 deviations 35,
+// of 1000 44.)
 #include <cuda_fp16.h>
 
 #include <atomic>

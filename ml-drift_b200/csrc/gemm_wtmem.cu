@@ -390,7 +390,10 @@ __global__ void __launch_bounds__(kWtThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------ producer of the activation tiles
     if (lane == 0) prefetch_tmap(&tmap_x);
-    // Everything else that this kernel reads was complete when the transposition ahead of it let it begin.
+    // What the other roles read ahead of this wait (weights, scales, the work's split) was complete when the transposition ahead let this
+    // kernel begin; callers of products on codes, which have no such pass, see to it that no launch still writes it.  The codes are
+    // read behind the wait, which ends when the launch ahead has, and every launch ends behind its own wait: back to the norm.  What
+    // this kernel writes follows products of rows fetched behind the wait, so nothing ahead reads or writes there any more.
     pdl_wait();
     int stage = 0;
     uint32_t phase = 0;

@@ -231,7 +231,9 @@ bool takes_many(const mld_moe_desc& d, int tokens) {
   if (d.force_path != MLD_MOE_PATH_AUTO) return d.force_path == MLD_MOE_PATH_MANY_ROWS;
   // By the rows of an expert, were all alike.  us, few / many, at 6, 8 and 10: 64 experts of 2048 x 1024 in 4 bits 86 / 105, 101 / 106,
   // 115 / 105; 8 of 4096 x 4096 76 / 108, 89 / 109, 113 / 109, in 8 bits 91 / 124, 107 / 124, 134 / 124; 128 of 2048 x 768
-  // 121 / 130, 144 / 141, 166 / 141.
+  // 121 / 130, 144 / 141, 166 / 141.  (Measured with rows spread evenly.  The host does not see the ids: a batch of up to this many rows
+  // that goes to a few of many experts takes tiles of eight, each of which streams its expert's weights; force_path is for callers
+  // who know.)
   return static_cast<int64_t>(tokens) * d.top_k > kFewShare * static_cast<int64_t>(d.experts);
 }
 

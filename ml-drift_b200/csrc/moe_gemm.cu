@@ -20,8 +20,8 @@
 // With few rows bound by what a stage costs each role, whatever is in it (the warps that fetch and the one that issues MMAs 300 to
 // 500 cycles, the dequantisation about 1700 for a quarter of the stages): hence 128 inputs to a stage, where 64 took 122 us against
 // 107 (128 tokens through 8 of 64 experts, 2048 x 1024) and 139 against 127 (512 tokens), at a cost of 1 to 2 % at 1531 and 2048.  With
-// many rows by the MMAs, 4 cycles a row and stage, and by the clock that the power limit leaves: 1531 tokens through 2 of 8 experts of
-// 4096 x 14336 take 1035 us, 1.04 PFLOP/s.
+// many rows by the MMAs, 4 cycles a row and stage, and by the clock that the power limit leaves: 1501 tokens through 2 of 8 experts of
+// 4096 x 14336 take 1051 us, 1.01 PFLOP/s.
 // Every wait is bounded.
 #include <cuda_fp16.h>
 
