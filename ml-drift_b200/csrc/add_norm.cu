@@ -477,10 +477,10 @@ extern "C" int mld_add_rms_norm(const mld_add_norm_desc* d, const mld_add_norm_i
   MLD_REQUIRE(d->eps >= 0.0f && d->eps < INFINITY && d->weight_offset > -INFINITY && d->weight_offset < INFINITY,
               "eps must be finite and not negative, weight_offset finite");
   MLD_REQUIRE(tokens >= 0 && tokens <= 1 << 30, "tokens must be 0 to 2^30");
+  if (tokens == 0) return MLD_OK;  // (whose tensors may have no address)
   MLD_REQUIRE(io->out != nullptr || io->codes != nullptr, "neither out nor codes");
   MLD_REQUIRE((io->codes == nullptr) == (io->params == nullptr), "codes and params go together");
   MLD_REQUIRE(io->sum_out == nullptr || io->residual != nullptr, "sum_out needs a residual");
-  if (tokens == 0) return MLD_OK;
   MLD_REQUIRE(io->x != nullptr, "null tensor");
   const uintptr_t esz = d->f16 ? 2 : 4;
   const uintptr_t all = reinterpret_cast<uintptr_t>(io->x) | reinterpret_cast<uintptr_t>(io->residual) |
